@@ -1265,6 +1265,208 @@ def attn_decode(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, seg_q
     _check(code, "attn_decode", f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
 
 
+# ---------------------------------------------------------------------------
+# a cache held in 4 bits (csrc/q4.cuh: the format)
+
+Q4_HEAD_DIMS = (64, 128, 256)
+Q4_PAGE_STEP = 16   # a page's tokens are a multiple of this
+
+
+def q4_takes(head_dim: int, page_tokens: int) -> bool:
+    """Whether heads of this size and pages of so many tokens can be held in 4 bits."""
+    return head_dim in Q4_HEAD_DIMS and page_tokens > 0 and page_tokens % Q4_PAGE_STEP == 0
+
+
+def q4_page_bytes(head_dim: int, page_tokens: int) -> int:
+    """Bytes of a page of one key/value head, keys or values alone: ``page_tokens`` rows of ``head_dim / 2`` bytes of codes and
+    as many pairs (scale, mid) of bfloat16."""
+    return page_tokens * (head_dim // 2 + 4)
+
+
+def _q4_here(what: str, **tensors) -> None:
+    """Tensors that lie on the current device (launches go to its current stream)."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{what}: {name} must be a CUDA tensor")
+        if t.device.index != here:
+            raise KernelError(f"{what}: {name} lies on {t.device}, the current device is cuda:{here}")
+        if not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be contiguous")
+
+
+def _q4_pool(what: str, pool: torch.Tensor, n_kv_heads: int, head_dim: int, page_tokens: int, lead: int = 0) -> None:
+    _need(q4_takes(head_dim, page_tokens), f"{what}: heads of {head_dim} in pages of {page_tokens} tokens (known: heads of "
+          f"{', '.join(map(str, Q4_HEAD_DIMS))}, pages of a multiple of {Q4_PAGE_STEP})")
+    _need(pool.dtype == torch.uint8 and pool.dim() == 4 + lead
+          and tuple(pool.shape[1 + lead:]) == (2, n_kv_heads, q4_page_bytes(head_dim, page_tokens)),
+          f"{what}: the pool must be uint8 [{'layers, ' * lead}pages, 2, {n_kv_heads}, {q4_page_bytes(head_dim, page_tokens)}]")
+    _need(pool.data_ptr() % 16 == 0, f"{what}: the pool must start at a multiple of 16 bytes")
+
+
+def _q4_i32(what: str, least: int, **tensors) -> None:
+    for name, t in tensors.items():
+        _need(t.dtype == torch.int32 and t.numel() >= least, f"{what}: {name} must be int32 with at least {least} elements")
+
+
+def _q4_weights(what: str, weights: Optional[torch.Tensor], lead, n_kv_heads: int, page_tokens: int) -> None:
+    if weights is not None:
+        _need(weights.dtype == torch.float32 and tuple(weights.shape) == tuple(lead) + (n_kv_heads, page_tokens),
+              f"{what}: weights must be float32 {list(lead) + [n_kv_heads, page_tokens]}")
+
+
+def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], q_out: torch.Tensor,
+                     pool: torch.Tensor, slots: torch.Tensor, *, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int,
+                     interleaved: bool, page_tokens: int, write_kv: bool = True, weights: Optional[torch.Tensor] = None) -> None:
+    """:func:`rope_kv_write` into a cache held in 4 bits: q, rotated, to ``q_out`` in the model's type; k, rotated, and v, neither rounded to
+    the model's type first, to the rows of ``slots`` in ``pool`` uint8 [n_pages, 2, n_kv_heads, :func:`q4_page_bytes`].  A row x of a head is
+    held as one of sixteen codes per element and two bfloat16: scale = (max - min) / 15 and mid = (min + max) / 2, and stands for
+    mid + scale * (code - 7.5); a row with a value that is not finite reads as NaN.  The angles' product and reduction are 64 bits.
+    ``weights`` float32 [n_pages, n_kv_heads, page_tokens]: set to 0 for the slots written (see :func:`attn_decode_q4`)."""
+    what = "rope_kv_write_q4"
+    _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
+    T = qkv.shape[0]
+    _need(qkv.dim() == 2 and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim, f"{what}: qkv width")
+    _need(qkv.dtype == q_out.dtype, f"{what}: qkv and q_out share one element type")
+    _need(q_out.numel() >= T * n_heads * head_dim, f"{what}: q_out is too small")
+    _need(qkv.data_ptr() % 16 == 0 and q_out.data_ptr() % 16 == 0, f"{what}: qkv and q_out must start at multiples of 16 bytes")
+    _q4_i32(what, T, positions=positions, slots=slots)
+    _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
+    if inv_freq is not None:
+        _need(0 <= rot_dim <= head_dim and rot_dim % 2 == 0, f"{what}: rot_dim {rot_dim} of heads of {head_dim}")
+        _need(inv_freq.dtype == torch.float32 and inv_freq.numel() == rot_dim // 2, f"{what}: inv_freq must be float32 [rot_dim / 2]")
+    _q4_here(what, qkv=qkv, positions=positions, inv_freq=inv_freq, q_out=q_out, pool=pool, slots=slots, weights=weights)
+    code = _lib("cache_q4").locus_rope_kv_write_q4(
+        _p(qkv), I(dtype_code(qkv.dtype)), _p(positions), _p(inv_freq), _p(q_out), _p(pool), _p(slots), _p(weights), I(T), I(n_heads),
+        I(n_kv_heads), I(head_dim), I(rot_dim), I(1 if interleaved else 0), I(page_tokens), I(1 if write_kv else 0), _stream())
+    _check(code, what, f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
+
+
+def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: torch.Tensor, n_segs: int, seg_ctx: torch.Tensor, seg_qn: torch.Tensor,
+              block_table: torch.Tensor, n_kv_heads: int, head_dim: int, page_tokens: int, max_keys: int) -> None:
+    """The rows of positions 0 .. seg_ctx + seg_qn - 1 of the segments ``segs`` [n_segs], out of ``pool`` (4 bits) into ordinary pages
+    ``out`` [n_pages, 2, n_kv_heads, page_tokens, head_dim] of the same page ids, float32 or bfloat16 (rounded once): what the kernels of prompt
+    portions (:func:`attn_chunk` and the others) read.  Rows behind a segment's last token and pages that went back (-1) stay as they were.
+    ``max_keys``: at least the rows of the longest of these segments."""
+    what = "expand_q4"
+    _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
+    _need(tuple(out.shape) == (pool.shape[0], 2, n_kv_heads, page_tokens, head_dim), f"{what}: out must have the pool's pages in the model's type")
+    _need(out.data_ptr() % 16 == 0, f"{what}: out must start at a multiple of 16 bytes")
+    _need(block_table.dim() == 2, f"{what}: block_table [segments, width]")
+    _q4_i32(what, n_segs, segs=segs)
+    _q4_i32(what, 0, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
+    _q4_here(what, pool=pool, out=out, segs=segs, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
+    code = _lib("cache_q4").locus_expand_q4(
+        _p(pool), _p(out), I(dtype_code(out.dtype)), _p(segs), I(n_segs), _p(seg_ctx), _p(seg_qn), _p(block_table), I(block_table.shape[1]),
+        I(n_kv_heads), I(head_dim), I(page_tokens), I(max_keys), _stream())
+    _check(code, what, f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_segs} segments of up to {max_keys} keys)")
+
+
+def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Tensor, n_tokens: torch.Tensor, n_items: int, keep: int,
+             first: int, recent: int, kept: torch.Tensor, n_kv_heads: int, head_dim: int, page_tokens: int, max_tokens: int,
+             dst_table: Optional[torch.Tensor] = None) -> None:
+    """Let go of the keys that mattered least.  Of every layer of ``pool`` uint8 [layers, pages, 2, n_kv_heads, :func:`q4_page_bytes`], request (row of
+    ``block_table`` [n_items, width], ``n_tokens`` [n_items] tokens) and key/value head at most ``keep`` keys stay: the first ``first``,
+    the last ``recent`` and the heaviest of the others by ``weights`` float32 [layers, pages, n_kv_heads, page_tokens] (:func:`attn_decode_q4`
+    adds them up).  Of equal weights the earlier key stays; a weight that is NaN counts as the lightest.  The keys that stay keep their order: their
+    rows, factors and weights become those of slots 0 .. keep - 1, of the request's own pages (``dst_table`` None: in place; a page that is not
+    needed any more may go back) or of ``dst_table``'s, which must be other pages than any that ``block_table`` lists.  ``kept`` int32 [layers,
+    n_items, n_kv_heads, keep]: which keys stayed, -1 behind the keys of a request that has fewer than ``keep``, and stays whole.  Each head keeps keys
+    of its own; every head of a request has the same number.  Keys keep the rotation of the position that they were written at.
+    ``max_tokens``: at least the tokens of the longest request."""
+    what = "evict_q4"
+    _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens, 1)
+    _q4_weights(what, weights, pool.shape[:2], n_kv_heads, page_tokens)
+    _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep, f"{what}: keep {keep} with the first {first} and the last {recent}")
+    _need(block_table.dim() == 2 and block_table.shape[0] >= n_items, f"{what}: block_table [requests, width]")
+    _need(kept.dtype == torch.int32 and tuple(kept.shape) == (pool.shape[0], n_items, n_kv_heads, keep), f"{what}: kept must be int32 [layers, requests, kv heads, keep]")
+    _q4_i32(what, n_items, n_tokens=n_tokens)
+    _q4_i32(what, 0, block_table=block_table)
+    _need(0 < max_tokens <= block_table.shape[1] * page_tokens, f"{what}: max_tokens {max_tokens} beyond what block_table describes")
+    to = block_table if dst_table is None else dst_table
+    if dst_table is not None:
+        _q4_i32(what, 0, dst_table=dst_table)
+        _need(dst_table.dim() == 2 and dst_table.shape[0] >= n_items and dst_table.shape[1] * page_tokens >= min(keep, max_tokens),
+              f"{what}: dst_table [requests, pages for the keys that stay]")
+    _q4_here(what, pool=pool, weights=weights, block_table=block_table, n_tokens=n_tokens, kept=kept, dst_table=dst_table)
+    code = _lib("cache_q4").locus_evict_q4(
+        _p(pool), _p(weights), _p(block_table), I(block_table.shape[1]), _p(to), I(to.shape[1]), _p(n_tokens), I(n_items), I(pool.shape[0]),
+        LL(pool.shape[1]), I(n_kv_heads), I(head_dim), I(page_tokens), I(keep), I(first), I(recent), I(max_tokens), _p(kept), _stream())
+    if code == 0:
+        _count_launches(1)
+    _check(code, what, f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_items} requests, keep {keep})")
+
+
+# The range cut's cost model of the 4-bit kernel, in keys (see GQA_COST_RANGE).
+Q4_COST_RANGE, Q4_COST_MERGE_PER_HEAD = 64, 2
+Q4_MAX_ITEMS = 1024
+
+
+def decode_units_q4(max_items: int, n_heads: int, device, fixed_ranges: bool = False) -> int:
+    """How many partial results (``head_dim`` floats of ``part_o``, two of ``part_ml``) the scratch of :func:`attn_decode_q4` should hold for
+    batches of up to ``max_items`` requests; ``fixed_ranges``: with a window that keeps first tokens."""
+    try:
+        n_sm = torch.cuda.get_device_properties(device).multi_processor_count
+    except Exception:  # no GPU (host tests with emulated kernels)
+        n_sm = 148
+    return max_items * n_heads * (2 if fixed_ranges else 1) + 8 * 16 * n_sm
+
+
+def attn_q4_error() -> int:
+    """Error word of the 4-bit decode attention module (0 = fine; 1 = a wait for a bulk copy ran out); reading it synchronises the device and
+    clears it."""
+    return int(_lib("attention_q4").locus_attn_q4_error())
+
+
+def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, seg_q0: torch.Tensor, seg_ctx: torch.Tensor,
+                   block_table: torch.Tensor, items: torch.Tensor, n_items: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                   page_tokens: int, window: int, scale: float, part_o: torch.Tensor, part_ml: torch.Tensor, counters: torch.Tensor,
+                   keep_first: int = 0, sink=False, chunk: int = 0, slopes: Optional[torch.Tensor] = None,
+                   weights: Optional[torch.Tensor] = None, scores: Optional[torch.Tensor] = None) -> None:
+    """:func:`attn_decode` over a cache held in 4 bits (``pool`` uint8 [n_pages, 2, n_kv_heads, :func:`q4_page_bytes`], written by
+    :func:`rope_kv_write_q4`): the codes are multiplied as they are, nothing is laid out in between.  q and out float32 or bfloat16, any number of
+    query heads per key/value head; masks, sinks and distance biases as there.
+
+    ``part_o``, ``part_ml``: scratch for :func:`decode_units_q4` partial results; ``counters`` (int32, n_items * n_heads) must be zero before
+    the call and is zero after it.  ``weights`` float32 [n_pages, n_kv_heads, page_tokens] (without a window or chunks): the softmax weight that
+    each key gets, summed over the query heads of its group, is added to the key's slot; ``scores`` is scratch for that, float32 with
+    n_items * n_heads * block_table.shape[1] * page_tokens elements."""
+    what = "attn_decode_q4"
+    _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
+    _need(n_heads > 0 and n_heads % n_kv_heads == 0, f"{what}: {n_heads} heads are not a multiple of {n_kv_heads} kv heads")
+    _need(q.dtype == out.dtype and q.numel() % (n_heads * head_dim) == 0 and out.numel() % (n_heads * head_dim) == 0,
+          f"{what}: q and out must be rows of {n_heads} heads of {head_dim}, of one element type")
+    _need(q.data_ptr() % 16 == 0 and part_o.data_ptr() % 16 == 0 and part_ml.data_ptr() % 8 == 0, f"{what}: q and the scratch must start at multiples of 16 bytes")
+    _need(block_table.dim() == 2, f"{what}: block_table [segments, width]")
+    _need(n_items <= Q4_MAX_ITEMS, f"{what}: {n_items} requests (at most {Q4_MAX_ITEMS})")
+    _q4_i32(what, n_items, items=items)
+    _q4_i32(what, n_items * n_heads, counters=counters)
+    _q4_i32(what, 0, seg_q0=seg_q0, seg_ctx=seg_ctx, block_table=block_table)
+    _need(part_o.dtype == torch.float32 and part_ml.dtype == torch.float32, f"{what}: float32 scratch")
+    lse, floats = None, part_o.numel()
+    if weights is not None:
+        _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
+        _need(window == 0 and chunk == 0, f"{what}: weights go with neither a window nor chunks")
+        _need(scores is not None and scores.dtype == torch.float32 and scores.numel() >= n_items * n_heads * block_table.shape[1] * page_tokens,
+              f"{what}: scores too small for weights")
+        floats = max(0, (floats - 2 * n_items * n_heads) // 4 * 4)   # a head's maximum and denominator lie behind the partial results
+        lse = part_o.view(-1)[floats:]
+    max_units = min(floats // head_dim, part_ml.numel() // 2)
+    _need(max_units >= n_items * n_heads * (2 if keep_first > 0 and window > 0 else 1), f"{what}: scratch too small")
+    _q4_here(what, q=q, pool=pool, out=out, seg_q0=seg_q0, seg_ctx=seg_ctx, block_table=block_table, items=items, part_o=part_o, part_ml=part_ml,
+             counters=counters, slopes=slopes, weights=weights, scores=scores)
+    code = _lib("attention_q4").locus_attn_decode_q4(
+        _p(q), I(dtype_code(q.dtype)), _p(pool), _p(out), _p(seg_q0), _p(seg_ctx), _p(block_table), I(block_table.shape[1]), _p(items), I(n_items),
+        I(n_heads), I(n_kv_heads), I(head_dim), I(page_tokens), I(window), I(chunk), F(scale), _p(part_o), _p(part_ml), _p(counters),
+        LL(max_units), I(Q4_COST_RANGE), I(Q4_COST_MERGE_PER_HEAD * (n_heads // n_kv_heads)), I(keep_first if window > 0 else 0),
+        *_sink_args(sink, n_heads), _slopes_arg(slopes, n_heads), _p(weights), _p(scores if weights is not None else None), _p(lse), _stream())
+    if weights is not None and code == 0 and n_items > 0:
+        _count_launches(1)
+    _check(code, what, f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
+
+
 SCORE_FUNCTIONS = {"softmax": 0, "sigmoid": 1}
 # what a group of experts is judged by when only some groups stay eligible: the sum of its two best selection scores,
 # or its best one (a flag beside the score function's code, see csrc/route_select.cuh)
