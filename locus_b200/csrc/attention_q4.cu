@@ -3,36 +3,49 @@
 //   o_h = sum_t p_t v_t   p = softmax over the keys in sight of scale * q_h . k_t (a sink, a distance bias: as in attention.cu)
 //
 // with k_t and v_t read straight from their codes.  A key's row is mid + scale (code - 7.5) = z + scale (code - 7), z = mid - scale / 2, and codes
-// less 7 are small whole numbers that bfloat16 holds exactly, so
+// less 7 are small whole numbers that float16 holds exactly, so
 //
 //   q . k_t = scale_t (q . (code_t - 7)) + z_t sum(q)                      the product on the tensor cores, the rest per score in float32
 //   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t z_t             the same for the values
 //
-// and nothing is rounded but the weights p_t scale_t, to bfloat16 (an operand of the tensor cores; the unrounded p_t enter the denominator
-// and z's sum).  The 7 is taken off the codes rather than out of the sums: sums of codes of one sign would lose what cancels in them.
-// A float32 model's q and weights go through the tensor cores as three bfloat16 parts each (bf16_parts.cuh), so nothing is rounded there.
+// The tensor cores' operands are float16:
+//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
+//     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more;
+//   * the weights p_t scale_t, formed relative to the running maximum M of score + exponent of scale, so that they stay below 2^15, whatever the
+//     scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest where that is more; two parts for a float32 model).  The
+//     unrounded p_t enter the denominator and z's sum.  (bfloat16, the model's type, would round to 2^-9, and the unpacking below would cost
+//     more: its mantissa holds one nibble at a time.)
+// The 7 is taken off the codes rather than out of the sums: sums of codes of one sign would lose what cancels in them.
+// For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
+// over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
-// The work is cut as in attention_gqa.cu: a warp takes a range of keys of one (request, key/value head) for up to 16 query heads that share
-// it, in the transposed form (16 keys in the M dimension of mma.sync m16n8k16, eight heads in N):
-//   S^T [16 keys x 8 heads] = (C_k - 7) [16 x hd] . Q^T     a lane's words of a key row hold eight codes each: one shift, one mask-and-or and
-//                             one subtraction give two neighbouring dimensions as bfloat16, as the A fragment wants them;
+// A warp takes a range of keys of one (request, key/value head) for up to 16 query heads that share it, in the transposed form (16 keys in the M
+// dimension of mma.sync m16n8k16, eight heads in N):
+//   S^T [16 keys x 8 heads] = (C_k - 7) [16 x hd] . Q^T     a lane's words of a key row hold eight codes each: a mask-and-or and a subtraction (or a
+//                             multiply-add that also takes the nibble's place out) give two neighbouring dimensions as the A fragment wants them;
 //   O^T [hd x 8 heads] += (C_v - 7)^T [hd x 16 keys] . P^T  the A fragment wants one dimension of two keys in a register: a byte permute joins
 //                             the same byte of two keys' words, and its two nibbles are two dimensions (two row tiles' halves).
 // A group of more heads is served by several warps (that each read its rows, from the L2 after the first).
-// The running maximum of a head is raised only when a score exceeds it by more than 2^8: until then the weights are formed relative to the
-// old one (at most 2^8, well inside float32), which saves the exchange between lanes and the correction of the sums in nearly every chunk.
+// M is raised only when a score exceeds it by more than 2^4: until then the weights are formed relative to the old one, which saves the exchange
+// between lanes and the correction of the sums in nearly every chunk.
+//
+// The cut: every (request, key/value head) is cut into ranges of one length (plan_ranges), and the units (request, head, range), in this order, are
+// dealt to the blocks by runs of as many as a block has warps.  The warps of a block that have ranges of one (request, head) join them in shared
+// memory; what covers it whole is the output, else the block leaves one partial result, and the block that is the last to do so joins those, in
+// ascending order.  (With one partial result per warp, joined by the last warp, a request of 131,000 tokens took 270 us, most of it in that.)
 //
 // Memory: a warp's ring in shared memory is filled by bulk copies of up to 64 keys of one page: codes and factors of K, then of V.  (A whole
 // page of 64 tokens is one run of bytes per plane.)  Every wait is bounded: when the limit runs out the warp records it in the module's error
-// word, waits for its other copies with the same limit and leaves.
+// word, waits for its other copies with the same limit and goes on to the end without a further copy.
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
 //
 // With weights: the scores are written out as they are formed, and a second kernel (q4_weigh_kernel) adds every key's p_t, summed over the heads
 // of its group, to a number per (slot, key/value head).  The softmax's denominator is known only behind the last range.
-#include "attn_ranges.cuh"
-#include "bf16_parts.cuh"
+#include <cuda_fp16.h>
+
 #include "distance.cuh"
+#include "mask.cuh"
 #include "q4.cuh"
 #include "sink.cuh"
 
@@ -125,9 +138,9 @@ __device__ __forceinline__ void lds_words(uint32_t* v, uint32_t addr) {
     }
 }
 
-__device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -142,41 +155,149 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+// the codes in bits 0 .. 3 of a register's halves, less 7, as float16: 0x6400 | n is 1024 + n
+__device__ __forceinline__ uint32_t codes_low(uint32_t x) {
+    return bits(__hsub2(halves((x & 0x000f000fu) | 0x64006400u), halves(0x64076407u)));
 }
-// the low nibbles of a register's halves, less 7, as two bfloat16: 0x4300 | n is 128 + n, and 135 comes off exactly
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-    const uint32_t y = (x & 0x000f000fu) | 0x43004300u;
-    const uint32_t k = 0x43074307u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&k));
-    return *reinterpret_cast<const uint32_t*>(&d);
+// the codes in bits 4 .. 7: (1024 + 16 n) / 16 - 71
+__device__ __forceinline__ uint32_t codes_high(uint32_t x) {
+    return bits(__hfma2(halves((x & 0x00f000f0u) | 0x64006400u), halves(0x2c002c00u), halves(0xd470d470u)));
 }
-
-// a pair of values as PARTS pairs of bfloat16: one, rounded, or three that sum to them
+// a pair of values as PARTS pairs of float16: one, rounded, or two
 template <int PARTS>
 __device__ __forceinline__ void split2(float a, float b, uint32_t* out) {
-    if constexpr (PARTS == 3) bf16_parts(a, b, out[0], out[1], out[2]);
-    else out[0] = pack2(a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    out[0] = bits(h);
+    if constexpr (PARTS == 2) {
+        const float2 f = __half22float2(h);
+        out[1] = bits(__floats2half2_rn(a - f.x, b - f.y));
+    }
 }
-__device__ __forceinline__ void load_pair(const bf16* p, uint32_t* out) { out[0] = *reinterpret_cast<const uint32_t*>(p); }
-__device__ __forceinline__ void load_pair(const float* p, uint32_t* out) {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    split2<3>(v.x, v.y, out);
+__device__ __forceinline__ float pow2i(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }   // -126 .. 127
+
+__device__ __forceinline__ void load8(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const bf16* p, float* v) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The cut of a step's keys into ranges.
+#define Q4_MAX_ITEMS 1024
+#define Q4_CAND 256       // candidate range lengths looked at
+
+struct Q4Plan {
+    int first[Q4_MAX_ITEMS];     // first key of item i, rounded down to 16
+    int pos[Q4_MAX_ITEMS];       // position of its query
+    int seg[Q4_MAX_ITEMS];
+    int pref[Q4_MAX_ITEMS + 1];  // ranges of the items before i
+    unsigned long long best[32];
+    int len;
+};
+
+// kept first tokens of an item that lie in front of its window's first chunk: a range of their own, the item's first
+__device__ __forceinline__ int q4_kept(const Q4Args& a, int first) { return a.window > 0 ? min(a.keep_first, first) : 0; }
+// Ranges of `n` keys at a length of about len (inv its reciprocal).  By a product, which may be one more than need be; the same everywhere.
+__device__ __forceinline__ int q4_ranges(int n, int len, float inv) { return max(1, static_cast<int>(static_cast<float>(n + len - 1) * inv)); }
+// The length of an item's ranges: all alike, whole pieces of 16, 32 or 64 keys (long ranges begin where pages do).
+__device__ __forceinline__ int q4_length(int n, int ranges) {
+    const int even = (n + ranges - 1) / ranges;
+    const int step = even >= 512 ? 64 : even >= 128 ? 32 : 16;
+    return (even + step - 1) / step * step;
+}
+
+// Fills the plan (all threads of the block; ends with a barrier) and returns the length, 0 when not even one range per item fits max_ranges.
+// The length is the one of Q4_CAND with the least cost: rounds over the grid's warps x (length + cost_range) + cost_merge per partial result of
+// the longest item.
+__device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int n_warps, int block_warps,
+                                           int cost_range, int cost_merge) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < n_items; i += blockDim.x) {
+        const int seg = a.items[i], p = a.seg_ctx[seg];
+        pl.first[i] = first_key(a.window, a.chunk, p) & ~15;
+        pl.pos[i] = p;
+        pl.seg[i] = seg;
+    }
+    __syncthreads();
+    int longest = 1;
+    for (int i = 0; i < n_items; ++i) longest = max(longest, pl.pos[i] + 1 - pl.first[i]);
+    const int step = 16 * ((longest + 16 * Q4_CAND - 1) / (16 * Q4_CAND));
+    unsigned long long best = ~0ull;
+    for (int c = tid; c < Q4_CAND; c += blockDim.x) {
+        const int len = step * (c + 1);
+        if (len - step >= longest && c > 0) break;  // longer than any context: the same cut as the one before
+        const float inv = 1.f / static_cast<float>(len);
+        int ranges = 0;
+        for (int i = 0; i < n_items; ++i) {
+            const int first = pl.first[i];
+            ranges += q4_ranges(pl.pos[i] + 1 - first, len, inv) + (q4_kept(a, first) > 0);
+        }
+        if (ranges > max_ranges) continue;  // the scratch does not hold that many partial results
+        const unsigned rounds = (static_cast<unsigned>(ranges) * n_vh + n_warps - 1) / n_warps;
+        const unsigned long long cost = static_cast<unsigned long long>(rounds) * (len + cost_range) +
+                                        static_cast<unsigned long long>(cost_merge) * ((longest + len - 1) / len / block_warps);
+        best = min(best, (cost << 24) | static_cast<unsigned>(c));  // ties: the shorter range
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) pl.best[warp] = best;
+    __syncthreads();
+    if (warp == 0) {
+        unsigned long long b = lane < block_warps ? pl.best[lane] : ~0ull;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) b = min(b, __shfl_xor_sync(0xffffffffu, b, o));
+        const int len = b == ~0ull ? 0 : step * (static_cast<int>(b & 0xffffff) + 1);
+        const float inv = len ? 1.f / static_cast<float>(len) : 0.f;
+        int acc = 0;
+        for (int i0 = 0; i0 < n_items; i0 += 32) {
+            const int i = i0 + lane;
+            int mine = 0;
+            if (i < n_items && len) {
+                const int first = pl.first[i];
+                mine = q4_ranges(pl.pos[i] + 1 - first, len, inv) + (q4_kept(a, first) > 0);
+            }
+            int run = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += v;
+            }
+            if (i < n_items) pl.pref[i] = acc + run - mine;
+            acc += __shfl_sync(0xffffffffu, run, 31);
+        }
+        if (lane == 0) {
+            pl.pref[n_items] = acc;
+            pl.len = len;
+        }
+    }
+    __syncthreads();
+    return pl.len;
 }
 
 // T: the model's type.  HD: head size.  HT: tiles of eight heads per warp.  W warps of a block, S stages of SK keys in flight per warp.
 template <typename T, int HD, int HT, int W, int S, int SK, bool WEIGH>
 __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int n_items, long long max_units, int cost_range, int cost_merge) {
     pdl_trigger();  // every block of this grid is resident from the start
-    constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     constexpr int KW = HD / 32;      // words of a lane per key row (keys): HD / 4 dimensions
     constexpr int VW = HD / 64;      // words of a lane per value row: HD / 8 dimensions
     constexpr int MT = HD / 16;      // row tiles of O^T
+    constexpr int DL = HD / 32;      // dimensions of a lane where a warp has a head's row
     constexpr int RB = HD / 2;       // bytes of a row's codes
     constexpr uint32_t PLANE = SK * (RB + Q4_FACTOR_BYTES);   // K (or V) of a stage
     constexpr uint32_t STAGE = 2 * PLANE;
+    constexpr float RAISE = 4.f, TOP = 10.f;   // weights are 2^TOP at M, at most 2^(TOP + RAISE), times scale / 2^exponent < 2: below 65,504
+    constexpr int LEAST = -64;                 // smallest exponent of a scale that is taken out (smaller ones leave smaller weights)
     extern __shared__ __align__(16) unsigned char q4_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, t4 = lane & 3;   // row of the fragments, and the lane's place in its row
@@ -187,8 +308,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     const int P = a.page_tokens, G = a.nh / a.nkv;
     const int n_sub = (G + 8 * HT - 1) / (8 * HT), n_vh = a.nkv * n_sub;   // warps that serve a group, heads of a range
 
-    __shared__ KeyRanges kr;
+    __shared__ Q4Plan pl;
     __shared__ __align__(8) unsigned long long q4_bars[W * S];
+    __shared__ int is_last[W];
     const uint32_t bars = smem_u32(q4_bars) + warp * (S * 8);  // this warp's barriers, one per stage
     if (lane == 0) {
 #pragma unroll
@@ -198,359 +320,457 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     }
     __syncwarp();
     uint32_t parity = 0;  // bit i: the phase of stage i's barrier that the next wait on it looks for
-    const int n_warps = gridDim.x * W;
-    const int len = plan_key_ranges(kr, a.items, a.seg_ctx, a.seg_q0, a.window, a.chunk, n_items, n_vh, max_units / a.nh * n_vh, n_warps,
-                                    cost_range, cost_merge, a.keep_first);
+    bool ok = true;
+    const int len = plan_ranges(pl, a, n_items, n_vh, max_units / a.nh, gridDim.x * W, W, cost_range, cost_merge);
     // (the cut read only the step's descriptors; q and the newest rows come from the kernel in front)
     pdl_entry();
     if (len == 0) return;
-    const long long n_units = static_cast<long long>(kr.pref[n_items]) * n_vh;
+    const int n_units = pl.pref[n_items] * n_vh;
     const float qscale = a.scale * 1.4426950408889634f;  // scores in base 2
     const size_t plane_step = static_cast<size_t>(a.nkv) * P * (RB + Q4_FACTOR_BYTES);
     const uint32_t ring = smem_u32(q4_smem) + warp * (S * STAGE);
+    // a warp's result, in its ring's place once the ring is empty: [heads][HD] sums, then [heads] pairs (maximum, denominator)
+    constexpr int RES = 8 * HT * (HD + 2);
+    static_assert(RES * 4 <= S * static_cast<int>(STAGE), "a warp's result fits its ring");
+    float* const res0 = reinterpret_cast<float*>(q4_smem);
+    constexpr int RES_STEP = S * STAGE / 4;   // floats from a warp's result to the next one's
 
-    for (long long u = static_cast<long long>(blockIdx.x) * W + warp; u < n_units; u += n_warps) {
-        const int vh = static_cast<int>(u % n_vh);
+    for (int base = blockIdx.x * W; base < n_units; base += gridDim.x * W) {
+        const int u = base + warp;
+        const bool active = u < n_units;
+        // the unit: item, (virtual) head, range
+        int item = 0;
+        if (active) {
+            int hi = n_items;   // the last item whose units begin at or in front of u
+            while (hi - item > 1) {
+                const int mid = (item + hi) >> 1;
+                if (pl.pref[mid] * n_vh <= u) item = mid;
+                else hi = mid;
+            }
+        }
+        const int r0 = pl.pref[item], n_ranges = pl.pref[item + 1] - r0;
+        const int v = active ? u - r0 * n_vh : 0;
+        const int vh = v / n_ranges, range = v % n_ranges;
         const int kvh = vh / n_sub, g0 = (vh % n_sub) * 8 * HT;
         const int nG = min(G - g0, 8 * HT), h0 = kvh * G + g0;   // this warp's heads: h0 .. h0 + nG - 1
-        const int r = static_cast<int>(u / n_vh);
-        int item = 0;
-        while (kr.pref[item + 1] <= r) ++item;
-        const int seg = kr.seg[item], p = kr.pos[item], row = kr.row[item];
-        // an item's first range may be its kept first tokens (see attention_gqa.cu)
-        const int kept = kr.kept[item], keep = a.keep_first;
-        const bool kept_range = kept > 0 && r == kr.pref[item];
-        const int split = r - kr.pref[item] - (kept > 0);
-        const int t_lo = kept_range ? 0 : first_key(a.window, a.chunk, p);
-        const int k_begin = kept_range ? 0 : kr.first[item] + split * len;   // a multiple of 32
-        const int k_end = kept_range ? kept : min(p + 1, k_begin + len);      // exclusive
-        const int* table = a.block_table + static_cast<size_t>(seg) * a.table_stride;
+        const int seg = pl.seg[item], p = pl.pos[item], first = pl.first[item];
+        const int row = a.seg_q0[seg];
+        // the warps of this block that have ranges of the same (item, head): wa .. wb - 1
+        const int wa = max(0, warp - range), wb = min(min(W, n_units - base), warp - range + n_ranges);
+        const bool whole = wa == warp - range && wb - wa == n_ranges;
 
-        // Q as B fragments: head gq (and gq + 8 of the second tile), dimensions t4 HD / 4 + 8 w + 4 s + {0, 1} and + {2, 3}: words w, s = 0, 1
-        uint32_t qb[HT][2 * KW][2][PARTS];
-        float sq[HT][2];   // sum(q) of this lane's two heads per tile, times the scores' factor
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-            const int g = gq + 8 * ht;
-            const T* q0 = static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.nh + h0 + (g < nG ? g : 0)) * HD + t4 * (HD / 4);
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-#pragma unroll
-            for (int i = 0; i < 2 * KW; ++i) {
-                load_pair(q0 + 4 * i, qb[ht][i][0]);
-                load_pair(q0 + 4 * i + 2, qb[ht][i][1]);
-#pragma unroll
-                for (int x = PARTS - 1; x >= 0; --x) {
-                    if (g >= nG) qb[ht][i][0][x] = qb[ht][i][1][x] = 0u;
-                    mma_bf16(sum, ones, qb[ht][i][0][x], qb[ht][i][1][x]);
-                }
-            }
-            sq[ht][0] = sum[0] * qscale;
-            sq[ht][1] = sum[1] * qscale;
-        }
-        // O^T: byte b of word w of a lane's value row is row tile 4 w + b: its low nibble's dimension in row gq, its high nibble's in row
-        // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
-        float o[HT][MT][4], m[HT][2], l[HT][2], z[HT][2], slope[HT][2];
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-            for (int j = 0; j < MT; ++j) o[ht][j][0] = o[ht][j][1] = o[ht][j][2] = o[ht][j][3] = 0.f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int g = 8 * ht + 2 * t4 + c;
-                m[ht][c] = -INFINITY;
-                l[ht][c] = z[ht][c] = 0.f;
-                slope[ht][c] = a.slopes && g < nG ? slope_log2(a.slopes, h0 + g) : 0.f;
-            }
-        }
+        if (active) {
+            const int keep = a.keep_first, kept = q4_kept(a, first);
+            const bool kept_range = kept > 0 && range == 0;
+            const int t_lo = kept_range ? 0 : first_key(a.window, a.chunk, p);
+            const int n_even = n_ranges - (kept > 0);
+            const int length = q4_length(p + 1 - first, n_even);
+            const int k_begin = kept_range ? 0 : min(p + 1, first + (range - (kept > 0)) * length);   // a multiple of 16, or no key
+            const int k_end = kept_range ? kept : min(p + 1, k_begin + length);                         // exclusive
+            const int* table = a.block_table + static_cast<size_t>(seg) * a.table_stride;
 
-        // keys k0 .. end - 1 of one page into a stage of the ring
-        const int k_stop = (k_end + 15) & ~15;
-        auto stage_end = [&](int k0) { return min(min((k0 / P + 1) * P, k0 + SK), k_stop); };
-        auto issue = [&](int k0, int end, int st) {
-            if (lane == 0) {
-                const int n = end - k0, off = k0 % P;
-                const uint8_t* src = a.pool + q4_place(table[k0 / P], 0, kvh, a.nkv, P, HD);
-                const uint32_t dst = ring + st * STAGE, bar = bars + 8 * st;
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind this warp's reads of the stage
-                mbar_expect_tx(bar, 2 * n * (RB + Q4_FACTOR_BYTES));
-                if (n == SK && P == SK) {
-                    bulk_copy(dst, src, PLANE, bar);
-                    bulk_copy(dst + PLANE, src + plane_step, PLANE, bar);
-                } else {
-                    const uint8_t* codes = src + static_cast<size_t>(off) * RB;
-                    const uint8_t* factors = src + static_cast<size_t>(P) * RB + static_cast<size_t>(off) * Q4_FACTOR_BYTES;
-                    bulk_copy(dst, codes, n * RB, bar);
-                    bulk_copy(dst + SK * RB, factors, n * Q4_FACTOR_BYTES, bar);
-                    bulk_copy(dst + PLANE, codes + plane_step, n * RB, bar);
-                    bulk_copy(dst + PLANE + SK * RB, factors + plane_step, n * Q4_FACTOR_BYTES, bar);
+            // keys k0 .. end - 1 of one page into a stage of the ring.  (Every chunk holds a live key, so its page is the request's: the first
+            // of a window's ranges begins with the chunk of the window's first key, and kept tokens in front of that are a range of their own.)
+            const int k_stop = k_begin < k_end ? (k_end + 15) & ~15 : k_begin;
+            auto stage_end = [&](int k0) { return min(min((k0 / P + 1) * P, k0 + SK), k_stop); };
+            auto issue = [&](int k0, int end, int st) {
+                if (lane == 0) {
+                    const int n = end - k0, off = k0 % P;
+                    const uint8_t* src = a.pool + q4_place(table[k0 / P], 0, kvh, a.nkv, P, HD);
+                    const uint32_t dst = ring + st * STAGE, bar = bars + 8 * st;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the reads of what lies there
+                    mbar_expect_tx(bar, 2 * n * (RB + Q4_FACTOR_BYTES));
+                    if (n == SK && P == SK) {
+                        bulk_copy(dst, src, PLANE, bar);
+                        bulk_copy(dst + PLANE, src + plane_step, PLANE, bar);
+                    } else {
+                        const uint8_t* codes = src + static_cast<size_t>(off) * RB;
+                        const uint8_t* factors = src + static_cast<size_t>(P) * RB + static_cast<size_t>(off) * Q4_FACTOR_BYTES;
+                        bulk_copy(dst, codes, n * RB, bar);
+                        bulk_copy(dst + SK * RB, factors, n * Q4_FACTOR_BYTES, bar);
+                        bulk_copy(dst + PLANE, codes + plane_step, n * RB, bar);
+                        bulk_copy(dst + PLANE + SK * RB, factors + plane_step, n * Q4_FACTOR_BYTES, bar);
+                    }
+                }
+            };
+            int k0 = k_begin, k_next = k_begin;   // first key that is not read yet; that is not asked for yet
+            int st = 0;
+            if (ok) {
+#pragma unroll
+                for (int c = 0; c < S - 1; ++c)
+                    if (k_next < k_stop) {
+                        const int e = stage_end(k_next);
+                        issue(k_next, e, c);
+                        k_next = e;
+                    }
+            }
+
+            // Q as B fragments: head gq (and gq + 8 of the second tile), dimensions t4 HD / 4 + 8 w + 4 x + {0, 1} and + {2, 3}: words w, x = 0, 1
+            uint32_t qb[HT][2 * KW][2][PARTS];
+            float hq[HT][2], sq[HT][2];   // of this lane's two heads per tile: the scores' factor, and times sum(q)
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) {
+                const int g = gq + 8 * ht;
+                const T* q0 = static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.nh + h0 + (g < nG ? g : 0)) * HD + t4 * (HD / 4);
+                float x[8 * KW], top = 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; ++w) load8(q0 + 8 * w, x + 8 * w);
+#pragma unroll
+                for (int i = 0; i < 8 * KW; ++i) {
+                    if (g >= nG) x[i] = 0.f;
+                    top = fmaxf(top, fabsf(x[i]));
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int k = min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);   // (-114 for infinities)
+                const float up = pow2i(k);
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+                for (int i = 0; i < 2 * KW; ++i) {
+                    split2<PARTS>(x[4 * i] * up, x[4 * i + 1] * up, qb[ht][i][0]);
+                    split2<PARTS>(x[4 * i + 2] * up, x[4 * i + 3] * up, qb[ht][i][1]);
+#pragma unroll
+                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(sum, ones, qb[ht][i][0][y], qb[ht][i][1][y]);
+                }
+                const float down = qscale * pow2i(-k);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    hq[ht][c] = __shfl_sync(0xffffffffu, down, 4 * (2 * t4 + c));
+                    sq[ht][c] = sum[c] * hq[ht][c];
                 }
             }
-        };
-        // the first chunk that holds a live key (see attention_gqa.cu: every chunk from there on holds one, so its page is the request's)
-        int k0 = keep > k_begin ? k_begin : max(k_begin, t_lo & ~15);
-        int k_next = k0;   // first key that is not asked for yet
-        bool ok = true;
+            // O^T: byte b of word w of a lane's value row is row tile 4 w + b: its low nibble's dimension in row gq, its high nibble's in row
+            // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
+            float o[HT][MT][4], m[HT][2], l[HT][2], z[HT][2], slope[HT][2];
 #pragma unroll
-        for (int c = 0; c < S - 1; ++c)
-            if (k_next < k_stop) {
-                const int e = stage_end(k_next);
-                issue(k_next, e, c);
-                k_next = e;
-            }
-        int st = 0;
-        while (k0 < k_stop) {
-            __syncwarp();  // every lane has read the stage before this one: its place may be overwritten
-            if (k_next < k_stop) {
-                int st_new = st + S - 1;
-                if (st_new >= S) st_new -= S;
-                const int e = stage_end(k_next);
-                issue(k_next, e, st_new);
-                k_next = e;
-            }
-            const int end = stage_end(k0);
-            if (!mbar_wait(bars + 8 * st, (parity >> st) & 1u)) {
-                ok = false;
-                break;
-            }
-            parity ^= 1u << st;
-            const uint32_t src = ring + st * STAGE;
-            if (++st == S) st = 0;
-            for (int c0 = k0; c0 < end; c0 += 16) {
-                const uint32_t kbase = src + (c0 - k0) * RB, kfac = src + SK * RB + (c0 - k0) * Q4_FACTOR_BYTES;
-                // keys c0 + kr0 and c0 + 8 + kr0: words, factors of the key's and of the value's row
-                uint32_t k_lo[KW], k_hi[KW];
-                lds_words<KW>(k_lo, kbase + kr0 * RB + t4 * (RB / 4));
-                lds_words<KW>(k_hi, kbase + (kr0 + 8) * RB + t4 * (RB / 4));
-                uint32_t kf[2], vf[2];
-                kf[0] = lds4(kfac + 4 * kr0);
-                kf[1] = lds4(kfac + 4 * (kr0 + 8));
-                vf[0] = lds4(kfac + PLANE + 4 * kr0);
-                vf[1] = lds4(kfac + PLANE + 4 * (kr0 + 8));
-                uint32_t v_a[2][VW], v_b[2][VW];
+            for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    lds_words<VW>(v_a[x], kbase + PLANE + (8 * x + va_row) * RB + gq * (RB / 8));
-                    lds_words<VW>(v_b[x], kbase + PLANE + (8 * x + vb_row) * RB + gq * (RB / 8));
+                for (int j = 0; j < MT; ++j) o[ht][j][0] = o[ht][j][1] = o[ht][j][2] = o[ht][j][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int g = 8 * ht + 2 * t4 + c;
+                    m[ht][c] = -INFINITY;
+                    l[ht][c] = z[ht][c] = 0.f;
+                    slope[ht][c] = a.slopes && g < nG ? slope_log2(a.slopes, h0 + g) : 0.f;
                 }
-                float s[HT][2][4];
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) s[ht][x][0] = s[ht][x][1] = s[ht][x][2] = s[ht][x][3] = 0.f;
-#pragma unroll
-                for (int w = 0; w < KW; ++w)
+            }
+
+            while (ok && k0 < k_stop) {
+                __syncwarp();  // every lane has read the stage before this one: its place may be overwritten
+                if (k_next < k_stop) {
+                    int st_new = st + S - 1;
+                    if (st_new >= S) st_new -= S;
+                    const int e = stage_end(k_next);
+                    issue(k_next, e, st_new);
+                    k_next = e;
+                }
+                const int end = stage_end(k0);
+                ok = mbar_wait(bars + 8 * st, (parity >> st) & 1u);
+                if (!ok) break;
+                parity ^= 1u << st;
+                const uint32_t src = ring + st * STAGE;
+                if (++st == S) st = 0;
+                for (int c0 = k0; c0 < end; c0 += 16) {
+                    const uint32_t kbase = src + (c0 - k0) * RB, kfac = src + SK * RB + (c0 - k0) * Q4_FACTOR_BYTES;
+                    // keys c0 + kr0 and c0 + 8 + kr0: words, factors of the key's and of the value's row
+                    uint32_t k_lo[KW], k_hi[KW];
+                    lds_words<KW>(k_lo, kbase + kr0 * RB + t4 * (RB / 4));
+                    lds_words<KW>(k_hi, kbase + (kr0 + 8) * RB + t4 * (RB / 4));
+                    uint32_t kf[2], vf[2];
+                    kf[0] = lds4(kfac + 4 * kr0);
+                    kf[1] = lds4(kfac + 4 * (kr0 + 8));
+                    vf[0] = lds4(kfac + PLANE + 4 * kr0);
+                    vf[1] = lds4(kfac + PLANE + 4 * (kr0 + 8));
+                    uint32_t v_a[2][VW], v_b[2][VW];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const uint32_t af[4] = {codes2(k_lo[w] >> (8 * x)), codes2(k_hi[w] >> (8 * x)), codes2(k_lo[w] >> (8 * x + 4)),
-                                                codes2(k_hi[w] >> (8 * x + 4))};
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                            for (int y = PARTS - 1; y >= 0; --y) mma_bf16(s[ht][x], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
+                        lds_words<VW>(v_a[x], kbase + PLANE + (8 * x + va_row) * RB + gq * (RB / 8));
+                        lds_words<VW>(v_b[x], kbase + PLANE + (8 * x + vb_row) * RB + gq * (RB / 8));
                     }
-                const int key0 = c0 + kr0, key1 = c0 + 8 + kr0;
-                const bool edge = c0 < t_lo || c0 + 16 > k_end;
-                bool live0 = true, live1 = true;
-                if (edge) {
-                    live0 = (key0 >= t_lo || key0 < keep) && key0 < k_end;
-                    live1 = (key1 >= t_lo || key1 < keep) && key1 < k_end;
-                    if (!live0) kf[0] = vf[0] = 0u;
-                    if (!live1) kf[1] = vf[1] = 0u;
-                }
-                const float ks0 = q4_scale(kf[0]), ks1 = q4_scale(kf[1]), vs0 = q4_scale(vf[0]), vs1 = q4_scale(vf[1]);
-                const float kz0 = fmaf(-0.5f, ks0, q4_mid(kf[0])), kz1 = fmaf(-0.5f, ks1, q4_mid(kf[1]));
-                const float vz0 = fmaf(-0.5f, vs0, q4_mid(vf[0])), vz1 = fmaf(-0.5f, vs1, q4_mid(vf[1]));
-                float sc[HT][4];
-                bool raise = false;
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = i & 1;
-                        float v = fmaf(s[ht][0][i] + s[ht][1][i], (i < 2 ? ks0 : ks1) * qscale, (i < 2 ? kz0 : kz1) * sq[ht][c]);
-                        if (a.slopes) v = fmaf(slope[ht][c], static_cast<float>((i < 2 ? key0 : key1) - p), v);
-                        if (edge && !(i < 2 ? live0 : live1)) v = -INFINITY;
-                        sc[ht][i] = v;
-                        raise |= v > m[ht][c] + 8.f;
-                    }
-                    if (WEIGH) {
-                        float* at = a.scores + (static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P * G + g0 + 8 * ht + 2 * t4;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (8 * ht + 2 * t4 + (i & 1) < nG && (i < 2 ? live0 : live1))
-                                at[static_cast<size_t>(i < 2 ? key0 : key1) * G + (i & 1)] = sc[ht][i];
-                    }
-                }
-                if (__any_sync(0xffffffffu, raise)) {
+                    float s[HT][2][4];
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float n = fmaxf(sc[ht][c], sc[ht][2 + c]);
-                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
-                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
-                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
-                            n = fmaxf(n, m[ht][c]);
-                            const float corr = m[ht][c] == -INFINITY ? 0.f : ex2(m[ht][c] - n);
-                            m[ht][c] = n;
-                            l[ht][c] *= corr;
-                            z[ht][c] *= corr;
+                        for (int x = 0; x < 2; ++x) s[ht][x][0] = s[ht][x][1] = s[ht][x][2] = s[ht][x][3] = 0.f;
 #pragma unroll
-                            for (int j = 0; j < MT; ++j) {
-                                o[ht][j][c] *= corr;
-                                o[ht][j][2 + c] *= corr;
-                            }
+                    for (int w = 0; w < KW; ++w)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
+                            const uint32_t af[4] = {codes_low(a0), codes_low(a1), codes_high(a0), codes_high(a1)};
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                                for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[ht][x], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
                         }
-                }
-                uint32_t pb[HT][2][PARTS];
+                    const int key[2] = {c0 + kr0, c0 + 8 + kr0};
+                    const bool edge = c0 < t_lo || c0 + 16 > k_end;
+                    bool live[2] = {true, true};
+                    if (edge) {
 #pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
-                    float e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float mu = m[ht][i & 1];
-                        e[i] = ex2(sc[ht][i] - (mu == -INFINITY ? 0.f : mu));   // (no live key yet: all weights 0)
+                        for (int i = 0; i < 2; ++i) {
+                            live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < k_end;
+                            if (!live[i]) kf[i] = vf[i] = 0u;
+                        }
                     }
+                    // of the two keys: scale of K, z of K; of V the scale's exponent, what is left of it, z, both over 2^exponent
+                    float ks[2], kz[2], ve[2], vs[2], vz[2], vi[2];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        l[ht][c] += e[c] + e[2 + c];
-                        z[ht][c] = fmaf(e[c], vz0, fmaf(e[2 + c], vz1, z[ht][c]));
+                    for (int i = 0; i < 2; ++i) {
+                        ks[i] = q4_scale(kf[i]);
+                        kz[i] = fmaf(-0.5f, ks[i], q4_mid(kf[i]));
+                        const float scale = q4_scale(vf[i]);
+                        const int e = min(max(static_cast<int>((vf[i] >> 7) & 0xffu) - 127, LEAST), 126);
+                        ve[i] = static_cast<float>(e);
+                        vi[i] = pow2i(-e);
+                        vs[i] = scale * vi[i];
+                        vz[i] = fmaf(-0.5f, scale, q4_mid(vf[i])) * vi[i];
                     }
-                    // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
-                    split2<PARTS>(e[0] * vs0, e[1] * vs0, pb[ht][0]);
-                    split2<PARTS>(e[2] * vs1, e[3] * vs1, pb[ht][1]);
+                    float sc[HT][4];   // score + exponent
+                    bool raise = false;
 #pragma unroll
-                    for (int y = 0; y < PARTS; ++y) {
-                        pb[ht][0][y] = movmatrix_trans(pb[ht][0][y]);
-                        pb[ht][1][y] = movmatrix_trans(pb[ht][1][y]);
+                    for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = i & 1, y = i >> 1;
+                            float w = fmaf(s[ht][0][i] + s[ht][1][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
+                            if (a.slopes) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
+                            if (WEIGH) {
+                                const int g = 8 * ht + 2 * t4 + c;
+                                if (g < nG && live[y])
+                                    a.scores[((static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P + key[y]) * G + g0 + g] = w;
+                                w += ve[y];
+                            }
+                            if (edge && !live[y]) w = -INFINITY;
+                            sc[ht][i] = w;
+                            raise |= w > m[ht][c] + RAISE;
+                        }
                     }
-                }
-#pragma unroll
-                for (int w = 0; w < VW; ++w)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
-                        const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
-                        const uint32_t af[4] = {codes2(x0), codes2(x0 >> 4), codes2(x1), codes2(x1 >> 4)};
+                    if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                         for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                            for (int y = PARTS - 1; y >= 0; --y) mma_bf16(o[ht][4 * w + b], af, pb[ht][0][y], pb[ht][1][y]);
+                            for (int c = 0; c < 2; ++c) {
+                                float n = fmaxf(sc[ht][c], sc[ht][2 + c]);
+                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
+                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
+                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
+                                n = fmaxf(n, m[ht][c]);
+                                const float corr = m[ht][c] == -INFINITY ? 0.f : ex2(m[ht][c] - n);
+                                m[ht][c] = n;
+                                l[ht][c] *= corr;
+                                z[ht][c] *= corr;
+#pragma unroll
+                                for (int j = 0; j < MT; ++j) {
+                                    o[ht][j][c] *= corr;
+                                    o[ht][j][2 + c] *= corr;
+                                }
+                            }
                     }
-            }
-            k0 = end;
-        }
-        if (!ok) {
-            // a copy never came: the error word is set.  Those still in flight are waited for, with the same limit, and the warp leaves
-            while (k0 < k_next) {
-                const int end = stage_end(k0);
-                if (++st == S) st = 0;
-                if (end < k_next) mbar_wait(bars + 8 * st, (parity >> st) & 1u);
+                    uint32_t pb[HT][2][PARTS];
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) {
+                        float e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float mu = m[ht][i & 1];
+                            e[i] = ex2(sc[ht][i] - (mu == -INFINITY ? 0.f : mu - TOP));   // (no live key yet: all weights 0)
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            l[ht][c] = fmaf(e[c], vi[0], fmaf(e[2 + c], vi[1], l[ht][c]));
+                            z[ht][c] = fmaf(e[c], vz[0], fmaf(e[2 + c], vz[1], z[ht][c]));
+                        }
+                        // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
+                        split2<PARTS>(e[0] * vs[0], e[1] * vs[0], pb[ht][0]);
+                        split2<PARTS>(e[2] * vs[1], e[3] * vs[1], pb[ht][1]);
+#pragma unroll
+                        for (int y = 0; y < PARTS; ++y) {
+                            pb[ht][0][y] = movmatrix_trans(pb[ht][0][y]);
+                            pb[ht][1][y] = movmatrix_trans(pb[ht][1][y]);
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < VW; ++w)
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
+                            const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
+                            const uint32_t af[4] = {codes_low(x0), codes_high(x0), codes_low(x1), codes_high(x1)};
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht) {
+                                float* t = o[ht][4 * w + b];
+                                if constexpr (PARTS == 1) {
+                                    mma_f16(t, af, pb[ht][0][0], pb[ht][1][0]);
+                                } else {
+                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(d, af, pb[ht][0][y], pb[ht][1][y]);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) t[i] += d[i];
+                                }
+                            }
+                        }
+                }
                 k0 = end;
             }
-            return;
-        }
-        // partial results: head h of range r is place r * nh + h.  A head's denominator lives in the eight lanes of its column.
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float lc = l[ht][c], zc = z[ht][c];
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) {
-                    lc += __shfl_xor_sync(0xffffffffu, lc, x);
-                    zc += __shfl_xor_sync(0xffffffffu, zc, x);
+            if (!ok) {
+                // a copy never came: the error word is set.  Those behind it are waited for, with the same limit
+                while (k0 < k_next) {
+                    const int end = stage_end(k0);
+                    if (++st == S) st = 0;
+                    if (end < k_next) mbar_wait(bars + 8 * st, (parity >> st) & 1u);
+                    k0 = end;
                 }
-                const int g = 8 * ht + 2 * t4 + c;
-                if (g < nG) {
-                    const size_t place = static_cast<size_t>(r) * a.nh + h0 + g;
-                    float* po = a.part_o + place * HD + gq * (HD / 8);
+            }
+            __syncwarp();
+            // this warp's result, into its ring.  A head's denominator lives in the eight lanes of its column.
+            float* res = res0 + warp * RES_STEP;
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        const float (*t)[4] = &o[ht][4 * w];
-                        *reinterpret_cast<float4*>(po + 8 * w) = make_float4(t[0][c] + zc, t[2][c] + zc, t[0][2 + c] + zc, t[2][2 + c] + zc);
-                        *reinterpret_cast<float4*>(po + 8 * w + 4) = make_float4(t[1][c] + zc, t[3][c] + zc, t[1][2 + c] + zc, t[3][2 + c] + zc);
+            for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float lc = l[ht][c], zc = z[ht][c];
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) {
+                        lc += __shfl_xor_sync(0xffffffffu, lc, x);
+                        zc += __shfl_xor_sync(0xffffffffu, zc, x);
                     }
-                    if (gq == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * place) = make_float2(m[ht][c], lc);
+                    const int g = 8 * ht + 2 * t4 + c;
+                    if (g < nG) {
+                        float* po = res + g * HD + gq * (HD / 8);
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) {
+                            const float (*t)[4] = &o[ht][4 * w];
+                            *reinterpret_cast<float4*>(po + 8 * w) = make_float4(t[0][c] + zc, t[2][c] + zc, t[0][2 + c] + zc, t[2][2 + c] + zc);
+                            *reinterpret_cast<float4*>(po + 8 * w + 4) = make_float4(t[1][c] + zc, t[3][c] + zc, t[1][2 + c] + zc, t[3][2 + c] + zc);
+                        }
+                        if (gq == 0) *reinterpret_cast<float2*>(res + 8 * HT * HD + 2 * g) = make_float2(m[ht][c], lc);
+                    }
                 }
             }
         }
-        // the warp that finishes the last range of these heads merges their ranges, in ascending order
-        __syncwarp();
-        int last = 0;
-        const int n_splits = kr.pref[item + 1] - kr.pref[item];
-        if (lane == 0) {
-            __threadfence();
-            int* counter = a.counters + static_cast<size_t>(item) * a.nh + vh;
-            last = atomicAdd(counter, 1) == n_splits - 1;
-            if (last) *counter = 0;
-        }
-        last = __shfl_sync(0xffffffffu, last, 0);
-        if (!last) continue;
-        __threadfence();
-        constexpr int GM = 4;          // heads at a time: a lane forms the weights of one range for all of them
-        constexpr int DL = HD / 32;    // dimensions of a lane
-        for (int g1 = 0; g1 < nG; g1 += GM) {
-            const int n_g = min(GM, nG - g1);
-            const size_t u0 = static_cast<size_t>(kr.pref[item]) * a.nh + h0 + g1;   // range s of head g1 + g: u0 + g + s nh
-            float M[GM], L[GM], acc[GM][DL];
+        __syncthreads();
+        // joins: weight of a part whose maximum is pm and denominator pl_, relative to M  (a part without a live key: 0, NaN stays)
+        auto part_weight = [](float2 ml, float M) { return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M); };
+        auto finish = [&](int g, const float* acc, float L, float M, int h_first, int at_row, int at_item) {
+            const int h = h_first + g;
+            // (the sink: one more term of score 0; scores are in base 2, and a weight is 2^TOP at M)
+            const float full = a.sink ? fmaf(sink_term2(a.sink_val, h, M), 1024.f, L) : L;
+            const float inv = 1.0f / full;
+            T* dst = static_cast<T*>(a.out) + (static_cast<size_t>(at_row) * a.nh + h) * HD + lane * DL;
 #pragma unroll
-            for (int g = 0; g < GM; ++g) {
-                M[g] = -INFINITY;
-                L[g] = 0.f;
-#pragma unroll
-                for (int d = 0; d < DL; ++d) acc[g][d] = 0.f;
+            for (int d = 0; d < DL; d += 2) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(dst + d) = make_float2(acc[d] * inv, acc[d + 1] * inv);
+                else *reinterpret_cast<__nv_bfloat162*>(dst + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
             }
-            for (int x = lane; x < n_splits; x += 32)
+            if (WEIGH && lane == 0) *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(at_item) * a.nh + h)) = make_float2(M - TOP, inv);
+        };
+        if (active) {
+            // the heads of a run of warps, dealt to its warps
+            for (int g = warp - wa; g < nG; g += wb - wa) {
+                const float* ml = res0 + 8 * HT * HD + 2 * g;
+                const int n = wb - wa;
+                const float2 mine = lane < n ? *reinterpret_cast<const float2*>(ml + (wa + lane) * RES_STEP) : make_float2(-INFINITY, 0.f);
+                const float M = warp_max(mine.x);
+                const float w = part_weight(mine, M);
+                const float L = warp_sum(w == 0.f ? 0.f : mine.y * w);
+                float acc[DL];
 #pragma unroll
-                for (int g = 0; g < GM; ++g)
-                    if (g < n_g) M[g] = fmaxf(M[g], __ldcg(a.part_ml + 2 * (u0 + g + static_cast<size_t>(x) * a.nh)));
-#pragma unroll
-            for (int g = 0; g < GM; ++g) M[g] = warp_max(M[g]);
-            for (int s0 = 0; s0 < n_splits; s0 += 32) {
-                float w[GM], lw[GM];   // of range s0 + lane
-#pragma unroll
-                for (int g = 0; g < GM; ++g) {
-                    w[g] = lw[g] = 0.f;
-                    if (g < n_g && s0 + lane < n_splits) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + 2 * (u0 + g + static_cast<size_t>(s0 + lane) * a.nh)));
-                        w[g] = ml.x == -INFINITY && !(ml.y != ml.y) ? 0.f : exp2f(ml.x - M[g]);
-                        lw[g] = ml.y;
-                    }
-                }
-                const int n = min(32, n_splits - s0);
-                const float* po = a.part_o + (u0 + static_cast<size_t>(s0) * a.nh) * HD + lane * DL;
+                for (int d = 0; d < DL; ++d) acc[d] = 0.f;
                 for (int j = 0; j < n; ++j) {
+                    const float wj = __shfl_sync(0xffffffffu, w, j);
+                    const float* src = res0 + (wa + j) * RES_STEP + g * HD + lane * DL;
 #pragma unroll
-                    for (int g = 0; g < GM; ++g) {
-                        if (g >= n_g) break;
-                        const float wj = __shfl_sync(0xffffffffu, w[g], j);
-                        L[g] = fmaf(__shfl_sync(0xffffffffu, lw[g], j), wj, L[g]);
-                        const float* src = po + (static_cast<size_t>(j) * a.nh + g) * HD;
+                    for (int d = 0; d < DL; d += 2) {
+                        const float2 x = *reinterpret_cast<const float2*>(src + d);
+                        acc[d] = fmaf(x.x, wj, acc[d]);
+                        acc[d + 1] = fmaf(x.y, wj, acc[d + 1]);
+                    }
+                }
+                if (whole) {
+                    finish(g, acc, L, M, h0, row, item);
+                } else {
+                    const size_t place = static_cast<size_t>(r0 + range - (warp - wa)) * a.nh + h0 + g;   // of the run's first range
+                    float* dst = a.part_o + place * HD + lane * DL;
 #pragma unroll
-                        for (int d = 0; d < DL; d += 2) {
-                            const float2 v = __ldcg(reinterpret_cast<const float2*>(src + d));
-                            acc[g][d] = fmaf(v.x, wj, acc[g][d]);
-                            acc[g][d + 1] = fmaf(v.y, wj, acc[g][d + 1]);
+                    for (int d = 0; d < DL; d += 2) *reinterpret_cast<float2*>(dst + d) = make_float2(acc[d], acc[d + 1]);
+                    if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * place) = make_float2(M, L);
+                    __threadfence();
+                }
+            }
+        }
+        if (!__syncthreads_or(active && !whole)) continue;   // (the rings are free again behind this)
+        // runs of warps that cover a (request, head) in part: the last block to bring one joins them all
+        const int u0 = r0 * n_vh + vh * n_ranges;            // the first unit of this (request, head)
+        const int n_parts = (u0 + n_ranges - 1) / W - u0 / W + 1;
+        if (lane == 0) {
+            int last = 0;
+            if (active && warp == wa && !whole) {
+                __threadfence();
+                int* counter = a.counters + static_cast<size_t>(item) * a.nh + vh;
+                last = atomicAdd(counter, 1) == n_parts - 1;
+                if (last) *counter = 0;
+                __threadfence();
+            }
+            is_last[warp] = last;
+        }
+        __syncthreads();
+        for (int lead = 0; lead < W; ++lead) {
+            if (!is_last[lead]) continue;
+            // (all warps of the block take part: the lead's unit again)
+            const int lu = base + lead;
+            int li = 0, hi = n_items;
+            while (hi - li > 1) {
+                const int mid = (li + hi) >> 1;
+                if (pl.pref[mid] * n_vh <= lu) li = mid;
+                else hi = mid;
+            }
+            const int lr0 = pl.pref[li], lnr = pl.pref[li + 1] - lr0, lvh = (lu - lr0 * n_vh) / lnr;
+            const int lg0 = (lvh % n_sub) * 8 * HT, lnG = min(G - lg0, 8 * HT), lh0 = (lvh / n_sub) * G + lg0;
+            const int lu0 = lr0 * n_vh + lvh * lnr, parts = (lu0 + lnr - 1) / W - lu0 / W + 1;
+            // range that part k begins with: 0, then where the blocks' runs begin
+            auto place = [&](int k, int g) {
+                const int first_range = k == 0 ? 0 : W * (lu0 / W + k) - lu0;
+                return static_cast<size_t>(lr0 + first_range) * a.nh + lh0 + g;
+            };
+            for (int g = warp; g < lnG; g += W) {
+                float M = -INFINITY;
+                for (int k = lane; k < parts; k += 32) M = fmaxf(M, __ldcg(a.part_ml + 2 * place(k, g)));
+                M = warp_max(M);
+                float L = 0.f, acc[DL];
+#pragma unroll
+                for (int d = 0; d < DL; ++d) acc[d] = 0.f;
+                for (int k0 = 0; k0 < parts; k0 += 32) {
+                    float2 mine = make_float2(-INFINITY, 0.f);
+                    if (k0 + lane < parts) mine = __ldcg(reinterpret_cast<const float2*>(a.part_ml + 2 * place(k0 + lane, g)));
+                    const float w = part_weight(mine, M);
+                    L += warp_sum(w == 0.f ? 0.f : mine.y * w);
+                    const int n = min(32, parts - k0);
+                    for (int j = 0; j < n; j += 8) {   // the rows of eight parts are on their way together
+                        float2 x[8][DL / 2];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y)
+#pragma unroll
+                            for (int d = 0; d < DL; d += 2)
+                                x[y][d / 2] = j + y < n ? __ldcg(reinterpret_cast<const float2*>(a.part_o + place(k0 + j + y, g) * HD + lane * DL + d))
+                                                        : make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            const float wj = __shfl_sync(0xffffffffu, w, j + y);
+#pragma unroll
+                            for (int d = 0; d < DL; d += 2) {
+                                acc[d] = fmaf(x[y][d / 2].x, wj, acc[d]);
+                                acc[d + 1] = fmaf(x[y][d / 2].y, wj, acc[d + 1]);
+                            }
                         }
                     }
                 }
-            }
-#pragma unroll
-            for (int g = 0; g < GM; ++g) {
-                if (g >= n_g) break;
-                // (the sink: one more term of score 0; scores are in base 2 here)
-                const int h = h0 + g1 + g;
-                const float full = a.sink ? L[g] + sink_term2(a.sink_val, h, M[g]) : L[g];
-                const float inv = 1.0f / full;
-                T* dst = static_cast<T*>(a.out) + (static_cast<size_t>(row) * a.nh + h) * HD + lane * DL;
-#pragma unroll
-                for (int d = 0; d < DL; ++d) dst[d] = from_f<T>(acc[g][d] * inv);
-                if (WEIGH && lane == 0)
-                    *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(item) * a.nh + h)) = make_float2(M[g], inv);
+                finish(g, acc, L, M, lh0, a.seg_q0[pl.seg[li]], li);
             }
         }
+        __syncthreads();   // (is_last is written again in the next round)
     }
 }
 
@@ -598,7 +818,7 @@ extern "C" int locus_attn_decode_q4(const void* q, int dt, const void* pool, voi
                                     cudaStream_t stream) {
     if (n_items <= 0) return 0;
     if ((dt != LOCUS_DT_F32 && dt != LOCUS_DT_BF16) || nkv <= 0 || nh <= 0 || nh % nkv != 0 || !q4_head_ok(hd) || page_tokens <= 0 ||
-        page_tokens % 16 != 0 || n_items > DS_MAX_ITEMS || !mask_ok(window, chunk, keep_first) || counters == nullptr || table_stride <= 0 ||
+        page_tokens % 16 != 0 || n_items > Q4_MAX_ITEMS || !mask_ok(window, chunk, keep_first) || counters == nullptr || table_stride <= 0 ||
         nkv > 65535 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(part_o)) & 15) != 0)
         return LOCUS_ERR_UNSUPPORTED;
     if (window == 0) keep_first = 0;
@@ -623,7 +843,7 @@ extern "C" int locus_attn_decode_q4(const void* q, int dt, const void* pool, voi
     } else if (hd == 64) {
         code = wide ? Q4_GO(bf16, 64, 2, 12, 3, 64) : Q4_GO(bf16, 64, 1, 12, 3, 64);
     } else if (hd == 128) {
-        code = wide ? Q4_GO(bf16, 128, 2, 11, 2, 64) : Q4_GO(bf16, 128, 1, 11, 2, 64);
+        code = wide ? Q4_GO(bf16, 128, 2, 8, 2, 64) : Q4_GO(bf16, 128, 1, 12, 2, 64);
     } else {
         code = Q4_GO(bf16, 256, 1, 8, 2, 32);
     }
