@@ -2,27 +2,29 @@
 //
 //   o_h = sum_t p_t v_t   p = softmax over the keys in sight of scale * q_h . k_t (a sink, a distance bias: as in attention.cu)
 //
-// with k_t and v_t read straight from their codes.  A key's row is mid + scale (code - 7.5) = z + scale (code - 7), z = mid - scale / 2, and codes
-// less 7 are small whole numbers that float16 holds exactly, so
+// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5), so
 //
-//   q . k_t = scale_t (q . (code_t - 7)) + z_t sum(q)                      the product on the tensor cores, the rest per score in float32
-//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t z_t             the same for the values
+//   q . k_t = scale_t (q . code_t) + (mid_t - 7.5 scale_t) sum(q)
+//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t (mid_t - scale_t / 2)
 //
-// The tensor cores' operands are float16:
-//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
-//     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more;
+// with the two products on the tensor cores and the rest in float32.  The tensor cores' operands are float16:
+//   * codes as they are: a nibble n in the low bits of a 16-bit half is the float16 n 2^-24 (a subnormal number, which the tensor cores take like any
+//     other), and n in the next four bits 16 n 2^-24, so that one AND unpacks two codes; the powers of two go into the other operand or out
+//     of the sums.  (Whole numbers by the usual or with 1024 and a subtraction behind it: twice the instructions.)
+//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15: a bfloat16 element loses bits only if it is 2^-25 of the
+//     largest, and then at most 2^-36 of that; a float32 q goes in as two parts, 22 bits and more;
 //   * the weights p_t scale_t, formed relative to the running maximum M of score + exponent of scale, so that they stay below 2^15, whatever the
 //     scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest where that is more; two parts for a float32 model).  The
-//     unrounded p_t enter the denominator and z's sum.  (bfloat16, the model's type, would round to 2^-9, and the unpacking below would cost
-//     more: its mantissa holds one nibble at a time.)
-// The 7 is taken off the codes rather than out of the sums: sums of codes of one sign would lose what cancels in them.
+//     unrounded p_t enter the denominator and the second sum.
+// The values' 7 is taken off inside the sums, by a product of the same weights with a constant: sums of codes of one sign would grow over the keys
+// and lose what cancels in them.  (In a score, a sum over one head's dimensions, the codes' mean costs one bit.)
 // For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
 // over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
 // A warp takes a range of keys of one (request, key/value head) for up to 16 query heads that share it, in the transposed form (16 keys in the M
 // dimension of mma.sync m16n8k16, eight heads in N):
-//   S^T [16 keys x 8 heads] = (C_k - 7) [16 x hd] . Q^T     a lane's words of a key row hold eight codes each: a mask-and-or and a subtraction (or a
-//                             multiply-add that also takes the nibble's place out) give two neighbouring dimensions as the A fragment wants them;
+//   S^T [16 keys x 8 heads] = C_k [16 x hd] . Q^T           a lane's words of a key row hold eight codes each, two neighbouring dimensions in a
+//                             register's halves as the A fragment wants them;
 //   O^T [hd x 8 heads] += (C_v - 7)^T [hd x 16 keys] . P^T  the A fragment wants one dimension of two keys in a register: a byte permute joins
 //                             the same byte of two keys' words, and its two nibbles are two dimensions (two row tiles' halves).
 // A group of more heads is served by several warps (that each read its rows, from the L2 after the first).
@@ -118,28 +120,25 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-// N (1, 2, 4 or 8) words from shared memory
+// N (1, 2, 4 or 8) words of shared memory
 template <int N>
-__device__ __forceinline__ void lds_words(uint32_t* v, uint32_t addr) {
-    if constexpr (N == 1) v[0] = lds4(addr);
-    else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory");
-    else {
+__device__ __forceinline__ void lds_words(uint32_t* v, const unsigned char* p) {
+    if constexpr (N == 1) {
+        v[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (N == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        v[0] = x.x; v[1] = x.y;
+    } else {
 #pragma unroll
-        for (int i = 0; i < N; i += 4)
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
-                         : "r"(addr + 4 * i)
-                         : "memory");
+        for (int i = 0; i < N; i += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * i);
+            v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+        }
     }
 }
 
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -147,7 +146,7 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
 // transpose of an 8 x 8 matrix of 16-bit elements held as mma fragments (two elements of a row per lane)
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -156,15 +155,6 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-// the codes in bits 0 .. 3 of a register's halves, less 7, as float16: 0x6400 | n is 1024 + n
-__device__ __forceinline__ uint32_t codes_low(uint32_t x) {
-    return bits(__hsub2(halves((x & 0x000f000fu) | 0x64006400u), halves(0x64076407u)));
-}
-// the codes in bits 4 .. 7: (1024 + 16 n) / 16 - 71
-__device__ __forceinline__ uint32_t codes_high(uint32_t x) {
-    return bits(__hfma2(halves((x & 0x00f000f0u) | 0x64006400u), halves(0x2c002c00u), halves(0xd470d470u)));
-}
 // a pair of values as PARTS pairs of float16: one, rounded, or two
 template <int PARTS>
 __device__ __forceinline__ void split2(float a, float b, uint32_t* out) {
@@ -200,8 +190,10 @@ struct Q4Plan {
     int first[Q4_MAX_ITEMS];     // first key of item i, rounded down to 16
     int pos[Q4_MAX_ITEMS];       // position of its query
     int seg[Q4_MAX_ITEMS];
+    int row[Q4_MAX_ITEMS];       // row of q / out
     int pref[Q4_MAX_ITEMS + 1];  // ranges of the items before i
     unsigned long long best[32];
+    int longest[32], total[32];
     int len;
 };
 
@@ -218,33 +210,48 @@ __device__ __forceinline__ int q4_length(int n, int ranges) {
 
 // Fills the plan (all threads of the block; ends with a barrier) and returns the length, 0 when not even one range per item fits max_ranges.
 // The length is the one of Q4_CAND with the least cost: rounds over the grid's warps x (length + cost_range) + cost_merge per partial result of
-// the longest item.
+// the longest item.  Candidates lie 1.45 % apart from a quarter of what fills every warp once to ten times that; the last one is the longest item's.
 __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int n_warps, int block_warps,
                                            int cost_range, int cost_merge) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int longest = 1, total = 0;
     for (int i = tid; i < n_items; i += blockDim.x) {
         const int seg = a.items[i], p = a.seg_ctx[seg];
-        pl.first[i] = first_key(a.window, a.chunk, p) & ~15;
+        const int first = first_key(a.window, a.chunk, p) & ~15;
+        pl.row[i] = a.seg_q0[seg];
+        pl.first[i] = first;
         pl.pos[i] = p;
         pl.seg[i] = seg;
+        longest = max(longest, p + 1 - first);
+        total += p + 1 - first;
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (lane == 0) {
+        pl.longest[warp] = longest;
+        pl.total[warp] = total;
     }
     __syncthreads();
-    int longest = 1;
-    for (int i = 0; i < n_items; ++i) longest = max(longest, pl.pos[i] + 1 - pl.first[i]);
-    const int step = 16 * ((longest + 16 * Q4_CAND - 1) / (16 * Q4_CAND));
+    longest = __reduce_max_sync(0xffffffffu, lane < block_warps ? pl.longest[lane] : 1);
+    total = __reduce_add_sync(0xffffffffu, lane < block_warps ? pl.total[lane] : 0);
+    const float fill = static_cast<float>(total) * static_cast<float>(n_vh) / static_cast<float>(n_warps);
+    auto length = [&](int c) {
+        if (c == Q4_CAND - 1) return (longest + 15) & ~15;
+        return 16 * max(1, static_cast<int>(fminf(fill * exp2f(static_cast<float>(c - 96) * (1.f / 48.f)), 1e8f) * (1.f / 16.f) + 0.5f));
+    };
     unsigned long long best = ~0ull;
     for (int c = tid; c < Q4_CAND; c += blockDim.x) {
-        const int len = step * (c + 1);
-        if (len - step >= longest && c > 0) break;  // longer than any context: the same cut as the one before
+        const int len = length(c);
         const float inv = 1.f / static_cast<float>(len);
         int ranges = 0;
-        for (int i = 0; i < n_items; ++i) {
-            const int first = pl.first[i];
-            ranges += q4_ranges(pl.pos[i] + 1 - first, len, inv) + (q4_kept(a, first) > 0);
-        }
+#pragma unroll 4
+        for (int i = 0; i < n_items; ++i) ranges += q4_ranges(pl.pos[i] + 1 - pl.first[i], len, inv);
+        if (a.window > 0 && a.keep_first > 0)
+            for (int i = 0; i < n_items; ++i) ranges += q4_kept(a, pl.first[i]) > 0;
         if (ranges > max_ranges) continue;  // the scratch does not hold that many partial results
         const unsigned rounds = (static_cast<unsigned>(ranges) * n_vh + n_warps - 1) / n_warps;
-        const unsigned long long cost = static_cast<unsigned long long>(rounds) * (len + cost_range) +
+        const int most = min(len, longest);
+        const unsigned long long cost = static_cast<unsigned long long>(rounds) * (most + cost_range) +
                                         static_cast<unsigned long long>(cost_merge) * ((longest + len - 1) / len / block_warps);
         best = min(best, (cost << 24) | static_cast<unsigned>(c));  // ties: the shorter range
     }
@@ -256,7 +263,7 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
         unsigned long long b = lane < block_warps ? pl.best[lane] : ~0ull;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) b = min(b, __shfl_xor_sync(0xffffffffu, b, o));
-        const int len = b == ~0ull ? 0 : step * (static_cast<int>(b & 0xffffff) + 1);
+        const int len = b == ~0ull ? 0 : length(static_cast<int>(b & 0xffffff));
         const float inv = len ? 1.f / static_cast<float>(len) : 0.f;
         int acc = 0;
         for (int i0 = 0; i0 < n_items; i0 += 32) {
@@ -354,7 +361,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
         const int kvh = vh / n_sub, g0 = (vh % n_sub) * 8 * HT;
         const int nG = min(G - g0, 8 * HT), h0 = kvh * G + g0;   // this warp's heads: h0 .. h0 + nG - 1
         const int seg = pl.seg[item], p = pl.pos[item], first = pl.first[item];
-        const int row = a.seg_q0[seg];
+        const int row = pl.row[item];
         // the warps of this block that have ranges of the same (item, head): wa .. wb - 1
         const int wa = max(0, warp - range), wb = min(min(W, n_units - base), warp - range + n_ranges);
         const bool whole = wa == warp - range && wb - wa == n_ranges;
@@ -372,11 +379,16 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // keys k0 .. end - 1 of one page into a stage of the ring.  (Every chunk holds a live key, so its page is the request's: the first
             // of a window's ranges begins with the chunk of the window's first key, and kept tokens in front of that are a range of their own.)
             const int k_stop = k_begin < k_end ? (k_end + 15) & ~15 : k_begin;
-            auto stage_end = [&](int k0) { return min(min((k0 / P + 1) * P, k0 + SK), k_stop); };
-            auto issue = [&](int k0, int end, int st) {
+            const uint8_t* const pool_head = a.pool + q4_place(0, 0, kvh, a.nkv, P, HD);
+            int k0 = k_begin, k_next = k_begin;   // first key that is not read yet; that is not asked for yet
+            int page_at = k_begin / P;            // page of k_next, and where it and the page of k0 end
+            int end_next = (page_at + 1) * P, end_read = end_next;
+            // the next stage: keys k_next .. of one page
+            auto issue = [&](int st) {
+                const int end = min(min(end_next, k_next + SK), k_stop);
                 if (lane == 0) {
-                    const int n = end - k0, off = k0 % P;
-                    const uint8_t* src = a.pool + q4_place(table[k0 / P], 0, kvh, a.nkv, P, HD);
+                    const int n = end - k_next, off = k_next - (end_next - P);
+                    const uint8_t* src = pool_head + table[page_at] * (2 * plane_step);
                     const uint32_t dst = ring + st * STAGE, bar = bars + 8 * st;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the reads of what lies there
                     mbar_expect_tx(bar, 2 * n * (RB + Q4_FACTOR_BYTES));
@@ -392,17 +404,23 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         bulk_copy(dst + PLANE + SK * RB, factors + plane_step, n * Q4_FACTOR_BYTES, bar);
                     }
                 }
+                k_next = end;
+                if (end == end_next) {
+                    ++page_at;
+                    end_next += P;
+                }
             };
-            int k0 = k_begin, k_next = k_begin;   // first key that is not read yet; that is not asked for yet
+            // end of the stage that begins with k0
+            auto stage_end = [&]() { return min(min(end_read, k0 + SK), k_stop); };
+            auto next_stage = [&](int end) {
+                if (end == end_read) end_read += P;
+                k0 = end;
+            };
             int st = 0;
             if (ok) {
 #pragma unroll
                 for (int c = 0; c < S - 1; ++c)
-                    if (k_next < k_stop) {
-                        const int e = stage_end(k_next);
-                        issue(k_next, e, c);
-                        k_next = e;
-                    }
+                    if (k_next < k_stop) issue(c);
             }
 
             // Q as B fragments: head gq (and gq + 8 of the second tile), dimensions t4 HD / 4 + 8 w + 4 x + {0, 1} and + {2, 3}: words w, x = 0, 1
@@ -423,26 +441,28 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int k = min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);   // (-114 for infinities)
-                const float up = pow2i(k);
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                // the codes that meet {2, 3} count sixteen times what those that meet {0, 1} do
+                const float up = pow2i(k), up16 = up * 0.0625f;
+                float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * KW; ++i) {
                     split2<PARTS>(x[4 * i] * up, x[4 * i + 1] * up, qb[ht][i][0]);
-                    split2<PARTS>(x[4 * i + 2] * up, x[4 * i + 3] * up, qb[ht][i][1]);
-#pragma unroll
-                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(sum, ones, qb[ht][i][0][y], qb[ht][i][1][y]);
+                    split2<PARTS>(x[4 * i + 2] * up16, x[4 * i + 3] * up16, qb[ht][i][1]);
+                    sum += (x[4 * i] + x[4 * i + 1]) + (x[4 * i + 2] + x[4 * i + 3]);
                 }
-                const float down = qscale * pow2i(-k);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                const float down = qscale * pow2i(-k) * 4096.f;   // (2^24 comes off the codes: half of it here, half with the key's scale)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     hq[ht][c] = __shfl_sync(0xffffffffu, down, 4 * (2 * t4 + c));
-                    sq[ht][c] = sum[c] * hq[ht][c];
+                    sq[ht][c] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t4 + c)) * qscale;
                 }
             }
             // O^T: byte b of word w of a lane's value row is row tile 4 w + b: its low nibble's dimension in row gq, its high nibble's in row
             // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
             float o[HT][MT][4], m[HT][2], l[HT][2], z[HT][2], slope[HT][2];
+            float from[HT][2];   // what a score's weight is formed relative to: M - TOP (0: no live key yet)
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
@@ -451,177 +471,173 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 for (int c = 0; c < 2; ++c) {
                     const int g = 8 * ht + 2 * t4 + c;
                     m[ht][c] = -INFINITY;
-                    l[ht][c] = z[ht][c] = 0.f;
+                    l[ht][c] = z[ht][c] = from[ht][c] = 0.f;
                     slope[ht][c] = a.slopes && g < nG ? slope_log2(a.slopes, h0 + g) : 0.f;
                 }
             }
 
-            while (ok && k0 < k_stop) {
-                __syncwarp();  // every lane has read the stage before this one: its place may be overwritten
-                if (k_next < k_stop) {
-                    int st_new = st + S - 1;
-                    if (st_new >= S) st_new -= S;
-                    const int e = stage_end(k_next);
-                    issue(k_next, e, st_new);
-                    k_next = e;
+            float* const scores = WEIGH ? a.scores + (static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P * G + g0 + 2 * t4 : nullptr;
+            // sixteen keys, from c0, whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
+            auto chunk = [&](int c0, const unsigned char* at, const unsigned char* fac) {
+                const bool edge = c0 < t_lo || c0 + 16 > k_end;   // (a chunk with dead keys)
+                // keys c0 + kr0 and c0 + 8 + kr0: words, factors of the key's and of the value's row
+                uint32_t k_lo[KW], k_hi[KW], v_a[2][VW], v_b[2][VW], kf[2], vf[2];
+                lds_words<KW>(k_lo, at + kr0 * RB + t4 * (RB / 4));
+                lds_words<KW>(k_hi, at + (kr0 + 8) * RB + t4 * (RB / 4));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    lds_words<1>(kf + i, fac + 4 * (kr0 + 8 * i));
+                    lds_words<1>(vf + i, fac + PLANE + 4 * (kr0 + 8 * i));
+                    lds_words<VW>(v_a[i], at + PLANE + (8 * i + va_row) * RB + gq * (RB / 8));
+                    lds_words<VW>(v_b[i], at + PLANE + (8 * i + vb_row) * RB + gq * (RB / 8));
                 }
-                const int end = stage_end(k0);
-                ok = mbar_wait(bars + 8 * st, (parity >> st) & 1u);
-                if (!ok) break;
-                parity ^= 1u << st;
-                const uint32_t src = ring + st * STAGE;
-                if (++st == S) st = 0;
-                for (int c0 = k0; c0 < end; c0 += 16) {
-                    const uint32_t kbase = src + (c0 - k0) * RB, kfac = src + SK * RB + (c0 - k0) * Q4_FACTOR_BYTES;
-                    // keys c0 + kr0 and c0 + 8 + kr0: words, factors of the key's and of the value's row
-                    uint32_t k_lo[KW], k_hi[KW];
-                    lds_words<KW>(k_lo, kbase + kr0 * RB + t4 * (RB / 4));
-                    lds_words<KW>(k_hi, kbase + (kr0 + 8) * RB + t4 * (RB / 4));
-                    uint32_t kf[2], vf[2];
-                    kf[0] = lds4(kfac + 4 * kr0);
-                    kf[1] = lds4(kfac + 4 * (kr0 + 8));
-                    vf[0] = lds4(kfac + PLANE + 4 * kr0);
-                    vf[1] = lds4(kfac + PLANE + 4 * (kr0 + 8));
-                    uint32_t v_a[2][VW], v_b[2][VW];
+                float s[HT][4];
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) s[ht][0] = s[ht][1] = s[ht][2] = s[ht][3] = 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; ++w)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        lds_words<VW>(v_a[x], kbase + PLANE + (8 * x + va_row) * RB + gq * (RB / 8));
-                        lds_words<VW>(v_b[x], kbase + PLANE + (8 * x + vb_row) * RB + gq * (RB / 8));
-                    }
-                    float s[HT][2][4];
-#pragma unroll
-                    for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) s[ht][x][0] = s[ht][x][1] = s[ht][x][2] = s[ht][x][3] = 0.f;
-#pragma unroll
-                    for (int w = 0; w < KW; ++w)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
-                            const uint32_t af[4] = {codes_low(a0), codes_low(a1), codes_high(a0), codes_high(a1)};
-#pragma unroll
-                            for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                                for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[ht][x], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
-                        }
-                    const int key[2] = {c0 + kr0, c0 + 8 + kr0};
-                    const bool edge = c0 < t_lo || c0 + 16 > k_end;
-                    bool live[2] = {true, true};
-                    if (edge) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < k_end;
-                            if (!live[i]) kf[i] = vf[i] = 0u;
-                        }
-                    }
-                    // of the two keys: scale of K, z of K; of V the scale's exponent, what is left of it, z, both over 2^exponent
-                    float ks[2], kz[2], ve[2], vs[2], vz[2], vi[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        ks[i] = q4_scale(kf[i]);
-                        kz[i] = fmaf(-0.5f, ks[i], q4_mid(kf[i]));
-                        const float scale = q4_scale(vf[i]);
-                        const int e = min(max(static_cast<int>((vf[i] >> 7) & 0xffu) - 127, LEAST), 126);
-                        ve[i] = static_cast<float>(e);
-                        vi[i] = pow2i(-e);
-                        vs[i] = scale * vi[i];
-                        vz[i] = fmaf(-0.5f, scale, q4_mid(vf[i])) * vi[i];
-                    }
-                    float sc[HT][4];   // score + exponent
-                    bool raise = false;
-#pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int c = i & 1, y = i >> 1;
-                            float w = fmaf(s[ht][0][i] + s[ht][1][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
-                            if (a.slopes) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
-                            if (WEIGH) {
-                                const int g = 8 * ht + 2 * t4 + c;
-                                if (g < nG && live[y])
-                                    a.scores[((static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P + key[y]) * G + g0 + g] = w;
-                                w += ve[y];
-                            }
-                            if (edge && !live[y]) w = -INFINITY;
-                            sc[ht][i] = w;
-                            raise |= w > m[ht][c] + RAISE;
-                        }
-                    }
-                    if (__any_sync(0xffffffffu, raise)) {
+                        const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
+                        const uint32_t af[4] = {a0 & 0x000f000fu, a1 & 0x000f000fu, a0 & 0x00f000f0u, a1 & 0x00f000f0u};
 #pragma unroll
                         for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                float n = fmaxf(sc[ht][c], sc[ht][2 + c]);
-                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
-                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
-                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
-                                n = fmaxf(n, m[ht][c]);
-                                const float corr = m[ht][c] == -INFINITY ? 0.f : ex2(m[ht][c] - n);
-                                m[ht][c] = n;
-                                l[ht][c] *= corr;
-                                z[ht][c] *= corr;
-#pragma unroll
-                                for (int j = 0; j < MT; ++j) {
-                                    o[ht][j][c] *= corr;
-                                    o[ht][j][2 + c] *= corr;
-                                }
-                            }
+                            for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
                     }
-                    uint32_t pb[HT][2][PARTS];
+                const int key[2] = {c0 + kr0, c0 + 8 + kr0};
+                bool live[2] = {true, true};
+                if (edge) {
 #pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) {
-                        float e[4];
+                    for (int i = 0; i < 2; ++i) {
+                        live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < k_end;
+                        if (!live[i]) kf[i] = vf[i] = 0u;
+                    }
+                }
+                // of the two keys: 2^12 scale of K, mid - 7.5 scale; of V the scale's exponent e, 2^-e, scale 2^-e, (mid - scale / 2) 2^-e
+                float ks[2], kz[2], ve[2], vs[2], vz[2], vi[2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float mu = m[ht][i & 1];
-                            e[i] = ex2(sc[ht][i] - (mu == -INFINITY ? 0.f : mu - TOP));   // (no live key yet: all weights 0)
+                for (int i = 0; i < 2; ++i) {
+                    const float k_scale = q4_scale(kf[i]), v_scale = q4_scale(vf[i]);
+                    ks[i] = k_scale * 4096.f;
+                    kz[i] = fmaf(-7.5f, k_scale, q4_mid(kf[i]));
+                    // (the exponent's field, LEAST + 127 .. 253, still in its place)
+                    const uint32_t e = min(max((vf[i] << 16) & 0x7f800000u, static_cast<uint32_t>(LEAST + 127) << 23), 253u << 23);
+                    ve[i] = __uint_as_float(0x4b000000u | (e >> 23)) - (8388608.f + 127.f);
+                    vi[i] = __uint_as_float((254u << 23) - e);
+                    vs[i] = v_scale * vi[i];
+                    vz[i] = fmaf(-0.5f, v_scale, q4_mid(vf[i])) * vi[i];
+                }
+                float sc[HT][4];   // score + e
+                bool raise = false;
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = i & 1, y = i >> 1;
+                        float w = fmaf(s[ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
+                        if (a.slopes) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
+                        if (WEIGH) {
+                            const int g = 8 * ht + 2 * t4 + c;
+                            if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
+                            w += ve[y];
                         }
+                        if (edge && !live[y]) w = -INFINITY;
+                        sc[ht][i] = w;
+                        raise |= w > m[ht][c] + RAISE;
+                    }
+                }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            l[ht][c] = fmaf(e[c], vi[0], fmaf(e[2 + c], vi[1], l[ht][c]));
-                            z[ht][c] = fmaf(e[c], vz[0], fmaf(e[2 + c], vz[1], z[ht][c]));
-                        }
-                        // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
-                        split2<PARTS>(e[0] * vs[0], e[1] * vs[0], pb[ht][0]);
-                        split2<PARTS>(e[2] * vs[1], e[3] * vs[1], pb[ht][1]);
+                            float n = fmaxf(sc[ht][c], sc[ht][2 + c]);
+                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
+                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
+                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
+                            n = fmaxf(n, m[ht][c]);
+                            const float corr = m[ht][c] == -INFINITY ? 0.f : ex2(m[ht][c] - n);
+                            m[ht][c] = n;
+                            from[ht][c] = n == -INFINITY ? 0.f : n - TOP;
+                            l[ht][c] *= corr;
+                            z[ht][c] *= corr;
 #pragma unroll
-                        for (int y = 0; y < PARTS; ++y) {
-                            pb[ht][0][y] = movmatrix_trans(pb[ht][0][y]);
-                            pb[ht][1][y] = movmatrix_trans(pb[ht][1][y]);
-                        }
-                    }
-#pragma unroll
-                    for (int w = 0; w < VW; ++w)
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
-                            const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
-                            const uint32_t af[4] = {codes_low(x0), codes_high(x0), codes_low(x1), codes_high(x1)};
-#pragma unroll
-                            for (int ht = 0; ht < HT; ++ht) {
-                                float* t = o[ht][4 * w + b];
-                                if constexpr (PARTS == 1) {
-                                    mma_f16(t, af, pb[ht][0][0], pb[ht][1][0]);
-                                } else {
-                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(d, af, pb[ht][0][y], pb[ht][1][y]);
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) t[i] += d[i];
-                                }
+                            for (int j = 0; j < MT; ++j) {
+                                o[ht][j][c] *= corr;
+                                o[ht][j][2 + c] *= corr;
                             }
                         }
                 }
-                k0 = end;
+                uint32_t pb[HT][2][PARTS];
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) {
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[i] = ex2(sc[ht][i] - from[ht][i & 1]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        l[ht][c] = fmaf(e[c], vi[0], fmaf(e[2 + c], vi[1], l[ht][c]));
+                        z[ht][c] = fmaf(e[c], vz[0], fmaf(e[2 + c], vz[1], z[ht][c]));
+                    }
+                    // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
+                    split2<PARTS>(e[0] * vs[0], e[1] * vs[0], pb[ht][0]);
+                    split2<PARTS>(e[2] * vs[1], e[3] * vs[1], pb[ht][1]);
+#pragma unroll
+                    for (int y = 0; y < PARTS; ++y) {
+                        pb[ht][0][y] = movmatrix_trans(pb[ht][0][y]);
+                        pb[ht][1][y] = movmatrix_trans(pb[ht][1][y]);
+                    }
+                }
+                const uint32_t seven[4] = {0x80078007u, 0x80708070u, 0x80078007u, 0x80708070u};   // -7 2^-24, -7 2^-20
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
+                        const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
+                        const uint32_t af[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) {
+                            float* t = o[ht][4 * w + b];
+                            if constexpr (PARTS == 1) {
+                                mma_f16(t, seven, pb[ht][0][0], pb[ht][1][0]);
+                                mma_f16(t, af, pb[ht][0][0], pb[ht][1][0]);
+                            } else {
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int y = PARTS - 1; y >= 0; --y) {
+                                    mma_f16(d, seven, pb[ht][0][y], pb[ht][1][y]);
+                                    mma_f16(d, af, pb[ht][0][y], pb[ht][1][y]);
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) t[i] += d[i];
+                            }
+                        }
+                    }
+            };
+
+            while (ok && k0 < k_stop) {
+                __syncwarp();  // every lane has read the stage before this one: its place may be overwritten
+                if (k_next < k_stop) issue(st + S - 1 < S ? st + S - 1 : st - 1);
+                const int end = stage_end();
+                ok = mbar_wait(bars + 8 * st, (parity >> st) & 1u);
+                if (!ok) break;
+                parity ^= 1u << st;
+                const unsigned char* src = q4_smem + warp * (S * STAGE) + st * STAGE;
+                if (++st == S) st = 0;
+                const int n = end - k0;
+#pragma unroll 1
+                for (int c = 0; c < n; c += 16) chunk(k0 + c, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                next_stage(end);
             }
             if (!ok) {
                 // a copy never came: the error word is set.  Those behind it are waited for, with the same limit
                 while (k0 < k_next) {
-                    const int end = stage_end(k0);
+                    const int end = stage_end();
                     if (++st == S) st = 0;
                     if (end < k_next) mbar_wait(bars + 8 * st, (parity >> st) & 1u);
-                    k0 = end;
+                    next_stage(end);
                 }
             }
             __syncwarp();
@@ -640,11 +656,13 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     const int g = 8 * ht + 2 * t4 + c;
                     if (g < nG) {
                         float* po = res + g * HD + gq * (HD / 8);
+                        auto low = [&](const float* t) { return fmaf(t[c], 16777216.f, zc); };        // 2^24, 2^20: the nibbles' places
+                        auto high = [&](const float* t) { return fmaf(t[2 + c], 1048576.f, zc); };
 #pragma unroll
                         for (int w = 0; w < VW; ++w) {
                             const float (*t)[4] = &o[ht][4 * w];
-                            *reinterpret_cast<float4*>(po + 8 * w) = make_float4(t[0][c] + zc, t[2][c] + zc, t[0][2 + c] + zc, t[2][2 + c] + zc);
-                            *reinterpret_cast<float4*>(po + 8 * w + 4) = make_float4(t[1][c] + zc, t[3][c] + zc, t[1][2 + c] + zc, t[3][2 + c] + zc);
+                            *reinterpret_cast<float4*>(po + 8 * w) = make_float4(low(t[0]), low(t[2]), high(t[0]), high(t[2]));
+                            *reinterpret_cast<float4*>(po + 8 * w + 4) = make_float4(low(t[1]), low(t[3]), high(t[1]), high(t[3]));
                         }
                         if (gq == 0) *reinterpret_cast<float2*>(res + 8 * HT * HD + 2 * g) = make_float2(m[ht][c], lc);
                     }
@@ -767,7 +785,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         }
                     }
                 }
-                finish(g, acc, L, M, lh0, a.seg_q0[pl.seg[li]], li);
+                finish(g, acc, L, M, lh0, pl.row[li], li);
             }
         }
         __syncthreads();   // (is_last is written again in the next round)
@@ -798,58 +816,75 @@ __global__ void __launch_bounds__(WG_THREADS) q4_weigh_kernel(Q4Args a, float* _
 }
 
 template <typename T, int HD, int HT, int W, int S, int SK, bool WEIGH>
-static int q4_decode_launch(const Q4Args& a, int n_items, long long max_units, int cost_range, int cost_merge, int n_sm, cudaStream_t stream) {
+static int q4_decode_launch(const Q4Args& a, int n_items, long long max_units, int cost_range, int cost_merge, int n_sm, int dev, cudaStream_t stream) {
     constexpr size_t smem = static_cast<size_t>(W) * S * 2 * SK * (HD / 2 + Q4_FACTOR_BYTES);
-    if (cudaFuncSetAttribute(attn_decode_q4_kernel<T, HD, HT, W, S, SK, WEIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-        return static_cast<int>(cudaGetLastError());
+    static unsigned long long asked = 0;   // devices that know of the kernel's shared memory (asked again at worst)
+    if (dev >= 64 || !(asked >> dev & 1)) {
+        if (cudaFuncSetAttribute(attn_decode_q4_kernel<T, HD, HT, W, S, SK, WEIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(smem)) != cudaSuccess)
+            return static_cast<int>(cudaGetLastError());
+        if (dev < 64) asked |= 1ull << dev;
+    }
     locus_launch(attn_decode_q4_kernel<T, HD, HT, W, S, SK, WEIGH>, n_sm, 32 * W, smem, stream, a, n_items, max_units, cost_range, cost_merge);
     return locus_launch_status();
 }
 
+// What a call brings.  (One pointer to all of it: a foreign-function call pays for each of its arguments, a tenth of a microsecond from Python.)
 // part_o holds max_units partial results of hd floats (at least n_items * nh; twice that with kept first tokens), part_ml two floats each, counters
 // n_items * nh ints that are zero before and after the call.  weights (or null) [n_pages][nkv][P] float32, with scores of n_items * nh *
 // table_stride * P floats and lse of 2 n_items * nh; then neither a window nor chunks.
-extern "C" int locus_attn_decode_q4(const void* q, int dt, const void* pool, void* out, const int* seg_q0, const int* seg_ctx,
-                                    const int* block_table, int table_stride, const int* items, int n_items, int nh, int nkv, int hd,
-                                    int page_tokens, int window, int chunk, float scale, float* part_o, float* part_ml, int* counters,
-                                    long long max_units, int cost_range, int cost_merge, int keep_first, int sink,
-                                    const float* sink_val, const float* slopes, float* weights, float* scores, float* lse,
-                                    cudaStream_t stream) {
-    if (n_items <= 0) return 0;
-    if ((dt != LOCUS_DT_F32 && dt != LOCUS_DT_BF16) || nkv <= 0 || nh <= 0 || nh % nkv != 0 || !q4_head_ok(hd) || page_tokens <= 0 ||
-        page_tokens % 16 != 0 || n_items > Q4_MAX_ITEMS || !mask_ok(window, chunk, keep_first) || counters == nullptr || table_stride <= 0 ||
-        nkv > 65535 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(part_o)) & 15) != 0)
+struct Q4DecodeCall {
+    const void *q, *pool;
+    void* out;
+    const int *seg_q0, *seg_ctx, *block_table, *items;
+    float *part_o, *part_ml;
+    int* counters;
+    const float *sink_val, *slopes;
+    float *weights, *scores, *lse;
+    long long dt, table_stride, n_items, nh, nkv, hd, page_tokens, window, chunk, max_units, cost_range, cost_merge, keep_first, sink;
+    double scale;
+};
+
+extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t stream) {
+    const Q4DecodeCall& v = *call;
+    if (v.n_items <= 0) return 0;
+    if ((v.dt != LOCUS_DT_F32 && v.dt != LOCUS_DT_BF16) || v.nkv <= 0 || v.nh <= 0 || v.nh % v.nkv != 0 || !q4_head_ok(static_cast<int>(v.hd)) ||
+        v.page_tokens <= 0 || v.page_tokens % 16 != 0 || v.n_items > Q4_MAX_ITEMS || v.table_stride <= 0 || v.nkv > 65535 || v.counters == nullptr ||
+        !mask_ok(static_cast<int>(v.window), static_cast<int>(v.chunk), static_cast<int>(v.keep_first)) ||
+        ((reinterpret_cast<uintptr_t>(v.q) | reinterpret_cast<uintptr_t>(v.pool) | reinterpret_cast<uintptr_t>(v.part_o)) & 15) != 0 ||
+        (reinterpret_cast<uintptr_t>(v.part_ml) & 7) != 0)
         return LOCUS_ERR_UNSUPPORTED;
-    if (window == 0) keep_first = 0;
-    if (max_units < static_cast<long long>(n_items) * nh * (keep_first > 0 ? 2 : 1)) return LOCUS_ERR_UNSUPPORTED;
-    if (weights && (scores == nullptr || lse == nullptr || window > 0 || chunk > 0)) return LOCUS_ERR_UNSUPPORTED;
+    const int keep_first = v.window == 0 ? 0 : static_cast<int>(v.keep_first);
+    if (v.max_units < v.n_items * v.nh * (keep_first > 0 ? 2 : 1)) return LOCUS_ERR_UNSUPPORTED;
+    if (v.weights && (v.scores == nullptr || v.lse == nullptr || v.window > 0 || v.chunk > 0)) return LOCUS_ERR_UNSUPPORTED;
     int dev = 0, n_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n_sm <= 0)
         return static_cast<int>(cudaGetLastError());
     Q4Args a;
-    a.q = q; a.pool = static_cast<const uint8_t*>(pool); a.out = out;
-    a.seg_q0 = seg_q0; a.seg_ctx = seg_ctx; a.block_table = block_table; a.table_stride = table_stride; a.items = items;
-    a.nh = nh; a.nkv = nkv; a.page_tokens = page_tokens; a.window = window; a.chunk = chunk; a.scale = scale;
-    a.keep_first = keep_first; a.sink = sink; a.sink_val = sink ? sink_val : nullptr; a.slopes = slopes;
-    a.part_o = part_o; a.part_ml = part_ml; a.counters = counters; a.scores = scores; a.lse = lse;
-    const bool wide = nh / nkv > 8;
-#define Q4_GO(T_, HD_, HT_, W_, S_, SK_)                                                                                        \
-    (weights ? q4_decode_launch<T_, HD_, HT_, W_, S_, SK_, true>(a, n_items, max_units, cost_range, cost_merge, n_sm, stream)   \
-             : q4_decode_launch<T_, HD_, HT_, W_, S_, SK_, false>(a, n_items, max_units, cost_range, cost_merge, n_sm, stream))
+    a.q = v.q; a.pool = static_cast<const uint8_t*>(v.pool); a.out = v.out;
+    a.seg_q0 = v.seg_q0; a.seg_ctx = v.seg_ctx; a.block_table = v.block_table; a.table_stride = static_cast<int>(v.table_stride); a.items = v.items;
+    a.nh = static_cast<int>(v.nh); a.nkv = static_cast<int>(v.nkv); a.page_tokens = static_cast<int>(v.page_tokens);
+    a.window = static_cast<int>(v.window); a.chunk = static_cast<int>(v.chunk); a.scale = static_cast<float>(v.scale);
+    a.keep_first = keep_first; a.sink = static_cast<int>(v.sink); a.sink_val = v.sink ? v.sink_val : nullptr; a.slopes = v.slopes;
+    a.part_o = v.part_o; a.part_ml = v.part_ml; a.counters = v.counters; a.scores = v.scores; a.lse = v.lse;
+    const int n = static_cast<int>(v.n_items), cr = static_cast<int>(v.cost_range), cm = static_cast<int>(v.cost_merge);
+    const bool wide = a.nh / a.nkv > 8;
+#define Q4_GO(T_, HD_, HT_, W_, S_, SK_)                                                                              \
+    (v.weights ? q4_decode_launch<T_, HD_, HT_, W_, S_, SK_, true>(a, n, v.max_units, cr, cm, n_sm, dev, stream)      \
+               : q4_decode_launch<T_, HD_, HT_, W_, S_, SK_, false>(a, n, v.max_units, cr, cm, n_sm, dev, stream))
     int code;
-    if (dt == LOCUS_DT_F32) {
-        code = hd == 64 ? Q4_GO(float, 64, 1, 8, 3, 64) : hd == 128 ? Q4_GO(float, 128, 1, 8, 2, 64) : Q4_GO(float, 256, 1, 8, 2, 32);
-    } else if (hd == 64) {
+    if (v.dt == LOCUS_DT_F32) {
+        code = v.hd == 64 ? Q4_GO(float, 64, 1, 8, 3, 64) : v.hd == 128 ? Q4_GO(float, 128, 1, 8, 2, 64) : Q4_GO(float, 256, 1, 8, 2, 32);
+    } else if (v.hd == 64) {
         code = wide ? Q4_GO(bf16, 64, 2, 12, 3, 64) : Q4_GO(bf16, 64, 1, 12, 3, 64);
-    } else if (hd == 128) {
+    } else if (v.hd == 128) {
         code = wide ? Q4_GO(bf16, 128, 2, 8, 2, 64) : Q4_GO(bf16, 128, 1, 12, 2, 64);
     } else {
         code = Q4_GO(bf16, 256, 1, 8, 2, 32);
     }
 #undef Q4_GO
-    if (code || !weights) return code;
-    const dim3 grid(ceil_div(table_stride * page_tokens, WG_THREADS), nkv, n_items);
-    locus_launch(q4_weigh_kernel, grid, WG_THREADS, 0, stream, a, weights);
+    if (code || !v.weights) return code;
+    const dim3 grid(ceil_div(a.table_stride * a.page_tokens, WG_THREADS), a.nkv, n);
+    locus_launch(q4_weigh_kernel, grid, WG_THREADS, 0, stream, a, v.weights);
     return locus_launch_status();
 }

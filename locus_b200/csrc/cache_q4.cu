@@ -168,20 +168,30 @@ static int write_launch(const void* qkv, const int* positions, const float* inv_
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// inv_freq null: no rotation (rot is then taken as 0).  weights (or null) [n_pages][nkv][P] float32: 0 for the slots that are written.
-extern "C" int locus_rope_kv_write_q4(const void* qkv, int dt, const int* positions, const float* inv_freq, void* q_out, void* pool,
-                                      const int* slots, float* weights, int T, int nh, int nkv, int hd, int rot, int pairing, int P,
-                                      int write_kv, cudaStream_t stream) {
-    if (T <= 0) return 0;
-    if (inv_freq == nullptr) rot = 0;
-    if (!q4_head_ok(hd) || nh <= 0 || nkv <= 0 || P <= 0 || P % 16 != 0 || rot < 0 || rot > hd || (rot & 1) || (pairing != 0 && pairing != 1) ||
-        !aligned16(qkv) || !aligned16(q_out) || !aligned16(pool) || (write_kv && slots == nullptr))
+// What a call brings, behind one pointer (see attention_q4.cu).  inv_freq null: no rotation (rot is then taken as 0).  weights (or null)
+// [n_pages][nkv][P] float32: 0 for the slots that are written.
+struct Q4WriteCall {
+    const void* qkv;
+    const int* positions;
+    const float* inv_freq;
+    void *q_out, *pool;
+    const int* slots;
+    float* weights;
+    long long dt, T, nh, nkv, hd, rot, pairing, P, write_kv;
+};
+extern "C" int locus_rope_kv_write_q4(const Q4WriteCall* call, cudaStream_t stream) {
+    const Q4WriteCall& v = *call;
+    if (v.T <= 0) return 0;
+    const int hd = static_cast<int>(v.hd), rot = v.inv_freq == nullptr ? 0 : static_cast<int>(v.rot), P = static_cast<int>(v.P);
+    if (!q4_head_ok(hd) || v.nh <= 0 || v.nkv <= 0 || P <= 0 || P % 16 != 0 || rot < 0 || rot > hd || (rot & 1) || (v.pairing != 0 && v.pairing != 1) ||
+        !aligned16(v.qkv) || !aligned16(v.q_out) || !aligned16(v.pool) || (v.write_kv && v.slots == nullptr))
         return LOCUS_ERR_UNSUPPORTED;
-    uint8_t* p8 = static_cast<uint8_t*>(pool);
-    if (dt == LOCUS_DT_F32)
-        return write_launch<float>(qkv, positions, inv_freq, q_out, p8, slots, weights, T, nh, nkv, hd, rot, pairing, P, write_kv, stream);
-    if (dt == LOCUS_DT_BF16)
-        return write_launch<bf16>(qkv, positions, inv_freq, q_out, p8, slots, weights, T, nh, nkv, hd, rot, pairing, P, write_kv, stream);
+    auto go = [&](auto launch) {
+        return launch(v.qkv, v.positions, v.inv_freq, v.q_out, static_cast<uint8_t*>(v.pool), v.slots, v.weights, static_cast<int>(v.T),
+                      static_cast<int>(v.nh), static_cast<int>(v.nkv), hd, rot, static_cast<int>(v.pairing), P, static_cast<int>(v.write_kv), stream);
+    };
+    if (v.dt == LOCUS_DT_F32) return go(write_launch<float>);
+    if (v.dt == LOCUS_DT_BF16) return go(write_launch<bf16>);
     return LOCUS_ERR_UNSUPPORTED;
 }
 
@@ -223,25 +233,33 @@ __global__ void __launch_bounds__(E_THREADS) q4_expand_kernel(const uint8_t* __r
 }
 
 // max_keys: at least the tokens of the longest of these segments.
-extern "C" int locus_expand_q4(const void* pool, void* out, int dt, const int* segs, int n_segs, const int* seg_ctx, const int* seg_qn,
-                               const int* block_table, int table_stride, int nkv, int hd, int P, int max_keys, cudaStream_t stream) {
-    if (n_segs <= 0 || max_keys <= 0) return 0;
-    const int pages = min(table_stride, ceil_div(max_keys, P > 0 ? P : 1));
-    if (!q4_head_ok(hd) || nkv <= 0 || P <= 0 || P % 16 != 0 || !aligned16(pool) || !aligned16(out) || pages > 65535 || n_segs > 65535)
+struct Q4ExpandCall {
+    const void* pool;
+    void* out;
+    const int *segs, *seg_ctx, *seg_qn, *block_table;
+    long long dt, n_segs, table_stride, nkv, hd, P, max_keys;
+};
+extern "C" int locus_expand_q4(const Q4ExpandCall* call, cudaStream_t stream) {
+    const Q4ExpandCall& v = *call;
+    if (v.n_segs <= 0 || v.max_keys <= 0) return 0;
+    const int hd = static_cast<int>(v.hd), P = static_cast<int>(v.P), nkv = static_cast<int>(v.nkv), table_stride = static_cast<int>(v.table_stride);
+    const long long pages = min(v.table_stride, (v.max_keys + max(P, 1) - 1) / max(P, 1));
+    if (!q4_head_ok(hd) || nkv <= 0 || P <= 0 || P % 16 != 0 || !aligned16(v.pool) || !aligned16(v.out) || pages > 65535 || v.n_segs > 65535)
         return LOCUS_ERR_UNSUPPORTED;
-    const dim3 grid(2 * nkv, pages, n_segs);
-    const uint8_t* p8 = static_cast<const uint8_t*>(pool);
+    if (pages <= 0) return 0;
+    const dim3 grid(2 * nkv, static_cast<unsigned>(pages), static_cast<unsigned>(v.n_segs));
+    const uint8_t* p8 = static_cast<const uint8_t*>(v.pool);
 #define Q4_EXPAND(T_, HD_)                                                                                                          \
-    locus_launch(q4_expand_kernel<T_, HD_>, grid, E_THREADS, 0, stream, p8, static_cast<T_*>(out), segs, seg_ctx, seg_qn,           \
-                 block_table, table_stride, nkv, P)
+    locus_launch(q4_expand_kernel<T_, HD_>, grid, E_THREADS, 0, stream, p8, static_cast<T_*>(v.out), v.segs, v.seg_ctx, v.seg_qn,   \
+                 v.block_table, table_stride, nkv, P)
 #define Q4_EXPAND_T(T_)                                                                                                             \
     do {                                                                                                                            \
         if (hd == 64) Q4_EXPAND(T_, 64);                                                                                            \
         else if (hd == 128) Q4_EXPAND(T_, 128);                                                                                     \
         else Q4_EXPAND(T_, 256);                                                                                                    \
     } while (0)
-    if (dt == LOCUS_DT_F32) Q4_EXPAND_T(float);
-    else if (dt == LOCUS_DT_BF16) Q4_EXPAND_T(bf16);
+    if (v.dt == LOCUS_DT_F32) Q4_EXPAND_T(float);
+    else if (v.dt == LOCUS_DT_BF16) Q4_EXPAND_T(bf16);
     else return LOCUS_ERR_UNSUPPORTED;
 #undef Q4_EXPAND_T
 #undef Q4_EXPAND
@@ -470,29 +488,44 @@ __global__ void __launch_bounds__(M_THREADS) q4_move_kernel(uint8_t* pool, float
 }
 
 // max_tokens: at least the tokens of the longest request (its weights' place in shared memory is sized by it).
-extern "C" int locus_evict_q4(void* pool, float* weights, const int* block_table, int table_stride, const int* dst_table, int dst_stride,
-                              const int* n_tokens, int n_items, int n_layers, long long layer_pages, int nkv, int hd, int P, int keep,
-                              int first, int recent, int max_tokens, int* kept, cudaStream_t stream) {
-    if (n_items <= 0 || n_layers <= 0) return 0;
+struct Q4EvictCall {
+    void* pool;
+    float* weights;
+    const int *block_table, *dst_table, *n_tokens;
+    int* kept;
+    long long table_stride, dst_stride, n_items, n_layers, layer_pages, nkv, hd, P, keep, first, recent, max_tokens;
+};
+extern "C" int locus_evict_q4(const Q4EvictCall* call, cudaStream_t stream) {
+    const Q4EvictCall& v = *call;
+    if (v.n_items <= 0 || v.n_layers <= 0) return 0;
+    const int hd = static_cast<int>(v.hd), P = static_cast<int>(v.P), nkv = static_cast<int>(v.nkv), keep = static_cast<int>(v.keep);
+    const int first = static_cast<int>(v.first), recent = static_cast<int>(v.recent), max_tokens = static_cast<int>(v.max_tokens);
+    const int n_items = static_cast<int>(v.n_items), table_stride = static_cast<int>(v.table_stride), dst_stride = static_cast<int>(v.dst_stride);
     if (!q4_head_ok(hd) || nkv <= 0 || P <= 0 || P % 16 != 0 || keep <= 0 || first < 0 || recent < 0 || first > keep - recent ||
-        n_items > 65535 || n_layers > 65535 || !aligned16(pool) || max_tokens <= 0)
+        n_items > 65535 || v.n_layers > 65535 || !aligned16(v.pool) || max_tokens <= 0)
         return LOCUS_ERR_UNSUPPORTED;
-    const size_t slots = static_cast<size_t>(layer_pages) * nkv * P, bytes = slots * 2 * q4_row_bytes(hd);
+    const size_t slots = static_cast<size_t>(v.layer_pages) * nkv * P, bytes = slots * 2 * q4_row_bytes(hd);
     const int between = max(0, max_tokens - first - recent);
-    const dim3 grid(nkv, n_items, n_layers);
+    const dim3 grid(nkv, n_items, static_cast<unsigned>(v.n_layers));
     const int room = between <= SK_MAX ? between : 0;   // (longer ones are read from memory in every pass)
-    if (cudaFuncSetAttribute(q4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_MAX * 4) != cudaSuccess)
-        return static_cast<int>(cudaGetLastError());
-    locus_launch(q4_select_kernel, grid, S_THREADS, static_cast<size_t>(room) * 4, stream, weights, block_table,
-                 table_stride, n_tokens, n_items, nkv, P, slots, keep, first, recent, room, kept);
-    int code = locus_launch_status();
+    static unsigned long long asked = 0;   // devices that know of the kernel's shared memory (asked again at worst)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return static_cast<int>(cudaGetLastError());
+    if (dev >= 64 || !(asked >> dev & 1)) {
+        if (cudaFuncSetAttribute(q4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_MAX * 4) != cudaSuccess)
+            return static_cast<int>(cudaGetLastError());
+        if (dev < 64) asked |= 1ull << dev;
+    }
+    locus_launch(q4_select_kernel, grid, S_THREADS, static_cast<size_t>(room) * 4, stream, v.weights, v.block_table, table_stride, v.n_tokens, n_items,
+                 nkv, P, slots, keep, first, recent, room, v.kept);
+    const int code = locus_launch_status();
     if (code) return code;
     const int tile = M_THREADS * M_UNROLL / (hd / 32);
-    const int n_parts = dst_table == block_table ? 1 : max(1, min(ceil_div(min(keep, max_tokens), tile), 16));
-    const dim3 mgrid(2 * nkv * n_parts, n_items, n_layers);
-#define Q4_MOVE(HD_)                                                                                                                \
-    locus_launch(q4_move_kernel<HD_>, mgrid, M_THREADS, 0, stream, static_cast<uint8_t*>(pool), weights, block_table, table_stride, \
-                 dst_table, dst_stride, n_tokens, n_items, nkv, P, bytes, slots, keep, n_parts, kept)
+    const int n_parts = v.dst_table == v.block_table ? 1 : max(1, min(ceil_div(min(keep, max_tokens), tile), 16));
+    const dim3 mgrid(2 * nkv * n_parts, n_items, static_cast<unsigned>(v.n_layers));
+#define Q4_MOVE(HD_)                                                                                                                        \
+    locus_launch(q4_move_kernel<HD_>, mgrid, M_THREADS, 0, stream, static_cast<uint8_t*>(v.pool), v.weights, v.block_table, table_stride,   \
+                 v.dst_table, dst_stride, v.n_tokens, n_items, nkv, P, bytes, slots, keep, n_parts, v.kept)
     if (hd == 64) Q4_MOVE(64);
     else if (hd == 128) Q4_MOVE(128);
     else Q4_MOVE(256);

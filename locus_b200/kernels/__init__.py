@@ -11,6 +11,7 @@ plain torch functions of the same signature to exercise the engine's host logic.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from typing import Optional, Tuple
 
@@ -1283,8 +1284,31 @@ def q4_page_bytes(head_dim: int, page_tokens: int) -> int:
     return page_tokens * (head_dim // 2 + 4)
 
 
+# The calls below are made once per layer and step, often for a few microseconds of work, so their checks are plain conditions (a message is
+# put together only when one fails) and their arguments travel as one packed record (a foreign-function call pays a tenth of a microsecond for each).
+_Q4_WRITE = struct.Struct("@7P9q")
+_Q4_EXPAND = struct.Struct("@6P7q")
+_Q4_EVICT = struct.Struct("@6P12q")
+_Q4_DECODE = struct.Struct("@15P14qd")
+_q4_entries = {}
+
+
+def _q4_entry(module: str, name: str):
+    fn = _q4_entries.get(name)
+    if fn is None:
+        fn = getattr(_lib(module), name)
+        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+        _q4_entries[name] = fn
+    return fn
+
+
+def _q4_stream(device: int):
+    return _stream_override if _stream_override is not None else torch._C._cuda_getCurrentRawStream(device)
+
+
 def _q4_here(what: str, **tensors) -> None:
-    """Tensors that lie on the current device (launches go to its current stream)."""
+    """Words what keeps these tensors from a launch on the current device."""
     here = torch.cuda.current_device() if torch.cuda.is_available() else -1
     for name, t in tensors.items():
         if t is None:
@@ -1298,23 +1322,21 @@ def _q4_here(what: str, **tensors) -> None:
 
 
 def _q4_pool(what: str, pool: torch.Tensor, n_kv_heads: int, head_dim: int, page_tokens: int, lead: int = 0) -> None:
-    _need(q4_takes(head_dim, page_tokens), f"{what}: heads of {head_dim} in pages of {page_tokens} tokens (known: heads of "
-          f"{', '.join(map(str, Q4_HEAD_DIMS))}, pages of a multiple of {Q4_PAGE_STEP})")
-    _need(pool.dtype == torch.uint8 and pool.dim() == 4 + lead
-          and tuple(pool.shape[1 + lead:]) == (2, n_kv_heads, q4_page_bytes(head_dim, page_tokens)),
-          f"{what}: the pool must be uint8 [{'layers, ' * lead}pages, 2, {n_kv_heads}, {q4_page_bytes(head_dim, page_tokens)}]")
-    _need(pool.data_ptr() % 16 == 0, f"{what}: the pool must start at a multiple of 16 bytes")
+    if head_dim not in Q4_HEAD_DIMS or page_tokens <= 0 or page_tokens % Q4_PAGE_STEP != 0:
+        raise KernelError(f"{what}: heads of {head_dim} in pages of {page_tokens} tokens (known: heads of "
+                          f"{', '.join(map(str, Q4_HEAD_DIMS))}, pages of a multiple of {Q4_PAGE_STEP})")
+    if pool.dtype is not torch.uint8 or pool.shape[1 + lead:] != (2, n_kv_heads, page_tokens * (head_dim // 2 + 4)):
+        raise KernelError(f"{what}: the pool must be uint8 [{'layers, ' * lead}pages, 2, {n_kv_heads}, {q4_page_bytes(head_dim, page_tokens)}]")
 
 
-def _q4_i32(what: str, least: int, **tensors) -> None:
-    for name, t in tensors.items():
-        _need(t.dtype == torch.int32 and t.numel() >= least, f"{what}: {name} must be int32 with at least {least} elements")
+def _q4_weights(what: str, weights: torch.Tensor, lead, n_kv_heads: int, page_tokens: int) -> None:
+    if weights.dtype is not torch.float32 or weights.shape != tuple(lead) + (n_kv_heads, page_tokens):
+        raise KernelError(f"{what}: weights must be float32 {list(lead) + [n_kv_heads, page_tokens]}")
 
 
-def _q4_weights(what: str, weights: Optional[torch.Tensor], lead, n_kv_heads: int, page_tokens: int) -> None:
-    if weights is not None:
-        _need(weights.dtype == torch.float32 and tuple(weights.shape) == tuple(lead) + (n_kv_heads, page_tokens),
-              f"{what}: weights must be float32 {list(lead) + [n_kv_heads, page_tokens]}")
+def _q4_aligned(what: str, addresses: int, step: int, names: str) -> None:
+    if addresses % step:
+        raise KernelError(f"{what}: {names} must start at multiples of {step} bytes")
 
 
 def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], q_out: torch.Tensor,
@@ -1327,21 +1349,33 @@ def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     ``weights`` float32 [n_pages, n_kv_heads, page_tokens]: set to 0 for the slots written (see :func:`attn_decode_q4`)."""
     what = "rope_kv_write_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
-    T = qkv.shape[0]
-    _need(qkv.dim() == 2 and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim, f"{what}: qkv width")
-    _need(qkv.dtype == q_out.dtype, f"{what}: qkv and q_out share one element type")
-    _need(q_out.numel() >= T * n_heads * head_dim, f"{what}: q_out is too small")
-    _need(qkv.data_ptr() % 16 == 0 and q_out.data_ptr() % 16 == 0, f"{what}: qkv and q_out must start at multiples of 16 bytes")
-    _q4_i32(what, T, positions=positions, slots=slots)
-    _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
+    T, width = qkv.shape
+    if width != (n_heads + 2 * n_kv_heads) * head_dim or n_heads <= 0:
+        raise KernelError(f"{what}: qkv width {width} for {n_heads} heads on {n_kv_heads} of {head_dim}")
+    _need(qkv.dtype is q_out.dtype, "rope_kv_write_q4: qkv and q_out share one element type")
+    _need(q_out.numel() >= T * n_heads * head_dim, "rope_kv_write_q4: q_out is too small")
+    _need(positions.dtype is torch.int32 and positions.numel() >= T, "rope_kv_write_q4: positions must be int32, one per row")
+    _need(slots.dtype is torch.int32 and slots.numel() >= T, "rope_kv_write_q4: slots must be int32, one per row")
+    if weights is not None:
+        _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
+    freq = 0
     if inv_freq is not None:
-        _need(0 <= rot_dim <= head_dim and rot_dim % 2 == 0, f"{what}: rot_dim {rot_dim} of heads of {head_dim}")
-        _need(inv_freq.dtype == torch.float32 and inv_freq.numel() == rot_dim // 2, f"{what}: inv_freq must be float32 [rot_dim / 2]")
-    _q4_here(what, qkv=qkv, positions=positions, inv_freq=inv_freq, q_out=q_out, pool=pool, slots=slots, weights=weights)
-    code = _lib("cache_q4").locus_rope_kv_write_q4(
-        _p(qkv), I(dtype_code(qkv.dtype)), _p(positions), _p(inv_freq), _p(q_out), _p(pool), _p(slots), _p(weights), I(T), I(n_heads),
-        I(n_kv_heads), I(head_dim), I(rot_dim), I(1 if interleaved else 0), I(page_tokens), I(1 if write_kv else 0), _stream())
-    _check(code, what, f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
+        _need(0 <= rot_dim <= head_dim and rot_dim % 2 == 0, "rope_kv_write_q4: rot_dim must be even and at most the heads' size")
+        _need(inv_freq.dtype is torch.float32 and inv_freq.numel() == rot_dim // 2, "rope_kv_write_q4: inv_freq must be float32 [rot_dim / 2]")
+        freq = inv_freq.data_ptr()
+    dev = qkv.get_device()
+    if not (dev >= 0 and dev == q_out.get_device() == pool.get_device() == positions.get_device() == slots.get_device()
+            and (inv_freq is None or (dev == inv_freq.get_device() and inv_freq.is_contiguous()))
+            and (weights is None or (dev == weights.get_device() and weights.is_contiguous()))
+            and qkv.is_contiguous() and q_out.is_contiguous() and pool.is_contiguous() and positions.is_contiguous() and slots.is_contiguous()
+            and dev == torch.cuda.current_device()):
+        _q4_here(what, qkv=qkv, positions=positions, inv_freq=inv_freq, q_out=q_out, pool=pool, slots=slots, weights=weights)
+    x, q, base = qkv.data_ptr(), q_out.data_ptr(), pool.data_ptr()
+    _q4_aligned(what, x | q | base, 16, "qkv, q_out and the pool")
+    code = _q4_entry("cache_q4", "locus_rope_kv_write_q4")(
+        _Q4_WRITE.pack(x, positions.data_ptr(), freq, q, base, slots.data_ptr(), 0 if weights is None else weights.data_ptr(), dtype_code(qkv.dtype), T,
+                       n_heads, n_kv_heads, head_dim, rot_dim, 1 if interleaved else 0, page_tokens, 1 if write_kv else 0), _q4_stream(dev))
+    _check(code, what, lambda: f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
 
 
 def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: torch.Tensor, n_segs: int, seg_ctx: torch.Tensor, seg_qn: torch.Tensor,
@@ -1352,16 +1386,21 @@ def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: torch.Tensor, n_se
     ``max_keys``: at least the rows of the longest of these segments."""
     what = "expand_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
-    _need(tuple(out.shape) == (pool.shape[0], 2, n_kv_heads, page_tokens, head_dim), f"{what}: out must have the pool's pages in the model's type")
-    _need(out.data_ptr() % 16 == 0, f"{what}: out must start at a multiple of 16 bytes")
-    _need(block_table.dim() == 2, f"{what}: block_table [segments, width]")
-    _q4_i32(what, n_segs, segs=segs)
-    _q4_i32(what, 0, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
-    _q4_here(what, pool=pool, out=out, segs=segs, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
-    code = _lib("cache_q4").locus_expand_q4(
-        _p(pool), _p(out), I(dtype_code(out.dtype)), _p(segs), I(n_segs), _p(seg_ctx), _p(seg_qn), _p(block_table), I(block_table.shape[1]),
-        I(n_kv_heads), I(head_dim), I(page_tokens), I(max_keys), _stream())
-    _check(code, what, f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_segs} segments of up to {max_keys} keys)")
+    _need(out.shape == (pool.shape[0], 2, n_kv_heads, page_tokens, head_dim), "expand_q4: out must have the pool's pages in the model's type")
+    _need(block_table.dtype is torch.int32 and block_table.dim() == 2, "expand_q4: block_table must be int32 [segments, width]")
+    _need(segs.dtype is torch.int32 and segs.numel() >= n_segs, "expand_q4: segs must be int32, one per segment to expand")
+    _need(seg_ctx.dtype is torch.int32 and seg_qn.dtype is torch.int32, "expand_q4: seg_ctx and seg_qn must be int32")
+    dev = pool.get_device()
+    if not (dev >= 0 and dev == out.get_device() == segs.get_device() == seg_ctx.get_device() == seg_qn.get_device() == block_table.get_device()
+            and pool.is_contiguous() and out.is_contiguous() and segs.is_contiguous() and seg_ctx.is_contiguous() and seg_qn.is_contiguous()
+            and block_table.is_contiguous() and dev == torch.cuda.current_device()):
+        _q4_here(what, pool=pool, out=out, segs=segs, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
+    base, to = pool.data_ptr(), out.data_ptr()
+    _q4_aligned(what, base | to, 16, "the pool and out")
+    code = _q4_entry("cache_q4", "locus_expand_q4")(
+        _Q4_EXPAND.pack(base, to, segs.data_ptr(), seg_ctx.data_ptr(), seg_qn.data_ptr(), block_table.data_ptr(), dtype_code(out.dtype), n_segs,
+                        block_table.shape[1], n_kv_heads, head_dim, page_tokens, max_keys), _q4_stream(dev))
+    _check(code, what, lambda: f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_segs} segments of up to {max_keys} keys)")
 
 
 def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Tensor, n_tokens: torch.Tensor, n_items: int, keep: int,
@@ -1378,29 +1417,39 @@ def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Te
     ``max_tokens``: at least the tokens of the longest request."""
     what = "evict_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens, 1)
-    _q4_weights(what, weights, pool.shape[:2], n_kv_heads, page_tokens)
-    _need(keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep, f"{what}: keep {keep} with the first {first} and the last {recent}")
-    _need(block_table.dim() == 2 and block_table.shape[0] >= n_items, f"{what}: block_table [requests, width]")
-    _need(kept.dtype == torch.int32 and tuple(kept.shape) == (pool.shape[0], n_items, n_kv_heads, keep), f"{what}: kept must be int32 [layers, requests, kv heads, keep]")
-    _q4_i32(what, n_items, n_tokens=n_tokens)
-    _q4_i32(what, 0, block_table=block_table)
-    _need(0 < max_tokens <= block_table.shape[1] * page_tokens, f"{what}: max_tokens {max_tokens} beyond what block_table describes")
+    layers, pages = pool.shape[:2]
+    _q4_weights(what, weights, (layers, pages), n_kv_heads, page_tokens)
+    if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+        raise KernelError(f"{what}: keep {keep} with the first {first} and the last {recent}")
+    _need(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= n_items, "evict_q4: block_table must be int32 [requests, width]")
+    _need(n_tokens.dtype is torch.int32 and n_tokens.numel() >= n_items, "evict_q4: n_tokens must be int32, one per request")
+    if kept.dtype is not torch.int32 or kept.shape != (layers, n_items, n_kv_heads, keep):
+        raise KernelError(f"{what}: kept must be int32 {[layers, n_items, n_kv_heads, keep]}")
+    width = block_table.shape[1]
+    if not 0 < max_tokens <= width * page_tokens:
+        raise KernelError(f"{what}: max_tokens {max_tokens} beyond what block_table describes")
     to = block_table if dst_table is None else dst_table
     if dst_table is not None:
-        _q4_i32(what, 0, dst_table=dst_table)
-        _need(dst_table.dim() == 2 and dst_table.shape[0] >= n_items and dst_table.shape[1] * page_tokens >= min(keep, max_tokens),
-              f"{what}: dst_table [requests, pages for the keys that stay]")
-    _q4_here(what, pool=pool, weights=weights, block_table=block_table, n_tokens=n_tokens, kept=kept, dst_table=dst_table)
-    code = _lib("cache_q4").locus_evict_q4(
-        _p(pool), _p(weights), _p(block_table), I(block_table.shape[1]), _p(to), I(to.shape[1]), _p(n_tokens), I(n_items), I(pool.shape[0]),
-        LL(pool.shape[1]), I(n_kv_heads), I(head_dim), I(page_tokens), I(keep), I(first), I(recent), I(max_tokens), _p(kept), _stream())
+        _need(to.dtype is torch.int32 and to.dim() == 2 and to.shape[0] >= n_items and to.shape[1] * page_tokens >= min(keep, max_tokens),
+              "evict_q4: dst_table must be int32 [requests, pages for the keys that stay]")
+    dev = pool.get_device()
+    if not (dev >= 0 and dev == weights.get_device() == block_table.get_device() == to.get_device() == n_tokens.get_device() == kept.get_device()
+            and pool.is_contiguous() and weights.is_contiguous() and block_table.is_contiguous() and to.is_contiguous() and n_tokens.is_contiguous()
+            and kept.is_contiguous() and dev == torch.cuda.current_device()):
+        _q4_here(what, pool=pool, weights=weights, block_table=block_table, n_tokens=n_tokens, kept=kept, dst_table=dst_table)
+    base = pool.data_ptr()
+    _q4_aligned(what, base, 16, "the pool")
+    code = _q4_entry("cache_q4", "locus_evict_q4")(
+        _Q4_EVICT.pack(base, weights.data_ptr(), block_table.data_ptr(), to.data_ptr(), n_tokens.data_ptr(), kept.data_ptr(), width, to.shape[1],
+                       n_items, layers, pages, n_kv_heads, head_dim, page_tokens, keep, first, recent, max_tokens), _q4_stream(dev))
     if code == 0:
         _count_launches(1)
-    _check(code, what, f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_items} requests, keep {keep})")
+    _check(code, what, lambda: f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_items} requests, keep {keep})")
 
 
-# The range cut's cost model of the 4-bit kernel, in keys (see GQA_COST_RANGE).
-Q4_COST_RANGE, Q4_COST_MERGE_PER_HEAD = 64, 2
+# The range cut's cost model of the 4-bit kernel, in keys: the fixed cost of a range, and of one more partial result (a block's) of the longest
+# request (csrc/attention_q4.cu: plan_ranges).
+Q4_COST_RANGE, Q4_COST_MERGE = 64, 16
 Q4_MAX_ITEMS = 1024
 
 
@@ -1435,36 +1484,60 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
     n_items * n_heads * block_table.shape[1] * page_tokens elements."""
     what = "attn_decode_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
-    _need(n_heads > 0 and n_heads % n_kv_heads == 0, f"{what}: {n_heads} heads are not a multiple of {n_kv_heads} kv heads")
-    _need(q.dtype == out.dtype and q.numel() % (n_heads * head_dim) == 0 and out.numel() % (n_heads * head_dim) == 0,
-          f"{what}: q and out must be rows of {n_heads} heads of {head_dim}, of one element type")
-    _need(q.data_ptr() % 16 == 0 and part_o.data_ptr() % 16 == 0 and part_ml.data_ptr() % 8 == 0, f"{what}: q and the scratch must start at multiples of 16 bytes")
-    _need(block_table.dim() == 2, f"{what}: block_table [segments, width]")
-    _need(n_items <= Q4_MAX_ITEMS, f"{what}: {n_items} requests (at most {Q4_MAX_ITEMS})")
-    _q4_i32(what, n_items, items=items)
-    _q4_i32(what, n_items * n_heads, counters=counters)
-    _q4_i32(what, 0, seg_q0=seg_q0, seg_ctx=seg_ctx, block_table=block_table)
-    _need(part_o.dtype == torch.float32 and part_ml.dtype == torch.float32, f"{what}: float32 scratch")
-    lse, floats = None, part_o.numel()
+    if n_heads <= 0 or n_heads % n_kv_heads:
+        raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv_heads} kv heads")
+    width = n_heads * head_dim
+    _need(q.dtype is out.dtype and q.numel() % width == 0 and out.numel() % width == 0, "attn_decode_q4: q and out must be rows of whole heads, of one element type")
+    _need(block_table.dtype is torch.int32 and block_table.dim() == 2, "attn_decode_q4: block_table must be int32 [segments, width]")
+    pages = block_table.shape[1]
+    _need(n_items <= Q4_MAX_ITEMS, "attn_decode_q4: at most 1024 requests")
+    _need(items.dtype is torch.int32 and items.numel() >= n_items, "attn_decode_q4: items must be int32, one per request")
+    _need(counters.dtype is torch.int32 and counters.numel() >= n_items * n_heads, "attn_decode_q4: counters must be int32 [n_items * n_heads]")
+    _need(seg_q0.dtype is torch.int32 and seg_ctx.dtype is torch.int32, "attn_decode_q4: seg_q0 and seg_ctx must be int32")
+    _need(part_o.dtype is torch.float32 and part_ml.dtype is torch.float32, "attn_decode_q4: float32 scratch")
+    floats, part, to, at, lse = part_o.numel(), part_o.data_ptr(), 0, 0, 0
     if weights is not None:
         _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
-        _need(window == 0 and chunk == 0, f"{what}: weights go with neither a window nor chunks")
-        _need(scores is not None and scores.dtype == torch.float32 and scores.numel() >= n_items * n_heads * block_table.shape[1] * page_tokens,
-              f"{what}: scores too small for weights")
+        _need(window == 0 and chunk == 0, "attn_decode_q4: weights go with neither a window nor chunks")
+        _need(scores is not None and scores.dtype is torch.float32 and scores.numel() >= n_items * n_heads * pages * page_tokens,
+              "attn_decode_q4: scores too small for weights")
         floats = max(0, (floats - 2 * n_items * n_heads) // 4 * 4)   # a head's maximum and denominator lie behind the partial results
-        lse = part_o.view(-1)[floats:]
+        to, at, lse = weights.data_ptr(), scores.data_ptr(), part + 4 * floats
     max_units = min(floats // head_dim, part_ml.numel() // 2)
-    _need(max_units >= n_items * n_heads * (2 if keep_first > 0 and window > 0 else 1), f"{what}: scratch too small")
-    _q4_here(what, q=q, pool=pool, out=out, seg_q0=seg_q0, seg_ctx=seg_ctx, block_table=block_table, items=items, part_o=part_o, part_ml=part_ml,
-             counters=counters, slopes=slopes, weights=weights, scores=scores)
-    code = _lib("attention_q4").locus_attn_decode_q4(
-        _p(q), I(dtype_code(q.dtype)), _p(pool), _p(out), _p(seg_q0), _p(seg_ctx), _p(block_table), I(block_table.shape[1]), _p(items), I(n_items),
-        I(n_heads), I(n_kv_heads), I(head_dim), I(page_tokens), I(window), I(chunk), F(scale), _p(part_o), _p(part_ml), _p(counters),
-        LL(max_units), I(Q4_COST_RANGE), I(Q4_COST_MERGE_PER_HEAD * (n_heads // n_kv_heads)), I(keep_first if window > 0 else 0),
-        *_sink_args(sink, n_heads), _slopes_arg(slopes, n_heads), _p(weights), _p(scores if weights is not None else None), _p(lse), _stream())
-    if weights is not None and code == 0 and n_items > 0:
+    _need(max_units >= n_items * n_heads * (2 if keep_first > 0 and window > 0 else 1), "attn_decode_q4: scratch too small")
+    sink_flag, sink_at, slopes_at = 0, 0, 0
+    if sink is not False:
+        if isinstance(sink, torch.Tensor):
+            _sink_args(sink, n_heads)
+            sink_at = sink.data_ptr()
+            sink_flag = 1
+        else:
+            sink_flag = 1 if sink else 0
+    if slopes is not None:
+        _slopes_arg(slopes, n_heads)
+        slopes_at = slopes.data_ptr()
+    dev = q.get_device()
+    if not (dev >= 0 and dev == pool.get_device() == out.get_device() == seg_q0.get_device() == seg_ctx.get_device() == block_table.get_device()
+            == items.get_device() == part_o.get_device() == part_ml.get_device() == counters.get_device()
+            and q.is_contiguous() and pool.is_contiguous() and out.is_contiguous() and seg_q0.is_contiguous() and seg_ctx.is_contiguous()
+            and block_table.is_contiguous() and items.is_contiguous() and part_o.is_contiguous() and part_ml.is_contiguous()
+            and counters.is_contiguous() and (weights is None or (dev == weights.get_device() == scores.get_device()
+                                                                  and weights.is_contiguous() and scores.is_contiguous()))
+            and (sink_at == 0 or dev == sink.get_device()) and (slopes is None or dev == slopes.get_device())
+            and dev == torch.cuda.current_device()):
+        _q4_here(what, q=q, pool=pool, out=out, seg_q0=seg_q0, seg_ctx=seg_ctx, block_table=block_table, items=items, part_o=part_o, part_ml=part_ml,
+                 counters=counters, slopes=slopes, weights=weights, scores=scores, sink=sink if sink_at else None)
+    qp, base, ml = q.data_ptr(), pool.data_ptr(), part_ml.data_ptr()
+    _q4_aligned(what, qp | base | part, 16, "q, the pool and part_o")
+    _q4_aligned(what, ml, 8, "part_ml")
+    code = _q4_entry("attention_q4", "locus_attn_decode_q4")(
+        _Q4_DECODE.pack(qp, base, out.data_ptr(), seg_q0.data_ptr(), seg_ctx.data_ptr(), block_table.data_ptr(), items.data_ptr(), part, ml,
+                        counters.data_ptr(), sink_at, slopes_at, to, at, lse, dtype_code(q.dtype), pages, n_items, n_heads, n_kv_heads, head_dim,
+                        page_tokens, window, chunk, max_units, Q4_COST_RANGE, Q4_COST_MERGE, keep_first if window > 0 else 0, sink_flag, scale),
+        _q4_stream(dev))
+    if to and code == 0 and n_items > 0:
         _count_launches(1)
-    _check(code, what, f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
+    _check(code, what, lambda: f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
 
 
 SCORE_FUNCTIONS = {"softmax": 0, "sigmoid": 1}
