@@ -2,28 +2,28 @@
 //
 //   o_h = sum_t p_t v_t   p = softmax over the keys in sight of scale * q_h . k_t (a sink, a distance bias: as in attention.cu)
 //
-// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5), so
+// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5) = z + scale (code - 7), z = mid - scale / 2, and codes less 7 are
+// small whole numbers that float16 holds exactly, so
 //
-//   q . k_t = scale_t (q . code_t) + (mid_t - 7.5 scale_t) sum(q)
-//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t (mid_t - scale_t / 2)
+//   q . k_t = scale_t (q . (code_t - 7)) + z_t sum(q)                      the product on the tensor cores, the rest per score in float32
+//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t z_t             the same for the values
 //
-// with the two products on the tensor cores and the rest in float32.  The tensor cores' operands are float16:
-//   * codes as they are: a nibble n in the low bits of a 16-bit half is the float16 n 2^-24 (a subnormal number, which the tensor cores take like any
-//     other), and n in the next four bits 16 n 2^-24, so that one AND unpacks two codes; the powers of two go into the other operand or out
-//     of the sums.  (Whole numbers by the usual or with 1024 and a subtraction behind it: twice the instructions.)
-//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15: a bfloat16 element loses bits only if it is 2^-25 of the
-//     largest, and then at most 2^-36 of that; a float32 q goes in as two parts, 22 bits and more;
+// The tensor cores' operands are float16:
+//   * codes less 7: a nibble n under the exponent of 1024 is 1024 + n, in the next four bits 1024 + 16 n, and one addition or multiply-add (two
+//     codes an instruction) leaves n - 7.  (A nibble alone is the subnormal number n 2^-24 and would need neither, but the tensor cores align what
+//     they add by the operands' exponent fields: sums of such products were off by 1e-4.  The 7 is taken off the codes rather than out of the
+//     sums, where it would grow over the keys and lose what cancels.)
+//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
+//     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more;
 //   * the weights p_t scale_t, formed relative to the running maximum M of score + exponent of scale, so that they stay below 2^15, whatever the
 //     scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest where that is more; two parts for a float32 model).  The
-//     unrounded p_t enter the denominator and the second sum.
-// The values' 7 is taken off inside the sums, by a product of the same weights with a constant: sums of codes of one sign would grow over the keys
-// and lose what cancels in them.  (In a score, a sum over one head's dimensions, the codes' mean costs one bit.)
+//     unrounded p_t enter the denominator and z's sum.
 // For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
 // over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
 // A warp takes a range of keys of one (request, key/value head) for up to 16 query heads that share it, in the transposed form (16 keys in the M
 // dimension of mma.sync m16n8k16, eight heads in N):
-//   S^T [16 keys x 8 heads] = C_k [16 x hd] . Q^T           a lane's words of a key row hold eight codes each, two neighbouring dimensions in a
+//   S^T [16 keys x 8 heads] = (C_k - 7) [16 x hd] . Q^T     a lane's words of a key row hold eight codes each, two neighbouring dimensions in a
 //                             register's halves as the A fragment wants them;
 //   O^T [hd x 8 heads] += (C_v - 7)^T [hd x 16 keys] . P^T  the A fragment wants one dimension of two keys in a register: a byte permute joins
 //                             the same byte of two keys' words, and its two nibbles are two dimensions (two row tiles' halves).
@@ -31,13 +31,12 @@
 // M is raised only when a score exceeds it by more than 2^4: until then the weights are formed relative to the old one, which saves the exchange
 // between lanes and the correction of the sums in nearly every chunk.
 //
-// The cut: every (request, key/value head) is cut into ranges of one length (plan_ranges), and the units (request, head, range), in this order, are
-// dealt to the blocks by runs of as many as a block has warps.  The warps of a block that have ranges of one (request, head) join them in shared
-// memory; what covers it whole is the output, else the block leaves one partial result, and the block that is the last to do so joins those, in
-// ascending order.  (With one partial result per warp, joined by the last warp, a request of 131,000 tokens took 270 us, most of it in that.)
+// The cut: every (request, key/value head) is cut into ranges of one length, a warp each (plan_ranges).  The warps of a block that have ranges of
+// one (request, head) join them in shared memory; what covers it whole is the output, else the block leaves one partial result, and the block that
+// is the last to do so joins those, in ascending order.  (With one partial result per warp, joined by the last warp, a request of 131,000 tokens took 270 us, most of it in that.)
 //
-// Memory: a warp's ring in shared memory is filled by bulk copies of up to 64 keys of one page: codes and factors of K, then of V.  (A whole
-// page of 64 tokens is one run of bytes per plane.)  Every wait is bounded: when the limit runs out the warp records it in the module's error
+// Memory: a warp's ring in shared memory is filled by bulk copies, up to 64 keys at a time: codes and factors of K, then of V.  (A whole page of
+// 64 tokens is one run of bytes per plane; of other pages a lane each asks for the codes and the factors.)  Every wait is bounded: when the limit runs out the warp records it in the module's error
 // word, waits for its other copies with the same limit and goes on to the end without a further copy.
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
@@ -69,7 +68,7 @@ struct Q4Args {
     float* part_ml;           // [ranges * nh][2]
     int* counters;            // [n_items * nh], zero between launches
     float* scores;            // with weights: [n_items][nkv][table_stride * P][heads of a group], in base 2
-    float* lse;               // with weights: [n_items * nh][2], a head's maximum and denominator
+    float* lse;               // with weights: [n_items * nh][2], what a head's weights are relative to, and 1 / denominator
 };
 
 #define Q4_WAIT_LIMIT 2000000000LL   // cycles a warp waits for a copy before it gives up (about a second)
@@ -155,6 +154,15 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+// the codes in bits 0 .. 3 of a register's halves, less 7: 0x6400 | n is 1024 + n
+__device__ __forceinline__ uint32_t codes_low(uint32_t x) {
+    return bits(__hsub2(halves((x & 0x000f000fu) | 0x64006400u), halves(0x64076407u)));
+}
+// the codes in bits 4 .. 7: (1024 + 16 n) / 16 - 71
+__device__ __forceinline__ uint32_t codes_high(uint32_t x) {
+    return bits(__hfma2(halves((x & 0x00f000f0u) | 0x64006400u), halves(0x2c002c00u), halves(0xd470d470u)));
+}
 // a pair of values as PARTS pairs of float16: one, rounded, or two
 template <int PARTS>
 __device__ __forceinline__ void split2(float a, float b, uint32_t* out) {
@@ -184,19 +192,21 @@ __device__ __forceinline__ void load8(const bf16* p, float* v) {
 // ---------------------------------------------------------------------------
 // The cut of a step's keys into ranges.
 #define Q4_MAX_ITEMS 1024
-#define Q4_CAND 256       // candidate range lengths looked at
+#define Q4_CAND 128       // candidate range lengths looked at
 
 struct Q4Plan {
-    int first[Q4_MAX_ITEMS];     // first key of item i, rounded down to 16
-    int pos[Q4_MAX_ITEMS];       // position of its query
+    int pos[Q4_MAX_ITEMS];       // position of item i's query
     int seg[Q4_MAX_ITEMS];
     int row[Q4_MAX_ITEMS];       // row of q / out
     int pref[Q4_MAX_ITEMS + 1];  // ranges of the items before i
+    int block_pref[Q4_MAX_ITEMS + 1];   // not packed: block-loads of the items before i
     unsigned long long best[32];
-    int longest[32], total[32];
-    int len;
+    int longest[32], total[32], blocks_of[32];
+    int len, packed, n_blocks;
 };
 
+// first key that a query at position p sees (besides kept first tokens), rounded down to 16
+__device__ __forceinline__ int q4_first(const Q4Args& a, int p) { return first_key(a.window, a.chunk, p) & ~15; }
 // kept first tokens of an item that lie in front of its window's first chunk: a range of their own, the item's first
 __device__ __forceinline__ int q4_kept(const Q4Args& a, int first) { return a.window > 0 ? min(a.keep_first, first) : 0; }
 // Ranges of `n` keys at a length of about len (inv its reciprocal).  By a product, which may be one more than need be; the same everywhere.
@@ -207,23 +217,36 @@ __device__ __forceinline__ int q4_length(int n, int ranges) {
     const int step = even >= 512 ? 64 : even >= 128 ? 32 : 16;
     return (even + step - 1) / step * step;
 }
+// Blocks of W warps that an item of `ranges` ranges takes when no block holds parts of a (request, head) that another one holds parts of, unless
+// it has more ranges than a block warps.  table[r], r 1 .. W: for r ranges.
+template <int W>
+__device__ __forceinline__ int q4_blocks(const int* table, int ranges, int n_vh) {
+    return ranges > W ? n_vh * ((ranges + W - 1) / W) : table[ranges];
+}
 
 // Fills the plan (all threads of the block; ends with a barrier) and returns the length, 0 when not even one range per item fits max_ranges.
-// The length is the one of Q4_CAND with the least cost: rounds over the grid's warps x (length + cost_range) + cost_merge per partial result of
-// the longest item.  Candidates lie 1.45 % apart from a quarter of what fills every warp once to ten times that; the last one is the longest item's.
-__device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int n_warps, int block_warps,
-                                           int cost_range, int cost_merge) {
+// Two ways to deal the units to blocks, for each of Q4_CAND lengths: `packed`, unit after unit, W to a block, and by whole blocks (q4_blocks), where
+// some warps may have nothing to do but fewer (request, head)s are joined across blocks.  The cost of a cut, in keys: rounds over the grid x
+// (length + cost_range), and cost_join once where blocks join, and cost_merge per partial result of the longest item.  Lengths
+// from what fills every warp once, 2 % apart, some shorter and longer ones, and the longest item's.
+// (8 requests of 4,096 keys on 16 heads: twelve ranges, a block each, 24.5 us; thirteen, unit after unit, 29.5.)
+template <int W>
+__device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int cost_range, int cost_join,
+                                           int cost_merge) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int longest = 1, total = 0;
-    for (int i = tid; i < n_items; i += blockDim.x) {
-        const int seg = a.items[i], p = a.seg_ctx[seg];
-        const int first = first_key(a.window, a.chunk, p) & ~15;
-        pl.row[i] = a.seg_q0[seg];
-        pl.first[i] = first;
+    for (int i = tid; i < n_items; i += 32 * W) {
+        const int seg = a.items[i], p = a.seg_ctx[seg], row = a.seg_q0[seg];
+        const int first = q4_first(a, p);
+        pl.row[i] = row;
         pl.pos[i] = p;
         pl.seg[i] = seg;
         longest = max(longest, p + 1 - first);
         total += p + 1 - first;
+    }
+    if (tid >= 1 && tid <= W) {
+        const int heads = W / tid;   // (request, head)s of tid ranges that a block holds
+        pl.blocks_of[tid] = (n_vh + heads - 1) / heads;
     }
     longest = __reduce_max_sync(0xffffffffu, longest);
     total = __reduce_add_sync(0xffffffffu, total);
@@ -232,68 +255,146 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
         pl.total[warp] = total;
     }
     __syncthreads();
-    longest = __reduce_max_sync(0xffffffffu, lane < block_warps ? pl.longest[lane] : 1);
-    total = __reduce_add_sync(0xffffffffu, lane < block_warps ? pl.total[lane] : 0);
+    longest = __reduce_max_sync(0xffffffffu, lane < W ? pl.longest[lane] : 1);
+    total = __reduce_add_sync(0xffffffffu, lane < W ? pl.total[lane] : 0);
+    const int n_warps = gridDim.x * W;
     const float fill = static_cast<float>(total) * static_cast<float>(n_vh) / static_cast<float>(n_warps);
     auto length = [&](int c) {
         if (c == Q4_CAND - 1) return (longest + 15) & ~15;
-        return 16 * max(1, static_cast<int>(fminf(fill * exp2f(static_cast<float>(c - 96) * (1.f / 48.f)), 1e8f) * (1.f / 16.f) + 0.5f));
+        const float x = static_cast<float>(c);
+        const float times = c < 100 ? 1.f + 0.02f * x : c < 108 ? 0.12f * (x - 99.f) : 3.f + 0.1f * (x - 107.f) * (x - 107.f);
+        return 16 * max(1, static_cast<int>(fminf(fill * times, 1e8f) * (1.f / 16.f) + 0.5f));
+    };
+    const bool kept_ranges = a.window > 0 && a.keep_first > 0;
+    auto ranges_of = [&](int i, int len, float inv) {
+        const int p = pl.pos[i], first = q4_first(a, p);
+        return q4_ranges(p + 1 - first, len, inv) + (kept_ranges && q4_kept(a, first) > 0);
     };
     unsigned long long best = ~0ull;
-    for (int c = tid; c < Q4_CAND; c += blockDim.x) {
+    const float grid_inv = 1.f / static_cast<float>(gridDim.x);
+    for (int c = tid; c < Q4_CAND; c += 32 * W) {
         const int len = length(c);
         const float inv = 1.f / static_cast<float>(len);
-        int ranges = 0;
+        int ranges = 0, blocks = 0;
 #pragma unroll 4
-        for (int i = 0; i < n_items; ++i) ranges += q4_ranges(pl.pos[i] + 1 - pl.first[i], len, inv);
-        if (a.window > 0 && a.keep_first > 0)
-            for (int i = 0; i < n_items; ++i) ranges += q4_kept(a, pl.first[i]) > 0;
+        for (int i = 0; i < n_items; ++i) {
+            const int r = ranges_of(i, len, inv);
+            ranges += r;
+            blocks += q4_blocks<W>(pl.blocks_of, r, n_vh);
+        }
         if (ranges > max_ranges) continue;  // the scratch does not hold that many partial results
-        const unsigned rounds = (static_cast<unsigned>(ranges) * n_vh + n_warps - 1) / n_warps;
-        const int most = min(len, longest);
-        const unsigned long long cost = static_cast<unsigned long long>(rounds) * (most + cost_range) +
-                                        static_cast<unsigned long long>(cost_merge) * ((longest + len - 1) / len / block_warps);
-        best = min(best, (cost << 24) | static_cast<unsigned>(c));  // ties: the shorter range
+        const int most = min(len, longest) + cost_range, merge = cost_merge * (static_cast<int>(static_cast<float>(longest) * inv) / W);
+        auto consider = [&](int loads, bool joins, int packed) {
+            const int rounds = static_cast<int>((static_cast<float>(loads) + static_cast<float>(gridDim.x - 1)) * grid_inv);
+            const unsigned long long cost = static_cast<unsigned long long>(rounds) * most + merge + (joins ? cost_join : 0);
+            best = min(best, (cost << 24) | static_cast<unsigned>(2 * c + packed));  // ties: the shorter range
+        };
+        consider(blocks, longest > len * W, 0);
+        consider((ranges * n_vh + W - 1) / W, ranges > n_items, 1);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) pl.best[warp] = best;
     __syncthreads();
     if (warp == 0) {
-        unsigned long long b = lane < block_warps ? pl.best[lane] : ~0ull;
+        unsigned long long b = lane < W ? pl.best[lane] : ~0ull;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) b = min(b, __shfl_xor_sync(0xffffffffu, b, o));
-        const int len = b == ~0ull ? 0 : length(static_cast<int>(b & 0xffffff));
+        const int c = static_cast<int>(b & 0xffffff), len = b == ~0ull ? 0 : length(c >> 1);
         const float inv = len ? 1.f / static_cast<float>(len) : 0.f;
-        int acc = 0;
+        int acc = 0, acc_blocks = 0;
         for (int i0 = 0; i0 < n_items; i0 += 32) {
             const int i = i0 + lane;
-            int mine = 0;
+            int mine = 0, mine_blocks = 0;
             if (i < n_items && len) {
-                const int first = pl.first[i];
-                mine = q4_ranges(pl.pos[i] + 1 - first, len, inv) + (q4_kept(a, first) > 0);
+                mine = ranges_of(i, len, inv);
+                if (!(c & 1)) mine_blocks = q4_blocks<W>(pl.blocks_of, mine, n_vh);
             }
-            int run = mine;
+            int run = mine, run_blocks = mine_blocks;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += v;
+                const int v = __shfl_up_sync(0xffffffffu, run, o), w = __shfl_up_sync(0xffffffffu, run_blocks, o);
+                if (lane >= o) {
+                    run += v;
+                    run_blocks += w;
+                }
             }
-            if (i < n_items) pl.pref[i] = acc + run - mine;
+            if (i < n_items) {
+                pl.pref[i] = acc + run - mine;
+                pl.block_pref[i] = acc_blocks + run_blocks - mine_blocks;
+            }
             acc += __shfl_sync(0xffffffffu, run, 31);
+            acc_blocks += __shfl_sync(0xffffffffu, run_blocks, 31);
         }
         if (lane == 0) {
             pl.pref[n_items] = acc;
+            pl.block_pref[n_items] = acc_blocks;
             pl.len = len;
+            pl.packed = c & 1;
+            pl.n_blocks = c & 1 ? (acc * n_vh + W - 1) / W : acc_blocks;
         }
     }
     __syncthreads();
     return pl.len;
 }
 
-// T: the model's type.  HD: head size.  HT: tiles of eight heads per warp.  W warps of a block, S stages of SK keys in flight per warp.
-template <typename T, int HD, int HT, int W, int S, int SK, bool WEIGH>
-__global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int n_items, long long max_units, int cost_range, int cost_merge) {
+// What warp `warp` of block-load `load` (of plan.n_blocks) does.
+struct Q4Unit {
+    bool active;
+    int item, vh, range, n_ranges;   // range of the item's n_ranges
+    int wa, wb;                       // the warps of the block that have ranges of the same (item, head)
+    int parts;                        // blocks that have some
+    int lead;                         // packed: ranges of this (item, head) that its first block has
+};
+template <int W>
+__device__ __forceinline__ Q4Unit q4_unit(const Q4Plan& pl, int load, int warp, int n_items, int n_vh) {
+    Q4Unit u;
+    const int at = pl.packed ? load * W + warp : load;
+    auto begin = [&](int i) { return pl.packed ? pl.pref[i] * n_vh : pl.block_pref[i]; };
+    int item = 0, hi = n_items;   // the last item that begins at or in front of `at`
+    while (hi - item > 1) {
+        const int mid = (item + hi) >> 1;
+        if (begin(mid) <= at) item = mid;
+        else hi = mid;
+    }
+    u.item = item;
+    u.n_ranges = pl.pref[item + 1] - pl.pref[item];
+    const int k = at - begin(item), nr = u.n_ranges;
+    if (pl.packed) {
+        const int left = pl.pref[n_items] * n_vh - load * W;   // units from this block's first on
+        u.active = warp < left;
+        u.vh = k / nr;
+        u.range = k - u.vh * nr;
+        const int u0 = at - u.range;                            // the (item, head)'s first unit
+        u.wa = max(0, warp - u.range);
+        u.wb = min(min(W, left), warp - u.range + nr);
+        u.parts = (u0 + nr - 1) / W - u0 / W + 1;
+        u.lead = W - u0 % W;
+    } else if (nr > W) {
+        const int loads = (nr + W - 1) / W;
+        u.vh = k / loads;
+        u.range = (k - u.vh * loads) * W + warp;
+        u.active = u.range < nr;
+        u.wa = 0;
+        u.wb = min(W, nr - (u.range - warp));
+        u.parts = loads;
+        u.lead = W;
+    } else {
+        const int heads = W / nr, h = warp / nr;
+        u.vh = k * heads + h;
+        u.range = warp - h * nr;
+        u.active = h < heads && u.vh < n_vh;
+        u.wa = h * nr;
+        u.wb = u.wa + nr;
+        u.parts = 1;
+        u.lead = W;
+    }
+    return u;
+}
+
+// T: the model's type.  HD: head size.  HT: tiles of eight heads per warp.  N: chunks of 16 keys at a time.  W warps of a block, S stages of SK keys in flight per warp.
+template <typename T, int HD, int HT, int N, int W, int S, int SK, bool WEIGH>
+__global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int n_items, long long max_units, int cost_range, int cost_join, int cost_merge) {
     pdl_trigger();  // every block of this grid is resident from the start
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     constexpr int KW = HD / 32;      // words of a lane per key row (keys): HD / 4 dimensions
@@ -328,11 +429,10 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     __syncwarp();
     uint32_t parity = 0;  // bit i: the phase of stage i's barrier that the next wait on it looks for
     bool ok = true;
-    const int len = plan_ranges(pl, a, n_items, n_vh, max_units / a.nh, gridDim.x * W, W, cost_range, cost_merge);
+    const int len = plan_ranges<W>(pl, a, n_items, n_vh, max_units / a.nh, cost_range, cost_join, cost_merge);
     // (the cut read only the step's descriptors; q and the newest rows come from the kernel in front)
     pdl_entry();
     if (len == 0) return;
-    const int n_units = pl.pref[n_items] * n_vh;
     const float qscale = a.scale * 1.4426950408889634f;  // scores in base 2
     const size_t plane_step = static_cast<size_t>(a.nkv) * P * (RB + Q4_FACTOR_BYTES);
     const uint32_t ring = smem_u32(q4_smem) + warp * (S * STAGE);
@@ -342,29 +442,15 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     float* const res0 = reinterpret_cast<float*>(q4_smem);
     constexpr int RES_STEP = S * STAGE / 4;   // floats from a warp's result to the next one's
 
-    for (int base = blockIdx.x * W; base < n_units; base += gridDim.x * W) {
-        const int u = base + warp;
-        const bool active = u < n_units;
-        // the unit: item, (virtual) head, range
-        int item = 0;
-        if (active) {
-            int hi = n_items;   // the last item whose units begin at or in front of u
-            while (hi - item > 1) {
-                const int mid = (item + hi) >> 1;
-                if (pl.pref[mid] * n_vh <= u) item = mid;
-                else hi = mid;
-            }
-        }
-        const int r0 = pl.pref[item], n_ranges = pl.pref[item + 1] - r0;
-        const int v = active ? u - r0 * n_vh : 0;
-        const int vh = v / n_ranges, range = v % n_ranges;
+    for (int load = blockIdx.x; load < pl.n_blocks; load += gridDim.x) {
+        const Q4Unit un = q4_unit<W>(pl, load, warp, n_items, n_vh);
+        const bool active = un.active;
+        const int item = un.item, vh = un.vh, range = un.range, n_ranges = un.n_ranges, wa = un.wa, wb = un.wb;
         const int kvh = vh / n_sub, g0 = (vh % n_sub) * 8 * HT;
         const int nG = min(G - g0, 8 * HT), h0 = kvh * G + g0;   // this warp's heads: h0 .. h0 + nG - 1
-        const int seg = pl.seg[item], p = pl.pos[item], first = pl.first[item];
+        const int seg = pl.seg[item], p = pl.pos[item], first = q4_first(a, p), r0 = pl.pref[item];
         const int row = pl.row[item];
-        // the warps of this block that have ranges of the same (item, head): wa .. wb - 1
-        const int wa = max(0, warp - range), wb = min(min(W, n_units - base), warp - range + n_ranges);
-        const bool whole = wa == warp - range && wb - wa == n_ranges;
+        const bool whole = un.parts == 1;
 
         if (active) {
             const int keep = a.keep_first, kept = q4_kept(a, first);
@@ -376,45 +462,56 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             const int k_end = kept_range ? kept : min(p + 1, k_begin + length);                         // exclusive
             const int* table = a.block_table + static_cast<size_t>(seg) * a.table_stride;
 
-            // keys k0 .. end - 1 of one page into a stage of the ring.  (Every chunk holds a live key, so its page is the request's: the first
-            // of a window's ranges begins with the chunk of the window's first key, and kept tokens in front of that are a range of their own.)
+            // A stage of the ring: the keys of one run of SK, counted from position 0, that lie in the range.  (Every chunk holds a live key, so
+            // its page is the request's: the first of a window's ranges begins with the chunk of the window's first key, and kept tokens in front
+            // of that are a range of their own.)
             const int k_stop = k_begin < k_end ? (k_end + 15) & ~15 : k_begin;
             const uint8_t* const pool_head = a.pool + q4_place(0, 0, kvh, a.nkv, P, HD);
-            int k0 = k_begin, k_next = k_begin;   // first key that is not read yet; that is not asked for yet
-            int page_at = k_begin / P;            // page of k_next, and where it and the page of k0 end
-            int end_next = (page_at + 1) * P, end_read = end_next;
-            // the next stage: keys k_next .. of one page
+            int k0 = k_begin, k_next = k_begin;                          // first key that is not read yet; that is not asked for yet
+            int page_at = k_begin / P, end_next = (page_at + 1) * P;     // page of k_next, and where it ends
+            // the ids of 32 pages from page_from on, one a lane (looked up one by one, each lookup would stand in front of its copy)
+            const int last_page = k_begin < k_stop ? (k_stop - 1) / P : 0;
+            int page_from = page_at, page_ids = table[min(page_from + lane, last_page)];
+            auto stage_end = [&](int k) { return min((k / SK + 1) * SK, k_stop); };
             auto issue = [&](int st) {
-                const int end = min(min(end_next, k_next + SK), k_stop);
+                constexpr int MOST = SK / 16;   // pages of a stage
+                const int end = stage_end(k_next), n = end - k_next;
+                if (page_at - page_from > 32 - MOST) {
+                    page_from = page_at;
+                    page_ids = table[min(page_from + lane, last_page)];
+                }
+                const int page = __shfl_sync(0xffffffffu, page_ids, (page_at - page_from + lane) & 31);
+                const uint32_t dst = ring + st * STAGE, bar = bars + 8 * st;
                 if (lane == 0) {
-                    const int n = end - k_next, off = k_next - (end_next - P);
-                    const uint8_t* src = pool_head + table[page_at] * (2 * plane_step);
-                    const uint32_t dst = ring + st * STAGE, bar = bars + 8 * st;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the reads of what lies there
                     mbar_expect_tx(bar, 2 * n * (RB + Q4_FACTOR_BYTES));
                     if (n == SK && P == SK) {
+                        const uint8_t* src = pool_head + page * (2 * plane_step);
                         bulk_copy(dst, src, PLANE, bar);
                         bulk_copy(dst + PLANE, src + plane_step, PLANE, bar);
-                    } else {
+                    }
+                }
+                if (n != SK || P != SK) {
+                    __syncwarp();
+                    // a page a lane
+                    const int lo = lane == 0 ? k_next : end_next + (lane - 1) * P, hi = min(end, end_next + lane * P);
+                    if (lane < MOST && lo < hi) {
+                        const int off = lane == 0 ? k_next - (end_next - P) : 0, m = hi - lo, at = lo - k_next;
+                        const uint8_t* src = pool_head + page * (2 * plane_step);
                         const uint8_t* codes = src + static_cast<size_t>(off) * RB;
                         const uint8_t* factors = src + static_cast<size_t>(P) * RB + static_cast<size_t>(off) * Q4_FACTOR_BYTES;
-                        bulk_copy(dst, codes, n * RB, bar);
-                        bulk_copy(dst + SK * RB, factors, n * Q4_FACTOR_BYTES, bar);
-                        bulk_copy(dst + PLANE, codes + plane_step, n * RB, bar);
-                        bulk_copy(dst + PLANE + SK * RB, factors + plane_step, n * Q4_FACTOR_BYTES, bar);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        bulk_copy(dst + at * RB, codes, m * RB, bar);
+                        bulk_copy(dst + SK * RB + at * Q4_FACTOR_BYTES, factors, m * Q4_FACTOR_BYTES, bar);
+                        bulk_copy(dst + PLANE + at * RB, codes + plane_step, m * RB, bar);
+                        bulk_copy(dst + PLANE + SK * RB + at * Q4_FACTOR_BYTES, factors + plane_step, m * Q4_FACTOR_BYTES, bar);
                     }
                 }
                 k_next = end;
-                if (end == end_next) {
+                while (end_next <= end) {
                     ++page_at;
                     end_next += P;
                 }
-            };
-            // end of the stage that begins with k0
-            auto stage_end = [&]() { return min(min(end_read, k0 + SK), k_stop); };
-            auto next_stage = [&](int end) {
-                if (end == end_read) end_read += P;
-                k0 = end;
             };
             int st = 0;
             if (ok) {
@@ -441,18 +538,17 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int k = min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);   // (-114 for infinities)
-                // the codes that meet {2, 3} count sixteen times what those that meet {0, 1} do
-                const float up = pow2i(k), up16 = up * 0.0625f;
+                const float up = pow2i(k);
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * KW; ++i) {
                     split2<PARTS>(x[4 * i] * up, x[4 * i + 1] * up, qb[ht][i][0]);
-                    split2<PARTS>(x[4 * i + 2] * up16, x[4 * i + 3] * up16, qb[ht][i][1]);
+                    split2<PARTS>(x[4 * i + 2] * up, x[4 * i + 3] * up, qb[ht][i][1]);
                     sum += (x[4 * i] + x[4 * i + 1]) + (x[4 * i + 2] + x[4 * i + 3]);
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                const float down = qscale * pow2i(-k) * 4096.f;   // (2^24 comes off the codes: half of it here, half with the key's scale)
+                const float down = qscale * pow2i(-k);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     hq[ht][c] = __shfl_sync(0xffffffffu, down, 4 * (2 * t4 + c));
@@ -461,8 +557,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             }
             // O^T: byte b of word w of a lane's value row is row tile 4 w + b: its low nibble's dimension in row gq, its high nibble's in row
             // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
-            float o[HT][MT][4], m[HT][2], l[HT][2], z[HT][2], slope[HT][2];
-            float from[HT][2];   // what a score's weight is formed relative to: M - TOP (0: no live key yet)
+            float o[HT][MT][4], l[HT][2], z[HT][2], slope[HT][2];
+            float limit[HT][2], from[HT][2];   // a score's weight is formed relative to `from` (M - TOP), up to `limit` (M + RAISE; no live key yet: -infinity)
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
@@ -470,81 +566,86 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int g = 8 * ht + 2 * t4 + c;
-                    m[ht][c] = -INFINITY;
+                    limit[ht][c] = -INFINITY;
                     l[ht][c] = z[ht][c] = from[ht][c] = 0.f;
                     slope[ht][c] = a.slopes && g < nG ? slope_log2(a.slopes, h0 + g) : 0.f;
                 }
             }
 
             float* const scores = WEIGH ? a.scores + (static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P * G + g0 + 2 * t4 : nullptr;
-            // sixteen keys, from c0, whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
-            auto chunk = [&](int c0, const unsigned char* at, const unsigned char* fac) {
-                const bool edge = c0 < t_lo || c0 + 16 > k_end;   // (a chunk with dead keys)
-                // keys c0 + kr0 and c0 + 8 + kr0: words, factors of the key's and of the value's row
-                uint32_t k_lo[KW], k_hi[KW], v_a[2][VW], v_b[2][VW], kf[2], vf[2];
-                lds_words<KW>(k_lo, at + kr0 * RB + t4 * (RB / 4));
-                lds_words<KW>(k_hi, at + (kr0 + 8) * RB + t4 * (RB / 4));
+            // N chunks of sixteen keys, from c0, whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
+            auto step = [&](int c0, const unsigned char* at, const unsigned char* fac) {
+                const bool edge = c0 < t_lo || c0 + 16 * N > k_end;   // (a step with dead keys)
+                // chunk n: keys c0 + 16 n + kr0 and + 8 + kr0
+                float s[N][HT][4];
+                uint32_t kf[N][2], vf[N][2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    lds_words<1>(kf + i, fac + 4 * (kr0 + 8 * i));
-                    lds_words<1>(vf + i, fac + PLANE + 4 * (kr0 + 8 * i));
-                    lds_words<VW>(v_a[i], at + PLANE + (8 * i + va_row) * RB + gq * (RB / 8));
-                    lds_words<VW>(v_b[i], at + PLANE + (8 * i + vb_row) * RB + gq * (RB / 8));
-                }
-                float s[HT][4];
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht) s[ht][0] = s[ht][1] = s[ht][2] = s[ht][3] = 0.f;
-#pragma unroll
-                for (int w = 0; w < KW; ++w)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
-                        const uint32_t af[4] = {a0 & 0x000f000fu, a1 & 0x000f000fu, a0 & 0x00f000f0u, a1 & 0x00f000f0u};
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                            for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
-                    }
-                const int key[2] = {c0 + kr0, c0 + 8 + kr0};
-                bool live[2] = {true, true};
-                if (edge) {
+                for (int n = 0; n < N; ++n) {
+                    uint32_t k_lo[KW], k_hi[KW];
+                    lds_words<KW>(k_lo, at + (16 * n + kr0) * RB + t4 * (RB / 4));
+                    lds_words<KW>(k_hi, at + (16 * n + kr0 + 8) * RB + t4 * (RB / 4));
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < k_end;
-                        if (!live[i]) kf[i] = vf[i] = 0u;
+                        lds_words<1>(&kf[n][i], fac + 4 * (16 * n + kr0 + 8 * i));
+                        lds_words<1>(&vf[n][i], fac + PLANE + 4 * (16 * n + kr0 + 8 * i));
                     }
-                }
-                // of the two keys: 2^12 scale of K, mid - 7.5 scale; of V the scale's exponent e, 2^-e, scale 2^-e, (mid - scale / 2) 2^-e
-                float ks[2], kz[2], ve[2], vs[2], vz[2], vi[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float k_scale = q4_scale(kf[i]), v_scale = q4_scale(vf[i]);
-                    ks[i] = k_scale * 4096.f;
-                    kz[i] = fmaf(-7.5f, k_scale, q4_mid(kf[i]));
-                    // (the exponent's field, LEAST + 127 .. 253, still in its place)
-                    const uint32_t e = min(max((vf[i] << 16) & 0x7f800000u, static_cast<uint32_t>(LEAST + 127) << 23), 253u << 23);
-                    ve[i] = __uint_as_float(0x4b000000u | (e >> 23)) - (8388608.f + 127.f);
-                    vi[i] = __uint_as_float((254u << 23) - e);
-                    vs[i] = v_scale * vi[i];
-                    vz[i] = fmaf(-0.5f, v_scale, q4_mid(vf[i])) * vi[i];
+                    for (int ht = 0; ht < HT; ++ht) s[n][ht][0] = s[n][ht][1] = s[n][ht][2] = s[n][ht][3] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < KW; ++w)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
+                            const uint32_t af[4] = {codes_low(a0), codes_low(a1), codes_high(a0), codes_high(a1)};
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                                for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
+                        }
                 }
-                float sc[HT][4];   // score + e
+                // of the two keys of a chunk: scale and z of K; of V the scale's exponent e, 2^-e, scale 2^-e, z 2^-e
+                float sc[N][HT][4], vs[N][2], vz[N][2], vi[N][2];   // sc: score + e
                 bool raise = false;
 #pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
+                for (int n = 0; n < N; ++n) {
+                    const int key[2] = {c0 + 16 * n + kr0, c0 + 16 * n + 8 + kr0};
+                    bool live[2] = {true, true};
+                    if (edge) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = i & 1, y = i >> 1;
-                        float w = fmaf(s[ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
-                        if (a.slopes) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
-                        if (WEIGH) {
-                            const int g = 8 * ht + 2 * t4 + c;
-                            if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
-                            w += ve[y];
+                        for (int i = 0; i < 2; ++i) {
+                            live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < k_end;
+                            if (!live[i]) kf[n][i] = vf[n][i] = 0u;
                         }
-                        if (edge && !live[y]) w = -INFINITY;
-                        sc[ht][i] = w;
-                        raise |= w > m[ht][c] + RAISE;
+                    }
+                    float ks[2], kz[2], ve[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float v_scale = q4_scale(vf[n][i]);
+                        ks[i] = q4_scale(kf[n][i]);
+                        kz[i] = fmaf(-0.5f, ks[i], q4_mid(kf[n][i]));
+                        // (the exponent's field, LEAST + 127 .. 253, still in its place)
+                        const uint32_t e = min(max((vf[n][i] << 16) & 0x7f800000u, static_cast<uint32_t>(LEAST + 127) << 23), 253u << 23);
+                        ve[i] = __uint_as_float(0x4b000000u | (e >> 23)) - (8388608.f + 127.f);
+                        vi[n][i] = __uint_as_float((254u << 23) - e);
+                        vs[n][i] = v_scale * vi[n][i];
+                        vz[n][i] = fmaf(-0.5f, v_scale, q4_mid(vf[n][i])) * vi[n][i];
+                    }
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = i & 1, y = i >> 1;
+                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
+                            if (a.slopes) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
+                            if (WEIGH) {
+                                const int g = 8 * ht + 2 * t4 + c;
+                                if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
+                                w += ve[y];
+                            }
+                            if (edge && !live[y]) w = -INFINITY;
+                            sc[n][ht][i] = w;
+                            raise |= w > limit[ht][c];
+                        }
                     }
                 }
                 if (__any_sync(0xffffffffu, raise)) {
@@ -552,14 +653,17 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float n = fmaxf(sc[ht][c], sc[ht][2 + c]);
-                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
-                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
-                            n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
-                            n = fmaxf(n, m[ht][c]);
-                            const float corr = m[ht][c] == -INFINITY ? 0.f : ex2(m[ht][c] - n);
-                            m[ht][c] = n;
-                            from[ht][c] = n == -INFINITY ? 0.f : n - TOP;
+                            float top = fmaxf(sc[0][ht][c], sc[0][ht][2 + c]);
+#pragma unroll
+                            for (int n = 1; n < N; ++n) top = fmaxf(top, fmaxf(sc[n][ht][c], sc[n][ht][2 + c]));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            const bool none = limit[ht][c] == -INFINITY;   // (no live key so far)
+                            const float now = none ? top - TOP : fmaxf(from[ht][c], top - TOP);
+                            const float corr = none ? 0.f : ex2(from[ht][c] - now);
+                            limit[ht][c] = now + (TOP + RAISE);
+                            from[ht][c] = now == -INFINITY ? 0.f : now;
                             l[ht][c] *= corr;
                             z[ht][c] *= corr;
 #pragma unroll
@@ -569,75 +673,80 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             }
                         }
                 }
-                uint32_t pb[HT][2][PARTS];
 #pragma unroll
-                for (int ht = 0; ht < HT; ++ht) {
-                    float e[4];
+                for (int n = 0; n < N; ++n) {
+                    uint32_t pb[HT][2][PARTS];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[i] = ex2(sc[ht][i] - from[ht][i & 1]);
+                    for (int ht = 0; ht < HT; ++ht) {
+                        float e[4];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        l[ht][c] = fmaf(e[c], vi[0], fmaf(e[2 + c], vi[1], l[ht][c]));
-                        z[ht][c] = fmaf(e[c], vz[0], fmaf(e[2 + c], vz[1], z[ht][c]));
-                    }
-                    // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
-                    split2<PARTS>(e[0] * vs[0], e[1] * vs[0], pb[ht][0]);
-                    split2<PARTS>(e[2] * vs[1], e[3] * vs[1], pb[ht][1]);
+                        for (int i = 0; i < 4; ++i) e[i] = ex2(sc[n][ht][i] - from[ht][i & 1]);
 #pragma unroll
-                    for (int y = 0; y < PARTS; ++y) {
-                        pb[ht][0][y] = movmatrix_trans(pb[ht][0][y]);
-                        pb[ht][1][y] = movmatrix_trans(pb[ht][1][y]);
-                    }
-                }
-                const uint32_t seven[4] = {0x80078007u, 0x80708070u, 0x80078007u, 0x80708070u};   // -7 2^-24, -7 2^-20
+                        for (int c = 0; c < 2; ++c) {
+                            l[ht][c] = fmaf(e[c], vi[n][0], fmaf(e[2 + c], vi[n][1], l[ht][c]));
+                            z[ht][c] = fmaf(e[c], vz[n][0], fmaf(e[2 + c], vz[n][1], z[ht][c]));
+                        }
+                        // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
+                        split2<PARTS>(e[0] * vs[n][0], e[1] * vs[n][0], pb[ht][0]);
+                        split2<PARTS>(e[2] * vs[n][1], e[3] * vs[n][1], pb[ht][1]);
 #pragma unroll
-                for (int w = 0; w < VW; ++w)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
-                        const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
-                        const uint32_t af[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) {
-                            float* t = o[ht][4 * w + b];
-                            if constexpr (PARTS == 1) {
-                                mma_f16(t, seven, pb[ht][0][0], pb[ht][1][0]);
-                                mma_f16(t, af, pb[ht][0][0], pb[ht][1][0]);
-                            } else {
-                                float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                for (int y = PARTS - 1; y >= 0; --y) {
-                                    mma_f16(d, seven, pb[ht][0][y], pb[ht][1][y]);
-                                    mma_f16(d, af, pb[ht][0][y], pb[ht][1][y]);
-                                }
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) t[i] += d[i];
-                            }
+                        for (int y = 0; y < PARTS; ++y) {
+                            pb[ht][0][y] = movmatrix_trans(pb[ht][0][y]);
+                            pb[ht][1][y] = movmatrix_trans(pb[ht][1][y]);
                         }
                     }
+                    uint32_t v_a[2][VW], v_b[2][VW];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        lds_words<VW>(v_a[i], at + PLANE + (16 * n + 8 * i + va_row) * RB + gq * (RB / 8));
+                        lds_words<VW>(v_b[i], at + PLANE + (16 * n + 8 * i + vb_row) * RB + gq * (RB / 8));
+                    }
+#pragma unroll
+                    for (int w = 0; w < VW; ++w)
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
+                            const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
+                            const uint32_t af[4] = {codes_low(x0), codes_high(x0), codes_low(x1), codes_high(x1)};
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht) {
+                                float* t = o[ht][4 * w + b];
+                                if constexpr (PARTS == 1) {
+                                    mma_f16(t, af, pb[ht][0][0], pb[ht][1][0]);
+                                } else {
+                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(d, af, pb[ht][0][y], pb[ht][1][y]);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) t[i] += d[i];
+                                }
+                            }
+                        }
+                }
             };
 
             while (ok && k0 < k_stop) {
                 __syncwarp();  // every lane has read the stage before this one: its place may be overwritten
                 if (k_next < k_stop) issue(st + S - 1 < S ? st + S - 1 : st - 1);
-                const int end = stage_end();
+                const int end = stage_end(k0);
                 ok = mbar_wait(bars + 8 * st, (parity >> st) & 1u);
                 if (!ok) break;
                 parity ^= 1u << st;
                 const unsigned char* src = q4_smem + warp * (S * STAGE) + st * STAGE;
                 if (++st == S) st = 0;
                 const int n = end - k0;
+                // (a second chunk behind the stage's last key reads what an earlier stage left, as dead keys)
 #pragma unroll 1
-                for (int c = 0; c < n; c += 16) chunk(k0 + c, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
-                next_stage(end);
+                for (int c = 0; c < n; c += 16 * N) step(k0 + c, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                k0 = end;
             }
             if (!ok) {
                 // a copy never came: the error word is set.  Those behind it are waited for, with the same limit
                 while (k0 < k_next) {
-                    const int end = stage_end();
+                    const int end = stage_end(k0);
                     if (++st == S) st = 0;
                     if (end < k_next) mbar_wait(bars + 8 * st, (parity >> st) & 1u);
-                    next_stage(end);
+                    k0 = end;
                 }
             }
             __syncwarp();
@@ -656,26 +765,26 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     const int g = 8 * ht + 2 * t4 + c;
                     if (g < nG) {
                         float* po = res + g * HD + gq * (HD / 8);
-                        auto low = [&](const float* t) { return fmaf(t[c], 16777216.f, zc); };        // 2^24, 2^20: the nibbles' places
-                        auto high = [&](const float* t) { return fmaf(t[2 + c], 1048576.f, zc); };
+                        auto low = [&](const float* t) { return t[c] + zc; };        // the low nibbles' dimensions, the high ones'
+                        auto high = [&](const float* t) { return t[2 + c] + zc; };
 #pragma unroll
                         for (int w = 0; w < VW; ++w) {
                             const float (*t)[4] = &o[ht][4 * w];
                             *reinterpret_cast<float4*>(po + 8 * w) = make_float4(low(t[0]), low(t[2]), high(t[0]), high(t[2]));
                             *reinterpret_cast<float4*>(po + 8 * w + 4) = make_float4(low(t[1]), low(t[3]), high(t[1]), high(t[3]));
                         }
-                        if (gq == 0) *reinterpret_cast<float2*>(res + 8 * HT * HD + 2 * g) = make_float2(m[ht][c], lc);
+                        if (gq == 0) *reinterpret_cast<float2*>(res + 8 * HT * HD + 2 * g) = make_float2(limit[ht][c] == -INFINITY ? -INFINITY : from[ht][c], lc);
                     }
                 }
             }
         }
         __syncthreads();
-        // joins: weight of a part whose maximum is pm and denominator pl_, relative to M  (a part without a live key: 0, NaN stays)
+        // joins: the weight of a part whose sums are relative to ml.x, relative to M (a part without a live key: 0; NaN stays)
         auto part_weight = [](float2 ml, float M) { return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M); };
         auto finish = [&](int g, const float* acc, float L, float M, int h_first, int at_row, int at_item) {
             const int h = h_first + g;
-            // (the sink: one more term of score 0; scores are in base 2, and a weight is 2^TOP at M)
-            const float full = a.sink ? fmaf(sink_term2(a.sink_val, h, M), 1024.f, L) : L;
+            // (the sink: one more term of score 0; scores are in base 2)
+            const float full = a.sink ? L + sink_term2(a.sink_val, h, M) : L;
             const float inv = 1.0f / full;
             T* dst = static_cast<T*>(a.out) + (static_cast<size_t>(at_row) * a.nh + h) * HD + lane * DL;
 #pragma unroll
@@ -683,7 +792,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(dst + d) = make_float2(acc[d] * inv, acc[d + 1] * inv);
                 else *reinterpret_cast<__nv_bfloat162*>(dst + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
             }
-            if (WEIGH && lane == 0) *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(at_item) * a.nh + h)) = make_float2(M - TOP, inv);
+            if (WEIGH && lane == 0) *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(at_item) * a.nh + h)) = make_float2(M, inv);
         };
         if (active) {
             // the heads of a run of warps, dealt to its warps
@@ -715,20 +824,17 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 #pragma unroll
                     for (int d = 0; d < DL; d += 2) *reinterpret_cast<float2*>(dst + d) = make_float2(acc[d], acc[d + 1]);
                     if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * place) = make_float2(M, L);
-                    __threadfence();
                 }
             }
         }
         if (!__syncthreads_or(active && !whole)) continue;   // (the rings are free again behind this)
-        // runs of warps that cover a (request, head) in part: the last block to bring one joins them all
-        const int u0 = r0 * n_vh + vh * n_ranges;            // the first unit of this (request, head)
-        const int n_parts = (u0 + n_ranges - 1) / W - u0 / W + 1;
+        // (request, head)s that several blocks have ranges of: the last block to bring its partial result joins them all
         if (lane == 0) {
             int last = 0;
             if (active && warp == wa && !whole) {
-                __threadfence();
+                __threadfence();   // (with the barrier in front: the whole block's results are out before the count is)
                 int* counter = a.counters + static_cast<size_t>(item) * a.nh + vh;
-                last = atomicAdd(counter, 1) == n_parts - 1;
+                last = atomicAdd(counter, 1) == un.parts - 1;
                 if (last) *counter = 0;
                 __threadfence();
             }
@@ -738,54 +844,47 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
         for (int lead = 0; lead < W; ++lead) {
             if (!is_last[lead]) continue;
             // (all warps of the block take part: the lead's unit again)
-            const int lu = base + lead;
-            int li = 0, hi = n_items;
-            while (hi - li > 1) {
-                const int mid = (li + hi) >> 1;
-                if (pl.pref[mid] * n_vh <= lu) li = mid;
-                else hi = mid;
-            }
-            const int lr0 = pl.pref[li], lnr = pl.pref[li + 1] - lr0, lvh = (lu - lr0 * n_vh) / lnr;
-            const int lg0 = (lvh % n_sub) * 8 * HT, lnG = min(G - lg0, 8 * HT), lh0 = (lvh / n_sub) * G + lg0;
-            const int lu0 = lr0 * n_vh + lvh * lnr, parts = (lu0 + lnr - 1) / W - lu0 / W + 1;
-            // range that part k begins with: 0, then where the blocks' runs begin
+            const Q4Unit lu = q4_unit<W>(pl, load, lead, n_items, n_vh);
+            const int lg0 = (lu.vh % n_sub) * 8 * HT, lnG = min(G - lg0, 8 * HT), lh0 = (lu.vh / n_sub) * G + lg0, parts = lu.parts;
+            // a part begins with the first range that its block has
             auto place = [&](int k, int g) {
-                const int first_range = k == 0 ? 0 : W * (lu0 / W + k) - lu0;
-                return static_cast<size_t>(lr0 + first_range) * a.nh + lh0 + g;
+                const int first_range = k == 0 ? 0 : lu.lead + (k - 1) * W;
+                return static_cast<size_t>(pl.pref[lu.item] + first_range) * a.nh + lh0 + g;
             };
             for (int g = warp; g < lnG; g += W) {
-                float M = -INFINITY;
-                for (int k = lane; k < parts; k += 32) M = fmaxf(M, __ldcg(a.part_ml + 2 * place(k, g)));
-                M = warp_max(M);
-                float L = 0.f, acc[DL];
+                constexpr int ROWS = 16;   // rows on their way together, with the first of the factors
+                float M = -INFINITY, L = 0.f, acc[DL];
 #pragma unroll
                 for (int d = 0; d < DL; ++d) acc[d] = 0.f;
-                for (int k0 = 0; k0 < parts; k0 += 32) {
+                for (int k0 = 0; k0 < parts; k0 += ROWS) {
+                    const int n = min(ROWS, parts - k0);
                     float2 mine = make_float2(-INFINITY, 0.f);
-                    if (k0 + lane < parts) mine = __ldcg(reinterpret_cast<const float2*>(a.part_ml + 2 * place(k0 + lane, g)));
-                    const float w = part_weight(mine, M);
-                    L += warp_sum(w == 0.f ? 0.f : mine.y * w);
-                    const int n = min(32, parts - k0);
-                    for (int j = 0; j < n; j += 8) {   // the rows of eight parts are on their way together
-                        float2 x[8][DL / 2];
+                    if (lane < n) mine = __ldcg(reinterpret_cast<const float2*>(a.part_ml + 2 * place(k0 + lane, g)));
+                    float2 x[ROWS][DL / 2];
 #pragma unroll
-                        for (int y = 0; y < 8; ++y)
+                    for (int y = 0; y < ROWS; ++y)
 #pragma unroll
-                            for (int d = 0; d < DL; d += 2)
-                                x[y][d / 2] = j + y < n ? __ldcg(reinterpret_cast<const float2*>(a.part_o + place(k0 + j + y, g) * HD + lane * DL + d))
-                                                        : make_float2(0.f, 0.f);
+                        for (int d = 0; d < DL; d += 2)
+                            x[y][d / 2] = y < n ? __ldcg(reinterpret_cast<const float2*>(a.part_o + place(k0 + y, g) * HD + lane * DL + d))
+                                                : make_float2(0.f, 0.f);
+                    const float top = fmaxf(M, warp_max(mine.x)), corr = M == -INFINITY ? 0.f : exp2f(M - top);
+                    const float w = part_weight(mine, top);
+                    L = (M == -INFINITY && L == 0.f ? 0.f : L * corr) + warp_sum(w == 0.f ? 0.f : mine.y * w);
 #pragma unroll
-                        for (int y = 0; y < 8; ++y) {
-                            const float wj = __shfl_sync(0xffffffffu, w, j + y);
+                    for (int d = 0; d < DL; ++d) acc[d] = k0 == 0 ? 0.f : acc[d] * corr;
+                    M = top;
 #pragma unroll
-                            for (int d = 0; d < DL; d += 2) {
-                                acc[d] = fmaf(x[y][d / 2].x, wj, acc[d]);
-                                acc[d + 1] = fmaf(x[y][d / 2].y, wj, acc[d + 1]);
-                            }
+                    for (int y = 0; y < ROWS; ++y) {
+                        if (y >= n) break;
+                        const float wj = __shfl_sync(0xffffffffu, w, y);
+#pragma unroll
+                        for (int d = 0; d < DL; d += 2) {
+                            acc[d] = fmaf(x[y][d / 2].x, wj, acc[d]);
+                            acc[d + 1] = fmaf(x[y][d / 2].y, wj, acc[d + 1]);
                         }
                     }
                 }
-                finish(g, acc, L, M, lh0, pl.row[li], li);
+                finish(g, acc, L, M, lh0, pl.row[lu.item], lu.item);
             }
         }
         __syncthreads();   // (is_last is written again in the next round)
@@ -815,17 +914,17 @@ __global__ void __launch_bounds__(WG_THREADS) q4_weigh_kernel(Q4Args a, float* _
     atomicAdd(weights + (static_cast<size_t>(page) * a.nkv + kvh) * P + t % P, sum);
 }
 
-template <typename T, int HD, int HT, int W, int S, int SK, bool WEIGH>
-static int q4_decode_launch(const Q4Args& a, int n_items, long long max_units, int cost_range, int cost_merge, int n_sm, int dev, cudaStream_t stream) {
+template <typename T, int HD, int HT, int N, int W, int S, int SK, bool WEIGH>
+static int q4_decode_launch(const Q4Args& a, int n_items, long long max_units, int cost_range, int cost_join, int cost_merge, int n_sm, int dev, cudaStream_t stream) {
     constexpr size_t smem = static_cast<size_t>(W) * S * 2 * SK * (HD / 2 + Q4_FACTOR_BYTES);
     static unsigned long long asked = 0;   // devices that know of the kernel's shared memory (asked again at worst)
     if (dev >= 64 || !(asked >> dev & 1)) {
-        if (cudaFuncSetAttribute(attn_decode_q4_kernel<T, HD, HT, W, S, SK, WEIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(attn_decode_q4_kernel<T, HD, HT, N, W, S, SK, WEIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(smem)) != cudaSuccess)
             return static_cast<int>(cudaGetLastError());
         if (dev < 64) asked |= 1ull << dev;
     }
-    locus_launch(attn_decode_q4_kernel<T, HD, HT, W, S, SK, WEIGH>, n_sm, 32 * W, smem, stream, a, n_items, max_units, cost_range, cost_merge);
+    locus_launch(attn_decode_q4_kernel<T, HD, HT, N, W, S, SK, WEIGH>, n_sm, 32 * W, smem, stream, a, n_items, max_units, cost_range, cost_join, cost_merge);
     return locus_launch_status();
 }
 
@@ -841,7 +940,7 @@ struct Q4DecodeCall {
     int* counters;
     const float *sink_val, *slopes;
     float *weights, *scores, *lse;
-    long long dt, table_stride, n_items, nh, nkv, hd, page_tokens, window, chunk, max_units, cost_range, cost_merge, keep_first, sink;
+    long long dt, table_stride, n_items, nh, nkv, hd, page_tokens, window, chunk, max_units, cost_range, cost_join, cost_merge, keep_first, sink;
     double scale;
 };
 
@@ -867,20 +966,20 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
     a.window = static_cast<int>(v.window); a.chunk = static_cast<int>(v.chunk); a.scale = static_cast<float>(v.scale);
     a.keep_first = keep_first; a.sink = static_cast<int>(v.sink); a.sink_val = v.sink ? v.sink_val : nullptr; a.slopes = v.slopes;
     a.part_o = v.part_o; a.part_ml = v.part_ml; a.counters = v.counters; a.scores = v.scores; a.lse = v.lse;
-    const int n = static_cast<int>(v.n_items), cr = static_cast<int>(v.cost_range), cm = static_cast<int>(v.cost_merge);
+    const int n = static_cast<int>(v.n_items), cr = static_cast<int>(v.cost_range), cj = static_cast<int>(v.cost_join), cm = static_cast<int>(v.cost_merge);
     const bool wide = a.nh / a.nkv > 8;
-#define Q4_GO(T_, HD_, HT_, W_, S_, SK_)                                                                              \
-    (v.weights ? q4_decode_launch<T_, HD_, HT_, W_, S_, SK_, true>(a, n, v.max_units, cr, cm, n_sm, dev, stream)      \
-               : q4_decode_launch<T_, HD_, HT_, W_, S_, SK_, false>(a, n, v.max_units, cr, cm, n_sm, dev, stream))
+#define Q4_GO(T_, HD_, HT_, N_, W_, S_, SK_)                                                                            \
+    (v.weights ? q4_decode_launch<T_, HD_, HT_, N_, W_, S_, SK_, true>(a, n, v.max_units, cr, cj, cm, n_sm, dev, stream)      \
+               : q4_decode_launch<T_, HD_, HT_, N_, W_, S_, SK_, false>(a, n, v.max_units, cr, cj, cm, n_sm, dev, stream))
     int code;
     if (v.dt == LOCUS_DT_F32) {
-        code = v.hd == 64 ? Q4_GO(float, 64, 1, 8, 3, 64) : v.hd == 128 ? Q4_GO(float, 128, 1, 8, 2, 64) : Q4_GO(float, 256, 1, 8, 2, 32);
+        code = v.hd == 64 ? Q4_GO(float, 64, 1, 1, 8, 3, 64) : v.hd == 128 ? Q4_GO(float, 128, 1, 1, 8, 2, 64) : Q4_GO(float, 256, 1, 1, 8, 2, 32);
     } else if (v.hd == 64) {
-        code = wide ? Q4_GO(bf16, 64, 2, 12, 3, 64) : Q4_GO(bf16, 64, 1, 12, 3, 64);
+        code = wide ? Q4_GO(bf16, 64, 2, 1, 12, 3, 64) : Q4_GO(bf16, 64, 1, 2, 12, 3, 64);
     } else if (v.hd == 128) {
-        code = wide ? Q4_GO(bf16, 128, 2, 8, 2, 64) : Q4_GO(bf16, 128, 1, 12, 2, 64);
+        code = wide ? Q4_GO(bf16, 128, 2, 1, 8, 2, 64) : Q4_GO(bf16, 128, 1, 2, 12, 2, 64);
     } else {
-        code = Q4_GO(bf16, 256, 1, 8, 2, 32);
+        code = Q4_GO(bf16, 256, 1, 1, 8, 2, 32);
     }
 #undef Q4_GO
     if (code || !v.weights) return code;

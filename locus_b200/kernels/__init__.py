@@ -1289,7 +1289,7 @@ def q4_page_bytes(head_dim: int, page_tokens: int) -> int:
 _Q4_WRITE = struct.Struct("@7P9q")
 _Q4_EXPAND = struct.Struct("@6P7q")
 _Q4_EVICT = struct.Struct("@6P12q")
-_Q4_DECODE = struct.Struct("@15P14qd")
+_Q4_DECODE = struct.Struct("@15P15qd")
 _q4_entries = {}
 
 
@@ -1447,9 +1447,9 @@ def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Te
     _check(code, what, lambda: f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_items} requests, keep {keep})")
 
 
-# The range cut's cost model of the 4-bit kernel, in keys: the fixed cost of a range, and of one more partial result (a block's) of the longest
-# request (csrc/attention_q4.cu: plan_ranges).
-Q4_COST_RANGE, Q4_COST_MERGE = 64, 16
+# The range cut's cost model of the 4-bit kernel, in keys: the fixed cost of a range, of joining partial results across blocks, and of one more
+# of them (csrc/attention_q4.cu: plan_ranges).
+Q4_COST_RANGE, Q4_COST_JOIN, Q4_COST_MERGE = 64, 96, 4
 Q4_MAX_ITEMS = 1024
 
 
@@ -1533,7 +1533,7 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
     code = _q4_entry("attention_q4", "locus_attn_decode_q4")(
         _Q4_DECODE.pack(qp, base, out.data_ptr(), seg_q0.data_ptr(), seg_ctx.data_ptr(), block_table.data_ptr(), items.data_ptr(), part, ml,
                         counters.data_ptr(), sink_at, slopes_at, to, at, lse, dtype_code(q.dtype), pages, n_items, n_heads, n_kv_heads, head_dim,
-                        page_tokens, window, chunk, max_units, Q4_COST_RANGE, Q4_COST_MERGE, keep_first if window > 0 else 0, sink_flag, scale),
+                        page_tokens, window, chunk, max_units, Q4_COST_RANGE, Q4_COST_JOIN, Q4_COST_MERGE, keep_first if window > 0 else 0, sink_flag, scale),
         _q4_stream(dev))
     if to and code == 0 and n_items > 0:
         _count_launches(1)
