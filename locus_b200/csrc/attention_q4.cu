@@ -69,6 +69,7 @@ struct Q4Args {
     int* counters;            // [n_items * nh], zero between launches
     float* scores;            // with weights: [n_items][nkv][table_stride * P][heads of a group], in base 2
     float* lse;               // with weights: [n_items * nh][2], what a head's weights are relative to, and 1 / denominator
+    uint32_t k1024;           // 0x64006400, 1024 twice in float16: as an argument it stays in a register (codes_low)
 };
 
 #define Q4_WAIT_LIMIT 2000000000LL   // cycles a warp waits for a copy before it gives up (about a second)
@@ -155,13 +156,14 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-// the codes in bits 0 .. 3 of a register's halves, less 7: 0x6400 | n is 1024 + n
-__device__ __forceinline__ uint32_t codes_low(uint32_t x) {
-    return bits(__hsub2(halves((x & 0x000f000fu) | 0x64006400u), halves(0x64076407u)));
+// the codes in bits 0 .. 3 of a register's halves, less 7: 0x6400 | n is 1024 + n.  (Mask and exponent in one LOP3 need one of the two constants in
+// a register; from two immediates the compiler makes two instructions, which cost a quarter of the loop's time.)
+__device__ __forceinline__ uint32_t codes_low(uint32_t x, uint32_t k1024) {
+    return bits(__hsub2(halves((x & 0x000f000fu) | k1024), halves(0x64076407u)));
 }
 // the codes in bits 4 .. 7: (1024 + 16 n) / 16 - 71
-__device__ __forceinline__ uint32_t codes_high(uint32_t x) {
-    return bits(__hfma2(halves((x & 0x00f000f0u) | 0x64006400u), halves(0x2c002c00u), halves(0xd470d470u)));
+__device__ __forceinline__ uint32_t codes_high(uint32_t x, uint32_t k1024) {
+    return bits(__hfma2(halves((x & 0x00f000f0u) | k1024), halves(0x2c002c00u), halves(0xd470d470u)));
 }
 // a pair of values as PARTS pairs of float16: one, rounded, or two
 template <int PARTS>
@@ -188,6 +190,11 @@ __device__ __forceinline__ void load8(const bf16* p, float* v) {
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
+
+template <bool B>
+struct Bool {
+    static constexpr bool value = B;
+};
 
 // ---------------------------------------------------------------------------
 // The cut of a step's keys into ranges.
@@ -413,6 +420,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     // and of odd keys alternate both among the rows 2 t4 (values) and among neighbouring rows (keys), half the banks each
     const int kr0 = gq ^ ((gq >> 1) & 1);
     const int va_row = (2 * t4) ^ (t4 & 1), vb_row = (2 * t4 + 1) ^ (t4 & 1);
+    const uint32_t k1024 = a.k1024;
     const int P = a.page_tokens, G = a.nh / a.nkv;
     const int n_sub = (G + 8 * HT - 1) / (8 * HT), n_vh = a.nkv * n_sub;   // warps that serve a group, heads of a range
 
@@ -573,9 +581,12 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             }
 
             float* const scores = WEIGH ? a.scores + (static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P * G + g0 + 2 * t4 : nullptr;
-            // N chunks of sixteen keys, from c0, whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
-            auto step = [&](int c0, const unsigned char* at, const unsigned char* fac) {
-                const bool edge = c0 < t_lo || c0 + 16 * N > k_end;   // (a step with dead keys)
+            // N chunks of sixteen keys, from c0 (those from `stop` on are dead), whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
+            // (SPECIAL: dead keys among them, or a distance bias; a copy of its own, for the plain steps' sake)
+            const bool biased_call = a.slopes != nullptr;
+            auto step = [&](auto special, int c0, int stop, const unsigned char* at, const unsigned char* fac) {
+                constexpr bool SPECIAL = decltype(special)::value;
+                const bool edge = SPECIAL && (c0 < t_lo || c0 + 16 * N > stop), biased = SPECIAL && biased_call;
                 // chunk n: keys c0 + 16 n + kr0 and + 8 + kr0
                 float s[N][HT][4];
                 uint32_t kf[N][2], vf[N][2];
@@ -596,7 +607,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
-                            const uint32_t af[4] = {codes_low(a0), codes_low(a1), codes_high(a0), codes_high(a1)};
+                            const uint32_t af[4] = {codes_low(a0, k1024), codes_low(a1, k1024), codes_high(a0, k1024), codes_high(a1, k1024)};
 #pragma unroll
                             for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
@@ -613,7 +624,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     if (edge) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < k_end;
+                            live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < stop;
                             if (!live[i]) kf[n][i] = vf[n][i] = 0u;
                         }
                     }
@@ -636,7 +647,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         for (int i = 0; i < 4; ++i) {
                             const int c = i & 1, y = i >> 1;
                             float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
-                            if (a.slopes) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
+                            if (biased) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
                             if (WEIGH) {
                                 const int g = 8 * ht + 2 * t4 + c;
                                 if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
@@ -707,7 +718,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         for (int b = 0; b < 4; ++b) {
                             const uint32_t sel = b | ((4 + b) << 8);   // byte b of one key and of the other; the bytes between do not count
                             const uint32_t x0 = __byte_perm(v_a[0][w], v_b[0][w], sel), x1 = __byte_perm(v_a[1][w], v_b[1][w], sel);
-                            const uint32_t af[4] = {codes_low(x0), codes_high(x0), codes_low(x1), codes_high(x1)};
+                            const uint32_t af[4] = {codes_low(x0, k1024), codes_high(x0, k1024), codes_low(x1, k1024), codes_high(x1, k1024)};
 #pragma unroll
                             for (int ht = 0; ht < HT; ++ht) {
                                 float* t = o[ht][4 * w + b];
@@ -736,8 +747,13 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 if (++st == S) st = 0;
                 const int n = end - k0;
                 // (a second chunk behind the stage's last key reads what an earlier stage left, as dead keys)
+                const int stop = min(end, k_end);
 #pragma unroll 1
-                for (int c = 0; c < n; c += 16 * N) step(k0 + c, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                for (int c = 0; c < n; c += 16 * N) {
+                    const int c0 = k0 + c;
+                    if (biased_call || c0 < t_lo || c0 + 16 * N > stop) step(Bool<true>(), c0, stop, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                    else step(Bool<false>(), c0, stop, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                }
                 k0 = end;
             }
             if (!ok) {
@@ -965,7 +981,7 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
     a.nh = static_cast<int>(v.nh); a.nkv = static_cast<int>(v.nkv); a.page_tokens = static_cast<int>(v.page_tokens);
     a.window = static_cast<int>(v.window); a.chunk = static_cast<int>(v.chunk); a.scale = static_cast<float>(v.scale);
     a.keep_first = keep_first; a.sink = static_cast<int>(v.sink); a.sink_val = v.sink ? v.sink_val : nullptr; a.slopes = v.slopes;
-    a.part_o = v.part_o; a.part_ml = v.part_ml; a.counters = v.counters; a.scores = v.scores; a.lse = v.lse;
+    a.part_o = v.part_o; a.part_ml = v.part_ml; a.counters = v.counters; a.scores = v.scores; a.lse = v.lse; a.k1024 = 0x64006400u;
     const int n = static_cast<int>(v.n_items), cr = static_cast<int>(v.cost_range), cj = static_cast<int>(v.cost_join), cm = static_cast<int>(v.cost_merge);
     const bool wide = a.nh / a.nkv > 8;
 #define Q4_GO(T_, HD_, HT_, N_, W_, S_, SK_)                                                                            \

@@ -221,6 +221,24 @@ def test_decode(dtype, H, kv, D, P, lens):
     check(out, plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5), dtype, H, D)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,kv,D,P", [(7, 1, 128, 64), (4, 4, 64, 48), (2, 1, 256, 16)])
+def test_decode_at_every_cut(dtype, H, kv, D, P):
+    """Lengths and numbers of requests that end ranges, stages and pages at many places.  Values are sums of few terms, so the output's error is that
+    of the weights alone: float32 to a few units of 2^-22 of the rows' sizes."""
+    for lens in ([33 * i + 7 for i in range(12)], [641], [16 * i + 1 for i in range(1, 30)], [1000, 17, 480, 481, 479, 64, 63], [48, 80, 112, 144, 176, 208, 240]):
+        table, n_pages = tables(lens, P, 25)
+        pool = filled(table, lens, kv, D, P, 26, n_pages).to(DEV)
+        q = rnd(len(lens), H * D, dtype=dtype, seed=27, scale=1.5)
+        out, ctx = run_decode(q, pool, table, lens, H, kv, D, P)
+        ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
+        check(out, ref, dtype, H, D)
+        if dtype == F32:
+            # the norm of a request's error: scores of up to some ten, each off by some units of 2^-24, and as many roundings of the sums
+            err = (out.cpu().double().view(-1, H * D) - ref[0].view(-1, H * D)).norm(dim=1) / ref[0].view(-1, H * D).norm(dim=1)
+            assert float(err.max()) <= 2.0 ** -18
+
+
 MASKS = [dict(window=1), dict(window=40), dict(window=100, keep_first=5), dict(window=33, keep_first=70), dict(chunk=48), dict(sink=True), dict(window=20, sink=True, keep_first=3),
          dict(sink="learned"), dict(slopes=True), dict(slopes=True, window=50)]
 
