@@ -41,8 +41,34 @@ __device__ __forceinline__ void store8(bf16* p, const float* v) {
 // k and v are not rounded to the model's type on the way.
 //
 // A block takes one token: its angles' sines and cosines, once, then its heads by groups of hd / 8 lanes, eight values (one word of codes) a
-// lane.  The pair's other half comes by a shuffle where halves lie a multiple of eight values apart, else through shared memory.
+// lane.  A pair's other half comes by a shuffle where halves lie a multiple of eight values apart, else through shared memory.  The rows of the first
+// W_AHEAD rounds are asked for in front of the angles.  (8,192 tokens of 16 + 16 heads of 128: bound by instructions, 93 us, until the quotient
+// was formed by a product and a remainder, q's rows went past the quantising, and the rows came ahead.)
 #define W_THREADS 256
+#define W_AHEAD 3
+__device__ __forceinline__ uint32_t q4_word(const float* x, float scale, float mid) {
+    if (scale == 0.f) return 0x88888888u;
+    if (scale < 1e-30f) {   // (no reciprocal to rely on)
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word |= static_cast<uint32_t>(fminf(fmaxf(floorf((x[i] - mid) / scale), -8.f), 7.f) + 8.f) << q4_shift(i);
+        return word;
+    }
+    // cell = floor((x - mid) / scale): the nearest whole number to the quotient, formed by the reciprocal, and one less where the remainder is negative
+    const float inv = 1.f / scale;
+    float half[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 6; i >= 0; i -= 2)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const float d = x[i + y] - mid;
+            const float near = (fminf(fmaxf(d * inv, -9.f), 9.f) + 12582912.f) - 12582912.f;
+            const float cell = fmaf(-near, scale, d) < 0.f ? near - 1.f : near;
+            half[y] = fmaf(half[y], 16.f, fminf(fmaxf(cell, -8.f), 7.f) + 8.f);   // (nibbles of the word's halves: whole numbers below 2^16)
+        }
+    return static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict__ qkv, const int* __restrict__ positions,
                                                             const float* __restrict__ inv_freq, T* __restrict__ q_out,
@@ -52,33 +78,34 @@ __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict
     constexpr int GL = HD / 8;            // lanes of a row
     constexpr int ROWS = W_THREADS / GL;  // rows of the block at a time
     __shared__ float cs[HD / 2], sn[HD / 2];
-    __shared__ __align__(16) float stage[W_THREADS * 8];
+    extern __shared__ __align__(16) float stage[];   // W_THREADS * 8 floats where halves lie apart by other than a multiple of eight
     const int t = blockIdx.x, tid = threadIdx.x;
     const int half = rot / 2;
-    const double pos = positions[t];
     const int slot = slots ? slots[t] : 0;
-    for (int i = tid; i < half; i += W_THREADS) {
-        const double turns = pos * static_cast<double>(inv_freq[i]) * 0.15915494309189533577;
-        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn[i], &cs[i]);
-    }
-    __syncthreads();
-    pdl_entry();
-    pdl_trigger();
-    const T* src = qkv + static_cast<size_t>(t) * (nh + 2 * nkv) * HD;
-    const int page = slot / P, off = slot % P;
+    const int page = slot / P, off = slot - page * P;
     const int n_rows = nh + (write_kv ? 2 * nkv : 0);
     const int g = tid / GL, l = tid % GL, d0 = 8 * l;
-    const bool aligned = half % 8 == 0;
-    const bool staged = pairing == 0 && !aligned && rot > 0;
-    for (int r0 = 0; r0 < n_rows; r0 += ROWS) {
-        const int r = r0 + g;
-        const bool live = r < n_rows;
-        float x[8];
-        if (live) load8(src + static_cast<size_t>(r) * HD + d0, x);
+    const T* src = qkv + static_cast<size_t>(t) * (nh + 2 * nkv) * HD + d0;
+    const bool staged = pairing == 0 && half % 8 != 0;
+    // (positions, slots and frequencies were there before the kernel in front)
+    pdl_entry();
+    pdl_trigger();
+    float x[W_AHEAD][8];
+    auto load = [&](int r, float* v) {
+        if (r < n_rows) load8(src + static_cast<size_t>(r) * HD, v);
         else
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        if (rot > 0) {   // (q and k; the rows of v take the shuffles with the others and keep their values)
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    };
+#pragma unroll
+    for (int u = 0; u < W_AHEAD; ++u) load(u * ROWS + g, x[u]);
+    if (tid < half) {
+        const double turns = static_cast<double>(positions[t]) * static_cast<double>(inv_freq[tid]) * 0.15915494309189533577;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn[tid], &cs[tid]);
+    }
+    __syncthreads();
+    auto row = [&](int r, float* x) {
+        if (rot > 0) {   // (q and k; rows of v beside rows of k take the shuffles with them and keep their values)
             const bool turn = r < nh + nkv;
             if (pairing == 1) {
 #pragma unroll
@@ -92,13 +119,14 @@ __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict
                 }
             } else if (!staged) {
                 const bool low = d0 < half;
-                const int lane = tid & 31, other = (lane - l) + (low ? l + half / 8 : l - half / 8);
+                const int lane = tid & 31, other = d0 < rot ? (lane - l) + (low ? l + half / 8 : l - half / 8) : lane;
                 const bool in = turn && d0 < rot;
                 const int p = low ? d0 : d0 - half;
+                const float sign = low ? -1.f : 1.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float y = __shfl_sync(0xffffffffu, x[i], d0 < rot ? other : lane);
-                    if (in) x[i] = low ? x[i] * cs[p + i] - y * sn[p + i] : y * sn[p + i] + x[i] * cs[p + i];
+                    const float y = __shfl_sync(0xffffffffu, x[i], other);
+                    if (in) x[i] = fmaf(x[i], cs[p + i], sign * y * sn[p + i]);
                 }
             } else {
                 float* mine = stage + static_cast<size_t>(g) * HD;
@@ -115,49 +143,49 @@ __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict
                 __syncwarp();
             }
         }
-        // (all lanes of a warp take part: rows of q leave theirs unused)
-        float lo = x[0], hi = x[0];
-        bool bad = false;
+        if (r < nh) store8(q_out + (static_cast<size_t>(t) * nh + r) * HD + d0, x);
+        if (!__any_sync(0xffffffffu, r >= nh && r < n_rows)) return;   // (a warp of q's rows alone)
+        float lo = x[0], hi = x[0], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             lo = fminf(lo, x[i]);
             hi = fmaxf(hi, x[i]);
-            bad = bad || !(fabsf(x[i]) <= 3.402823466e38f);
+            sum = fmaf(x[i], 0.f, sum);   // NaN if a value is not finite
         }
-        if (bad) hi = INFINITY;
+        if (sum != 0.f) hi = INFINITY;
 #pragma unroll
         for (int m = 1; m < GL; m <<= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
         }
-        if (!live) continue;
-        if (r < nh) {
-            store8(q_out + (static_cast<size_t>(t) * nh + r) * HD + d0, x);
-            continue;
-        }
-        const int plane = (r - nh) / nkv, h = (r - nh) % nkv;
+        if (r < nh || r >= n_rows) return;
+        const int plane = r >= nh + nkv, h = r - nh - (plane ? nkv : 0);
         const float scale = to_f(from_f<bf16>((0.5f * hi - 0.5f * lo) / 7.5f)), mid = to_f(from_f<bf16>(0.5f * lo + 0.5f * hi));
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float c = scale == 0.f ? 8.f : floorf((x[i] - mid) / scale) + 8.f;
-            word |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << q4_shift(i);
-        }
         uint8_t* at = pool + q4_place(page, plane, h, nkv, P, HD);
-        reinterpret_cast<uint32_t*>(at + static_cast<size_t>(off) * (HD / 2))[l] = word;
+        reinterpret_cast<uint32_t*>(at + static_cast<size_t>(off) * (HD / 2))[l] = q4_word(x, scale, mid);
         if (l == 0) {
             reinterpret_cast<uint32_t*>(at + static_cast<size_t>(P) * (HD / 2))[off] =
                 hi == INFINITY ? 0x7fff7fffu : q4_factors(scale, mid);
             if (weights && plane == 0) weights[(static_cast<size_t>(page) * nkv + h) * P + off] = 0.f;
         }
+    };
+    for (int r0 = 0; r0 < n_rows; r0 += W_AHEAD * ROWS) {
+        if (r0 > 0) {
+#pragma unroll
+            for (int u = 0; u < W_AHEAD; ++u) load(r0 + u * ROWS + g, x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < W_AHEAD; ++u)
+            if (r0 + u * ROWS < n_rows) row(r0 + u * ROWS + g, x[u]);
     }
 }
 
 template <typename T>
 static int write_launch(const void* qkv, const int* positions, const float* inv_freq, void* q_out, uint8_t* pool, const int* slots,
                         float* weights, int n, int nh, int nkv, int hd, int rot, int pairing, int P, int write_kv, cudaStream_t stream) {
+    const bool staged = pairing == 0 && (rot / 2) % 8 != 0;
 #define Q4_WRITE(HD_)                                                                                                               \
-    locus_launch(q4_write_kernel<T, HD_>, n, W_THREADS, 0, stream, static_cast<const T*>(qkv), positions, inv_freq,                \
+    locus_launch(q4_write_kernel<T, HD_>, n, W_THREADS, staged ? W_THREADS * 8 * sizeof(float) : 0, stream, static_cast<const T*>(qkv), positions, inv_freq,                \
                  static_cast<T*>(q_out), pool, slots, weights, nh, nkv, rot, pairing, P, write_kv)
     if (hd == 64) Q4_WRITE(64);
     else if (hd == 128) Q4_WRITE(128);
@@ -199,8 +227,33 @@ extern "C" int locus_rope_kv_write_q4(const Q4WriteCall* call, cudaStream_t stre
 // expand: the rows of positions 0 .. seg_ctx + seg_qn - 1 of the listed segments into ordinary pages [n_pages][2][nkv][P][hd] of the same
 // page ids, in the model's type (float32: as they are; bfloat16: one rounding, the tensor cores' operand).  Rows behind a request's last
 // token and pages that went back (-1) stay as they were.
-// One block per (page of the request, plane, head): P rows, a lane takes words of eight values.
+// One block per (page of the request, plane, head): P rows, a lane takes words of eight values, E_AHEAD at a time.
+// bfloat16 without a detour: 16 + code is 0x4180 | code << 3, 23.5 off is exact, and one fused multiply-add rounds once.
 #define E_THREADS 256
+#define E_AHEAD 4
+__device__ __forceinline__ void q4_eight(uint32_t w, uint32_t f, float* out) {
+    float v[8];
+    const float scale = q4_scale(f), mid = q4_mid(f);
+#pragma unroll
+    for (int d = 0; d < 8; ++d)   // (2^23 + code less 2^23 + 7.5, exactly)
+        v[d] = fmaf(scale, (__uint_as_float(((w >> q4_shift(d)) & 15u) | 0x4b000000u) - 8388608.f) - 7.5f, mid);
+    store8(out, v);
+}
+__device__ __forceinline__ void q4_eight(uint32_t w, uint32_t f, bf16* out) {
+    const __nv_bfloat162 factors = *reinterpret_cast<const __nv_bfloat162*>(&f);
+    const __nv_bfloat162 scale = __low2bfloat162(factors), mid = __high2bfloat162(factors);
+    const uint32_t k = 0x41bc41bcu;   // 23.5 twice
+    uint4 o;
+    uint32_t* v = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t y = ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
+        const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&k));
+        const __nv_bfloat162 r = __hfma2(scale, c, mid);
+        v[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    *reinterpret_cast<uint4*>(out) = o;
+}
 template <typename T, int HD>
 __global__ void __launch_bounds__(E_THREADS) q4_expand_kernel(const uint8_t* __restrict__ pool, T* __restrict__ out,
                                                               const int* __restrict__ segs, const int* __restrict__ seg_ctx,
@@ -221,14 +274,21 @@ __global__ void __launch_bounds__(E_THREADS) q4_expand_kernel(const uint8_t* __r
     const int words = min(P, n - first) * WR;
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(src);
     const uint32_t* factors = reinterpret_cast<const uint32_t*>(src + static_cast<size_t>(P) * (HD / 2));
-#pragma unroll 4
-    for (int i = threadIdx.x; i < words; i += E_THREADS) {
-        const uint32_t w = codes[i], f = factors[i / WR];
-        const float scale = q4_scale(f), mid = q4_mid(f);
-        float v[8];
+    for (int i0 = threadIdx.x; i0 < words; i0 += E_AHEAD * E_THREADS) {
+        uint32_t w[E_AHEAD], f[E_AHEAD];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) v[d] = fmaf(scale, static_cast<float>((w >> q4_shift(d)) & 15u) - 7.5f, mid);
-        store8(dst + static_cast<size_t>(i) * 8, v);
+        for (int u = 0; u < E_AHEAD; ++u) {
+            const int i = i0 + u * E_THREADS;
+            if (i < words) {
+                w[u] = codes[i];
+                f[u] = factors[i / WR];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < E_AHEAD; ++u) {
+            const int i = i0 + u * E_THREADS;
+            if (i < words) q4_eight(w[u], f[u], dst + static_cast<size_t>(i) * 8);
+        }
     }
 }
 
@@ -271,14 +331,16 @@ extern "C" int locus_expand_q4(const Q4ExpandCall* call, cudaStream_t stream) {
 // `keep` in all; of equal weights the earlier key counts as the heavier one, and a weight that is not a number as lighter than all others.
 // kept [layers][n_items][nkv][keep]: their indices, ascending; -1 behind a request of fewer than `keep` tokens, all of which stay.
 //
-// One block per (layer, request, head) finds the weight of the last key that stays digit by digit: the weights as unsigned numbers of the same
-// order, three digits of 11, 11 and 10 bits, a histogram in shared memory of those that agree in the digits before.  Then every warp takes
-// a run of keys, counts those that stay, and behind a sum over the warps writes their indices in order.  The keys are read once into shared
-// memory where they fit (SK_MAX), else from memory (the L2) in every pass.
-#define S_THREADS 1024
-#define S_WARPS (S_THREADS / 32)
+// One block per (layer, request, head).  The weights are read once, as unsigned numbers of the same order, into shared memory where they fit (SK_MAX; else
+// from memory, the L2, in every pass).  The weight of the last key that stays is found by histograms of S_BINS bins over the range of numbers that
+// it must lie in, at first from the smallest to the largest, then one bin of the pass before: three passes at most, mostly two, and only keys of that
+// range are counted, so that bins are hit evenly and seldom by a warp's lanes at once.  Then every warp takes a run of keys, counts those that stay,
+// and behind a sum over the warps writes their indices in order.
+// (24 layers of 16 heads of one request of 4,096 tokens: with a fixed cut of the 32 bits by 11, 11 and 10 and blocks of 1,024 threads 31 us, most
+// of it atomics on the few bins that exponents hit.)
 #define SK_MAX 49152      // weights in shared memory (192 KB)
 #define S_BINS 2048
+#define S_SHORT 8192      // up to so many keys: blocks of 256 threads, several to an SM; else 1,024
 
 // an unsigned number of the weight's order
 __device__ __forceinline__ uint32_t ordered(float w) {
@@ -286,14 +348,19 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     const uint32_t u = __float_as_uint(w + 0.f);   // (-0 and 0 are one weight)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// t / P for t and 2^40 / P below 2^27 and 2^37: a multiplication by ceil(2^40 / P)
+__device__ __forceinline__ int by_page(int t, unsigned long long page_inv) { return static_cast<int>((static_cast<unsigned long long>(t) * page_inv) >> 40); }
 
-__global__ void __launch_bounds__(S_THREADS) q4_select_kernel(const float* __restrict__ weights, const int* __restrict__ block_table,
-                                                              int table_stride, const int* __restrict__ n_tokens, int n_items, int nkv,
-                                                              int P, size_t layer_slots, int keep, int first, int recent,
-                                                              int room, int* __restrict__ kept) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) q4_select_kernel(const float* __restrict__ weights, const int* __restrict__ block_table, int table_stride,
+                                                            const int* __restrict__ n_tokens, int n_items, int nkv, int P,
+                                                            unsigned long long page_inv, size_t layer_slots, int keep, int first, int recent,
+                                                            int room, int* __restrict__ kept) {
+    constexpr int WARPS = THREADS / 32, BT = S_BINS / THREADS;   // bins of a thread
     extern __shared__ uint32_t s_keys[];
-    __shared__ int hist[S_BINS];
-    __shared__ int warp_sum_[S_WARPS], warp_tie[S_WARPS];
+    __shared__ __align__(16) int hist[S_BINS];
+    __shared__ int warp_a[WARPS], warp_b[WARPS];
+    __shared__ uint32_t warp_lo[WARPS], warp_hi[WARPS];
     __shared__ int chosen_bin, above_bin;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_entry();
@@ -302,108 +369,151 @@ __global__ void __launch_bounds__(S_THREADS) q4_select_kernel(const float* __res
     const int n = min(n_tokens[item], table_stride * P);
     int* dst = kept + ((static_cast<size_t>(layer) * n_items + item) * nkv + h) * keep;
     if (n <= keep) {
-        for (int j = tid; j < keep; j += S_THREADS) dst[j] = j < n ? j : -1;
+        for (int j = tid; j < keep; j += THREADS) dst[j] = j < n ? j : -1;
         return;
     }
-    const float* w = weights + static_cast<size_t>(layer) * layer_slots;
+    const float* w = weights + static_cast<size_t>(layer) * layer_slots + static_cast<size_t>(h) * P;
     const int* table = block_table + static_cast<size_t>(item) * table_stride;
-    const int lo = first, hi = n - recent;       // the keys between, of which `want` stay
-    const int want = keep - first - recent;
+    const size_t page_step = static_cast<size_t>(nkv) * P;
+    const int lo = first, hi = n - recent;       // the keys between, of which `left` stay
+    int left = keep - first - recent;
     auto read = [&](int t) {
-        const int page = table[t / P];
-        return page < 0 ? 0u : ordered(w[(static_cast<size_t>(page) * nkv + h) * P + t % P]);
+        const int at = by_page(t, page_inv), page = table[at];
+        return page < 0 ? 0u : ordered(w[page * page_step + (t - at * P)]);
     };
     const bool in_smem = hi - lo <= room;
-    if (in_smem && want > 0) {
-        for (int t = lo + tid; t < hi; t += S_THREADS) s_keys[t - lo] = read(t);
-    }
     auto key = [&](int t) { return in_smem ? s_keys[t - lo] : read(t); };
-    uint32_t prefix = 0;   // the digits found so far, in place
-    int left = want;       // keys of those digits that still stay
-    if (want > 0) {
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-            for (int i = tid; i < S_BINS; i += S_THREADS) hist[i] = 0;
+    uint32_t from = 0, to = 0;    // the numbers that the last key to stay lies between
+    bool ties = false;            // keys equal to `from`: the first `left` of them stay; else all from `from` on
+    if (left > 0) {
+        uint32_t least = 0xffffffffu, most = 0u;
+        constexpr int AHEAD = 4;
+        for (int t0 = lo + tid; t0 < hi; t0 += AHEAD * THREADS) {
+            uint32_t u[AHEAD];
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) u[x] = t0 + x * THREADS < hi ? read(t0 + x * THREADS) : 0u;
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x)
+                if (t0 + x * THREADS < hi) {
+                    least = min(least, u[x]);
+                    most = max(most, u[x]);
+                    if (in_smem) s_keys[t0 + x * THREADS - lo] = u[x];
+                }
+        }
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) {
+            warp_lo[warp] = least;
+            warp_hi[warp] = most;
+        }
+        __syncthreads();
+        from = __reduce_min_sync(0xffffffffu, lane < WARPS ? warp_lo[lane] : 0xffffffffu);
+        to = __reduce_max_sync(0xffffffffu, lane < WARPS ? warp_hi[lane] : 0u);
+        while (true) {
+            const uint32_t span = to - from;
+            const int shift = span ? max(0, 32 - __clz(span) - 11) : 0;   // (span >> shift) < 2048
+#pragma unroll
+            for (int i = 0; i < BT; ++i) hist[tid + i * THREADS] = 0;
             __syncthreads();
-            for (int t = lo + tid; t < hi; t += S_THREADS) {
-                const uint32_t u = key(t);
-                if (pass == 0 || (u >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1);
+#pragma unroll 4
+            for (int t = lo + tid; t < hi; t += THREADS) {
+                const uint32_t u = key(t) - from;
+                if (u <= span) atomicAdd(&hist[u >> shift], 1);
             }
             __syncthreads();
-            // keys in higher bins, from the top: thread i has bins 2047 - 2 i and 2046 - 2 i
-            const int b0 = hist[S_BINS - 1 - 2 * tid], b1 = hist[S_BINS - 2 - 2 * tid];
-            int run = b0 + b1;
+            // keys in higher bins, from the top: thread i has bins from S_BINS - 1 - BT i down
+            int mine[BT], run = 0;
+#pragma unroll
+            for (int i = 0; i < BT; ++i) {
+                mine[i] = hist[S_BINS - 1 - BT * tid - i];
+                run += mine[i];
+            }
+            const int own_sum = run;
 #pragma unroll
             for (int m = 1; m < 32; m <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, run, m);
                 if (lane >= m) run += v;
             }
-            if (lane == 31) warp_sum_[warp] = run;
+            if (lane == 31) warp_a[warp] = run;
             __syncthreads();
-            if (warp == 0) {
-                int v = warp_sum_[lane];
+            int before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_a[lane] : 0) + run - own_sum;   // keys above this thread's bins
 #pragma unroll
-                for (int m = 1; m < 32; m <<= 1) {
-                    const int o = __shfl_up_sync(0xffffffffu, v, m);
-                    if (lane >= m) v += o;
+            for (int i = 0; i < BT; ++i) {
+                if (before < left && before + mine[i] >= left) {
+                    chosen_bin = S_BINS - 1 - BT * tid - i;
+                    above_bin = before;
                 }
-                warp_sum_[lane] = v;
+                before += mine[i];
             }
             __syncthreads();
-            const int before = (warp ? warp_sum_[warp - 1] : 0) + run - b0 - b1;   // keys above this thread's bins
-            if (before < left && before + b0 >= left) {
-                chosen_bin = S_BINS - 1 - 2 * tid;
-                above_bin = before;
-            } else if (before + b0 < left && before + b0 + b1 >= left) {
-                chosen_bin = S_BINS - 2 - 2 * tid;
-                above_bin = before + b0;
-            }
-            __syncthreads();
-            prefix |= static_cast<uint32_t>(chosen_bin) << shift;
+            const int bin = chosen_bin, count = hist[bin];
             left -= above_bin;
-            __syncthreads();
+            from += static_cast<uint32_t>(bin) << shift;
+            to = from + min(to - from, (1u << shift) - 1u);
+            if (count == left) break;   // the whole bin stays
+            if (shift == 0) {           // (equal weights)
+                ties = true;
+                break;
+            }
+            __syncthreads();            // (hist is cleared again)
         }
+    } else {
+        from = 0xffffffffu;             // none of those between stays
+        ties = true;
     }
-    // keys above `prefix` stay, and the first `left` of those equal to it
-    const int per = ((n + S_WARPS - 1) / S_WARPS + 31) & ~31;
+    // keys from `from` on stay, of those equal to it with `ties` only the first `left`
+    const int per = ((n + WARPS - 1) / WARPS + 31) & ~31;
     const int a = min(n, warp * per), b = min(n, a + per);
     auto look = [&](int t, bool& stays, bool& tie) {
         stays = t < b && (t < lo || t >= hi);
         tie = false;
-        if (t < b && !stays && want > 0) {
+        if (t < b && !stays) {
             const uint32_t u = key(t);
-            stays = u > prefix;
-            tie = u == prefix;
+            tie = ties && u == from;
+            stays = u >= from && !tie;
         }
     };
     int n_stay = 0, n_tie = 0;
-    for (int t0 = a; t0 < b; t0 += 32) {
-        bool s, e;
-        look(t0 + lane, s, e);
-        n_stay += __popc(__ballot_sync(0xffffffffu, s));
-        n_tie += __popc(__ballot_sync(0xffffffffu, e));
+    if (left > 0 || !ties) {
+        for (int t0 = a; t0 < b; t0 += 32) {
+            bool s, e;
+            look(t0 + lane, s, e);
+            n_stay += s;
+            n_tie += e;
+        }
+    } else {   // (first and recent alone)
+        for (int t0 = a; t0 < b; t0 += 32) n_stay += t0 + lane < b && (t0 + lane < lo || t0 + lane >= hi);
     }
+    n_stay = __reduce_add_sync(0xffffffffu, n_stay);
+    n_tie = __reduce_add_sync(0xffffffffu, n_tie);
+    __syncthreads();
     if (lane == 0) {
-        warp_sum_[warp] = n_stay;
-        warp_tie[warp] = n_tie;
+        warp_a[warp] = n_stay;
+        warp_b[warp] = n_tie;
     }
     __syncthreads();
     // ties taken and keys written by the warps in front
-    int ties = 0, at = 0;
+    int taken = 0, at = 0;
     for (int v = 0; v < warp; ++v) {
-        at += warp_sum_[v] + max(0, min(warp_tie[v], left - ties));
-        ties += warp_tie[v];
+        at += warp_a[v] + max(0, min(warp_b[v], left - taken));
+        taken += warp_b[v];
     }
     const uint32_t below = (1u << lane) - 1;
+    const bool none = left <= 0 && ties;
     for (int t0 = a; t0 < b; t0 += 32) {
-        bool s, e;
-        look(t0 + lane, s, e);
-        const uint32_t tie_mask = __ballot_sync(0xffffffffu, e);
-        const bool in = s || (e && ties + __popc(tie_mask & below) < left);
-        const uint32_t in_mask = __ballot_sync(0xffffffffu, in);
+        bool s, e = false;
+        if (none) s = t0 + lane < b && (t0 + lane < lo || t0 + lane >= hi);
+        else look(t0 + lane, s, e);
+        uint32_t in_mask;
+        bool in = s;
+        if (ties) {
+            const uint32_t tie_mask = __ballot_sync(0xffffffffu, e);
+            in = s || (e && taken + __popc(tie_mask & below) < left);
+            taken += __popc(tie_mask);
+        }
+        in_mask = __ballot_sync(0xffffffffu, in);
         if (in) dst[at + __popc(in_mask & below)] = t0 + lane;
         at += __popc(in_mask);
-        ties += __popc(tie_mask);
     }
 }
 
@@ -412,14 +522,21 @@ __global__ void __launch_bounds__(S_THREADS) q4_select_kernel(const float* __res
 // (kept[j] >= j): a block takes (layer, request, head, plane) and walks its rows from the front, a tile at a time, and reads a tile before it
 // writes it.  Into other pages the order is free, and several blocks share the rows.
 #define M_THREADS 256
-#define M_UNROLL 4       // 16-byte pieces of a thread in flight per tile, two tiles
+#define M_UNROLL 8       // 16-byte pieces of a thread in flight
+
+// 16 bytes of a row; rows are read once, and rows that do not stay lie between them
+__device__ __forceinline__ uint4 ld_row(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
 
 template <int HD>
 __global__ void __launch_bounds__(M_THREADS) q4_move_kernel(uint8_t* pool, float* weights, const int* __restrict__ block_table,
                                                             int table_stride, const int* __restrict__ dst_table, int dst_stride,
                                                             const int* __restrict__ n_tokens, int n_items, int nkv, int P,
-                                                            size_t layer_bytes, size_t layer_slots, int keep, int n_parts,
-                                                            const int* __restrict__ kept) {
+                                                            unsigned long long page_inv, size_t layer_bytes, size_t layer_slots, int keep,
+                                                            int n_parts, const int* __restrict__ kept) {
     constexpr int PR = HD / 32;                           // pieces of a row
     constexpr int TILE = M_THREADS * M_UNROLL / PR;       // rows of a tile
     constexpr int FU = (TILE + M_THREADS - 1) / M_THREADS;
@@ -441,46 +558,48 @@ __global__ void __launch_bounds__(M_THREADS) q4_move_kernel(uint8_t* pool, float
     float wt[FU];
     bool has[M_UNROLL], fhas[FU];
     for (int j0 = part * TILE; j0 < n; j0 += n_parts * TILE) {
+        int t[M_UNROLL];
 #pragma unroll
         for (int u = 0; u < M_UNROLL; ++u) {
-            const int e = u * M_THREADS + tid, j = j0 + e / PR;
-            has[u] = false;
-            if (j < n) {
-                const int t = idx[j], page = table[t / P];
-                has[u] = page >= 0;
-                if (has[u]) piece[u] = *reinterpret_cast<const uint4*>(place(page) + static_cast<size_t>(t % P) * (HD / 2) + (e % PR) * 16);
-            }
+            const int j = j0 + (u * M_THREADS + tid) / PR;
+            t[u] = j < n ? idx[j] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < M_UNROLL; ++u) {
+            const int at = by_page(max(t[u], 0), page_inv), page = t[u] >= 0 ? table[at] : -1;
+            has[u] = page >= 0;
+            if (has[u]) piece[u] = ld_row(place(page) + static_cast<size_t>(t[u] - at * P) * (HD / 2) + (tid % PR) * 16);
         }
 #pragma unroll
         for (int u = 0; u < FU; ++u) {
             const int e = u * M_THREADS + tid, j = j0 + e;
             fhas[u] = false;
             if (e < TILE && j < n) {
-                const int t = idx[j], page = table[t / P];
+                const int s = idx[j], at = by_page(s, page_inv), page = table[at], off = s - at * P;
                 fhas[u] = page >= 0;
                 if (fhas[u]) {
-                    fac[u] = reinterpret_cast<const uint32_t*>(place(page) + static_cast<size_t>(P) * (HD / 2))[t % P];
-                    if (plane == 0) wt[u] = w[(static_cast<size_t>(page) * nkv + h) * P + t % P];
+                    fac[u] = reinterpret_cast<const uint32_t*>(place(page) + static_cast<size_t>(P) * (HD / 2))[off];
+                    if (plane == 0) wt[u] = w[(static_cast<size_t>(page) * nkv + h) * P + off];
                 }
             }
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < M_UNROLL; ++u) {
-            const int e = u * M_THREADS + tid, j = j0 + e / PR;
+            const int j = j0 + (u * M_THREADS + tid) / PR;
             if (has[u]) {
-                const int page = to[j / P];
-                if (page >= 0) *reinterpret_cast<uint4*>(place(page) + static_cast<size_t>(j % P) * (HD / 2) + (e % PR) * 16) = piece[u];
+                const int at = by_page(j, page_inv), page = to[at];
+                if (page >= 0) *reinterpret_cast<uint4*>(place(page) + static_cast<size_t>(j - at * P) * (HD / 2) + (tid % PR) * 16) = piece[u];
             }
         }
 #pragma unroll
         for (int u = 0; u < FU; ++u) {
             const int j = j0 + u * M_THREADS + tid;
             if (fhas[u]) {
-                const int page = to[j / P];
+                const int at = by_page(j, page_inv), page = to[at], off = j - at * P;
                 if (page >= 0) {
-                    reinterpret_cast<uint32_t*>(place(page) + static_cast<size_t>(P) * (HD / 2))[j % P] = fac[u];
-                    if (plane == 0) w[(static_cast<size_t>(page) * nkv + h) * P + j % P] = wt[u];
+                    reinterpret_cast<uint32_t*>(place(page) + static_cast<size_t>(P) * (HD / 2))[off] = fac[u];
+                    if (plane == 0) w[(static_cast<size_t>(page) * nkv + h) * P + off] = wt[u];
                 }
             }
         }
@@ -512,12 +631,17 @@ extern "C" int locus_evict_q4(const Q4EvictCall* call, cudaStream_t stream) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return static_cast<int>(cudaGetLastError());
     if (dev >= 64 || !(asked >> dev & 1)) {
-        if (cudaFuncSetAttribute(q4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_MAX * 4) != cudaSuccess)
+        if (cudaFuncSetAttribute(q4_select_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_MAX * 4) != cudaSuccess)
             return static_cast<int>(cudaGetLastError());
         if (dev < 64) asked |= 1ull << dev;
     }
-    locus_launch(q4_select_kernel, grid, S_THREADS, static_cast<size_t>(room) * 4, stream, v.weights, v.block_table, table_stride, v.n_tokens, n_items,
-                 nkv, P, slots, keep, first, recent, room, v.kept);
+    const unsigned long long page_inv = ((1ull << 40) + P - 1) / P;
+    if (between <= S_SHORT)
+        locus_launch(q4_select_kernel<256>, grid, 256, static_cast<size_t>(room) * 4, stream, v.weights, v.block_table, table_stride, v.n_tokens,
+                     n_items, nkv, P, page_inv, slots, keep, first, recent, room, v.kept);
+    else
+        locus_launch(q4_select_kernel<1024>, grid, 1024, static_cast<size_t>(room) * 4, stream, v.weights, v.block_table, table_stride, v.n_tokens,
+                     n_items, nkv, P, page_inv, slots, keep, first, recent, room, v.kept);
     const int code = locus_launch_status();
     if (code) return code;
     const int tile = M_THREADS * M_UNROLL / (hd / 32);
@@ -525,7 +649,7 @@ extern "C" int locus_evict_q4(const Q4EvictCall* call, cudaStream_t stream) {
     const dim3 mgrid(2 * nkv * n_parts, n_items, static_cast<unsigned>(v.n_layers));
 #define Q4_MOVE(HD_)                                                                                                                        \
     locus_launch(q4_move_kernel<HD_>, mgrid, M_THREADS, 0, stream, static_cast<uint8_t*>(v.pool), v.weights, v.block_table, table_stride,   \
-                 v.dst_table, dst_stride, v.n_tokens, n_items, nkv, P, bytes, slots, keep, n_parts, v.kept)
+                 v.dst_table, dst_stride, v.n_tokens, n_items, nkv, P, page_inv, bytes, slots, keep, n_parts, v.kept)
     if (hd == 64) Q4_MOVE(64);
     else if (hd == 128) Q4_MOVE(128);
     else Q4_MOVE(256);

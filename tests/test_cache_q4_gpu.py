@@ -111,7 +111,7 @@ def test_rows_that_are_written(dtype, nh, nkv, D, rot, swap, P, T):
 
 
 def test_rows_without_a_range_and_rows_that_are_not_finite():
-    nh, nkv, D, P, T = 1, 1, 128, 16, 7
+    nh, nkv, D, P, T = 1, 1, 128, 16, 9
     qkv = rnd(T, 3 * D, seed=4)
     v = qkv[:, 2 * D:]
     v[0] = 1.5
@@ -122,6 +122,8 @@ def test_rows_without_a_range_and_rows_that_are_not_finite():
     v[5] = torch.linspace(-3e38, 3e38, D)            # (float32 steps overflow: infinities and NaN)
     v[6] = torch.linspace(-3e38, 3e38, D, dtype=torch.float64).float()
     assert not torch.isfinite(v[5]).all() and torch.isfinite(v[6]).all()
+    v[7] *= 1e-36
+    v[8] = torch.where(torch.arange(D) < 64, 1.0, -1.0) * 1e-44   # (subnormal)
     pool = poison(1, nkv, D, P).to(DEV)
     K.rope_kv_write_q4(qkv.to(DEV), torch.zeros(T, dtype=I32, device=DEV), None, torch.empty(T, D, device=DEV), pool,
                        torch.arange(T, dtype=I32, device=DEV), n_heads=nh, rot_dim=0, interleaved=False, **sizes(nkv, D, P))
@@ -130,6 +132,10 @@ def test_rows_without_a_range_and_rows_that_are_not_finite():
     assert torch.isnan(got[2:6]).all()
     step = 6e38 / 15
     assert ((got[6] - v[6].double()).abs() <= step * (0.5 + 2.0 ** -8 * 7.5)).all()
+    for i in (7, 8):
+        codes, scale, mid = plain.codes_of(v[i].double())
+        c, s, m = (f[0, 1, 0, i] for f in plain.fields(pool, P, D))
+        assert torch.equal(c, codes) and s == scale and m == mid
 
 
 def test_q_alone_is_rotated_where_another_call_owns_the_cache():
@@ -398,6 +404,29 @@ def test_evict(in_place, kv, D, P, lens, keep, first, recent):
         assert torch.equal(kept[l].cpu(), want[0]), f"layer {l}"
         assert torch.equal(dpool[l].cpu(), want[1])
         assert torch.equal(dweights[l].cpu().view(I32), want[2].view(I32))
+
+
+@pytest.mark.parametrize("n,keep,first,recent", [(9000, 4000, 4, 300), (8193, 8192, 0, 0), (8192, 1, 0, 0), (8194, 5000, 1, 1), (20000, 19999, 0, 7)])
+@pytest.mark.parametrize("kind", ["close", "equal", "wide", "two", "infinite", "negative"])
+def test_which_keys_stay(n, keep, first, recent, kind):
+    """The choice alone, over weights that crowd a few numbers or span all of float32, against a sort (ties: the earlier key)."""
+    kv, D, P = 1, 64, 64
+    pages = -(-n // P)
+    w = {"close": lambda: 1 + 1e-6 * rnd(pages * P, seed=n).abs(), "equal": lambda: torch.full((pages * P,), 0.25),
+         "wide": lambda: torch.exp(40 * rnd(pages * P, seed=n)), "two": lambda: (rnd(pages * P, seed=n) > 0).float(),
+         "infinite": lambda: torch.where(rnd(pages * P, seed=n) > 0, math.inf, rnd(pages * P, seed=n + 1)), "negative": lambda: rnd(pages * P, seed=n).round(decimals=2)}[kind]()
+    pool = torch.zeros(1, pages, 2, kv, K.q4_page_bytes(D, P), dtype=torch.uint8, device=DEV)
+    kept = torch.empty(1, 1, kv, keep, dtype=I32, device=DEV)
+    K.evict_q4(pool, w.view(1, pages, kv, P).to(DEV), block_table=torch.arange(pages, dtype=I32, device=DEV).view(1, -1), n_items=1, keep=keep, first=first,
+               n_tokens=torch.tensor([n], dtype=I32, device=DEV), recent=recent, kept=kept, max_tokens=n, **sizes(kv, D, P))
+    rank = w[:n].double()
+    rank[:first] = rank[n - recent:] = math.inf
+    order = torch.argsort(rank, descending=True, stable=True)
+    if kind == "infinite":   # (the first and the last stay whatever the others are)
+        sure = torch.zeros(n, dtype=torch.bool)
+        sure[:first] = sure[n - recent:] = True
+        order = torch.cat([sure.nonzero().view(-1), order[~sure[order]]])
+    assert kept.view(-1).tolist() == sorted(order[:keep].tolist())
 
 
 def test_evict_from_a_request_longer_than_shared_memory_holds():
