@@ -40,79 +40,147 @@ __device__ __forceinline__ void store8(bf16* p, const float* v) {
 // to one turn are 64 bits (in 32 a position of 30,000 is off by up to 1/1000 of a radian, a hundredth of a cell, and codes near a border change).
 // k and v are not rounded to the model's type on the way.
 //
-// A block takes one token: its angles' sines and cosines, once, then its heads by groups of hd / 8 lanes, eight values (one word of codes) a
-// lane.  A pair's other half comes by a shuffle where halves lie a multiple of eight values apart, else through shared memory.  The rows of the first
-// W_AHEAD rounds are asked for in front of the angles.  (8,192 tokens of 16 + 16 heads of 128: bound by instructions, 93 us, until the quotient
-// was formed by a product and a remainder, q's rows went past the quantising, and the rows came ahead.)
+// A block takes one token: its angles' sines and cosines, once, then its heads by groups of hd / 8 lanes, eight values a lane.  Two layouts:
+//   SPLIT (the whole head is rotated by halves)   a lane has values 4 l .. + 3 of either half: a pair's two values lie in one lane, and two lanes
+//                                                 put their nibbles together to two words;
+//   else                                          a lane has eight values in a row, one word; a pair's other half comes by a shuffle where halves lie a
+//                                                 multiple of eight values apart, else through shared memory.
+// The rows of the first W_AHEAD rounds are asked for in front of the angles.  Bound by instructions (8,192 tokens of 16 + 16 heads of 128, of which the
+// bytes alone take 26 us: 93 us with divisions and all rows through the quantising, 64 with a product and a remainder in their place).
 #define W_THREADS 256
 #define W_AHEAD 3
-__device__ __forceinline__ uint32_t q4_word(const float* x, float scale, float mid) {
-    if (scale == 0.f) return 0x88888888u;
-    if (scale < 1e-30f) {   // (no reciprocal to rely on)
-        uint32_t word = 0;
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// a row's factors, of all its lanes' values (NaN or an infinity among them: not a number)
+template <int GL>
+__device__ __forceinline__ void q4_row_factors(const float* x, float& scale, float& mid, bool& bad) {
+    float lo = min3_nan(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
+    lo = min3_nan(lo, x[3], x[4]); hi = max3_nan(hi, x[3], x[4]);
+    lo = min3_nan(lo, x[5], x[6]); hi = max3_nan(hi, x[5], x[6]);
+    lo = min3_nan(lo, x[7], x[7]); hi = max3_nan(hi, x[7], x[7]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word |= static_cast<uint32_t>(fminf(fmaxf(floorf((x[i] - mid) / scale), -8.f), 7.f) + 8.f) << q4_shift(i);
-        return word;
+    for (int m = 1; m < GL; m <<= 1) {
+        const float l = __shfl_xor_sync(0xffffffffu, lo, m), h = __shfl_xor_sync(0xffffffffu, hi, m);
+        lo = min3_nan(lo, l, l);
+        hi = max3_nan(hi, h, h);
     }
-    // cell = floor((x - mid) / scale): the nearest whole number to the quotient, formed by the reciprocal, and one less where the remainder is negative
-    const float inv = 1.f / scale;
-    float half[2] = {0.f, 0.f};
+    bad = !(hi <= 3.402823466e38f && lo >= -3.402823466e38f);
+    scale = to_f(from_f<bf16>((0.5f * hi - 0.5f * lo) / 7.5f));
+    mid = to_f(from_f<bf16>(0.5f * lo + 0.5f * hi));
+}
+// N codes (N a power of two) into their places in a word: code i goes to bit at(i).
+// floor((x - mid) / scale): the quotient by the reciprocal, raised by 2^-22 of itself, which is more than its rounding took off (so that a whole
+// quotient counts as one; two bfloat16 and their difference never give a quotient that close below a whole number), plus 3 2^22, rounded down.
+template <int N, typename At>
+__device__ __forceinline__ uint32_t q4_codes(const float* x, float scale, float mid, At&& at) {
+    uint32_t word = 0;
+    if (scale >= 1e-30f) {
+        const float inv = 1.f / scale, more = inv * 2.384185791e-07f;
 #pragma unroll
-    for (int i = 6; i >= 0; i -= 2)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            const float d = x[i + y] - mid;
-            const float near = (fminf(fmaxf(d * inv, -9.f), 9.f) + 12582912.f) - 12582912.f;
-            const float cell = fmaf(-near, scale, d) < 0.f ? near - 1.f : near;
-            half[y] = fmaf(half[y], 16.f, fminf(fmaxf(cell, -8.f), 7.f) + 8.f);   // (nibbles of the word's halves: whole numbers below 2^16)
+        for (int i = 0; i < N; ++i) {
+            const float d = x[i] - mid;
+            const int cell = __float_as_int(__fadd_rd(fmaf(fabsf(d), more, d * inv), 12582912.f)) - (0x4b400000 - 8);
+            word += static_cast<uint32_t>(max(min(cell, 15), 0)) << at(i);
         }
-    return static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
+    } else {   // (no reciprocal to rely on; a row of equal values; not a number)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float c = scale > 0.f ? floorf((x[i] - mid) / scale) : 0.f;
+            word += static_cast<uint32_t>(fminf(fmaxf(c, -8.f), 7.f) + 8.f) << at(i);
+        }
+    }
+    return word;
+}
+__device__ __forceinline__ void load4(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void load4(const bf16* p, float* v) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
+    v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(bf16* p, const float* v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict__ qkv, const int* __restrict__ positions,
+template <typename T, int HD, bool SPLIT>
+__global__ void __launch_bounds__(W_THREADS, 4) q4_write_kernel(const T* __restrict__ qkv, const int* __restrict__ positions,
                                                             const float* __restrict__ inv_freq, T* __restrict__ q_out,
                                                             uint8_t* __restrict__ pool, const int* __restrict__ slots,
                                                             float* __restrict__ weights, int nh, int nkv, int rot, int pairing, int P,
                                                             int write_kv) {
     constexpr int GL = HD / 8;            // lanes of a row
     constexpr int ROWS = W_THREADS / GL;  // rows of the block at a time
-    __shared__ float cs[HD / 2], sn[HD / 2];
+    __shared__ __align__(16) float cs[HD / 2], sn[2][HD / 2];   // sines, negative and as they are
     extern __shared__ __align__(16) float stage[];   // W_THREADS * 8 floats where halves lie apart by other than a multiple of eight
     const int t = blockIdx.x, tid = threadIdx.x;
-    const int half = rot / 2;
+    const int half = SPLIT ? HD / 2 : rot / 2;
     const int slot = slots ? slots[t] : 0;
     const int page = slot / P, off = slot - page * P;
     const int n_rows = nh + (write_kv ? 2 * nkv : 0);
-    const int g = tid / GL, l = tid % GL, d0 = 8 * l;
+    const int g = tid / GL, l = tid % GL, d0 = SPLIT ? 4 * l : 8 * l;
     const T* src = qkv + static_cast<size_t>(t) * (nh + 2 * nkv) * HD + d0;
-    const bool staged = pairing == 0 && half % 8 != 0;
+    T* const q_row = q_out + static_cast<size_t>(t) * nh * HD + d0;
+    const bool staged = !SPLIT && pairing == 0 && half % 8 != 0;
+    uint8_t* const page_bytes = pool + q4_place(page, 0, 0, nkv, P, HD);
+    const unsigned head_bytes = static_cast<unsigned>(P) * (HD / 2 + Q4_FACTOR_BYTES);
     // (positions, slots and frequencies were there before the kernel in front)
     pdl_entry();
     pdl_trigger();
-    float x[W_AHEAD][8];
+    float x[W_AHEAD][8];   // SPLIT: four of the lower half, four of the upper
     auto load = [&](int r, float* v) {
-        if (r < n_rows) load8(src + static_cast<size_t>(r) * HD, v);
-        else
+        if (r >= n_rows) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        } else if (SPLIT) {
+            load4(src + static_cast<size_t>(r) * HD, v);
+            load4(src + static_cast<size_t>(r) * HD + HD / 2, v + 4);
+        } else {
+            load8(src + static_cast<size_t>(r) * HD, v);
+        }
     };
 #pragma unroll
     for (int u = 0; u < W_AHEAD; ++u) load(u * ROWS + g, x[u]);
     if (tid < half) {
         const double turns = static_cast<double>(positions[t]) * static_cast<double>(inv_freq[tid]) * 0.15915494309189533577;
-        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn[tid], &cs[tid]);
+        float s;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &cs[tid]);
+        sn[0][tid] = -s;
+        sn[1][tid] = s;
     }
     __syncthreads();
     auto row = [&](int r, float* x) {
-        if (rot > 0) {   // (q and k; rows of v beside rows of k take the shuffles with them and keep their values)
-            const bool turn = r < nh + nkv;
+        const bool turn = r < nh + nkv;   // (q and k)
+        if constexpr (SPLIT) {
+            if (turn) {
+                float c[4], s[4];
+                load4(cs + d0, c);
+                load4(sn[1] + d0, s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = x[i], b = x[4 + i];
+                    x[i] = a * c[i] - b * s[i];
+                    x[4 + i] = a * s[i] + b * c[i];
+                }
+            }
+        } else if (half > 0 && __any_sync(0xffffffffu, turn)) {   // (rows of v beside rows of k take the shuffles with them and keep their values)
             if (pairing == 1) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int p = d0 / 2 + i;
                     if (turn && p < half) {
-                        const float c = cs[p], s = sn[p], a = x[2 * i], b = x[2 * i + 1];
+                        const float c = cs[p], s = sn[1][p], a = x[2 * i], b = x[2 * i + 1];
                         x[2 * i] = a * c - b * s;
                         x[2 * i + 1] = a * s + b * c;
                     }
@@ -122,11 +190,14 @@ __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict
                 const int lane = tid & 31, other = d0 < rot ? (lane - l) + (low ? l + half / 8 : l - half / 8) : lane;
                 const bool in = turn && d0 < rot;
                 const int p = low ? d0 : d0 - half;
-                const float sign = low ? -1.f : 1.f;
+                float y[8], c[8], s[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float y = __shfl_sync(0xffffffffu, x[i], other);
-                    if (in) x[i] = fmaf(x[i], cs[p + i], sign * y * sn[p + i]);
+                for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], other);
+                if (in) {
+                    load8(cs + p, c);
+                    load8(sn[low ? 0 : 1] + p, s);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], c[i], y[i] * s[i]);
                 }
             } else {
                 float* mine = stage + static_cast<size_t>(g) * HD;
@@ -137,36 +208,44 @@ __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int d = d0 + i;
-                        if (d < half) x[i] = x[i] * cs[d] - mine[d + half] * sn[d];
-                        else if (d < rot) x[i] = mine[d - half] * sn[d - half] + x[i] * cs[d - half];
+                        if (d < half) x[i] = x[i] * cs[d] - mine[d + half] * sn[1][d];
+                        else if (d < rot) x[i] = mine[d - half] * sn[1][d - half] + x[i] * cs[d - half];
                     }
                 __syncwarp();
             }
         }
-        if (r < nh) store8(q_out + (static_cast<size_t>(t) * nh + r) * HD + d0, x);
-        if (!__any_sync(0xffffffffu, r >= nh && r < n_rows)) return;   // (a warp of q's rows alone)
-        float lo = x[0], hi = x[0], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
-            sum = fmaf(x[i], 0.f, sum);   // NaN if a value is not finite
+        if (r < nh) {
+            if (SPLIT) {
+                store4(q_row + static_cast<size_t>(r) * HD, x);
+                store4(q_row + static_cast<size_t>(r) * HD + HD / 2, x + 4);
+            } else {
+                store8(q_row + static_cast<size_t>(r) * HD, x);
+            }
         }
-        if (sum != 0.f) hi = INFINITY;
-#pragma unroll
-        for (int m = 1; m < GL; m <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+        if (!__any_sync(0xffffffffu, r >= nh && r < n_rows)) return;   // (a warp of q's rows alone)
+        float scale, mid;
+        bool bad;
+        q4_row_factors<GL>(x, scale, mid, bad);
+        uint32_t word;
+        int place;   // of the word in its row
+        if constexpr (SPLIT) {
+            // values 4 l .. + 3 of a half: the even lane's are its word's first four (nibbles 0, 4, 1, 5), the odd lane's the last (2, 6, 3, 7)
+            const int odd = l & 1;
+            auto at = [&](int i) { return 16 * (i & 1) + 4 * (i >> 1) + 8 * odd; };
+            const uint32_t low = q4_codes<4>(x, scale, mid, at), high = q4_codes<4>(x + 4, scale, mid, at);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? low : high, 1);   // the even lane stores the lower half's word
+            word = (odd ? high : low) | other;
+            place = (l >> 1) + odd * (GL / 2);
+        } else {
+            word = q4_codes<8>(x, scale, mid, [](int i) { return q4_shift(i); });
+            place = l;
         }
         if (r < nh || r >= n_rows) return;
-        const int plane = r >= nh + nkv, h = r - nh - (plane ? nkv : 0);
-        const float scale = to_f(from_f<bf16>((0.5f * hi - 0.5f * lo) / 7.5f)), mid = to_f(from_f<bf16>(0.5f * lo + 0.5f * hi));
-        uint8_t* at = pool + q4_place(page, plane, h, nkv, P, HD);
-        reinterpret_cast<uint32_t*>(at + static_cast<size_t>(off) * (HD / 2))[l] = q4_word(x, scale, mid);
+        uint8_t* at = page_bytes + static_cast<unsigned>(r - nh) * head_bytes;   // (planes and heads lie as the rows of k and v do)
+        reinterpret_cast<uint32_t*>(at + off * (HD / 2))[place] = word;
         if (l == 0) {
-            reinterpret_cast<uint32_t*>(at + static_cast<size_t>(P) * (HD / 2))[off] =
-                hi == INFINITY ? 0x7fff7fffu : q4_factors(scale, mid);
-            if (weights && plane == 0) weights[(static_cast<size_t>(page) * nkv + h) * P + off] = 0.f;
+            reinterpret_cast<uint32_t*>(at + P * (HD / 2))[off] = bad ? 0x7fff7fffu : q4_factors(scale, mid);
+            if (weights && r < nh + nkv) weights[(static_cast<size_t>(page) * nkv + (r - nh)) * P + off] = 0.f;
         }
     };
     for (int r0 = 0; r0 < n_rows; r0 += W_AHEAD * ROWS) {
@@ -183,14 +262,21 @@ __global__ void __launch_bounds__(W_THREADS) q4_write_kernel(const T* __restrict
 template <typename T>
 static int write_launch(const void* qkv, const int* positions, const float* inv_freq, void* q_out, uint8_t* pool, const int* slots,
                         float* weights, int n, int nh, int nkv, int hd, int rot, int pairing, int P, int write_kv, cudaStream_t stream) {
-    const bool staged = pairing == 0 && (rot / 2) % 8 != 0;
-#define Q4_WRITE(HD_)                                                                                                               \
-    locus_launch(q4_write_kernel<T, HD_>, n, W_THREADS, staged ? W_THREADS * 8 * sizeof(float) : 0, stream, static_cast<const T*>(qkv), positions, inv_freq,                \
-                 static_cast<T*>(q_out), pool, slots, weights, nh, nkv, rot, pairing, P, write_kv)
+    const bool staged = pairing == 0 && (rot / 2) % 8 != 0, split = pairing == 0 && rot == hd;
+#define Q4_WRITE_S(HD_, SPLIT_)                                                                                                         \
+    locus_launch(q4_write_kernel<T, HD_, SPLIT_>, n, W_THREADS, staged ? W_THREADS * 8 * sizeof(float) : 0, stream,                    \
+                 static_cast<const T*>(qkv), positions, inv_freq, static_cast<T*>(q_out), pool, slots, weights, nh, nkv, rot, pairing, \
+                 P, write_kv)
+#define Q4_WRITE(HD_)                     \
+    do {                                  \
+        if (split) Q4_WRITE_S(HD_, true); \
+        else Q4_WRITE_S(HD_, false);      \
+    } while (0)
     if (hd == 64) Q4_WRITE(64);
     else if (hd == 128) Q4_WRITE(128);
     else Q4_WRITE(256);
 #undef Q4_WRITE
+#undef Q4_WRITE_S
     return locus_launch_status();
 }
 
@@ -331,16 +417,15 @@ extern "C" int locus_expand_q4(const Q4ExpandCall* call, cudaStream_t stream) {
 // `keep` in all; of equal weights the earlier key counts as the heavier one, and a weight that is not a number as lighter than all others.
 // kept [layers][n_items][nkv][keep]: their indices, ascending; -1 behind a request of fewer than `keep` tokens, all of which stay.
 //
-// One block per (layer, request, head).  The weights are read once, as unsigned numbers of the same order, into shared memory where they fit (SK_MAX; else
-// from memory, the L2, in every pass).  The weight of the last key that stays is found by histograms of S_BINS bins over the range of numbers that
-// it must lie in, at first from the smallest to the largest, then one bin of the pass before: three passes at most, mostly two, and only keys of that
-// range are counted, so that bins are hit evenly and seldom by a warp's lanes at once.  Then every warp takes a run of keys, counts those that stay,
-// and behind a sum over the warps writes their indices in order.
-// (24 layers of 16 heads of one request of 4,096 tokens: with a fixed cut of the 32 bits by 11, 11 and 10 and blocks of 1,024 threads 31 us, most
-// of it atomics on the few bins that exponents hit.)
+// One block per (layer, request, head).  The weights are read once, as unsigned numbers of the same order: into registers, a run of KPT x 32 keys a warp,
+// where the block's threads hold them, else into shared memory (SK_MAX), else from memory (the L2) in every pass.  The weight of the last key that
+// stays is found by histograms of S_BINS bins over the range of numbers that it must lie in, at first from the smallest to the largest, then one bin
+// of the pass before: three passes at most, mostly two, and only keys of that range are counted, so that bins are hit evenly and seldom by a
+// warp's lanes at once.  Then every warp counts the keys of its run that stay, and behind a sum over the warps writes their indices in order.
+// (24 layers of 16 heads of one request of 4,096 tokens: a fixed cut of the 32 bits by 11, 11 and 10 and blocks of 1,024 threads 31 us, most of it
+// atomics on the few bins that exponents hit; by ranges, blocks of 256 threads with the keys in shared memory 24.)
 #define SK_MAX 49152      // weights in shared memory (192 KB)
 #define S_BINS 2048
-#define S_SHORT 8192      // up to so many keys: blocks of 256 threads, several to an SM; else 1,024
 
 // an unsigned number of the weight's order
 __device__ __forceinline__ uint32_t ordered(float w) {
@@ -351,12 +436,14 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 // t / P for t and 2^40 / P below 2^27 and 2^37: a multiplication by ceil(2^40 / P)
 __device__ __forceinline__ int by_page(int t, unsigned long long page_inv) { return static_cast<int>((static_cast<unsigned long long>(t) * page_inv) >> 40); }
 
-template <int THREADS>
+// KPT keys of a thread in registers (n_tokens at most THREADS * KPT); 0: keys in shared memory (up to `room`) or in memory.
+template <int THREADS, int KPT>
 __global__ void __launch_bounds__(THREADS) q4_select_kernel(const float* __restrict__ weights, const int* __restrict__ block_table, int table_stride,
                                                             const int* __restrict__ n_tokens, int n_items, int nkv, int P,
                                                             unsigned long long page_inv, size_t layer_slots, int keep, int first, int recent,
                                                             int room, int* __restrict__ kept) {
     constexpr int WARPS = THREADS / 32, BT = S_BINS / THREADS;   // bins of a thread
+    constexpr uint32_t SURE = 0xffffffffu;                        // the first and the last keys (no weight maps to it), and keys behind the last
     extern __shared__ uint32_t s_keys[];
     __shared__ __align__(16) int hist[S_BINS];
     __shared__ int warp_a[WARPS], warp_b[WARPS];
@@ -366,7 +453,8 @@ __global__ void __launch_bounds__(THREADS) q4_select_kernel(const float* __restr
     pdl_entry();
     pdl_trigger();
     const int h = blockIdx.x, item = blockIdx.y, layer = blockIdx.z;
-    const int n = min(n_tokens[item], table_stride * P);
+    int n = min(n_tokens[item], table_stride * P);
+    if (KPT > 0) n = min(n, THREADS * KPT);
     int* dst = kept + ((static_cast<size_t>(layer) * n_items + item) * nkv + h) * keep;
     if (n <= keep) {
         for (int j = tid; j < keep; j += THREADS) dst[j] = j < n ? j : -1;
@@ -377,56 +465,80 @@ __global__ void __launch_bounds__(THREADS) q4_select_kernel(const float* __restr
     const size_t page_step = static_cast<size_t>(nkv) * P;
     const int lo = first, hi = n - recent;       // the keys between, of which `left` stay
     int left = keep - first - recent;
-    auto read = [&](int t) {
+    auto read = [&](int t) -> uint32_t {
+        if (t < lo || t >= hi) return SURE;
         const int at = by_page(t, page_inv), page = table[at];
         return page < 0 ? 0u : ordered(w[page * page_step + (t - at * P)]);
     };
-    const bool in_smem = hi - lo <= room;
-    auto key = [&](int t) { return in_smem ? s_keys[t - lo] : read(t); };
-    uint32_t from = 0, to = 0;    // the numbers that the last key to stay lies between
-    bool ties = false;            // keys equal to `from`: the first `left` of them stay; else all from `from` on
-    if (left > 0) {
-        uint32_t least = 0xffffffffu, most = 0u;
-        constexpr int AHEAD = 4;
-        for (int t0 = lo + tid; t0 < hi; t0 += AHEAD * THREADS) {
-            uint32_t u[AHEAD];
+    const bool in_smem = KPT == 0 && n <= room;
+    // a warp's run of keys: a .. b - 1, key i * 32 + lane of it in mine[i]
+    const int per = KPT > 0 ? KPT * 32 : ((n + WARPS - 1) / WARPS + 31) & ~31;
+    const int a = min(n, warp * per), b = min(n, a + per);
+    uint32_t mine[KPT > 0 ? KPT : 1];
+    auto each = [&](auto&& f) {   // f(key) for every key of the run: this lane's
+        if constexpr (KPT > 0) {
 #pragma unroll
-            for (int x = 0; x < AHEAD; ++x) u[x] = t0 + x * THREADS < hi ? read(t0 + x * THREADS) : 0u;
-#pragma unroll
-            for (int x = 0; x < AHEAD; ++x)
-                if (t0 + x * THREADS < hi) {
-                    least = min(least, u[x]);
-                    most = max(most, u[x]);
-                    if (in_smem) s_keys[t0 + x * THREADS - lo] = u[x];
-                }
+            for (int i = 0; i < KPT; ++i) f(mine[i]);
+        } else {
+#pragma unroll 4
+            for (int t = a + lane; t < b; t += 32) f(in_smem ? s_keys[t] : read(t));
         }
+    };
+    if constexpr (KPT > 0) {
+        // pages first, then weights: eight of either on their way together
+#pragma unroll
+        for (int i0 = 0; i0 < KPT; i0 += 8) {
+            int page[8];
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = a + (i0 + i) * 32 + lane;
+                page[i] = t >= lo && t < hi ? table[by_page(t, page_inv)] : -2;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = a + (i0 + i) * 32 + lane;
+                v[i] = page[i] >= 0 ? w[page[i] * page_step + (t - by_page(t, page_inv) * P)] : __int_as_float(0x7fffffff);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mine[i0 + i] = page[i] == -2 ? SURE : ordered(v[i]);
+        }
+    } else if (in_smem) {
+#pragma unroll 4
+        for (int t = a + lane; t < b; t += 32) s_keys[t] = read(t);
+    }
+    uint32_t from = SURE - 1, to = 0;   // the numbers that the last key to stay lies between
+    bool ties = false;                  // keys equal to `from`: the first `left` of them stay; else all from `from` on
+    if (left > 0) {
+        uint32_t least = SURE, most = 0u;
+        each([&](uint32_t u) {
+            least = min(least, u);
+            if (u != SURE) most = max(most, u);
+        });
         least = __reduce_min_sync(0xffffffffu, least);
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) {
             warp_lo[warp] = least;
             warp_hi[warp] = most;
         }
+        for (int i = tid; i < S_BINS / 4; i += THREADS) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
         __syncthreads();
-        from = __reduce_min_sync(0xffffffffu, lane < WARPS ? warp_lo[lane] : 0xffffffffu);
+        from = __reduce_min_sync(0xffffffffu, lane < WARPS ? warp_lo[lane] : SURE);
         to = __reduce_max_sync(0xffffffffu, lane < WARPS ? warp_hi[lane] : 0u);
         while (true) {
             const uint32_t span = to - from;
-            const int shift = span ? max(0, 32 - __clz(span) - 11) : 0;   // (span >> shift) < 2048
-#pragma unroll
-            for (int i = 0; i < BT; ++i) hist[tid + i * THREADS] = 0;
-            __syncthreads();
-#pragma unroll 4
-            for (int t = lo + tid; t < hi; t += THREADS) {
-                const uint32_t u = key(t) - from;
+            const int shift = span ? max(0, 32 - __clz(span) - 11) : 0;   // (span >> shift) < S_BINS
+            each([&](uint32_t u) {
+                u -= from;
                 if (u <= span) atomicAdd(&hist[u >> shift], 1);
-            }
+            });
             __syncthreads();
             // keys in higher bins, from the top: thread i has bins from S_BINS - 1 - BT i down
-            int mine[BT], run = 0;
+            int bins[BT], run = 0;
 #pragma unroll
             for (int i = 0; i < BT; ++i) {
-                mine[i] = hist[S_BINS - 1 - BT * tid - i];
-                run += mine[i];
+                bins[i] = hist[S_BINS - 1 - BT * tid - i];
+                run += bins[i];
             }
             const int own_sum = run;
 #pragma unroll
@@ -439,14 +551,16 @@ __global__ void __launch_bounds__(THREADS) q4_select_kernel(const float* __restr
             int before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_a[lane] : 0) + run - own_sum;   // keys above this thread's bins
 #pragma unroll
             for (int i = 0; i < BT; ++i) {
-                if (before < left && before + mine[i] >= left) {
+                if (before < left && before + bins[i] >= left) {
                     chosen_bin = S_BINS - 1 - BT * tid - i;
                     above_bin = before;
+                    warp_b[0] = bins[i];
                 }
-                before += mine[i];
+                before += bins[i];
+                hist[S_BINS - 1 - BT * tid - i] = 0;   // (for the next pass)
             }
             __syncthreads();
-            const int bin = chosen_bin, count = hist[bin];
+            const int bin = chosen_bin, count = warp_b[0];
             left -= above_bin;
             from += static_cast<uint32_t>(bin) << shift;
             to = from + min(to - from, (1u << shift) - 1u);
@@ -455,65 +569,52 @@ __global__ void __launch_bounds__(THREADS) q4_select_kernel(const float* __restr
                 ties = true;
                 break;
             }
-            __syncthreads();            // (hist is cleared again)
         }
-    } else {
-        from = 0xffffffffu;             // none of those between stays
-        ties = true;
+        __syncthreads();
     }
-    // keys from `from` on stay, of those equal to it with `ties` only the first `left`
-    const int per = ((n + WARPS - 1) / WARPS + 31) & ~31;
-    const int a = min(n, warp * per), b = min(n, a + per);
-    auto look = [&](int t, bool& stays, bool& tie) {
-        stays = t < b && (t < lo || t >= hi);
-        tie = false;
-        if (t < b && !stays) {
-            const uint32_t u = key(t);
-            tie = ties && u == from;
-            stays = u >= from && !tie;
-        }
-    };
+    // of the keys between those from `from` on stay, of those equal to it with `ties` only the first `left`
     int n_stay = 0, n_tie = 0;
-    if (left > 0 || !ties) {
-        for (int t0 = a; t0 < b; t0 += 32) {
-            bool s, e;
-            look(t0 + lane, s, e);
-            n_stay += s;
-            n_tie += e;
-        }
-    } else {   // (first and recent alone)
-        for (int t0 = a; t0 < b; t0 += 32) n_stay += t0 + lane < b && (t0 + lane < lo || t0 + lane >= hi);
+    each([&](uint32_t u) {
+        const bool tie = ties && u == from;
+        n_stay += u >= from && !tie;
+        n_tie += tie;
+    });
+    if constexpr (KPT > 0) {   // (less the places behind the last key)
+        int dead = 0;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) dead += a + i * 32 + lane >= b;
+        n_stay -= dead;
     }
     n_stay = __reduce_add_sync(0xffffffffu, n_stay);
     n_tie = __reduce_add_sync(0xffffffffu, n_tie);
-    __syncthreads();
     if (lane == 0) {
         warp_a[warp] = n_stay;
         warp_b[warp] = n_tie;
     }
     __syncthreads();
     // ties taken and keys written by the warps in front
-    int taken = 0, at = 0;
-    for (int v = 0; v < warp; ++v) {
-        at += warp_a[v] + max(0, min(warp_b[v], left - taken));
-        taken += warp_b[v];
-    }
+    int taken = __reduce_add_sync(0xffffffffu, lane < warp ? warp_b[lane] : 0);
+    int at = __reduce_add_sync(0xffffffffu, lane < warp ? warp_a[lane] : 0) + min(taken, max(left, 0));
     const uint32_t below = (1u << lane) - 1;
-    const bool none = left <= 0 && ties;
-    for (int t0 = a; t0 < b; t0 += 32) {
-        bool s, e = false;
-        if (none) s = t0 + lane < b && (t0 + lane < lo || t0 + lane >= hi);
-        else look(t0 + lane, s, e);
-        uint32_t in_mask;
-        bool in = s;
+    int t = a + lane;
+    auto put = [&](uint32_t u) {
+        const bool tie = ties && u == from;
+        bool in = t < b && u >= from && !tie;
         if (ties) {
-            const uint32_t tie_mask = __ballot_sync(0xffffffffu, e);
-            in = s || (e && taken + __popc(tie_mask & below) < left);
+            const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
+            in = in || (tie && taken + __popc(tie_mask & below) < left);
             taken += __popc(tie_mask);
         }
-        in_mask = __ballot_sync(0xffffffffu, in);
-        if (in) dst[at + __popc(in_mask & below)] = t0 + lane;
-        at += __popc(in_mask);
+        const uint32_t mask = __ballot_sync(0xffffffffu, in);
+        if (in) dst[at + __popc(mask & below)] = t;
+        at += __popc(mask);
+        t += 32;
+    };
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) put(mine[i]);
+    } else {
+        for (int t0 = a; t0 < b; t0 += 32) put(t0 + lane >= b ? 0u : in_smem ? s_keys[t0 + lane] : read(t0 + lane));
     }
 }
 
@@ -553,60 +654,58 @@ __global__ void __launch_bounds__(M_THREADS) q4_move_kernel(uint8_t* pool, float
     float* w = weights + static_cast<size_t>(layer) * layer_slots;
     auto place = [&](int page) { return base + q4_place(page, plane, h, nkv, P, HD); };
 
-    uint4 piece[M_UNROLL];
-    uint32_t fac[FU];
-    float wt[FU];
-    bool has[M_UNROLL], fhas[FU];
+    // a row's old and new place in its layer, in pieces (of 16 bytes); rows without a page: none
+    constexpr unsigned NONE = 0xffffffffu;
+    __shared__ uint2 places[TILE];
+    const unsigned page_pieces = 2u * nkv * P * (HD / 2 + Q4_FACTOR_BYTES) / 16;
+    const unsigned head_pieces = (static_cast<unsigned>(plane) * nkv + h) * (P * (HD / 2 + Q4_FACTOR_BYTES) / 16);
     for (int j0 = part * TILE; j0 < n; j0 += n_parts * TILE) {
-        int t[M_UNROLL];
-#pragma unroll
-        for (int u = 0; u < M_UNROLL; ++u) {
-            const int j = j0 + (u * M_THREADS + tid) / PR;
-            t[u] = j < n ? idx[j] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < M_UNROLL; ++u) {
-            const int at = by_page(max(t[u], 0), page_inv), page = t[u] >= 0 ? table[at] : -1;
-            has[u] = page >= 0;
-            if (has[u]) piece[u] = ld_row(place(page) + static_cast<size_t>(t[u] - at * P) * (HD / 2) + (tid % PR) * 16);
-        }
+        uint32_t fac[FU];
+        float wt[FU];
+        int new_page[FU], new_off[FU];
 #pragma unroll
         for (int u = 0; u < FU; ++u) {
             const int e = u * M_THREADS + tid, j = j0 + e;
-            fhas[u] = false;
-            if (e < TILE && j < n) {
-                const int s = idx[j], at = by_page(s, page_inv), page = table[at], off = s - at * P;
-                fhas[u] = page >= 0;
-                if (fhas[u]) {
-                    fac[u] = reinterpret_cast<const uint32_t*>(place(page) + static_cast<size_t>(P) * (HD / 2))[off];
-                    if (plane == 0) wt[u] = w[(static_cast<size_t>(page) * nkv + h) * P + off];
+            new_page[u] = -1;
+            if (e < TILE) {
+                uint2 at = make_uint2(NONE, NONE);
+                if (j < n) {
+                    const int s = idx[j], sp = by_page(max(s, 0), page_inv), so = s - sp * P, page = s < 0 ? -1 : table[sp];
+                    const int dp = by_page(j, page_inv), dpage = to[dp];
+                    if (page >= 0 && dpage >= 0) {
+                        at = make_uint2(page * page_pieces + head_pieces + so * PR, dpage * page_pieces + head_pieces + (j - dp * P) * PR);
+                        fac[u] = reinterpret_cast<const uint32_t*>(place(page) + P * (HD / 2))[so];
+                        if (plane == 0) wt[u] = w[(static_cast<size_t>(page) * nkv + h) * P + so];
+                        new_page[u] = dpage;
+                        new_off[u] = j - dp * P;
+                    }
                 }
+                places[e] = at;
             }
         }
         __syncthreads();
+        uint4 piece[M_UNROLL];
+        unsigned dst[M_UNROLL];
 #pragma unroll
         for (int u = 0; u < M_UNROLL; ++u) {
-            const int j = j0 + (u * M_THREADS + tid) / PR;
-            if (has[u]) {
-                const int at = by_page(j, page_inv), page = to[at];
-                if (page >= 0) *reinterpret_cast<uint4*>(place(page) + static_cast<size_t>(j - at * P) * (HD / 2) + (tid % PR) * 16) = piece[u];
-            }
+            const uint2 at = places[(u * M_THREADS + tid) / PR];
+            dst[u] = at.y;
+            if (at.x != NONE) piece[u] = ld_row(base + (static_cast<size_t>(at.x) + tid % PR) * 16);
         }
+        __syncthreads();   // (in place: every row of the tile is read before one is written; and `places` is free)
 #pragma unroll
-        for (int u = 0; u < FU; ++u) {
-            const int j = j0 + u * M_THREADS + tid;
-            if (fhas[u]) {
-                const int at = by_page(j, page_inv), page = to[at], off = j - at * P;
-                if (page >= 0) {
-                    reinterpret_cast<uint32_t*>(place(page) + static_cast<size_t>(P) * (HD / 2))[off] = fac[u];
-                    if (plane == 0) w[(static_cast<size_t>(page) * nkv + h) * P + off] = wt[u];
-                }
+        for (int u = 0; u < M_UNROLL; ++u)
+            if (dst[u] != NONE) *reinterpret_cast<uint4*>(base + (static_cast<size_t>(dst[u]) + tid % PR) * 16) = piece[u];
+#pragma unroll
+        for (int u = 0; u < FU; ++u)
+            if (new_page[u] >= 0) {
+                reinterpret_cast<uint32_t*>(place(new_page[u]) + P * (HD / 2))[new_off[u]] = fac[u];
+                if (plane == 0) w[(static_cast<size_t>(new_page[u]) * nkv + h) * P + new_off[u]] = wt[u];
             }
-        }
     }
 }
 
-// max_tokens: at least the tokens of the longest request (its weights' place in shared memory is sized by it).
+// max_tokens: at least the tokens of the longest request (a request's tokens behind that are not seen).  A layer of at most 64 GB.
 struct Q4EvictCall {
     void* pool;
     float* weights;
@@ -621,27 +720,29 @@ extern "C" int locus_evict_q4(const Q4EvictCall* call, cudaStream_t stream) {
     const int first = static_cast<int>(v.first), recent = static_cast<int>(v.recent), max_tokens = static_cast<int>(v.max_tokens);
     const int n_items = static_cast<int>(v.n_items), table_stride = static_cast<int>(v.table_stride), dst_stride = static_cast<int>(v.dst_stride);
     if (!q4_head_ok(hd) || nkv <= 0 || P <= 0 || P % 16 != 0 || keep <= 0 || first < 0 || recent < 0 || first > keep - recent ||
-        n_items > 65535 || v.n_layers > 65535 || !aligned16(v.pool) || max_tokens <= 0)
+        n_items > 65535 || v.n_layers > 65535 || !aligned16(v.pool) || max_tokens <= 0 || max_tokens >= 1 << 27 ||
+        static_cast<unsigned long long>(v.layer_pages) * 2 * nkv * P * q4_row_bytes(hd) / 16 >= 0xffffffffull)
         return LOCUS_ERR_UNSUPPORTED;
     const size_t slots = static_cast<size_t>(v.layer_pages) * nkv * P, bytes = slots * 2 * q4_row_bytes(hd);
-    const int between = max(0, max_tokens - first - recent);
     const dim3 grid(nkv, n_items, static_cast<unsigned>(v.n_layers));
-    const int room = between <= SK_MAX ? between : 0;   // (longer ones are read from memory in every pass)
     static unsigned long long asked = 0;   // devices that know of the kernel's shared memory (asked again at worst)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return static_cast<int>(cudaGetLastError());
     if (dev >= 64 || !(asked >> dev & 1)) {
-        if (cudaFuncSetAttribute(q4_select_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_MAX * 4) != cudaSuccess)
+        if (cudaFuncSetAttribute(q4_select_kernel<1024, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_MAX * 4) != cudaSuccess)
             return static_cast<int>(cudaGetLastError());
         if (dev < 64) asked |= 1ull << dev;
     }
     const unsigned long long page_inv = ((1ull << 40) + P - 1) / P;
-    if (between <= S_SHORT)
-        locus_launch(q4_select_kernel<256>, grid, 256, static_cast<size_t>(room) * 4, stream, v.weights, v.block_table, table_stride, v.n_tokens,
-                     n_items, nkv, P, page_inv, slots, keep, first, recent, room, v.kept);
-    else
-        locus_launch(q4_select_kernel<1024>, grid, 1024, static_cast<size_t>(room) * 4, stream, v.weights, v.block_table, table_stride, v.n_tokens,
-                     n_items, nkv, P, page_inv, slots, keep, first, recent, room, v.kept);
+#define Q4_SELECT(THREADS_, KPT_, ROOM_)                                                                                                    \
+    locus_launch(q4_select_kernel<THREADS_, KPT_>, grid, THREADS_, static_cast<size_t>(ROOM_) * 4, stream, v.weights, v.block_table,        \
+                 table_stride, v.n_tokens, n_items, nkv, P, page_inv, slots, keep, first, recent, ROOM_, v.kept)
+    if (max_tokens <= 256 * 8) Q4_SELECT(256, 8, 0);
+    else if (max_tokens <= 256 * 16) Q4_SELECT(256, 16, 0);
+    else if (max_tokens <= 512 * 16) Q4_SELECT(512, 16, 0);
+    else if (max_tokens <= 1024 * 16) Q4_SELECT(1024, 16, 0);
+    else Q4_SELECT(1024, 0, (max_tokens <= SK_MAX ? max_tokens : 0));
+#undef Q4_SELECT
     const int code = locus_launch_status();
     if (code) return code;
     const int tile = M_THREADS * M_UNROLL / (hd / 32);
