@@ -18,6 +18,11 @@ the step function the native object that assembles a step's descriptors from the
 
 Device layout of a group: ``pool[call, page, 0=K|1=V, kv_head, slot_in_page, head_dim]``;
 a layer call sees ``pool[call]``.  A page id means the same page in every call of the group.
+
+``kv_bits`` 4: rows are held in 4 bits (``kernels.rope_kv_write_q4``), the pool is bytes, ``pool[call, page, 0=K|1=V, kv_head, :]``.
+``weigh``: beside it lie the attention weights that every cached key has received, ``weights[call, page, kv_head, slot_in_page]``, by
+which :meth:`CacheManager.evict` chooses the keys that a request lets go of.  A request that was evicted from holds fewer tokens than
+its positions count (``SeqCache.position``); each layer and head keeps tokens of its own.
 """
 from __future__ import annotations
 
@@ -26,6 +31,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .. import kernels as K
 from ..engine.batch import LayerCache
 from ..parts.base import PagedKvSpec, StateSpec
 from . import native
@@ -56,6 +62,11 @@ class SeqCache:
         return max(0, self._cache._lib.locus_cache_n_tokens(self._cache._core, self._handle))
 
     @property
+    def position(self) -> int:
+        """Position of the next token: the cached tokens and the evicted ones together."""
+        return max(0, self._cache._lib.locus_cache_position(self._cache._core, self._handle))
+
+    @property
     def state_slot(self) -> int:
         return self._cache._lib.locus_cache_state_slot(self._cache._core, self._handle)
 
@@ -76,6 +87,7 @@ class _Group:
         self.n_pages = 0
         self.pool: Optional[torch.Tensor] = None    # [calls, pages, planes, kv heads, page_tokens, head_dim]
         self.extra: Optional[torch.Tensor] = None   # [calls, pages, page_tokens, extra_width]
+        self.weights: Optional[torch.Tensor] = None  # [calls, pages, kv heads, page_tokens] (``weigh``)
 
 
 class _StateSlots:
@@ -97,13 +109,15 @@ class CacheManager:
     def __init__(self, needs: Sequence[Tuple[Optional[PagedKvSpec], Optional[StateSpec], Optional[int]]], *,
                  page_tokens: int, n_pages: int, n_state_slots: int, max_seq_tokens: int,
                  dtype: torch.dtype = torch.float32, device="cpu", allocate_device: bool = True,
-                 poison: bool = False, max_step_tokens: int = 0) -> None:
+                 poison: bool = False, max_step_tokens: int = 0, kv_bits: int = 0, weigh: bool = False, bound: int = 0) -> None:
         """``needs``: per entry of the model's run order, what its mixer keeps and whose cache
         it reads.  ``n_pages``: pages of a group that keeps all tokens.  ``max_step_tokens`` > 0: the most
         tokens that one step feeds to one request; a group with a window then gets only the pages that
         ``n_state_slots`` requests can hold at once (window + step, rounded up to pages, plus one each)
         instead of ``n_pages``.  ``poison``: fill pages with NaN when they are created and when they are
-        given back (tests: a read of a stale or unwritten slot then shows in the logits)."""
+        given back (tests: a read of a stale or unwritten slot then shows in the logits).  ``kv_bits``: 0, rows in ``dtype``, or 4.
+        ``weigh`` (with 4 bits, without windows and chunks): keep what every key has received, for :meth:`evict`.  ``bound`` (with
+        ``weigh``): the most tokens that a request holds at once, a step's included; the caller evicts so that this holds."""
         if page_tokens <= 0 or n_pages < 0 or n_state_slots <= 0:
             raise ValueError("page_tokens and n_state_slots must be positive")
         self.page_tokens = page_tokens
@@ -111,6 +125,11 @@ class CacheManager:
         self.max_seq_tokens = max_seq_tokens
         self.table_width = max(1, -(-max_seq_tokens // page_tokens))
         self.dtype, self.device, self.poison = dtype, torch.device(device), poison
+        self.kv_bits, self.weigh, self.bound = int(kv_bits), bool(weigh), int(bound)
+        if self.kv_bits not in (0, 4):
+            raise ValueError(f"kv_bits {kv_bits} (known: 0, the model's type, and 4)")
+        if self.weigh and self.kv_bits != 4 or self.bound and not self.weigh:
+            raise ValueError("attention weights are kept beside a cache of 4 bits, and a bound needs them")
         self.groups: List[_Group] = []
         self._call_group: List[Optional[int]] = []
         self._call_index: List[int] = []
@@ -136,6 +155,13 @@ class CacheManager:
             self._call_group.append(gid)
             self._call_index.append(len(g.calls))
             g.calls.append(i)
+        for g in self.groups:
+            s = g.spec
+            if self.kv_bits == 4 and not (s.has_v and s.extra_width == 0 and K.q4_takes(s.head_dim, page_tokens)):
+                raise ValueError(f"a cache of 4 bits takes keys and values of heads of {', '.join(map(str, K.Q4_HEAD_DIMS))} in pages of a multiple of "
+                                 f"{K.Q4_PAGE_STEP} tokens, not {s} in pages of {page_tokens}")
+            if self.weigh and (s.window > 0 or s.chunk > 0):
+                raise ValueError("attention weights are kept for groups without a window and without chunks")
         self._lib = native.lib()
         self.max_step_tokens = max(0, int(max_step_tokens))
         for g in self.groups:
@@ -155,6 +181,10 @@ class CacheManager:
                 self._lib.locus_cache_set_keep(self._core, g.gid, g.spec.keep_first)
             if g.spec.chunk > 0 and self._lib.locus_cache_set_aligned(self._core, g.gid, g.spec.chunk) != 0:
                 raise ValueError("a cache group has either a window or chunks, not both")
+        if self.bound > 0:
+            if self._lib.locus_cache_set_bound(self._core, self.bound) != 0:
+                raise ValueError(f"a bound of {self.bound} tokens")
+            self.table_width = self._lib.locus_cache_table_width(self._core)
         assert self._lib.locus_cache_table_width(self._core) == self.table_width
         self.state_slots = _StateSlots(self)
         # (group, page) pairs that a commit or a release made free
@@ -172,18 +202,25 @@ class CacheManager:
         if allocate_device:
             for g in self.groups:
                 shape = (len(g.calls), g.n_pages, g.spec.planes, g.spec.n_kv_heads, page_tokens, g.spec.head_dim)
-                g.pool = torch.empty(shape, dtype=dtype, device=self.device)
+                if self.kv_bits == 4:
+                    shape = shape[:4] + (K.q4_page_bytes(g.spec.head_dim, page_tokens),)
+                g.pool = torch.empty(shape, dtype=torch.uint8 if self.kv_bits == 4 else dtype, device=self.device)
+                if self.weigh:
+                    g.weights = torch.zeros(shape[:2] + (g.spec.n_kv_heads, page_tokens), dtype=torch.float32, device=self.device)
                 if g.spec.extra_width > 0:
                     g.extra = torch.empty((len(g.calls), g.n_pages, page_tokens, g.spec.extra_width), dtype=dtype,
                                           device=self.device)
                 if poison:
-                    g.pool.fill_(float("nan"))
+                    g.pool.fill_(self._nothing)
                     if g.extra is not None:
                         g.extra.fill_(float("nan"))
         self._live: Dict[object, SeqCache] = {}
 
     # -- geometry -----------------------------------------------------------
     def bytes_per_token(self) -> int:
+        if self.kv_bits == 4:
+            row = lambda s: s.planes * s.n_kv_heads * (s.head_dim // 2 + 4) + (4 * s.n_kv_heads if self.weigh else 0)  # noqa: E731
+            return sum(len(g.calls) * row(g.spec) for g in self.groups)
         el = torch.empty((), dtype=self.dtype).element_size()
         return sum(len(g.calls) * g.spec.elements_per_token() * el for g in self.groups)
 
@@ -221,8 +258,11 @@ class CacheManager:
             extra = None
             if gid is not None and self.groups[gid].extra is not None:
                 extra = self.groups[gid].extra[self._call_index[i]]
+            weights = None
+            if gid is not None and self.groups[gid].weights is not None:
+                weights = self.groups[gid].weights[self._call_index[i]]
             out.append(LayerCache(group=gid, pool=pool, page_tokens=self.page_tokens,
-                                  state=self._state[i], writes=self._call_writes[i], extra=extra))
+                                  state=self._state[i], writes=self._call_writes[i], extra=extra, weights=weights))
         return out
 
     # -- requests -----------------------------------------------------------
@@ -267,7 +307,7 @@ class CacheManager:
             for i in range(0, len(pairs) - 1, 2):
                 g = self.groups[pairs[i]]
                 if g.pool is not None:
-                    g.pool[:, pairs[i + 1]].fill_(float("nan"))
+                    g.pool[:, pairs[i + 1]].fill_(self._nothing)
                     if g.extra is not None:
                         g.extra[:, pairs[i + 1]].fill_(float("nan"))
 
@@ -291,8 +331,9 @@ class CacheManager:
         self._check_open(seq)
         r = self._lib.locus_cache_ensure(self._core, seq._handle, int(n_more))
         if r == -2:
+            limit = min(self.max_seq_tokens, self.table_width * self.page_tokens) if self.bound else self.max_seq_tokens
             raise CacheError(f"request {seq.seq_id!r}: {seq.n_tokens + n_more} tokens exceed the "
-                             f"limit of {self.max_seq_tokens}")
+                             f"limit of {limit}")
         if r < 0:
             self._not_open(seq)
         return r == 1
@@ -319,6 +360,46 @@ class CacheManager:
         self.commit(seq, n)
         return True
 
+    def evict(self, seqs: Sequence[SeqCache], keep: int, first: int = 0, recent: int = 0) -> int:
+        """Let go of the keys that mattered least: of every request of ``seqs`` that holds more than ``keep`` tokens, in each layer and for each
+        key/value head the first ``first``, the last ``recent`` and the heaviest others stay, ``keep`` in all (``kernels.evict_q4``), in the
+        first slots of the request's pages; the pages behind them go back.  The requests' positions go on.  Returns how many requests
+        were evicted from."""
+        if not self.weigh:
+            raise CacheError("eviction needs a cache that keeps attention weights (weigh)")
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+            raise ValueError(f"keep {keep} with the first {first} and the last {recent}")
+        for seq in seqs:
+            self._check_open(seq)
+        if len({id(seq) for seq in seqs}) != len(seqs):
+            raise CacheError("a request appears twice in an eviction")
+        seqs = [seq for seq in seqs if seq.n_tokens > keep]
+        if not seqs:
+            return 0
+        counts = [seq.n_tokens for seq in seqs]
+        n_tokens = torch.tensor(counts, dtype=torch.int32).to(self.device)
+        for g in self.groups:
+            width = self.pages_for(max(counts))
+            rows = torch.full((len(seqs), width), -1, dtype=torch.int32)
+            for i, seq in enumerate(seqs):
+                row = self.table_row(seq, g.gid)[:width]
+                rows[i, : len(row)] = torch.tensor(row, dtype=torch.int32)
+            kept = torch.empty((len(g.calls), len(seqs), g.spec.n_kv_heads, keep), dtype=torch.int32, device=self.device)
+            K.evict_q4(g.pool, g.weights, block_table=rows.to(self.device), n_tokens=n_tokens, n_items=len(seqs), keep=keep, first=first,
+                       recent=recent, kept=kept, n_kv_heads=g.spec.n_kv_heads, head_dim=g.spec.head_dim, page_tokens=self.page_tokens,
+                       max_tokens=max(counts))
+        for seq in seqs:
+            r = self._lib.locus_cache_evict(self._core, seq._handle, keep, self._freed, len(self._freed))
+            if r < 0:
+                self._not_open(seq)
+            self._poison_freed(r)
+        return len(seqs)
+
+    @property
+    def _nothing(self):
+        """What ``poison`` fills pages with: values that read as NaN."""
+        return 255 if self.kv_bits == 4 else float("nan")
+
     def release(self, seq: SeqCache) -> None:
         """The request ends (or is preempted): everything it holds goes back."""
         self._check_open(seq)
@@ -335,7 +416,7 @@ class CacheManager:
         for i in range(n_pairs):
             g = self.groups[self._freed[2 * i]]
             if g.pool is not None:
-                g.pool[:, self._freed[2 * i + 1]].fill_(float("nan"))
+                g.pool[:, self._freed[2 * i + 1]].fill_(self._nothing)
                 if g.extra is not None:
                     g.extra[:, self._freed[2 * i + 1]].fill_(float("nan"))
 

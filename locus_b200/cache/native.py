@@ -30,6 +30,9 @@ def lib() -> ctypes.CDLL:
             "locus_cache_new": (c_void_p, [c_int, P_INT, c_int, P_INT, c_int, c_int]),
             "locus_cache_set_keep": (c_int, [c_void_p, c_int, c_int]),
             "locus_cache_set_aligned": (c_int, [c_void_p, c_int, c_int]),
+            "locus_cache_set_bound": (c_int, [c_void_p, c_int]),
+            "locus_cache_position": (c_int, [c_void_p, c_int64]),
+            "locus_cache_evict": (c_int, [c_void_p, c_int64, c_int, P_INT, c_int]),
             "locus_cache_total_pages": (c_int, [c_void_p, c_int]),
             "locus_cache_pages_needed": (c_int, [c_void_p, c_int, c_int, c_int]),
             "locus_cache_delete": (None, [c_void_p]),

@@ -40,15 +40,14 @@ __device__ __forceinline__ void store8(bf16* p, const float* v) {
 // to one turn are 64 bits (in 32 a position of 30,000 is off by up to 1/1000 of a radian, a hundredth of a cell, and codes near a border change).
 // k and v are not rounded to the model's type on the way.
 //
-// A block takes one token: its angles' sines and cosines, once, then its heads by groups of hd / 8 lanes, eight values a lane.  Two layouts:
-//   SPLIT (the whole head is rotated by halves)   a lane has values 4 l .. + 3 of either half: a pair's two values lie in one lane, and two lanes
-//                                                 put their nibbles together to two words;
-//   else                                          a lane has eight values in a row, one word; a pair's other half comes by a shuffle where halves lie a
-//                                                 multiple of eight values apart, else through shared memory.
-// The rows of the first W_AHEAD rounds are asked for in front of the angles.  Bound by instructions (8,192 tokens of 16 + 16 heads of 128, of which the
-// bytes alone take 26 us: 93 us with divisions and all rows through the quantising, 64 with a product and a remainder in their place).
-#define W_THREADS 256
-#define W_AHEAD 3
+// A block takes one token: its angles' sines and cosines, once, then its heads by groups of hd / 16 lanes, sixteen values (two words of codes) a
+// lane: eight of either half of the head where the whole head is rotated by halves (SPLIT: a pair's two values lie in one lane), else sixteen in a row
+// (a pair's other half comes by a shuffle where halves lie a multiple of sixteen values apart, else through shared memory).  The rows of the first
+// W_AHEAD rounds are asked for in front of the angles.
+// Bound by instructions (8,192 tokens of 16 + 16 heads of 128, of which the bytes alone take 26 us: 93 us with divisions and all rows through the
+// quantising, 64 with a product and a remainder in their place, 54 with eight values a lane and a row's factors formed by twice as many, now 37.)
+#define W_THREADS 128
+#define W_AHEAD 1
 __device__ __forceinline__ float min3_nan(float a, float b, float c) {
     float d;
     asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -59,95 +58,85 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// a row's factors, of all its lanes' values (NaN or an infinity among them: not a number)
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// a row's factors, of the sixteen values of each of its GL lanes (NaN or an infinity among them: `bad`)
 template <int GL>
 __device__ __forceinline__ void q4_row_factors(const float* x, float& scale, float& mid, bool& bad) {
-    float lo = min3_nan(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
-    lo = min3_nan(lo, x[3], x[4]); hi = max3_nan(hi, x[3], x[4]);
-    lo = min3_nan(lo, x[5], x[6]); hi = max3_nan(hi, x[5], x[6]);
-    lo = min3_nan(lo, x[7], x[7]); hi = max3_nan(hi, x[7], x[7]);
+    float lo = min_nan(x[0], x[1]), hi = max_nan(x[0], x[1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) {
+        lo = min3_nan(lo, x[i], x[i + 1]);
+        hi = max3_nan(hi, x[i], x[i + 1]);
+    }
 #pragma unroll
     for (int m = 1; m < GL; m <<= 1) {
-        const float l = __shfl_xor_sync(0xffffffffu, lo, m), h = __shfl_xor_sync(0xffffffffu, hi, m);
-        lo = min3_nan(lo, l, l);
-        hi = max3_nan(hi, h, h);
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
     }
     bad = !(hi <= 3.402823466e38f && lo >= -3.402823466e38f);
     scale = to_f(from_f<bf16>((0.5f * hi - 0.5f * lo) / 7.5f));
     mid = to_f(from_f<bf16>(0.5f * lo + 0.5f * hi));
 }
-// N codes (N a power of two) into their places in a word: code i goes to bit at(i).
-// floor((x - mid) / scale): the quotient by the reciprocal, raised by 2^-22 of itself, which is more than its rounding took off (so that a whole
-// quotient counts as one; two bfloat16 and their difference never give a quotient that close below a whole number), plus 3 2^22, rounded down.
-template <int N, typename At>
-__device__ __forceinline__ uint32_t q4_codes(const float* x, float scale, float mid, At&& at) {
+// The word of eight values.  floor((x - mid) / scale): the quotient by the reciprocal, raised by 2^-22 of itself, which is more than its rounding took
+// off (so that a whole quotient counts as one; two bfloat16 and their difference never give a quotient that close below a whole number), plus
+// 3 2^22, rounded down; a sum with a bound and one at zero clamps it.
+__device__ __forceinline__ uint32_t q4_word(const float* x, float scale, float mid, float inv) {
     uint32_t word = 0;
     if (scale >= 1e-30f) {
-        const float inv = 1.f / scale, more = inv * 2.384185791e-07f;
+        const float more = inv * 2.384185791e-07f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const float d = x[i] - mid;
-            const int cell = __float_as_int(__fadd_rd(fmaf(fabsf(d), more, d * inv), 12582912.f)) - (0x4b400000 - 8);
-            word += static_cast<uint32_t>(max(min(cell, 15), 0)) << at(i);
+            const int cell = __float_as_int(__fadd_rd(fmaf(fabsf(d), more, d * inv), 12582912.f));
+            word += static_cast<uint32_t>(__viaddmin_s32_relu(cell, 8 - 0x4b400000, 15)) << q4_shift(i);
         }
     } else {   // (no reciprocal to rely on; a row of equal values; not a number)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const float c = scale > 0.f ? floorf((x[i] - mid) / scale) : 0.f;
-            word += static_cast<uint32_t>(fminf(fmaxf(c, -8.f), 7.f) + 8.f) << at(i);
+            word += static_cast<uint32_t>(fminf(fmaxf(c, -8.f), 7.f) + 8.f) << q4_shift(i);
         }
     }
     return word;
 }
-__device__ __forceinline__ void load4(const float* p, float* v) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-}
-__device__ __forceinline__ void load4(const bf16* p, float* v) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
-    v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
-}
-__device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void store4(bf16* p, const float* v) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
 
 template <typename T, int HD, bool SPLIT>
-__global__ void __launch_bounds__(W_THREADS, 4) q4_write_kernel(const T* __restrict__ qkv, const int* __restrict__ positions,
+__global__ void __launch_bounds__(W_THREADS, 8) q4_write_kernel(const T* __restrict__ qkv, const int* __restrict__ positions,
                                                             const float* __restrict__ inv_freq, T* __restrict__ q_out,
                                                             uint8_t* __restrict__ pool, const int* __restrict__ slots,
                                                             float* __restrict__ weights, int nh, int nkv, int rot, int pairing, int P,
                                                             int write_kv) {
-    constexpr int GL = HD / 8;            // lanes of a row
+    constexpr int GL = HD / 16;           // lanes of a row
     constexpr int ROWS = W_THREADS / GL;  // rows of the block at a time
+    constexpr int NEXT = SPLIT ? HD / 2 : 8;   // from a lane's first eight values to its other eight
     __shared__ __align__(16) float cs[HD / 2], sn[2][HD / 2];   // sines, negative and as they are
-    extern __shared__ __align__(16) float stage[];   // W_THREADS * 8 floats where halves lie apart by other than a multiple of eight
+    extern __shared__ __align__(16) float stage[];   // W_THREADS * 16 floats where halves lie apart by other than a multiple of sixteen
     const int t = blockIdx.x, tid = threadIdx.x;
     const int half = SPLIT ? HD / 2 : rot / 2;
-    const int slot = slots ? slots[t] : 0;
-    const int page = slot / P, off = slot - page * P;
     const int n_rows = nh + (write_kv ? 2 * nkv : 0);
-    const int g = tid / GL, l = tid % GL, d0 = SPLIT ? 4 * l : 8 * l;
+    const int g = tid / GL, l = tid % GL, d0 = SPLIT ? 8 * l : 16 * l;
     const T* src = qkv + static_cast<size_t>(t) * (nh + 2 * nkv) * HD + d0;
-    T* const q_row = q_out + static_cast<size_t>(t) * nh * HD + d0;
-    const bool staged = !SPLIT && pairing == 0 && half % 8 != 0;
-    uint8_t* const page_bytes = pool + q4_place(page, 0, 0, nkv, P, HD);
-    const unsigned head_bytes = static_cast<unsigned>(P) * (HD / 2 + Q4_FACTOR_BYTES);
+    const bool staged = !SPLIT && pairing == 0 && half % 16 != 0;
     // (positions, slots and frequencies were there before the kernel in front)
     pdl_entry();
     pdl_trigger();
-    float x[W_AHEAD][8];   // SPLIT: four of the lower half, four of the upper
+    float x[W_AHEAD][16];
     auto load = [&](int r, float* v) {
-        if (r >= n_rows) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        } else if (SPLIT) {
-            load4(src + static_cast<size_t>(r) * HD, v);
-            load4(src + static_cast<size_t>(r) * HD + HD / 2, v + 4);
-        } else {
+        if (r < n_rows) {
             load8(src + static_cast<size_t>(r) * HD, v);
+            load8(src + static_cast<size_t>(r) * HD + NEXT, v + 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0.f;
         }
     };
 #pragma unroll
@@ -159,25 +148,30 @@ __global__ void __launch_bounds__(W_THREADS, 4) q4_write_kernel(const T* __restr
         sn[0][tid] = -s;
         sn[1][tid] = s;
     }
+    const int slot = slots ? slots[t] : 0;
+    const int page = slot / P, off = slot - page * P;
+    T* const q_row = q_out + static_cast<size_t>(t) * nh * HD + d0;
+    uint8_t* const page_bytes = pool + q4_place(page, 0, 0, nkv, P, HD);
+    const unsigned head_bytes = static_cast<unsigned>(P) * (HD / 2 + Q4_FACTOR_BYTES);
     __syncthreads();
     auto row = [&](int r, float* x) {
         const bool turn = r < nh + nkv;   // (q and k)
         if constexpr (SPLIT) {
             if (turn) {
-                float c[4], s[4];
-                load4(cs + d0, c);
-                load4(sn[1] + d0, s);
+                float c[8], s[8];
+                load8(cs + d0, c);
+                load8(sn[1] + d0, s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = x[i], b = x[4 + i];
+                for (int i = 0; i < 8; ++i) {
+                    const float a = x[i], b = x[8 + i];
                     x[i] = a * c[i] - b * s[i];
-                    x[4 + i] = a * s[i] + b * c[i];
+                    x[8 + i] = a * s[i] + b * c[i];
                 }
             }
         } else if (half > 0 && __any_sync(0xffffffffu, turn)) {   // (rows of v beside rows of k take the shuffles with them and keep their values)
             if (pairing == 1) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     const int p = d0 / 2 + i;
                     if (turn && p < half) {
                         const float c = cs[p], s = sn[1][p], a = x[2 * i], b = x[2 * i + 1];
@@ -187,26 +181,23 @@ __global__ void __launch_bounds__(W_THREADS, 4) q4_write_kernel(const T* __restr
                 }
             } else if (!staged) {
                 const bool low = d0 < half;
-                const int lane = tid & 31, other = d0 < rot ? (lane - l) + (low ? l + half / 8 : l - half / 8) : lane;
+                const int lane = tid & 31, other = d0 < rot ? (lane - l) + (low ? l + half / 16 : l - half / 16) : lane;
                 const bool in = turn && d0 < rot;
                 const int p = low ? d0 : d0 - half;
-                float y[8], c[8], s[8];
+                const float* sines = sn[low ? 0 : 1];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], other);
-                if (in) {
-                    load8(cs + p, c);
-                    load8(sn[low ? 0 : 1] + p, s);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], c[i], y[i] * s[i]);
+                for (int i = 0; i < 16; ++i) {
+                    const float y = __shfl_sync(0xffffffffu, x[i], other);
+                    if (in) x[i] = fmaf(x[i], cs[p + i], y * sines[p + i]);
                 }
             } else {
                 float* mine = stage + static_cast<size_t>(g) * HD;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mine[d0 + i] = x[i];
+                for (int i = 0; i < 16; ++i) mine[d0 + i] = x[i];
                 __syncwarp();
                 if (turn)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         const int d = d0 + i;
                         if (d < half) x[i] = x[i] * cs[d] - mine[d + half] * sn[1][d];
                         else if (d < rot) x[i] = mine[d - half] * sn[1][d - half] + x[i] * cs[d - half];
@@ -215,37 +206,27 @@ __global__ void __launch_bounds__(W_THREADS, 4) q4_write_kernel(const T* __restr
             }
         }
         if (r < nh) {
-            if (SPLIT) {
-                store4(q_row + static_cast<size_t>(r) * HD, x);
-                store4(q_row + static_cast<size_t>(r) * HD + HD / 2, x + 4);
-            } else {
-                store8(q_row + static_cast<size_t>(r) * HD, x);
-            }
+            store8(q_row + static_cast<size_t>(r) * HD, x);
+            store8(q_row + static_cast<size_t>(r) * HD + NEXT, x + 8);
         }
         if (!__any_sync(0xffffffffu, r >= nh && r < n_rows)) return;   // (a warp of q's rows alone)
         float scale, mid;
         bool bad;
         q4_row_factors<GL>(x, scale, mid, bad);
-        uint32_t word;
-        int place;   // of the word in its row
-        if constexpr (SPLIT) {
-            // values 4 l .. + 3 of a half: the even lane's are its word's first four (nibbles 0, 4, 1, 5), the odd lane's the last (2, 6, 3, 7)
-            const int odd = l & 1;
-            auto at = [&](int i) { return 16 * (i & 1) + 4 * (i >> 1) + 8 * odd; };
-            const uint32_t low = q4_codes<4>(x, scale, mid, at), high = q4_codes<4>(x + 4, scale, mid, at);
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? low : high, 1);   // the even lane stores the lower half's word
-            word = (odd ? high : low) | other;
-            place = (l >> 1) + odd * (GL / 2);
-        } else {
-            word = q4_codes<8>(x, scale, mid, [](int i) { return q4_shift(i); });
-            place = l;
-        }
         if (r < nh || r >= n_rows) return;
+        const float inv = 1.f / scale;
         uint8_t* at = page_bytes + static_cast<unsigned>(r - nh) * head_bytes;   // (planes and heads lie as the rows of k and v do)
-        reinterpret_cast<uint32_t*>(at + off * (HD / 2))[place] = word;
+        uint32_t* words = reinterpret_cast<uint32_t*>(at + off * (HD / 2));
+        const uint32_t w0 = q4_word(x, scale, mid, inv), w1 = q4_word(x + 8, scale, mid, inv);
+        if (SPLIT) {
+            words[l] = w0;
+            words[l + GL] = w1;
+        } else {
+            reinterpret_cast<uint2*>(words)[l] = make_uint2(w0, w1);
+        }
         if (l == 0) {
             reinterpret_cast<uint32_t*>(at + P * (HD / 2))[off] = bad ? 0x7fff7fffu : q4_factors(scale, mid);
-            if (weights && r < nh + nkv) weights[(static_cast<size_t>(page) * nkv + (r - nh)) * P + off] = 0.f;
+            if (weights && turn) weights[(static_cast<size_t>(page) * nkv + (r - nh)) * P + off] = 0.f;
         }
     };
     for (int r0 = 0; r0 < n_rows; r0 += W_AHEAD * ROWS) {
@@ -262,9 +243,9 @@ __global__ void __launch_bounds__(W_THREADS, 4) q4_write_kernel(const T* __restr
 template <typename T>
 static int write_launch(const void* qkv, const int* positions, const float* inv_freq, void* q_out, uint8_t* pool, const int* slots,
                         float* weights, int n, int nh, int nkv, int hd, int rot, int pairing, int P, int write_kv, cudaStream_t stream) {
-    const bool staged = pairing == 0 && (rot / 2) % 8 != 0, split = pairing == 0 && rot == hd;
+    const bool staged = pairing == 0 && (rot / 2) % 16 != 0, split = pairing == 0 && rot == hd;
 #define Q4_WRITE_S(HD_, SPLIT_)                                                                                                         \
-    locus_launch(q4_write_kernel<T, HD_, SPLIT_>, n, W_THREADS, staged ? W_THREADS * 8 * sizeof(float) : 0, stream,                    \
+    locus_launch(q4_write_kernel<T, HD_, SPLIT_>, n, W_THREADS, staged ? W_THREADS * 16 * sizeof(float) : 0, stream,                    \
                  static_cast<const T*>(qkv), positions, inv_freq, static_cast<T*>(q_out), pool, slots, weights, nh, nkv, rot, pairing, \
                  P, write_kv)
 #define Q4_WRITE(HD_)                     \
@@ -297,7 +278,7 @@ extern "C" int locus_rope_kv_write_q4(const Q4WriteCall* call, cudaStream_t stre
     const Q4WriteCall& v = *call;
     if (v.T <= 0) return 0;
     const int hd = static_cast<int>(v.hd), rot = v.inv_freq == nullptr ? 0 : static_cast<int>(v.rot), P = static_cast<int>(v.P);
-    if (!q4_head_ok(hd) || v.nh <= 0 || v.nkv <= 0 || P <= 0 || P % 16 != 0 || rot < 0 || rot > hd || (rot & 1) || (v.pairing != 0 && v.pairing != 1) ||
+    if (!q4_head_ok(hd) || v.nh < 0 || v.nkv <= 0 || P <= 0 || P % 16 != 0 || rot < 0 || rot > hd || (rot & 1) || (v.pairing != 0 && v.pairing != 1) ||
         !aligned16(v.qkv) || !aligned16(v.q_out) || !aligned16(v.pool) || (v.write_kv && v.slots == nullptr))
         return LOCUS_ERR_UNSUPPORTED;
     auto go = [&](auto launch) {
@@ -310,7 +291,7 @@ extern "C" int locus_rope_kv_write_q4(const Q4WriteCall* call, cudaStream_t stre
 }
 
 // ---------------------------------------------------------------------------
-// expand: the rows of positions 0 .. seg_ctx + seg_qn - 1 of the listed segments into ordinary pages [n_pages][2][nkv][P][hd] of the same
+// expand: the rows of positions 0 .. seg_ctx + seg_qn - 1 of the listed segments (null: the first ones) that have at least min_new new tokens into ordinary pages [n_pages][2][nkv][P][hd] of the same
 // page ids, in the model's type (float32: as they are; bfloat16: one rounding, the tensor cores' operand).  Rows behind a request's last
 // token and pages that went back (-1) stay as they were.
 // One block per (page of the request, plane, head): P rows, a lane takes words of eight values, E_AHEAD at a time.
@@ -344,12 +325,13 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(E_THREADS) q4_expand_kernel(const uint8_t* __restrict__ pool, T* __restrict__ out,
                                                               const int* __restrict__ segs, const int* __restrict__ seg_ctx,
                                                               const int* __restrict__ seg_qn, const int* __restrict__ block_table,
-                                                              int table_stride, int nkv, int P) {
+                                                              int table_stride, int nkv, int P, int min_new) {
     constexpr int WR = HD / 8;   // words of a row
     pdl_entry();
     pdl_trigger();
-    const int seg = segs[blockIdx.z];
-    const int n = seg_ctx[seg] + seg_qn[seg];
+    const int seg = segs ? segs[blockIdx.z] : static_cast<int>(blockIdx.z);
+    const int fresh = seg_qn[seg], n = seg_ctx[seg] + fresh;
+    if (fresh < min_new) return;
     const int first = blockIdx.y * P;
     if (first >= n) return;
     const int page = block_table[static_cast<size_t>(seg) * table_stride + blockIdx.y];
@@ -383,7 +365,7 @@ struct Q4ExpandCall {
     const void* pool;
     void* out;
     const int *segs, *seg_ctx, *seg_qn, *block_table;
-    long long dt, n_segs, table_stride, nkv, hd, P, max_keys;
+    long long dt, n_segs, table_stride, nkv, hd, P, max_keys, min_new;
 };
 extern "C" int locus_expand_q4(const Q4ExpandCall* call, cudaStream_t stream) {
     const Q4ExpandCall& v = *call;
@@ -397,7 +379,7 @@ extern "C" int locus_expand_q4(const Q4ExpandCall* call, cudaStream_t stream) {
     const uint8_t* p8 = static_cast<const uint8_t*>(v.pool);
 #define Q4_EXPAND(T_, HD_)                                                                                                          \
     locus_launch(q4_expand_kernel<T_, HD_>, grid, E_THREADS, 0, stream, p8, static_cast<T_*>(v.out), v.segs, v.seg_ctx, v.seg_qn,   \
-                 v.block_table, table_stride, nkv, P)
+                 v.block_table, table_stride, nkv, P, static_cast<int>(v.min_new))
 #define Q4_EXPAND_T(T_)                                                                                                             \
     do {                                                                                                                            \
         if (hd == 64) Q4_EXPAND(T_, 64);                                                                                            \

@@ -55,6 +55,7 @@ struct Seq {
     uint32_t generation = 0;
     bool open = false;
     int n_tokens = 0;
+    int gone = 0;        // tokens that were evicted: the next token's position is n_tokens + gone
     int state_slot = -1;
     std::vector<std::vector<int>> tables;  // per group; -1 = page given back (window)
 };
@@ -63,6 +64,7 @@ inline int pages_of(int tokens, int page_tokens) { return (tokens + page_tokens 
 
 struct Cache {
     int page_tokens, n_pages, max_seq_tokens, table_width;  // n_pages: of the largest group
+    int bound = 0;            // > 0: requests are evicted down, and hold at most so many tokens at once
     std::vector<int> window;  // per group, 0 = all keys
     std::vector<int> keep;    // per group with a window: a request's first tokens that stay in sight (their pages never go back)
     std::vector<int> aligned;  // per group without a window: > 0, queries see the keys of their own chunk of that many positions
@@ -88,7 +90,7 @@ struct Cache {
     // Pages that a request of n_tokens tokens holds in group g at most, when no step feeds it more than
     // step_tokens at once: all of them, or in a group with a window (or chunks) those that cover it and the step.
     int pages_needed(int g, int n_tokens, int step_tokens) const {
-        const int all = pages_of(n_tokens, page_tokens);
+        const int all = pages_of(bound > 0 && n_tokens > bound ? bound : n_tokens, page_tokens);
         const int w = window[static_cast<size_t>(g)] > 0 ? window[static_cast<size_t>(g)] : aligned[static_cast<size_t>(g)];
         if (w <= 0 || step_tokens <= 0) return all;
         const int span = pages_of(w + step_tokens, page_tokens) + 1 + pages_of(keep[static_cast<size_t>(g)], page_tokens);
@@ -185,6 +187,7 @@ int64_t locus_cache_open(void* cv) {
     if (s.generation == 0) s.generation = 1;
     s.open = true;
     s.n_tokens = 0;
+    s.gone = 0;
     s.state_slot = slot;
     s.tables.assign(static_cast<size_t>(c->n_groups()), std::vector<int>());
     return static_cast<int64_t>((static_cast<uint64_t>(s.generation) << 32) | idx);
@@ -220,6 +223,7 @@ int locus_cache_ensure(void* cv, int64_t h, int n_more) {
     if (!s) return -1;
     if (static_cast<int64_t>(s->n_tokens) + n_more > c->max_seq_tokens) return -2;
     const int want = pages_of(s->n_tokens + n_more, c->page_tokens);
+    if (want > c->table_width) return -2;
     for (int g = 0; g < c->n_groups(); ++g) {
         const int missing = want - static_cast<int>(s->tables[static_cast<size_t>(g)].size());
         if (missing > c->pools[static_cast<size_t>(g)].n_free()) return 0;
@@ -247,6 +251,47 @@ int locus_cache_set_aligned(void* cv, int g, int size) {
     if (g < 0 || g >= c->n_groups() || size < 0 || c->window[static_cast<size_t>(g)] > 0) return -1;
     c->aligned[static_cast<size_t>(g)] = size;
     return 0;
+}
+
+// Requests are evicted down (locus_cache_evict) so that none holds more than `tokens` at once, the most tokens of a step included: what a
+// request needs of the pools, and the width of the tables, are bounded by that.  Set before the first request opens.  0 ok; -1 not positive.
+int locus_cache_set_bound(void* cv, int tokens) {
+    Cache* c = as_cache(cv);
+    if (tokens <= 0) return -1;
+    c->bound = tokens;
+    const int width = pages_of(tokens, c->page_tokens);
+    if (width < c->table_width) c->table_width = width;
+    return 0;
+}
+
+// Position of the request's next token: cached and evicted ones together; -1 not open.
+int locus_cache_position(void* c, int64_t h) {
+    Seq* s = as_cache(c)->find(h);
+    return s ? s->n_tokens + s->gone : -1;
+}
+
+// Of a request's cached tokens n stay (in every group its first n slots; which tokens those are is the caller's business), the pages behind
+// them go back.  Positions go on.  Writes the (group, page) pairs that became free to freed (cap ints) and returns their number; -1 not
+// open; -2 n is not within 1 .. the cached tokens; -3 a group with a window or chunks.
+int locus_cache_evict(void* cv, int64_t h, int n, int* freed, int cap) {
+    Cache* c = as_cache(cv);
+    Seq* s = c->find(h);
+    if (!s) return -1;
+    if (n < 1 || n > s->n_tokens) return -2;
+    for (int g = 0; g < c->n_groups(); ++g)
+        if (c->window[static_cast<size_t>(g)] > 0 || c->aligned[static_cast<size_t>(g)] > 0) return -3;
+    int n_freed = 0;
+    const size_t keep = static_cast<size_t>(pages_of(n, c->page_tokens));
+    for (int g = 0; g < c->n_groups(); ++g) {
+        auto& t = s->tables[static_cast<size_t>(g)];
+        while (t.size() > keep) {
+            if (c->pools[static_cast<size_t>(g)].release(t.back()) == 1) note_freed(freed, cap, n_freed, g, t.back());
+            t.pop_back();
+        }
+    }
+    s->gone += s->n_tokens - n;
+    s->n_tokens = n;
+    return n_freed;
 }
 
 // n tokens were written after the cached ones.  In a group with a window or chunks, pages that no later
@@ -295,6 +340,7 @@ int locus_cache_release(void* cv, int64_t h, int* freed, int cap) {
     c->slots.release(s->state_slot);
     s->state_slot = -1;
     s->n_tokens = 0;
+    s->gone = 0;
     s->open = false;
     c->spare.push_back(static_cast<int>(h & 0xffffffff));
     return n_freed;
@@ -384,7 +430,7 @@ int locus_step_build(void* cv, int n_entries, const int64_t* handles, const int*
             if (n <= 0) return 4;
             for (int i = 0; i < n; ++i)
                 if (tok[i] < 0 || tok[i] >= vocab) { info[7] = i; return 5; }
-            if (static_cast<int64_t>(s->n_tokens) + n > max_positions) { info[7] = s->n_tokens + n; return 6; }
+            if (static_cast<int64_t>(s->n_tokens) + s->gone + n > max_positions) { info[7] = s->n_tokens + s->gone + n; return 6; }
             if (s->n_tokens + n > c->capacity(*s)) { info[7] = n; return 8; }
             for (int i = 0; i < want_counts[e]; ++i)
                 if (wnt[i] < 0 || wnt[i] >= n) { info[7] = i; return 9; }
@@ -435,7 +481,7 @@ int locus_step_build(void* cv, int n_entries, const int64_t* handles, const int*
         for (int i = 0; i < want_counts[e]; ++i) *o_want++ = row + static_cast<int>(wnt[i]);
         for (int i = 0; i < n; ++i) {
             o_tok[row + i] = static_cast<int>(tok[i]);
-            o_pos[row + i] = ctx + i;
+            o_pos[row + i] = s->gone + ctx + i;
         }
         if (ctx + n > longest) longest = ctx + n;
         for (int g = 0; g < G; ++g) {

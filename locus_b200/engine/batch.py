@@ -170,8 +170,11 @@ class LayerCache:
     descriptors of its group, and its per-request state (if it has any)."""
 
     group: Optional[int]              # cache group id, key into StepBatch.groups
-    pool: Optional[torch.Tensor]      # [n_pages, planes (K, V or K alone), n_kv_heads, page_tokens, head_dim]
+    # [n_pages, planes (K, V or K alone), n_kv_heads, page_tokens, head_dim]; held in 4 bits: uint8 [n_pages, 2, n_kv_heads, bytes of a page]
+    pool: Optional[torch.Tensor]
     page_tokens: int
     state: Optional[torch.Tensor]     # [n_state_slots, *StateSpec.shape]
     writes: bool = True               # False: the call reads another call's cache
     extra: Optional[torch.Tensor] = None  # [n_pages, page_tokens, extra_width] per-token fields beside the rows
+    # [n_pages, n_kv_heads, page_tokens] float32: the attention weight that every cached key has received in all, for the keys' eviction
+    weights: Optional[torch.Tensor] = None

@@ -29,6 +29,7 @@ class Engine:
         self.cfg = config or SchedulerConfig()
         self.sched = Scheduler(cache, self.cfg, max_positions, eos_token_id)
         self.on_token: Optional[Callable[[Request, int], None]] = None
+        self.keep = None   # (tokens, first, recent) that a request is evicted down to (from_model: keep_tokens)
         self.timing = {"steps": 0, "prefill_tokens": 0, "decode_tokens": 0, "step_seconds": 0.0}
 
     # -- construction from a model folder -------------------------------------
@@ -36,29 +37,54 @@ class Engine:
     def from_model_dir(cls, model_dir: str, *, dtype: str = "bfloat16", ctx: int = 0, page_tokens: int = 64,
                        max_batch_tokens: int = 2048, chunk: int = 2048, max_running: int = 64,
                        decode_headroom: int = 16, device: str = "cuda:0", use_graphs: bool = True,
-                       max_seq_tokens: int = 0, kv_fraction: float = 0.0) -> "Engine":
+                       max_seq_tokens: int = 0, kv_fraction: float = 0.0, kv_bits: int = 0, keep_tokens: int = 0,
+                       keep_first: int = 4, keep_recent: int = 0) -> "Engine":
         """``ctx``: tokens the cache pool holds in all (default: min(model context, 4096), the
         reference's default, src/locus/model/llama.cpp:389-398).  ``kv_fraction`` > 0 instead sizes
         the pool to that fraction of the device memory that is free once the weights are loaded (the
         way to use a 180 GB device for many long requests); a request may then grow to the model's
-        context."""
+        context.
+
+        ``kv_bits`` 4: keys and values are held in 4 bits (0.53 bytes a value at heads of 128 instead of 2), for models whose paged mixers are
+        plain attention with heads of 64, 128 or 256.  ``keep_tokens`` > 0 (with 4 bits): a request that holds a page's tokens more than that
+        lets go of the keys that received the least attention so far, in each layer and for each key/value head, down to ``keep_tokens``: the
+        first ``keep_first``, the last ``keep_recent`` (0: a quarter) and the heaviest others stay.  Weights are counted from single tokens
+        and from the last token of every portion of a prompt.  A preempted request is evicted from anew as its tokens are fed again."""
         from ..models.model import load_model
 
         model = load_model(model_dir, parse_dtype(dtype), device)
         return cls.from_model(model, ctx=ctx, page_tokens=page_tokens, max_batch_tokens=max_batch_tokens,
                               chunk=chunk, max_running=max_running, decode_headroom=decode_headroom,
-                              use_graphs=use_graphs, max_seq_tokens=max_seq_tokens, kv_fraction=kv_fraction)
+                              use_graphs=use_graphs, max_seq_tokens=max_seq_tokens, kv_fraction=kv_fraction, kv_bits=kv_bits,
+                              keep_tokens=keep_tokens, keep_first=keep_first, keep_recent=keep_recent)
 
     @classmethod
     def from_model(cls, model, *, ctx: int = 0, page_tokens: int = 64, max_batch_tokens: int = 2048,
                    chunk: int = 2048, max_running: int = 64, decode_headroom: int = 16,
-                   use_graphs: bool = True, max_seq_tokens: int = 0, kv_fraction: float = 0.0) -> "Engine":
+                   use_graphs: bool = True, max_seq_tokens: int = 0, kv_fraction: float = 0.0, kv_bits: int = 0,
+                   keep_tokens: int = 0, keep_first: int = 4, keep_recent: int = 0) -> "Engine":
         plan = model.plan
+        weigh = keep_tokens > 0
+        if kv_bits:
+            mixers = [model.blocks[call.layer].mixer for call in plan.order]
+            paged = [m for m in mixers if m.cache_needs()[0] is not None]
+            if not all(m.reads_q4 for m in paged):
+                raise ValueError("kv_bits: a mixer of this model keeps pages that cannot be held in 4 bits")
+            if weigh and not all(m.weighs for m in paged):
+                raise ValueError("keep_tokens: a mixer of this model has a window, chunks or a distance bias, or reads pages in another way")
+        elif weigh:
+            raise ValueError("keep_tokens goes with a cache of 4 bits (kv_bits=4)")
+        bound = 0
+        if weigh:
+            keep_recent = keep_recent if keep_recent > 0 else keep_tokens // 4
+            if keep_first < 0 or keep_first + keep_recent > keep_tokens:
+                raise ValueError(f"keep_tokens {keep_tokens} with the first {keep_first} and the last {keep_recent}")
+            bound = keep_tokens + page_tokens + min(chunk, max_batch_tokens)
         if kv_fraction > 0:
             if not (kv_fraction <= 1.0) or model.device.type != "cuda":
                 raise ValueError("kv_fraction is a share (0, 1] of the free memory of a CUDA device")
             per_token = CacheManager(model.cache_needs(), page_tokens=page_tokens, n_pages=0, n_state_slots=1,
-                                     max_seq_tokens=1, dtype=model.dtype, allocate_device=False).bytes_per_token()
+                                     max_seq_tokens=1, dtype=model.dtype, allocate_device=False, kv_bits=kv_bits, weigh=weigh).bytes_per_token()
             free, _ = torch.cuda.mem_get_info(model.device)
             ctx = int(free * kv_fraction) // max(1, per_token * page_tokens) * page_tokens
             if ctx < page_tokens:
@@ -67,12 +93,16 @@ class Engine:
                 max_seq_tokens = min(plan.max_positions, ctx)
         if ctx <= 0:
             ctx = min(plan.max_positions, 4096)
-        if max_seq_tokens <= 0:
-            max_seq_tokens = min(plan.max_positions, ctx)
+        if max_seq_tokens <= 0:   # (an evicted request's positions may go beyond the pool)
+            max_seq_tokens = plan.max_positions if weigh else min(plan.max_positions, ctx)
         n_pages = -(-ctx // page_tokens)
         cache = CacheManager(model.cache_needs(), page_tokens=page_tokens, n_pages=n_pages,
                              n_state_slots=max_running, max_seq_tokens=max_seq_tokens, dtype=model.dtype,
-                             device=model.device, max_step_tokens=min(chunk, max_batch_tokens))
+                             device=model.device, max_step_tokens=min(chunk, max_batch_tokens), kv_bits=kv_bits, weigh=weigh, bound=bound)
+        if kv_bits:
+            from ..csrc import build
+
+            build.ensure(["cache_q4", "attention_q4"])
         max_tokens = max(max_batch_tokens, max_running)
         runner = ModelRunner(model, cache, max_tokens=max_tokens, max_segments=max_running,
                              max_wanted=max_running, use_graphs=use_graphs)
@@ -82,6 +112,8 @@ class Engine:
         eng = cls(runner, cache, sampler, max_positions=plan.max_positions, eos_token_id=plan.eos_token_id,
                   config=cfg)
         eng.model = model
+        if weigh:
+            eng.keep = (keep_tokens, keep_first, keep_recent)
         return eng
 
     # -- requests -------------------------------------------------------------
@@ -127,6 +159,10 @@ class Engine:
                     s.accept_token(r, tok)
                     if self.on_token is not None:
                         self.on_token(r, int(tok))
+            if self.keep is not None:
+                n, first, recent = self.keep
+                over = [r.seq for r in (p.request for p in planned) if r.seq is not None and r.seq.n_tokens >= n + self.cache.page_tokens]
+                self.timing["evictions"] = self.timing.get("evictions", 0) + self.cache.evict(over, n, first, recent)
             self.timing["steps"] += 1
             if self.timing["steps"] % 256 == 1 and hasattr(self.runner, "check_device_errors"):
                 self.runner.check_device_errors()  # the first step and every 256th

@@ -255,6 +255,11 @@ class ModelRunner:
             if code:
                 raise RuntimeError(f"grouped-query decode attention fault (code {code}): a wait for a bulk copy ran out; "
                                    "results since the last check are invalid")
+        if self.device.type == "cuda" and "attention_q4" in K._LIBS:
+            code = K.attn_q4_error()
+            if code:
+                raise RuntimeError(f"4-bit decode attention fault (code {code}): a wait for a bulk copy ran out; "
+                                   "results since the last check are invalid")
         if self.device.type == "cuda" and "gla" in K._LIBS:
             code = K.gla_error()
             if code:

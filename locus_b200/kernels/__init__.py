@@ -1287,7 +1287,7 @@ def q4_page_bytes(head_dim: int, page_tokens: int) -> int:
 # The calls below are made once per layer and step, often for a few microseconds of work, so their checks are plain conditions (a message is
 # put together only when one fails) and their arguments travel as one packed record (a foreign-function call pays a tenth of a microsecond for each).
 _Q4_WRITE = struct.Struct("@7P9q")
-_Q4_EXPAND = struct.Struct("@6P7q")
+_Q4_EXPAND = struct.Struct("@6P8q")
 _Q4_EVICT = struct.Struct("@6P12q")
 _Q4_DECODE = struct.Struct("@15P15qd")
 _q4_entries = {}
@@ -1339,19 +1339,23 @@ def _q4_aligned(what: str, addresses: int, step: int, names: str) -> None:
         raise KernelError(f"{what}: {names} must start at multiples of {step} bytes")
 
 
-def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], q_out: torch.Tensor,
+def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], q_out: Optional[torch.Tensor],
                      pool: torch.Tensor, slots: torch.Tensor, *, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int,
                      interleaved: bool, page_tokens: int, write_kv: bool = True, weights: Optional[torch.Tensor] = None) -> None:
     """:func:`rope_kv_write` into a cache held in 4 bits: q, rotated, to ``q_out`` in the model's type; k, rotated, and v, neither rounded to
     the model's type first, to the rows of ``slots`` in ``pool`` uint8 [n_pages, 2, n_kv_heads, :func:`q4_page_bytes`].  A row x of a head is
     held as one of sixteen codes per element and two bfloat16: scale = (max - min) / 15 and mid = (min + max) / 2, and stands for
     mid + scale * (code - 7.5); a row with a value that is not finite reads as NaN.  The angles' product and reduction are 64 bits.
-    ``weights`` float32 [n_pages, n_kv_heads, page_tokens]: set to 0 for the slots written (see :func:`attn_decode_q4`)."""
+    ``weights`` float32 [n_pages, n_kv_heads, page_tokens]: set to 0 for the slots written (see :func:`attn_decode_q4`).  ``n_heads`` 0 with
+    ``q_out`` None: rows of k and v alone."""
     what = "rope_kv_write_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
     T, width = qkv.shape
-    if width != (n_heads + 2 * n_kv_heads) * head_dim or n_heads <= 0:
+    if width != (n_heads + 2 * n_kv_heads) * head_dim or n_heads < 0:
         raise KernelError(f"{what}: qkv width {width} for {n_heads} heads on {n_kv_heads} of {head_dim}")
+    if q_out is None:
+        _need(n_heads == 0, "rope_kv_write_q4: q_out may only be left out without query heads")
+        q_out = qkv
     _need(qkv.dtype is q_out.dtype, "rope_kv_write_q4: qkv and q_out share one element type")
     _need(q_out.numel() >= T * n_heads * head_dim, "rope_kv_write_q4: q_out is too small")
     _need(positions.dtype is torch.int32 and positions.numel() >= T, "rope_kv_write_q4: positions must be int32, one per row")
@@ -1378,9 +1382,10 @@ def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     _check(code, what, lambda: f"(heads {n_heads}/{n_kv_heads}, head_dim {head_dim})")
 
 
-def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: torch.Tensor, n_segs: int, seg_ctx: torch.Tensor, seg_qn: torch.Tensor,
-              block_table: torch.Tensor, n_kv_heads: int, head_dim: int, page_tokens: int, max_keys: int) -> None:
-    """The rows of positions 0 .. seg_ctx + seg_qn - 1 of the segments ``segs`` [n_segs], out of ``pool`` (4 bits) into ordinary pages
+def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: Optional[torch.Tensor], n_segs: int, seg_ctx: torch.Tensor, seg_qn: torch.Tensor,
+              block_table: torch.Tensor, n_kv_heads: int, head_dim: int, page_tokens: int, max_keys: int, min_new: int = 1) -> None:
+    """The rows of positions 0 .. seg_ctx + seg_qn - 1 of the segments ``segs`` [n_segs] (None: the first ``n_segs``), of those with at least
+    ``min_new`` new tokens, out of ``pool`` (4 bits) into ordinary pages
     ``out`` [n_pages, 2, n_kv_heads, page_tokens, head_dim] of the same page ids, float32 or bfloat16 (rounded once): what the kernels of prompt
     portions (:func:`attn_chunk` and the others) read.  Rows behind a segment's last token and pages that went back (-1) stay as they were.
     ``max_keys``: at least the rows of the longest of these segments."""
@@ -1388,18 +1393,20 @@ def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: torch.Tensor, n_se
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
     _need(out.shape == (pool.shape[0], 2, n_kv_heads, page_tokens, head_dim), "expand_q4: out must have the pool's pages in the model's type")
     _need(block_table.dtype is torch.int32 and block_table.dim() == 2, "expand_q4: block_table must be int32 [segments, width]")
-    _need(segs.dtype is torch.int32 and segs.numel() >= n_segs, "expand_q4: segs must be int32, one per segment to expand")
+    _need(segs is None or (segs.dtype is torch.int32 and segs.numel() >= n_segs), "expand_q4: segs must be int32, one per segment to expand")
+    _need(segs is not None or min(seg_ctx.numel(), seg_qn.numel(), block_table.shape[0]) >= n_segs, "expand_q4: fewer segments than n_segs")
     _need(seg_ctx.dtype is torch.int32 and seg_qn.dtype is torch.int32, "expand_q4: seg_ctx and seg_qn must be int32")
     dev = pool.get_device()
-    if not (dev >= 0 and dev == out.get_device() == segs.get_device() == seg_ctx.get_device() == seg_qn.get_device() == block_table.get_device()
-            and pool.is_contiguous() and out.is_contiguous() and segs.is_contiguous() and seg_ctx.is_contiguous() and seg_qn.is_contiguous()
+    if not (dev >= 0 and dev == out.get_device() == seg_ctx.get_device() == seg_qn.get_device() == block_table.get_device()
+            and (segs is None or (dev == segs.get_device() and segs.is_contiguous()))
+            and pool.is_contiguous() and out.is_contiguous() and seg_ctx.is_contiguous() and seg_qn.is_contiguous()
             and block_table.is_contiguous() and dev == torch.cuda.current_device()):
         _q4_here(what, pool=pool, out=out, segs=segs, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
     base, to = pool.data_ptr(), out.data_ptr()
     _q4_aligned(what, base | to, 16, "the pool and out")
     code = _q4_entry("cache_q4", "locus_expand_q4")(
-        _Q4_EXPAND.pack(base, to, segs.data_ptr(), seg_ctx.data_ptr(), seg_qn.data_ptr(), block_table.data_ptr(), dtype_code(out.dtype), n_segs,
-                        block_table.shape[1], n_kv_heads, head_dim, page_tokens, max_keys), _q4_stream(dev))
+        _Q4_EXPAND.pack(base, to, 0 if segs is None else segs.data_ptr(), seg_ctx.data_ptr(), seg_qn.data_ptr(), block_table.data_ptr(), dtype_code(out.dtype), n_segs,
+                        block_table.shape[1], n_kv_heads, head_dim, page_tokens, max_keys, min_new), _q4_stream(dev))
     _check(code, what, lambda: f"(kv heads {n_kv_heads}, head_dim {head_dim}, {n_segs} segments of up to {max_keys} keys)")
 
 

@@ -302,6 +302,12 @@ class Attention(Mixer):
         if bqkv is not None:
             P["bqkv"] = bqkv
 
+    reads_q4 = True
+
+    @property
+    def weighs(self) -> bool:
+        return not (self.window or self.chunk or self.cache_window or self.slopes is not None)
+
     def kernel_modules(self, dtype):
         special = bool(self.keep_first or self.sink)   # such an attention runs on the kernels that know of both
         return (["elementwise", "gemm_simt", "gemv", "attention"] + (["short_conv"] if self.shaped else [])
@@ -340,16 +346,26 @@ class Attention(Mixer):
         if self.keys_are_values:
             offsets[2] = offsets[1]
         extra = {"q_temp": self.q_temp} if self.q_temp else {}
+        pool, slots, page_tokens = cache.pool if kv else None, gb.slots if kv else None, gb.page_tokens
+        q4 = kv and cache.pool.dtype == torch.uint8
+        if q4:
+            # k and v of the step's tokens in pages of one token, from where they are held in 4 bits
+            rows = rt.rows("attention.q4_rows", 2 * kv * D, rt.dtype, T)
+            pool, page_tokens = rows.view(T, 2, kv, 1, D), 1
+            slots = rt.shared_object(("attention.q4_slots", rt.max_tokens), lambda: torch.arange(rt.max_tokens, dtype=torch.int32, device=rt.device))
         K.head_prep(proj, offsets=offsets, heads=(self.n_heads, kv, kv),
                     dims=(self.qk_dim, self.qk_dim, self.v_dim), laid=(D, D, D), state_slots=batch.state_slots,
                     seg_q0=batch.seg_q0, seg_qn=batch.seg_qn, n_seg=batch.n_seg,
                     longest_new=max(batch.host_seg_qn) if batch.host_seg_qn else T, positions=batch.positions, q_out=q,
-                    pool=cache.pool if kv else None, slots=gb.slots if kv else None, page_tokens=gb.page_tokens,
+                    pool=pool, slots=slots, page_tokens=page_tokens,
                     write_kv=cache.writes, conv=self.params.get("conv"), state=cache.state if self.conv_taps > 1 else None,
                     inv_freq=table.inv_freq if table else None, rot=table.rot_dim if table else 0,
                     interleaved=table.interleaved if table else False, n_rows=T,
                     norm=None if self.qk_norm == "whole" else self.qk_norm, eps=self.qk_norm_eps,
                     norm_weights=(self.params["q_norm"], self.params.get("k_norm")) if self.qk_norm == "head" else None, **extra)
+        if q4 and cache.writes:
+            K.rope_kv_write_q4(rows, batch.positions, None, None, cache.pool, gb.slots, n_heads=0, n_kv_heads=self.n_kv_heads, head_dim=D,
+                               rot_dim=0, interleaved=False, page_tokens=gb.page_tokens, weights=cache.weights)
         o = rt.rows("attention.o", self.q_dim, rt.dtype, T)
         self._attend(q, o, batch, cache, gb, rt)
         if self.out_gate:
@@ -371,11 +387,13 @@ class Attention(Mixer):
             self.position.apply(qkv[:, : self.q_dim], qkv[:, self.q_dim : self.q_dim + self.kv_dim],
                                 batch.positions)
         q = rt.rows("attention.q", self.q_dim, rt.dtype, T)
-        K.rope_kv_write(
+        q4 = cache.pool.dtype == torch.uint8   # (a cache held in 4 bits)
+        write = K.rope_kv_write_q4 if q4 else K.rope_kv_write
+        write(
             qkv, batch.positions, table.inv_freq if table else None, q, cache.pool, gb.slots,
             n_heads=self.n_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim,
             rot_dim=table.rot_dim if table else 0, interleaved=table.interleaved if table else False,
-            page_tokens=gb.page_tokens, write_kv=cache.writes,
+            page_tokens=gb.page_tokens, write_kv=cache.writes, **({"weights": cache.weights} if q4 else {}),
         )
         o = rt.rows("attention.o", self.q_dim, rt.dtype, T)
         self._attend(q, o, batch, cache, gb, rt)
@@ -395,6 +413,14 @@ class Attention(Mixer):
                       head_dim=self.head_dim, page_tokens=gb.page_tokens, window=self.window,
                       scale=self.scale)
         tiles = batch.plans[AttentionTiles.key]
+        pool = cache.pool
+        if pool.dtype == torch.uint8:
+            if tiles["n_chunk_items"]:
+                # the kernels of portions read ordinary pages: those of the portions' requests, laid out for this layer
+                pool = rt.buf("attention.q4_wide", (pool.shape[0], 2, self.n_kv_heads, gb.page_tokens, self.head_dim), rt.dtype)
+                K.expand_q4(cache.pool, pool, segs=None, n_segs=batch.n_seg, seg_ctx=batch.seg_ctx, seg_qn=batch.seg_qn, min_new=2,
+                            block_table=gb.block_table, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, page_tokens=gb.page_tokens,
+                            max_keys=batch.longest)
         # splits of 128 keys that cover the longest context (all that the block table can describe when the
         # step's launches must not depend on its lengths)
         cap_splits = (gb.block_table.shape[1] * gb.page_tokens - 1) // K.DECODE_SPLIT + 1
@@ -411,7 +437,7 @@ class Attention(Mixer):
                     n_o, n_ml = K.attn_chunk_tc_scratch()
                     part_o = rt.buf("attention.chunk_tc_part_o", (n_o,), torch.float32)
                     part_ml = rt.buf("attention.chunk_tc_part_ml", (n_ml,), torch.float32)
-                K.attn_chunk_tc(q, cache.pool, o, items=tiles["chunk_items64"], n_items=tiles["n_chunk_items64"],
+                K.attn_chunk_tc(q, pool, o, items=tiles["chunk_items64"], n_items=tiles["n_chunk_items64"],
                                 n_splits=n_splits, part_o=part_o, part_ml=part_ml, **extra, **common)
             elif K.attn_chunk_mma_takes(q, self.head_dim) or K.attn_chunk_f32_takes(q, self.head_dim):
                 n_splits = K.attn_chunk_mma_splits(tiles["n_chunk_items64"], self.n_heads, keys)
@@ -421,10 +447,12 @@ class Attention(Mixer):
                     part_o = rt.buf("attention.chunk_part_o", (n_o,), torch.float32)
                     part_ml = rt.buf("attention.chunk_part_ml", (n_ml,), torch.float32)
                 call = K.attn_chunk_f32 if q.dtype == torch.float32 else K.attn_chunk_mma
-                call(q, cache.pool, o, items=tiles["chunk_items64"], n_items=tiles["n_chunk_items64"],
+                call(q, pool, o, items=tiles["chunk_items64"], n_items=tiles["n_chunk_items64"],
                      n_splits=n_splits, part_o=part_o, part_ml=part_ml, **extra, **common)
             else:
-                K.attn_chunk(q, cache.pool, o, items=tiles["chunk_items"], n_items=tiles["n_chunk_items"], **extra, **common)
+                K.attn_chunk(q, pool, o, items=tiles["chunk_items"], n_items=tiles["n_chunk_items"], **extra, **common)
+        if cache.pool.dtype == torch.uint8:
+            return self._attend_q4(q, o, batch, cache, gb, rt, tiles, common, extra)
         if tiles["n_decode_items"]:
             n = tiles["n_decode_items"]
             # scratch sized once, for the longest context that the block table can describe
@@ -438,6 +466,35 @@ class Attention(Mixer):
             )
             K.attn_decode(q, cache.pool, o, items=tiles["decode_items"], n_items=n, part_o=part_o,
                           part_ml=part_ml, counters=counters, max_splits=max_splits, **extra, **common)
+
+
+    def _attend_q4(self, q, o, batch, cache, gb, rt, tiles, common, extra) -> None:
+        """Single tokens over a cache held in 4 bits.  Where the keys' weights are kept, a portion's last token counts like a single one: its
+        attention runs here (again), and adds its weights up."""
+        n, items = tiles["n_decode_items"], tiles["decode_items"]
+        seg_q0, seg_ctx = batch.seg_q0, batch.seg_ctx
+        if cache.weights is not None and tiles["n_chunk_items"]:
+            n = batch.n_seg
+            items = rt.shared_object(("attention.q4_segments", rt.max_segments), lambda: torch.arange(rt.max_segments, dtype=torch.int32, device=rt.device))
+            last = rt.buf("attention.q4_last", (2, rt.max_segments), torch.int32)
+            seg_q0, seg_ctx = (torch.add(start, batch.seg_qn, out=last[i, :n]).sub_(1) for i, start in enumerate((batch.seg_q0, batch.seg_ctx)))
+        if not n:
+            return
+        units = K.decode_units_q4(rt.max_segments, self.n_heads, rt.device, fixed_ranges=self.keep_first > 0)
+        # (behind the partial results a pair of numbers per request and head, for the weights)
+        part_o = rt.buf("attention.q4_part_o", (units * self.head_dim + 2 * rt.max_segments * self.n_heads + 4,), torch.float32)
+        part_ml = rt.buf("attention.q4_part_ml", (2 * units,), torch.float32)
+        counters = rt.shared_object(
+            ("attention.counters", rt.max_segments * self.n_heads),
+            lambda: torch.zeros(rt.max_segments * self.n_heads, dtype=torch.int32, device=rt.device),
+        )
+        weigh = {}
+        if cache.weights is not None:
+            weigh = dict(weights=cache.weights, scores=rt.buf(
+                "attention.q4_scores", (rt.max_segments * self.n_heads * gb.block_table.shape[1] * gb.page_tokens,), torch.float32))
+        args = {k: v for k, v in common.items() if k not in ("seg_qn", "seg_q0", "seg_ctx")}
+        K.attn_decode_q4(q, cache.pool, o, seg_q0=seg_q0, seg_ctx=seg_ctx, items=items, n_items=n, part_o=part_o, part_ml=part_ml,
+                         counters=counters, **weigh, **extra, **args)
 
 
 register_mixer("attention", Attention)

@@ -275,6 +275,11 @@ class Mixer(Part):
         """Host-planned work lists this mixer wants for every step (see :class:`StepPlan`)."""
         return []
 
+    # Whether the mixer's pages may be held in 4 bits (``reads_q4``), and the weights that its keys receive be kept (``weighs``: every key stays in
+    # sight, and nothing depends on a key's place in the cache).
+    reads_q4 = False
+    weighs = False
+
     # A part with ``can_overwrite`` takes ``accumulate=False`` in ``forward``: it then WRITES its output into
     # ``residual`` (float32 rows whose old contents do not matter) instead of adding to it.
     can_overwrite = False

@@ -95,6 +95,14 @@ class ParallelMixers(Mixer):
             paged = paged or b.cache_needs()[0]
         return paged, self._state_spec
 
+    @property
+    def reads_q4(self) -> bool:
+        return all(b.reads_q4 for b in self.branches if b.cache_needs()[0] is not None)
+
+    @property
+    def weighs(self) -> bool:
+        return all(b.weighs for b in self.branches if b.cache_needs()[0] is not None)
+
     def _cache_of(self, i, cache):
         """The layer's cache as branch ``i`` sees it: with its own stretch of the state slot."""
         if i not in self._state_at or cache.state is None:
