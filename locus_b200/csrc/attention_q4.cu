@@ -15,9 +15,9 @@
 //     sums, where it would grow over the keys and lose what cancels.)
 //   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
 //     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more;
-//   * the weights p_t scale_t, formed relative to the running maximum M of score + exponent of scale, so that they stay below 2^15, whatever the
-//     scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest where that is more; two parts for a float32 model).  The
-//     unrounded p_t enter the denominator and z's sum.
+//   * the weights p_t scale_t, formed relative to the running maximum M of score + exponent, the exponent of the largest scale among the 64 keys of a
+//     stage, so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest where that
+//     is more; two parts for a float32 model).  The unrounded p_t enter the denominator and z's sum.
 // For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
 // over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
@@ -199,16 +199,25 @@ struct Bool {
 // ---------------------------------------------------------------------------
 // The cut of a step's keys into ranges.
 #define Q4_MAX_ITEMS 1024
-#define Q4_CAND 128       // candidate range lengths looked at
+#define Q4_CAND 64        // candidate range lengths looked at
 
+// What a warp of a block does in a round.
+struct Q4Unit {
+    int active;
+    int item, vh, range, n_ranges;   // range of the item's n_ranges
+    int wa, wb;                       // the warps of the block that have ranges of the same (item, head)
+    int parts;                        // blocks that have some
+    int lead;                         // packed: ranges of this (item, head) that its first block has
+};
 struct Q4Plan {
     int pos[Q4_MAX_ITEMS];       // position of item i's query
     int seg[Q4_MAX_ITEMS];
     int row[Q4_MAX_ITEMS];       // row of q / out
     int pref[Q4_MAX_ITEMS + 1];  // ranges of the items before i
     int block_pref[Q4_MAX_ITEMS + 1];   // not packed: block-loads of the items before i
-    unsigned long long best[32];
+    int ranges[Q4_CAND], blocks[Q4_CAND];
     int longest[32], total[32], blocks_of[32];
+    Q4Unit units[16];            // this round's, by warp
     int len, packed, n_blocks;
 };
 
@@ -255,6 +264,7 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
         const int heads = W / tid;   // (request, head)s of tid ranges that a block holds
         pl.blocks_of[tid] = (n_vh + heads - 1) / heads;
     }
+    if (tid < Q4_CAND) pl.ranges[tid] = pl.blocks[tid] = 0;
     longest = __reduce_max_sync(0xffffffffu, longest);
     total = __reduce_add_sync(0xffffffffu, total);
     if (lane == 0) {
@@ -264,12 +274,11 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
     __syncthreads();
     longest = __reduce_max_sync(0xffffffffu, lane < W ? pl.longest[lane] : 1);
     total = __reduce_add_sync(0xffffffffu, lane < W ? pl.total[lane] : 0);
-    const int n_warps = gridDim.x * W;
-    const float fill = static_cast<float>(total) * static_cast<float>(n_vh) / static_cast<float>(n_warps);
+    const float fill = static_cast<float>(total) * static_cast<float>(n_vh) / static_cast<float>(gridDim.x * W);
     auto length = [&](int c) {
         if (c == Q4_CAND - 1) return (longest + 15) & ~15;
         const float x = static_cast<float>(c);
-        const float times = c < 100 ? 1.f + 0.02f * x : c < 108 ? 0.12f * (x - 99.f) : 3.f + 0.1f * (x - 107.f) * (x - 107.f);
+        const float times = c < 56 ? 1.f + 0.03f * x : c < 60 ? 0.2f * (x - 55.f) : 3.f + (x - 60.f) * (x - 60.f);
         return 16 * max(1, static_cast<int>(fminf(fill * times, 1e8f) * (1.f / 16.f) + 0.5f));
     };
     const bool kept_ranges = a.window > 0 && a.keep_first > 0;
@@ -277,37 +286,44 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
         const int p = pl.pos[i], first = q4_first(a, p);
         return q4_ranges(p + 1 - first, len, inv) + (kept_ranges && q4_kept(a, first) > 0);
     };
-    unsigned long long best = ~0ull;
-    const float grid_inv = 1.f / static_cast<float>(gridDim.x);
-    for (int c = tid; c < Q4_CAND; c += 32 * W) {
-        const int len = length(c);
-        const float inv = 1.f / static_cast<float>(len);
-        int ranges = 0, blocks = 0;
-#pragma unroll 4
-        for (int i = 0; i < n_items; ++i) {
-            const int r = ranges_of(i, len, inv);
-            ranges += r;
-            blocks += q4_blocks<W>(pl.blocks_of, r, n_vh);
-        }
-        if (ranges > max_ranges) continue;  // the scratch does not hold that many partial results
-        const int most = min(len, longest) + cost_range, merge = cost_merge * (static_cast<int>(static_cast<float>(longest) * inv) / W);
-        auto consider = [&](int loads, bool joins, int packed) {
-            const int rounds = static_cast<int>((static_cast<float>(loads) + static_cast<float>(gridDim.x - 1)) * grid_inv);
-            const unsigned long long cost = static_cast<unsigned long long>(rounds) * most + merge + (joins ? cost_join : 0);
-            best = min(best, (cost << 24) | static_cast<unsigned>(2 * c + packed));  // ties: the shorter range
-        };
-        consider(blocks, longest > len * W, 0);
-        consider((ranges * n_vh + W - 1) / W, ranges > n_items, 1);
-    }
+    // every warp sums up some of the items, a lane two of the lengths
+    const int my_len[2] = {length(lane), length(lane + 32)};
+    const float my_inv[2] = {1.f / static_cast<float>(my_len[0]), 1.f / static_cast<float>(my_len[1])};
+    if (warp < n_items) {
+        int ranges[2] = {0, 0}, blocks[2] = {0, 0};
+        for (int i = warp; i < n_items; i += W)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) pl.best[warp] = best;
+            for (int k = 0; k < 2; ++k) {
+                const int r = ranges_of(i, my_len[k], my_inv[k]);
+                ranges[k] += r;
+                blocks[k] += q4_blocks<W>(pl.blocks_of, r, n_vh);
+            }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            atomicAdd(&pl.ranges[lane + 32 * k], ranges[k]);
+            atomicAdd(&pl.blocks[lane + 32 * k], blocks[k]);
+        }
+    }
     __syncthreads();
     if (warp == 0) {
-        unsigned long long b = lane < W ? pl.best[lane] : ~0ull;
+        const float grid_inv = 1.f / static_cast<float>(gridDim.x);
+        unsigned best = 0xffffffffu;   // cost << 7 | 2 candidate | packed: ties go to the shorter range
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) b = min(b, __shfl_xor_sync(0xffffffffu, b, o));
-        const int c = static_cast<int>(b & 0xffffff), len = b == ~0ull ? 0 : length(c >> 1);
+        for (int k = 0; k < 2; ++k) {
+            const int c = lane + 32 * k, ranges = pl.ranges[c];
+            const int most = min(my_len[k], longest) + cost_range, merge = cost_merge * (static_cast<int>(static_cast<float>(longest) * my_inv[k]) / W);
+            auto consider = [&](int loads, bool joins, int packed) {
+                const float rounds = floorf((static_cast<float>(loads) + static_cast<float>(gridDim.x - 1)) * grid_inv);
+                const float cost = fminf(rounds * static_cast<float>(most) + static_cast<float>(merge + (joins ? cost_join : 0)), 16777215.f);
+                best = min(best, static_cast<unsigned>(cost) << 7 | static_cast<unsigned>(2 * c + packed));
+            };
+            if (ranges <= max_ranges) {   // (the scratch holds that many partial results)
+                consider(pl.blocks[c], longest > my_len[k] * W, 0);
+                consider((ranges * n_vh + W - 1) / W, ranges > n_items, 1);
+            }
+        }
+        best = __reduce_min_sync(0xffffffffu, best);
+        const int packed = best & 1, len = best == 0xffffffffu ? 0 : length(static_cast<int>(best & 127u) >> 1);
         const float inv = len ? 1.f / static_cast<float>(len) : 0.f;
         int acc = 0, acc_blocks = 0;
         for (int i0 = 0; i0 < n_items; i0 += 32) {
@@ -315,7 +331,7 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
             int mine = 0, mine_blocks = 0;
             if (i < n_items && len) {
                 mine = ranges_of(i, len, inv);
-                if (!(c & 1)) mine_blocks = q4_blocks<W>(pl.blocks_of, mine, n_vh);
+                if (!packed) mine_blocks = q4_blocks<W>(pl.blocks_of, mine, n_vh);
             }
             int run = mine, run_blocks = mine_blocks;
 #pragma unroll
@@ -337,22 +353,19 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
             pl.pref[n_items] = acc;
             pl.block_pref[n_items] = acc_blocks;
             pl.len = len;
-            pl.packed = c & 1;
-            pl.n_blocks = c & 1 ? (acc * n_vh + W - 1) / W : acc_blocks;
+            pl.packed = packed;
+            pl.n_blocks = packed ? (acc * n_vh + W - 1) / W : acc_blocks;
         }
     }
     __syncthreads();
     return pl.len;
 }
 
+// a / b for small whole numbers (a below 2^20 by a product)
+__device__ __forceinline__ int q4_div(int a, int b) {
+    return a < 1 << 20 ? static_cast<int>(__fdividef(static_cast<float>(a) + 0.5f, static_cast<float>(b))) : a / b;
+}
 // What warp `warp` of block-load `load` (of plan.n_blocks) does.
-struct Q4Unit {
-    bool active;
-    int item, vh, range, n_ranges;   // range of the item's n_ranges
-    int wa, wb;                       // the warps of the block that have ranges of the same (item, head)
-    int parts;                        // blocks that have some
-    int lead;                         // packed: ranges of this (item, head) that its first block has
-};
 template <int W>
 __device__ __forceinline__ Q4Unit q4_unit(const Q4Plan& pl, int load, int warp, int n_items, int n_vh) {
     Q4Unit u;
@@ -370,7 +383,7 @@ __device__ __forceinline__ Q4Unit q4_unit(const Q4Plan& pl, int load, int warp, 
     if (pl.packed) {
         const int left = pl.pref[n_items] * n_vh - load * W;   // units from this block's first on
         u.active = warp < left;
-        u.vh = k / nr;
+        u.vh = q4_div(k, nr);
         u.range = k - u.vh * nr;
         const int u0 = at - u.range;                            // the (item, head)'s first unit
         u.wa = max(0, warp - u.range);
@@ -379,7 +392,7 @@ __device__ __forceinline__ Q4Unit q4_unit(const Q4Plan& pl, int load, int warp, 
         u.lead = W - u0 % W;
     } else if (nr > W) {
         const int loads = (nr + W - 1) / W;
-        u.vh = k / loads;
+        u.vh = q4_div(k, loads);
         u.range = (k - u.vh * loads) * W + warp;
         u.active = u.range < nr;
         u.wa = 0;
@@ -387,7 +400,7 @@ __device__ __forceinline__ Q4Unit q4_unit(const Q4Plan& pl, int load, int warp, 
         u.parts = loads;
         u.lead = W;
     } else {
-        const int heads = W / nr, h = warp / nr;
+        const int heads = q4_div(W, nr), h = q4_div(warp, nr);
         u.vh = k * heads + h;
         u.range = warp - h * nr;
         u.active = h < heads && u.vh < n_vh;
@@ -411,7 +424,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     constexpr int RB = HD / 2;       // bytes of a row's codes
     constexpr uint32_t PLANE = SK * (RB + Q4_FACTOR_BYTES);   // K (or V) of a stage
     constexpr uint32_t STAGE = 2 * PLANE;
-    constexpr float RAISE = 4.f, TOP = 10.f;   // weights are 2^TOP at M, at most 2^(TOP + RAISE), times scale / 2^exponent < 2: below 65,504
+    constexpr float RAISE = 4.f, TOP = 10.f;   // weights are 2^TOP at M, at most 2^(TOP + RAISE + 1/2), times scale / 2^exponent < 2: below 65,504
     constexpr int LEAST = -64;                 // smallest exponent of a scale that is taken out (smaller ones leave smaller weights)
     extern __shared__ __align__(16) unsigned char q4_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -452,9 +465,10 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 
     for (int load = blockIdx.x; load < pl.n_blocks; load += gridDim.x) {
         const Q4Unit un = q4_unit<W>(pl, load, warp, n_items, n_vh);
+        if (lane == 0) pl.units[warp] = un;   // (for the joins)
         const bool active = un.active;
         const int item = un.item, vh = un.vh, range = un.range, n_ranges = un.n_ranges, wa = un.wa, wb = un.wb;
-        const int kvh = vh / n_sub, g0 = (vh % n_sub) * 8 * HT;
+        const int kvh = n_sub == 1 ? vh : vh / n_sub, g0 = (vh - kvh * n_sub) * 8 * HT;
         const int nG = min(G - g0, 8 * HT), h0 = kvh * G + g0;   // this warp's heads: h0 .. h0 + nG - 1
         const int seg = pl.seg[item], p = pl.pos[item], first = q4_first(a, p), r0 = pl.pref[item];
         const int row = pl.row[item];
@@ -521,6 +535,15 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     end_next += P;
                 }
             };
+            // q is asked for in front of the copies, whose page ids are on their way
+            float x[HT][8 * KW];
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) {
+                const int g = gq + 8 * ht;
+                const T* q0 = static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.nh + h0 + (g < nG ? g : 0)) * HD + t4 * (HD / 4);
+#pragma unroll
+                for (int w = 0; w < KW; ++w) load8(q0 + 8 * w, x[ht] + 8 * w);
+            }
             int st = 0;
             if (ok) {
 #pragma unroll
@@ -534,14 +557,11 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
                 const int g = gq + 8 * ht;
-                const T* q0 = static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.nh + h0 + (g < nG ? g : 0)) * HD + t4 * (HD / 4);
-                float x[8 * KW], top = 0.f;
-#pragma unroll
-                for (int w = 0; w < KW; ++w) load8(q0 + 8 * w, x + 8 * w);
+                float top = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8 * KW; ++i) {
-                    if (g >= nG) x[i] = 0.f;
-                    top = fmaxf(top, fabsf(x[i]));
+                    if (g >= nG) x[ht][i] = 0.f;
+                    top = fmaxf(top, fabsf(x[ht][i]));
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -550,9 +570,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * KW; ++i) {
-                    split2<PARTS>(x[4 * i] * up, x[4 * i + 1] * up, qb[ht][i][0]);
-                    split2<PARTS>(x[4 * i + 2] * up, x[4 * i + 3] * up, qb[ht][i][1]);
-                    sum += (x[4 * i] + x[4 * i + 1]) + (x[4 * i + 2] + x[4 * i + 3]);
+                    split2<PARTS>(x[ht][4 * i] * up, x[ht][4 * i + 1] * up, qb[ht][i][0]);
+                    split2<PARTS>(x[ht][4 * i + 2] * up, x[ht][4 * i + 3] * up, qb[ht][i][1]);
+                    sum += (x[ht][4 * i] + x[ht][4 * i + 1]) + (x[ht][4 * i + 2] + x[ht][4 * i + 3]);
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -566,7 +586,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // O^T: byte b of word w of a lane's value row is row tile 4 w + b: its low nibble's dimension in row gq, its high nibble's in row
             // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
             float o[HT][MT][4], l[HT][2], z[HT][2], slope[HT][2];
-            float limit[HT][2], from[HT][2];   // a score's weight is formed relative to `from` (M - TOP), up to `limit` (M + RAISE; no live key yet: -infinity)
+            // A score's weight is formed relative to `from`, up to `limit`: M - TOP and M + RAISE, less the stage's exponent within a stage (M is a
+            // whole number, so that exponents come and go exactly); no live key yet: limit -infinity.
+            float limit[HT][2], from[HT][2], ls[HT][2], zs[HT][2];   // ls, zs: a stage's l and z, times 2^exponent
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
@@ -584,7 +606,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // N chunks of sixteen keys, from c0 (those from `stop` on are dead), whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
             // (SPECIAL: dead keys among them, or a distance bias; a copy of its own, for the plain steps' sake)
             const bool biased_call = a.slopes != nullptr;
-            auto step = [&](auto special, int c0, int stop, const unsigned char* at, const unsigned char* fac) {
+            auto step = [&](auto special, int c0, int stop, float shrink, const unsigned char* at, const unsigned char* fac) {
                 constexpr bool SPECIAL = decltype(special)::value;
                 const bool edge = SPECIAL && (c0 < t_lo || c0 + 16 * N > stop), biased = SPECIAL && biased_call;
                 // chunk n: keys c0 + 16 n + kr0 and + 8 + kr0
@@ -614,8 +636,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                                 for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
                         }
                 }
-                // of the two keys of a chunk: scale and z of K; of V the scale's exponent e, 2^-e, scale 2^-e, z 2^-e
-                float sc[N][HT][4], vs[N][2], vz[N][2], vi[N][2];   // sc: score + e
+                // of the two keys of a chunk: scale and z of K; of V scale 2^-exponent and z
+                float sc[N][HT][4], vs[N][2], vz[N][2];
                 bool raise = false;
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
@@ -628,30 +650,25 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             if (!live[i]) kf[n][i] = vf[n][i] = 0u;
                         }
                     }
-                    float ks[2], kz[2], ve[2];
+                    float ks[2], kz[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float v_scale = q4_scale(vf[n][i]);
                         ks[i] = q4_scale(kf[n][i]);
                         kz[i] = fmaf(-0.5f, ks[i], q4_mid(kf[n][i]));
-                        // (the exponent's field, LEAST + 127 .. 253, still in its place)
-                        const uint32_t e = min(max((vf[n][i] << 16) & 0x7f800000u, static_cast<uint32_t>(LEAST + 127) << 23), 253u << 23);
-                        ve[i] = __uint_as_float(0x4b000000u | (e >> 23)) - (8388608.f + 127.f);
-                        vi[n][i] = __uint_as_float((254u << 23) - e);
-                        vs[n][i] = v_scale * vi[n][i];
-                        vz[n][i] = fmaf(-0.5f, v_scale, q4_mid(vf[n][i])) * vi[n][i];
+                        vs[n][i] = v_scale * shrink;
+                        vz[n][i] = fmaf(-0.5f, v_scale, q4_mid(vf[n][i]));
                     }
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int c = i & 1, y = i >> 1;
-                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], WEIGH ? 0.f : ve[y]));
+                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], kz[y] * sq[ht][c]);
                             if (biased) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
                             if (WEIGH) {
                                 const int g = 8 * ht + 2 * t4 + c;
                                 if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
-                                w += ve[y];
                             }
                             if (edge && !live[y]) w = -INFINITY;
                             sc[n][ht][i] = w;
@@ -671,12 +688,14 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                             const bool none = limit[ht][c] == -INFINITY;   // (no live key so far)
-                            const float now = none ? top - TOP : fmaxf(from[ht][c], top - TOP);
+                            const float now = none ? rintf(top) - TOP : fmaxf(from[ht][c], rintf(top) - TOP);
                             const float corr = none ? 0.f : ex2(from[ht][c] - now);
                             limit[ht][c] = now + (TOP + RAISE);
                             from[ht][c] = now == -INFINITY ? 0.f : now;
                             l[ht][c] *= corr;
                             z[ht][c] *= corr;
+                            ls[ht][c] *= corr;
+                            zs[ht][c] *= corr;
 #pragma unroll
                             for (int j = 0; j < MT; ++j) {
                                 o[ht][j][c] *= corr;
@@ -694,8 +713,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         for (int i = 0; i < 4; ++i) e[i] = ex2(sc[n][ht][i] - from[ht][i & 1]);
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            l[ht][c] = fmaf(e[c], vi[n][0], fmaf(e[2 + c], vi[n][1], l[ht][c]));
-                            z[ht][c] = fmaf(e[c], vz[n][0], fmaf(e[2 + c], vz[n][1], z[ht][c]));
+                            ls[ht][c] += e[c] + e[2 + c];
+                            zs[ht][c] = fmaf(e[c], vz[n][0], fmaf(e[2 + c], vz[n][1], zs[ht][c]));
                         }
                         // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
                         split2<PARTS>(e[0] * vs[n][0], e[1] * vs[n][0], pb[ht][0]);
@@ -748,12 +767,38 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 const int n = end - k0;
                 // (a second chunk behind the stage's last key reads what an earlier stage left, as dead keys)
                 const int stop = min(end, k_end);
+                // the exponent of the largest of the live values' scales (infinite ones and NaN aside)
+                uint32_t top = 0u;
+                for (int i = lane; i < n; i += 32) {
+                    const uint32_t e = *reinterpret_cast<const uint32_t*>(src + PLANE + SK * RB + i * Q4_FACTOR_BYTES) << 16 & 0x7f800000u;
+                    const int t = k0 + i;
+                    if (e != 0x7f800000u && t < stop && (t >= t_lo || t < keep)) top = max(top, e);
+                }
+                top = max(__reduce_max_sync(0xffffffffu, top), static_cast<uint32_t>(LEAST + 127) << 23);
+                const float exponent = static_cast<float>(static_cast<int>(top >> 23) - 127), shrink = __uint_as_float((254u << 23) - top);
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        from[ht][c] -= exponent;
+                        limit[ht][c] -= exponent;
+                        ls[ht][c] = zs[ht][c] = 0.f;
+                    }
 #pragma unroll 1
                 for (int c = 0; c < n; c += 16 * N) {
                     const int c0 = k0 + c;
-                    if (biased_call || c0 < t_lo || c0 + 16 * N > stop) step(Bool<true>(), c0, stop, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
-                    else step(Bool<false>(), c0, stop, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                    if (biased_call || c0 < t_lo || c0 + 16 * N > stop) step(Bool<true>(), c0, stop, shrink, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                    else step(Bool<false>(), c0, stop, shrink, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
                 }
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        from[ht][c] += exponent;
+                        limit[ht][c] += exponent;
+                        l[ht][c] = fmaf(ls[ht][c], shrink, l[ht][c]);
+                        z[ht][c] = fmaf(zs[ht][c], shrink, z[ht][c]);
+                    }
                 k0 = end;
             }
             if (!ok) {
@@ -859,9 +904,10 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
         __syncthreads();
         for (int lead = 0; lead < W; ++lead) {
             if (!is_last[lead]) continue;
-            // (all warps of the block take part: the lead's unit again)
-            const Q4Unit lu = q4_unit<W>(pl, load, lead, n_items, n_vh);
-            const int lg0 = (lu.vh % n_sub) * 8 * HT, lnG = min(G - lg0, 8 * HT), lh0 = (lu.vh / n_sub) * G + lg0, parts = lu.parts;
+            // (all warps of the block take part)
+            const Q4Unit lu = pl.units[lead];
+            const int lkv = n_sub == 1 ? lu.vh : lu.vh / n_sub, lg0 = (lu.vh - lkv * n_sub) * 8 * HT, lnG = min(G - lg0, 8 * HT), lh0 = lkv * G + lg0;
+            const int parts = lu.parts;
             // a part begins with the first range that its block has
             auto place = [&](int k, int g) {
                 const int first_range = k == 0 ? 0 : lu.lead + (k - 1) * W;
