@@ -15,9 +15,9 @@
 //     sums, where it would grow over the keys and lose what cancels.)
 //   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
 //     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more;
-//   * the weights p_t scale_t, formed relative to the running maximum M of score + exponent, the exponent of the largest scale among the 64 keys of a
-//     stage, so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest where that
-//     is more; two parts for a float32 model).  The unrounded p_t enter the denominator and z's sum.
+//   * the weights p_t scale_t, formed relative to the running maximum M of score_t + e_t, e_t the exponent of the key's own scale (of its mid less 20
+//     where that is more), so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest
+//     where that is more; two parts for a float32 model).  The unrounded p_t enter the denominator and z's sum.
 // For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
 // over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
@@ -425,7 +425,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     constexpr uint32_t PLANE = SK * (RB + Q4_FACTOR_BYTES);   // K (or V) of a stage
     constexpr uint32_t STAGE = 2 * PLANE;
     constexpr float RAISE = 4.f, TOP = 10.f;   // weights are 2^TOP at M, at most 2^(TOP + RAISE + 1/2), times scale / 2^exponent < 2: below 65,504
-    constexpr int LEAST = -64;                 // smallest exponent of a scale that is taken out (smaller ones leave smaller weights)
+    constexpr int LEAST = -64;                 // smallest exponent that is taken out (smaller scales leave smaller weights)
+    constexpr int MID = 20;                    // a mid's exponent counts less this: products with z / 2^exponent < 2^(MID + 2) stay in range
     extern __shared__ __align__(16) unsigned char q4_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, t4 = lane & 3;   // row of the fragments, and the lane's place in its row
@@ -586,9 +587,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // O^T: byte b of word w of a lane's value row is row tile 4 w + b: its low nibble's dimension in row gq, its high nibble's in row
             // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
             float o[HT][MT][4], l[HT][2], z[HT][2], slope[HT][2];
-            // A score's weight is formed relative to `from`, up to `limit`: M - TOP and M + RAISE, less the stage's exponent within a stage (M is a
-            // whole number, so that exponents come and go exactly); no live key yet: limit -infinity.
-            float limit[HT][2], from[HT][2], ls[HT][2], zs[HT][2];   // ls, zs: a stage's l and z, times 2^exponent
+            // A weight times 2^exponent is formed relative to `from`, up to `limit`: M - TOP and M + RAISE; no live key yet: limit -infinity.
+            float limit[HT][2], from[HT][2];
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // N chunks of sixteen keys, from c0 (those from `stop` on are dead), whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
             // (SPECIAL: dead keys among them, or a distance bias; a copy of its own, for the plain steps' sake)
             const bool biased_call = a.slopes != nullptr;
-            auto step = [&](auto special, int c0, int stop, float shrink, const unsigned char* at, const unsigned char* fac) {
+            auto step = [&](auto special, int c0, int stop, const unsigned char* at, const unsigned char* fac) {
                 constexpr bool SPECIAL = decltype(special)::value;
                 const bool edge = SPECIAL && (c0 < t_lo || c0 + 16 * N > stop), biased = SPECIAL && biased_call;
                 // chunk n: keys c0 + 16 n + kr0 and + 8 + kr0
@@ -636,8 +636,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                                 for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
                         }
                 }
-                // of the two keys of a chunk: scale and z of K; of V scale 2^-exponent and z
-                float sc[N][HT][4], vs[N][2], vz[N][2];
+                // score + exponent of the two keys of a chunk; of V 2^-exponent, and scale and z times that
+                float sc[N][HT][4], down[N][2], vs[N][2], vz[N][2];
                 bool raise = false;
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
@@ -650,25 +650,28 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             if (!live[i]) kf[n][i] = vf[n][i] = 0u;
                         }
                     }
-                    float ks[2], kz[2];
+                    float ks[2], kz[2], ve[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float v_scale = q4_scale(vf[n][i]);
                         ks[i] = q4_scale(kf[n][i]);
                         kz[i] = fmaf(-0.5f, ks[i], q4_mid(kf[n][i]));
-                        vs[n][i] = v_scale * shrink;
-                        vz[n][i] = fmaf(-0.5f, v_scale, q4_mid(vf[n][i]));
+                        const int of_scale = static_cast<int>(vf[n][i] << 16 & 0x7f800000u), of_mid = static_cast<int>(vf[n][i] & 0x7f800000u);
+                        const int top = min(__vimax3_s32(of_scale, of_mid - (MID << 23), (LEAST + 127) << 23), 253 << 23);   // (NaN: any)
+                        ve[i] = __int_as_float(0x4b000000 | top >> 23) - 8388735.f;   // (2^23 + 127)
+                        down[n][i] = __int_as_float((254 << 23) - top);
+                        vs[n][i] = q4_scale(vf[n][i]) * down[n][i];
+                        vz[n][i] = fmaf(-0.5f, vs[n][i], q4_mid(vf[n][i]) * down[n][i]);
                     }
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int c = i & 1, y = i >> 1;
-                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], kz[y] * sq[ht][c]);
+                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], ve[y]));
                             if (biased) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
                             if (WEIGH) {
                                 const int g = 8 * ht + 2 * t4 + c;
-                                if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
+                                if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w - ve[y];
                             }
                             if (edge && !live[y]) w = -INFINITY;
                             sc[n][ht][i] = w;
@@ -694,8 +697,6 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             from[ht][c] = now == -INFINITY ? 0.f : now;
                             l[ht][c] *= corr;
                             z[ht][c] *= corr;
-                            ls[ht][c] *= corr;
-                            zs[ht][c] *= corr;
 #pragma unroll
                             for (int j = 0; j < MT; ++j) {
                                 o[ht][j][c] *= corr;
@@ -713,8 +714,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         for (int i = 0; i < 4; ++i) e[i] = ex2(sc[n][ht][i] - from[ht][i & 1]);
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            ls[ht][c] += e[c] + e[2 + c];
-                            zs[ht][c] = fmaf(e[c], vz[n][0], fmaf(e[2 + c], vz[n][1], zs[ht][c]));
+                            l[ht][c] = fmaf(e[c], down[n][0], fmaf(e[2 + c], down[n][1], l[ht][c]));
+                            z[ht][c] = fmaf(e[c], vz[n][0], fmaf(e[2 + c], vz[n][1], z[ht][c]));
                         }
                         // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
                         split2<PARTS>(e[0] * vs[n][0], e[1] * vs[n][0], pb[ht][0]);
@@ -767,38 +768,12 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 const int n = end - k0;
                 // (a second chunk behind the stage's last key reads what an earlier stage left, as dead keys)
                 const int stop = min(end, k_end);
-                // the exponent of the largest of the live values' scales (infinite ones and NaN aside)
-                uint32_t top = 0u;
-                for (int i = lane; i < n; i += 32) {
-                    const uint32_t e = *reinterpret_cast<const uint32_t*>(src + PLANE + SK * RB + i * Q4_FACTOR_BYTES) << 16 & 0x7f800000u;
-                    const int t = k0 + i;
-                    if (e != 0x7f800000u && t < stop && (t >= t_lo || t < keep)) top = max(top, e);
-                }
-                top = max(__reduce_max_sync(0xffffffffu, top), static_cast<uint32_t>(LEAST + 127) << 23);
-                const float exponent = static_cast<float>(static_cast<int>(top >> 23) - 127), shrink = __uint_as_float((254u << 23) - top);
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        from[ht][c] -= exponent;
-                        limit[ht][c] -= exponent;
-                        ls[ht][c] = zs[ht][c] = 0.f;
-                    }
 #pragma unroll 1
                 for (int c = 0; c < n; c += 16 * N) {
                     const int c0 = k0 + c;
-                    if (biased_call || c0 < t_lo || c0 + 16 * N > stop) step(Bool<true>(), c0, stop, shrink, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
-                    else step(Bool<false>(), c0, stop, shrink, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                    if (biased_call || c0 < t_lo || c0 + 16 * N > stop) step(Bool<true>(), c0, stop, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
+                    else step(Bool<false>(), c0, stop, src + c * RB, src + SK * RB + c * Q4_FACTOR_BYTES);
                 }
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        from[ht][c] += exponent;
-                        limit[ht][c] += exponent;
-                        l[ht][c] = fmaf(ls[ht][c], shrink, l[ht][c]);
-                        z[ht][c] = fmaf(zs[ht][c], shrink, z[ht][c]);
-                    }
                 k0 = end;
             }
             if (!ok) {

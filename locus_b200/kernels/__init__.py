@@ -1491,7 +1491,7 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
     n_items * n_heads * block_table.shape[1] * page_tokens elements."""
     what = "attn_decode_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
-    if n_heads <= 0 or n_heads % n_kv_heads:
+    if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
         raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv_heads} kv heads")
     width = n_heads * head_dim
     _need(q.dtype is out.dtype and q.numel() % width == 0 and out.numel() % width == 0, "attn_decode_q4: q and out must be rows of whole heads, of one element type")

@@ -314,6 +314,41 @@ def test_scores_far_apart_and_rows_that_are_not_numbers():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["spread", "hidden", "large", "level"])
+def test_values_of_very_different_sizes(dtype, kind):
+    """Rows of v from 2^-30 to 2^30 side by side; rows 2^60 times the others' size whose keys weigh nothing; rows near the type's largest number; and
+    rows far from zero with little range.  (The bound is relative to what the keys contribute, as everywhere.)"""
+    H, kv, D, P = 5, 1, 128, 64
+    lens = [200, 63]
+    table, n_pages = tables(lens, P, 91)
+    pool = poison(n_pages, kv, D, P)
+    side = torch.sign(rnd(1, D, seed=92))
+    for b, n in enumerate(lens):
+        k, v = 0.02 * rnd(n, D, seed=93 + b), rnd(n, D, seed=95 + b)
+        if kind == "spread":
+            v *= 2.0 ** torch.randint(-30, 31, (n, 1), generator=gen(97)).float()
+        elif kind == "hidden":
+            big = torch.arange(n) % 5 == 2
+            v[big] *= 2.0 ** 60
+            k[big] -= 30 * side          # (scores about 300 below the others')
+        elif kind == "large":
+            v *= 2.0 ** 120 / v.abs().max()
+        else:
+            v = 2.0 ** 118 * (1 + 2.0 ** -6 * v)
+        codes, scale, mid = plain.codes_of(torch.stack([k, v]))
+        for pg in range(-(-n // P)):
+            m = min(P, n - pg * P)
+            full = [torch.zeros(2, 1, P, D, dtype=torch.int64), torch.full((2, 1, P), math.nan, dtype=torch.float64), torch.zeros(2, 1, P, dtype=torch.float64)]
+            for f, x in zip(full, (codes, scale, mid)):
+                f[:, 0, :m] = x[:, pg * P:pg * P + m]
+            pool[int(table[b, pg])] = plain.pack(*full, P, D)
+    q = (side * (1 + 0.01 * rnd(H, D, seed=99))).reshape(1, -1).repeat(2, 1).to(dtype)
+    out, ctx = run_decode(q, pool.to(DEV), table, lens, H, kv, D, P)
+    assert torch.isfinite(out).all()
+    check(out, plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5), dtype, H, D)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("H,kv,D,P,lens", [(4, 4, 128, 64, [1, 70, 130]), (7, 1, 64, 16, [33, 18]), (20, 1, 128, 32, [50]), (6, 2, 256, 16, [20, 1])])
 def test_decode_adds_the_weights_up(dtype, H, kv, D, P, lens):
     table, n_pages = tables(lens, P, 61, extra_width=1)
