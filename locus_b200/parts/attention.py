@@ -52,7 +52,8 @@ CHUNK_TILE = 16  # queries per work item of the CUDA-core chunk kernel
 class AttentionTiles(StepPlan):
     """The work lists of this file's attention kernels: tiles of 16 queries (CUDA-core kernel) and of 64 queries
     (tensor-core kernels) over the segments with more than one new token, and the segments with exactly one
-    (the decode kernel).  One plan serves every attention layer of a model.  The lists are made by two small
+    (the decode kernel); in a step with portions also every segment's last new token, by its row and position (``last``: for
+    caches that keep the weight that a key receives).  One plan serves every attention layer of a model.  The lists are made by two small
     native helpers (csrc/host_core.cpp: ``locus_plan_query_tiles``, ``locus_plan_segments_with``).  The tiles are
     listed by the position of their first query, ascending, across requests: the kernels walk a list from its end,
     so the tiles with the most keys start first (``locus_sort_tiles_by_position``)."""
@@ -66,7 +67,7 @@ class AttentionTiles(StepPlan):
 
     def capacity(self, max_tokens: int, max_segments: int) -> int:
         tiles = max_tokens // CHUNK_TILE + max_tokens // K.MMA_QUERY_TILE + 2 * max_segments
-        return 2 * tiles + max_segments
+        return 2 * tiles + 4 * max_segments
 
     def build(self, seg_q0, seg_qn, seg_ctx, out):
         n_seg, qn, cap = len(seg_qn), seg_qn.ctypes.data, len(out)
@@ -81,9 +82,14 @@ class AttentionTiles(StepPlan):
         ctx = seg_ctx.ctypes.data
         self._lib.locus_sort_tiles_by_position(n16, base, ctx)
         self._lib.locus_sort_tiles_by_position(n64, base + 4 * o64, ctx)
+        o_last, n_last = o1 + n1, n_seg if n16 else 0
+        if n_last:
+            last = out[o_last : o_last + 3 * n_seg].reshape(3, n_seg)
+            last[0], last[1], last[2] = range(n_seg), seg_q0 + seg_qn - 1, seg_ctx + seg_qn - 1
         return {"chunk_items": (0, 2 * n16, (-1, 2)), "n_chunk_items": n16,
                 "chunk_items64": (o64, 2 * n64, (-1, 2)), "n_chunk_items64": n64,
-                "decode_items": (o1, n1, None), "n_decode_items": n1}
+                "decode_items": (o1, n1, None), "n_decode_items": n1,
+                "last": (o_last, 3 * n_last, (3, -1) if n_last else None), "n_last": n_last}
 
 
 # tensor names below an attention's prefix, by role; an architecture with other names passes its own
@@ -414,13 +420,15 @@ class Attention(Mixer):
                       scale=self.scale)
         tiles = batch.plans[AttentionTiles.key]
         pool = cache.pool
-        if pool.dtype == torch.uint8:
+        q4 = pool.dtype == torch.uint8
+        if q4:
             if tiles["n_chunk_items"]:
                 # the kernels of portions read ordinary pages: those of the portions' requests, laid out for this layer
                 pool = rt.buf("attention.q4_wide", (pool.shape[0], 2, self.n_kv_heads, gb.page_tokens, self.head_dim), rt.dtype)
                 K.expand_q4(cache.pool, pool, segs=None, n_segs=batch.n_seg, seg_ctx=batch.seg_ctx, seg_qn=batch.seg_qn, min_new=2,
                             block_table=gb.block_table, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, page_tokens=gb.page_tokens,
                             max_keys=batch.longest)
+            self._attend_q4(q, o, batch, cache, gb, rt, tiles, common, extra)
         # splits of 128 keys that cover the longest context (all that the block table can describe when the
         # step's launches must not depend on its lengths)
         cap_splits = (gb.block_table.shape[1] * gb.page_tokens - 1) // K.DECODE_SPLIT + 1
@@ -451,8 +459,8 @@ class Attention(Mixer):
                      n_splits=n_splits, part_o=part_o, part_ml=part_ml, **extra, **common)
             else:
                 K.attn_chunk(q, pool, o, items=tiles["chunk_items"], n_items=tiles["n_chunk_items"], **extra, **common)
-        if cache.pool.dtype == torch.uint8:
-            return self._attend_q4(q, o, batch, cache, gb, rt, tiles, common, extra)
+        if q4:
+            return
         if tiles["n_decode_items"]:
             n = tiles["n_decode_items"]
             # scratch sized once, for the longest context that the block table can describe
@@ -467,17 +475,13 @@ class Attention(Mixer):
             K.attn_decode(q, cache.pool, o, items=tiles["decode_items"], n_items=n, part_o=part_o,
                           part_ml=part_ml, counters=counters, max_splits=max_splits, **extra, **common)
 
-
     def _attend_q4(self, q, o, batch, cache, gb, rt, tiles, common, extra) -> None:
         """Single tokens over a cache held in 4 bits.  Where the keys' weights are kept, a portion's last token counts like a single one: its
-        attention runs here (again), and adds its weights up."""
+        attention runs here too and adds its weights up; the portion's own kernel then writes its output."""
         n, items = tiles["n_decode_items"], tiles["decode_items"]
         seg_q0, seg_ctx = batch.seg_q0, batch.seg_ctx
-        if cache.weights is not None and tiles["n_chunk_items"]:
-            n = batch.n_seg
-            items = rt.shared_object(("attention.q4_segments", rt.max_segments), lambda: torch.arange(rt.max_segments, dtype=torch.int32, device=rt.device))
-            last = rt.buf("attention.q4_last", (2, rt.max_segments), torch.int32)
-            seg_q0, seg_ctx = (torch.add(start, batch.seg_qn, out=last[i, :n]).sub_(1) for i, start in enumerate((batch.seg_q0, batch.seg_ctx)))
+        if cache.weights is not None and tiles["n_last"]:
+            n, (items, seg_q0, seg_ctx) = tiles["n_last"], tiles["last"]
         if not n:
             return
         units = K.decode_units_q4(rt.max_segments, self.n_heads, rt.device, fixed_ranges=self.keep_first > 0)

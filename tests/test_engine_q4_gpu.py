@@ -125,6 +125,26 @@ def test_replayed_steps_and_several_requests(model_case, weigh):
     assert runner.stats["graph_replays"] > 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_keeping_the_weights_changes_no_output(tmp_path, dtype):
+    """Bit for bit, single tokens beside portions too: a portion's last token has its weights added up by the kernel of single tokens, but its output
+    comes from the portion's kernel either way."""
+    from locus_b200.engine.step import StepEntry
+
+    raw = CASES["heads64"]
+    folder = make_model_dir(tmp_path, "A", raw=dict(raw))
+    tokens = random_tokens(80, raw["vocab_size"], 12)
+    seen = []
+    for weigh in (False, True):
+        runner, cache = runner_of(folder, dtype, weigh=weigh)
+        out = [feed(runner, cache, "a", tokens[:40], [33, 1, 6])]
+        a, b = cache.get("a"), cache.open("b")
+        assert cache.ensure_capacity(a, 1) and cache.ensure_capacity(b, 21)
+        out.append(runner.step([StepEntry(a, tokens[40:41], [0]), StepEntry(b, tokens[41:62], list(range(21)))]).double().cpu())
+        seen.append(torch.cat(out))
+    assert torch.equal(seen[0], seen[1])
+
+
 def test_generation_with_and_without_letting_go(tmp_path):
     from locus_b200.engine.engine import Engine
 
