@@ -2,6 +2,8 @@
 
     python -m locus_b200.tools.kernel_bench linear --m 2048 --n 6144 --k 2048 [--dual] [--accumulate] [--iters 20]
     python -m locus_b200.tools.kernel_bench attn_decode --batch 8 --ctx 4000 [--heads 16 --kv-heads 16 --head-dim 128]
+    python -m locus_b200.tools.kernel_bench attn_decode --kv-bits 4 --batch 8 --ctx 4000 [--weigh]
+    python -m locus_b200.tools.kernel_bench cache_q4 --tokens 2048 [--batch 8 --ctx 8192 --layers 12 --keep 2048]
     python -m locus_b200.tools.kernel_bench attn_chunk --tokens 2048 --ctx 0
     python -m locus_b200.tools.kernel_bench experts --tokens 2048 [--experts 60 --top-k 4 --k 2048 --n 1408] [--part up|down]
     python -m locus_b200.tools.kernel_bench recurrence --tokens 2048 --batch 1 [--heads 16 --head-dim 128 --v-dim 128]
@@ -156,7 +158,73 @@ def _paged(args, B: int, ctx: int, new: int):
     return pool, q, torch.empty_like(q), meta, kw, i32
 
 
+def _cache_q4(args, layers: int, pages: int) -> torch.Tensor:
+    """A pool of 4 bits with random codes and factors (scale 1/4, middle 1/16)."""
+    P, D = args.page_tokens, args.head_dim
+    pool = torch.randint(0, 256, (layers, pages, 2, args.kv_heads, K.q4_page_bytes(D, P)), dtype=torch.uint8, device="cuda:0")
+    pool[..., P * D // 2:] = torch.tensor([0.25, 0.0625], dtype=torch.bfloat16, device="cuda:0").view(torch.uint8).repeat(P)
+    return pool
+
+
+def _bench_attn_decode_q4(args) -> None:
+    B, ctx, P, D, H = args.batch, args.ctx, args.page_tokens, args.head_dim, args.heads
+    per = ctx // P + 1
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda:0")  # noqa: E731
+    pool = _cache_q4(args, 1, B * per)[0]
+    q = torch.randn(B, H * D, device="cuda:0").to(getattr(torch, args.dtype))
+    out, units = torch.empty_like(q), K.decode_units_q4(B, H, "cuda:0", fixed_ranges=args.keep_first > 0)
+    floats = lambda n: torch.empty(n, device="cuda:0")  # noqa: E731
+    kw = dict(seg_q0=i32(list(range(B))), seg_ctx=i32([ctx] * B), items=i32(list(range(B))), n_items=B, scale=D ** -0.5, window=args.window,
+              block_table=torch.randperm(B * per, device="cuda:0").to(torch.int32).view(B, per), n_heads=H, n_kv_heads=args.kv_heads, head_dim=D,
+              page_tokens=P, part_o=floats(units * D + 2 * B * H + 4), part_ml=floats(2 * units), keep_first=args.keep_first, sink=args.sink,
+              counters=torch.zeros(B * H, dtype=torch.int32, device="cuda:0"), chunk=args.chunk)
+    if args.slopes:
+        kw["slopes"] = torch.full((H,), 0.05, device="cuda:0")
+    if args.weigh:
+        kw.update(weights=torch.zeros(B * per, args.kv_heads, P, device="cuda:0"), scores=floats(B * H * per * P))
+    us = _time(lambda: K.attn_decode_q4(q, pool, out, **kw), args.iters, args.graph)
+    seen = ctx % args.chunk + 1 if args.chunk else ctx + 1 if not args.window else min(ctx + 1, args.window + args.keep_first)
+    byts = B * seen * 2 * args.kv_heads * (D // 2 + 4)
+    print(f"attn_decode 4 bits batch={B} ctx={ctx} heads={H}/{args.kv_heads} head_dim={D} weigh={args.weigh} {args.dtype}: "
+          f"{us:.1f} us/call  cache read {byts / us / 1e3:.1f} GB/s")
+
+
+def bench_cache_q4(args) -> None:
+    """Rows written for --tokens new tokens; those rows laid out in ordinary pages; --batch requests of --ctx tokens in --layers layers evicted
+    down to --keep (into other pages, so that every call does the same)."""
+    P, D, H, kv, T = args.page_tokens, args.head_dim, args.heads, args.kv_heads, args.tokens
+    dt = getattr(torch, args.dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda:0")  # noqa: E731
+    size = dict(n_kv_heads=kv, head_dim=D, page_tokens=P)
+    pages = -(-T // P)
+    pool = _cache_q4(args, 1, pages)[0]
+    qkv, q = torch.randn(T, (H + 2 * kv) * D, device="cuda:0").to(dt), torch.empty(T, H * D, dtype=dt, device="cuda:0")
+    at = torch.arange(T, dtype=torch.int32, device="cuda:0")
+    freq = torch.tensor([1e-4 ** (2 * i / D) for i in range(D // 2)], dtype=torch.float32, device="cuda:0")
+    us = _time(lambda: K.rope_kv_write_q4(qkv, at, freq, q, pool, at, n_heads=H, rot_dim=D, interleaved=False, **size), args.iters, args.graph)
+    row, elt = kv * 2 * (D // 2 + 4), qkv.element_size()
+    print(f"write 4 bits tokens={T} heads={H}/{kv} head_dim={D} {args.dtype}: {us:.1f} us/call  "
+          f"{(T * (elt * (2 * H + 2 * kv) * D + row)) / us / 1e3:.1f} GB/s")
+    wide = torch.empty(pages, 2, kv, P, D, dtype=dt, device="cuda:0")
+    zero, new, line = i32([0]), i32([T]), torch.arange(pages, dtype=torch.int32, device="cuda:0").view(1, -1)
+    us = _time(lambda: K.expand_q4(pool, wide, segs=None, n_segs=1, seg_ctx=zero, seg_qn=new, block_table=line, max_keys=T, **size), args.iters, args.graph)
+    print(f"expand 4 bits tokens={T} kv_heads={kv} head_dim={D} {args.dtype}: {us:.1f} us/call  {T * (row + 2 * kv * D * elt) / us / 1e3:.1f} GB/s")
+    del pool, wide
+    B, n, keep, L = args.batch, args.ctx, args.keep, args.layers
+    per, to = -(-n // P), -(-min(keep, n) // P)
+    pool = _cache_q4(args, L, B * (per + to))
+    weights = torch.rand(L, B * (per + to), kv, P, device="cuda:0")
+    order = torch.randperm(B * (per + to), device="cuda:0").to(torch.int32)
+    kw = dict(block_table=order[:B * per].view(B, per), dst_table=order[B * per:].view(B, to), n_tokens=i32([n] * B), n_items=B, keep=keep, first=4,
+              recent=keep // 4, kept=torch.empty(L, B, kv, keep, dtype=torch.int32, device="cuda:0"), max_tokens=n)
+    us = _time(lambda: K.evict_q4(pool, weights, **kw, **size), args.iters, args.graph)
+    byts = L * B * kv * (4 * n + min(keep, n) * (2 * 2 * (D // 2 + 4) + 8))
+    print(f"evict 4 bits batch={B} ctx={n} -> {keep} layers={L} kv_heads={kv} head_dim={D}: {us:.1f} us/call  {byts / us / 1e3:.1f} GB/s")
+
+
 def bench_attn_decode(args) -> None:
+    if args.kv_bits == 4:
+        return _bench_attn_decode_q4(args)
     B, ctx = args.batch, args.ctx
     pool, q, out, meta, kw, i32 = _paged(args, B, ctx, 1)
     ms = ctx // K.DECODE_SPLIT + 1
@@ -510,7 +578,7 @@ def bench_sample(args) -> None:
 
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="kernel_bench")
-    ap.add_argument("kernel", choices=["linear", "attn_decode", "attn_chunk", "experts", "sample", "recurrence", "head_prep", "rows", "latent"])
+    ap.add_argument("kernel", choices=["linear", "attn_decode", "attn_chunk", "experts", "sample", "recurrence", "head_prep", "rows", "latent", "cache_q4"])
     ap.add_argument("--rows", type=int, default=8, help="sample: rows of logits")
     ap.add_argument("--vocab", type=int, default=151936, help="sample: logits of a row")
     ap.add_argument("--one-block", action="store_true", help="sample: never the cluster kernel")
@@ -535,6 +603,10 @@ def main(argv=None) -> int:
     ap.add_argument("--delta", action="store_true", help="recurrence: the gated delta rule instead")
     ap.add_argument("--gla", action="store_true", help="recurrence: gated linear attention (a decay per key channel) instead")
     ap.add_argument("--page-tokens", type=int, default=64)
+    ap.add_argument("--kv-bits", type=int, default=0, choices=[0, 4], help="attn_decode: over a cache held in 4 bits")
+    ap.add_argument("--weigh", action="store_true", help="attn_decode: with --kv-bits 4, add up the weights that the keys get")
+    ap.add_argument("--layers", type=int, default=12, help="cache_q4: layers that are evicted from at once")
+    ap.add_argument("--keep", type=int, default=2048, help="cache_q4: keys of a head that stay")
     ap.add_argument("--rank", type=int, default=512, help="latent: the latent's size")
     ap.add_argument("--absorbed", action="store_true", help="latent: long portions over the cached latents, too")
     ap.add_argument("--window", type=int, default=0)
@@ -568,7 +640,8 @@ def main(argv=None) -> int:
         print("kernel_bench: no CUDA device", file=sys.stderr)
         return 1
     {"linear": bench_linear, "attn_decode": bench_attn_decode, "attn_chunk": bench_attn_chunk,
-     "experts": bench_experts, "sample": bench_sample, "recurrence": bench_recurrence, "head_prep": bench_head_prep, "rows": bench_rows, "latent": bench_latent}[args.kernel](args)
+     "experts": bench_experts, "sample": bench_sample, "recurrence": bench_recurrence, "head_prep": bench_head_prep, "rows": bench_rows, "latent": bench_latent,
+     "cache_q4": bench_cache_q4}[args.kernel](args)
     return 0
 
 
