@@ -468,10 +468,10 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
         const Q4Unit un = q4_unit<W>(pl, load, warp, n_items, n_vh);
         if (lane == 0) pl.units[warp] = un;   // (for the joins)
         const bool active = un.active;
-        const int item = un.item, vh = un.vh, range = un.range, n_ranges = un.n_ranges, wa = un.wa, wb = un.wb;
+        const int item = un.item, vh = un.vh, range = un.range, n_ranges = un.n_ranges, wa = un.wa;
         const int kvh = n_sub == 1 ? vh : vh / n_sub, g0 = (vh - kvh * n_sub) * 8 * HT;
         const int nG = min(G - g0, 8 * HT), h0 = kvh * G + g0;   // this warp's heads: h0 .. h0 + nG - 1
-        const int seg = pl.seg[item], p = pl.pos[item], first = q4_first(a, p), r0 = pl.pref[item];
+        const int seg = pl.seg[item], p = pl.pos[item], first = q4_first(a, p);
         const int row = pl.row[item];
         const bool whole = un.parts == 1;
 
@@ -830,21 +830,33 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             }
             if (WEIGH && lane == 0) *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(at_item) * a.nh + h)) = make_float2(M, inv);
         };
-        if (active) {
-            // the heads of a run of warps, dealt to its warps
-            for (int g = warp - wa; g < nG; g += wb - wa) {
+        // what a (request, head) that a warp leads is, and the first of its heads that this warp takes: the block's heads go round the warps
+        struct Led {
+            int item, range, n, h0, n_heads, parts, lead;
+        };
+        auto led = [&](int at) {
+            const Q4Unit& u = pl.units[at];
+            const int lkv = n_sub == 1 ? u.vh : u.vh / n_sub, g = (u.vh - lkv * n_sub) * 8 * HT;
+            return Led{u.item, u.range, u.wb - u.wa, lkv * G + g, min(G - g, 8 * HT), u.parts, u.lead};
+        };
+        int turn = warp;   // heads until this warp's next one
+        for (unsigned leads = __ballot_sync(0xffffffffu, lane < W && pl.units[lane].active && pl.units[lane].wa == lane); leads; leads &= leads - 1) {
+            const int at = __ffs(leads) - 1;
+            const Led r = led(at);
+            int g = turn;
+            for (; g < r.n_heads; g += W) {
                 const float* ml = res0 + 8 * HT * HD + 2 * g;
-                const int n = wb - wa;
-                const float2 mine = lane < n ? *reinterpret_cast<const float2*>(ml + (wa + lane) * RES_STEP) : make_float2(-INFINITY, 0.f);
+                const float2 mine = lane < r.n ? *reinterpret_cast<const float2*>(ml + (at + lane) * RES_STEP) : make_float2(-INFINITY, 0.f);
                 const float M = warp_max(mine.x);
                 const float w = part_weight(mine, M);
                 const float L = warp_sum(w == 0.f ? 0.f : mine.y * w);
                 float acc[DL];
 #pragma unroll
                 for (int d = 0; d < DL; ++d) acc[d] = 0.f;
-                for (int j = 0; j < n; ++j) {
+#pragma unroll 4
+                for (int j = 0; j < r.n; ++j) {
                     const float wj = __shfl_sync(0xffffffffu, w, j);
-                    const float* src = res0 + (wa + j) * RES_STEP + g * HD + lane * DL;
+                    const float* src = res0 + (at + j) * RES_STEP + g * HD + lane * DL;
 #pragma unroll
                     for (int d = 0; d < DL; d += 2) {
                         const float2 x = *reinterpret_cast<const float2*>(src + d);
@@ -852,16 +864,17 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         acc[d + 1] = fmaf(x.y, wj, acc[d + 1]);
                     }
                 }
-                if (whole) {
-                    finish(g, acc, L, M, h0, row, item);
+                if (r.parts == 1) {
+                    finish(g, acc, L, M, r.h0, pl.row[r.item], r.item);
                 } else {
-                    const size_t place = static_cast<size_t>(r0 + range - (warp - wa)) * a.nh + h0 + g;   // of the run's first range
+                    const size_t place = static_cast<size_t>(pl.pref[r.item] + r.range) * a.nh + r.h0 + g;   // of the run's first range
                     float* dst = a.part_o + place * HD + lane * DL;
 #pragma unroll
                     for (int d = 0; d < DL; d += 2) *reinterpret_cast<float2*>(dst + d) = make_float2(acc[d], acc[d + 1]);
                     if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * place) = make_float2(M, L);
                 }
             }
+            turn = g - r.n_heads;
         }
         if (!__syncthreads_or(active && !whole)) continue;   // (the rings are free again behind this)
         // (request, head)s that several blocks have ranges of: the last block to bring its partial result joins them all
@@ -877,18 +890,17 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             is_last[warp] = last;
         }
         __syncthreads();
-        for (int lead = 0; lead < W; ++lead) {
-            if (!is_last[lead]) continue;
-            // (all warps of the block take part)
-            const Q4Unit lu = pl.units[lead];
-            const int lkv = n_sub == 1 ? lu.vh : lu.vh / n_sub, lg0 = (lu.vh - lkv * n_sub) * 8 * HT, lnG = min(G - lg0, 8 * HT), lh0 = lkv * G + lg0;
-            const int parts = lu.parts;
+        turn = warp;   // (all warps of the block take part)
+        for (unsigned leads = __ballot_sync(0xffffffffu, lane < W && is_last[lane]); leads; leads &= leads - 1) {
+            const Led r = led(__ffs(leads) - 1);
+            const int parts = r.parts;
             // a part begins with the first range that its block has
             auto place = [&](int k, int g) {
-                const int first_range = k == 0 ? 0 : lu.lead + (k - 1) * W;
-                return static_cast<size_t>(pl.pref[lu.item] + first_range) * a.nh + lh0 + g;
+                const int first_range = k == 0 ? 0 : r.lead + (k - 1) * W;
+                return static_cast<size_t>(pl.pref[r.item] + first_range) * a.nh + r.h0 + g;
             };
-            for (int g = warp; g < lnG; g += W) {
+            int g = turn;
+            for (; g < r.n_heads; g += W) {
                 constexpr int ROWS = 16;   // rows on their way together, with the first of the factors
                 float M = -INFINITY, L = 0.f, acc[DL];
 #pragma unroll
@@ -921,8 +933,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         }
                     }
                 }
-                finish(g, acc, L, M, lh0, pl.row[lu.item], lu.item);
+                finish(g, acc, L, M, r.h0, pl.row[r.item], r.item);
             }
+            turn = g - r.n_heads;
         }
         __syncthreads();   // (is_last is written again in the next round)
     }
