@@ -2,29 +2,30 @@
 //
 //   o_h = sum_t p_t v_t   p = softmax over the keys in sight of scale * q_h . k_t (a sink, a distance bias: as in attention.cu)
 //
-// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5) = z + scale (code - 7), z = mid - scale / 2, and codes less 7 are
-// small whole numbers that float16 holds exactly, so
+// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5), so
 //
-//   q . k_t = scale_t (q . (code_t - 7)) + z_t sum(q)                      the product on the tensor cores, the rest per score in float32
-//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t z_t             the same for the values
+//   q . k_t = scale_t (q . code_t) + (mid_t - 7.5 scale_t) sum(q)              the product on the tensor cores, the rest per score in float32
+//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t (mid_t - scale_t / 2)   the same for the values
 //
-// The tensor cores' operands are float16:
-//   * codes less 7: a nibble n under the exponent of 1024 is 1024 + n, in the next four bits 1024 + 16 n, and one addition or multiply-add (two
-//     codes an instruction) leaves n - 7.  (A nibble alone is the subnormal number n 2^-24 and would need neither, but the tensor cores align what
-//     they add by the operands' exponent fields: sums of such products were off by 1e-4.  The 7 is taken off the codes rather than out of the
-//     sums, where it would grow over the keys and lose what cancels.)
-//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
-//     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more;
-//   * the weights p_t scale_t, formed relative to the running maximum M of score_t + e_t, e_t the exponent of the key's own scale (of its mid less 20
-//     where that is more), so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the largest
-//     where that is more; two parts for a float32 model).  The unrounded p_t enter the denominator and z's sum.
+// The tensor cores' operands:
+//   * scores of a bfloat16 model: codes as unsigned bytes (a mask, and a shift for every other one) times q as whole numbers of 16 bits, in a signed
+//     and an unsigned byte: a power of two per head brings its largest element to 2^14 .. 2^15 (taken out of the scores again).  Elements down to 2^-7 of
+//     the largest are exact, smaller ones off by at most 2^-15 of the largest, which itself stands for anything within 2^-9; sums are exact.
+//   * scores of a float32 model: codes less 7 and q in float16, q scaled likewise and in two parts, 22 bits and more;
+//   * values: codes less 7 in float16 (exact): a nibble n under the exponent of 1024 is 1024 + n, in the next four bits 1024 + 16 n, and one addition
+//     or multiply-add (two codes an instruction) leaves n - 7.  (A nibble alone is the subnormal number n 2^-24 and would need neither, but the tensor
+//     cores align what they add by the operands' exponent fields: sums of such products were off by 1e-4.  The 7 is taken off the codes rather than
+//     out of the sums, where it would grow over the keys and lose what cancels.)
+//   * the weights p_t scale_t in float16, formed relative to the running maximum M of score_t + e_t, e_t the exponent of the key's own scale (of its mid
+//     less 20 where that is more), so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the
+//     largest where that is more; two parts for a float32 model).  The unrounded p_t enter the denominator and the sum of the middles.
 // For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
 // over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
 // A warp takes a range of keys of one (request, key/value head) for up to 16 query heads that share it, in the transposed form (16 keys in the M
 // dimension of mma.sync m16n8k16, eight heads in N):
-//   S^T [16 keys x 8 heads] = (C_k - 7) [16 x hd] . Q^T     a lane's words of a key row hold eight codes each, two neighbouring dimensions in a
-//                             register's halves as the A fragment wants them;
+//   S^T [16 keys x 8 heads] = C_k [16 x hd] . Q^T           (m16n8k32 with bytes) a lane's words of a key row hold eight codes each, in a word's low and
+//                             high nibbles four dimensions as the A fragment wants them;
 //   O^T [hd x 8 heads] += (C_v - 7)^T [hd x 16 keys] . P^T  the A fragment wants one dimension of two keys in a register: a byte permute joins
 //                             the same byte of two keys' words, and its two nibbles are two dimensions (two row tiles' halves).
 // A group of more heads is served by several warps (that each read its rows, from the L2 after the first).
@@ -38,6 +39,8 @@
 // Memory: a warp's ring in shared memory is filled by bulk copies, up to 64 keys at a time: codes and factors of K, then of V.  (A whole page of
 // 64 tokens is one run of bytes per plane; of other pages a lane each asks for the codes and the factors.)  Every wait is bounded: when the limit runs out the warp records it in the module's error
 // word, waits for its other copies with the same limit and goes on to the end without a further copy.
+// What a key's four factors come to is worked out by one lane and left in the place of its chunks' codes of K, which are in registers by then: all
+// four lanes of a row of fragments need it (64 requests of up to 8,192 keys: 50.1 -> 47.7 us; scores by bytes before that: 52.6 -> 50.1).
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
 //
@@ -119,6 +122,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
+// this thread's accesses to shared memory so far come before copies into it that are issued behind the next barrier
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 // N (1, 2, 4 or 8) words of shared memory
 template <int N>
@@ -141,6 +146,19 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// codes as unsigned bytes times signed (unsigned) bytes, summed in 32-bit whole numbers
+__device__ __forceinline__ void mma_u8s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8u8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // transpose of an 8 x 8 matrix of 16-bit elements held as mma fragments (two elements of a row per lane)
@@ -506,7 +524,6 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 const int page = __shfl_sync(0xffffffffu, page_ids, (page_at - page_from + lane) & 31);
                 const uint32_t dst = ring + st * STAGE, bar = bars + 8 * st;
                 if (lane == 0) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the reads of what lies there
                     mbar_expect_tx(bar, 2 * n * (RB + Q4_FACTOR_BYTES));
                     if (n == SK && P == SK) {
                         const uint8_t* src = pool_head + page * (2 * plane_step);
@@ -523,7 +540,6 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         const uint8_t* src = pool_head + page * (2 * plane_step);
                         const uint8_t* codes = src + static_cast<size_t>(off) * RB;
                         const uint8_t* factors = src + static_cast<size_t>(P) * RB + static_cast<size_t>(off) * Q4_FACTOR_BYTES;
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         bulk_copy(dst + at * RB, codes, m * RB, bar);
                         bulk_copy(dst + SK * RB + at * Q4_FACTOR_BYTES, factors, m * Q4_FACTOR_BYTES, bar);
                         bulk_copy(dst + PLANE + at * RB, codes + plane_step, m * RB, bar);
@@ -571,9 +587,23 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * KW; ++i) {
-                    split2<PARTS>(x[ht][4 * i] * up, x[ht][4 * i + 1] * up, qb[ht][i][0]);
-                    split2<PARTS>(x[ht][4 * i + 2] * up, x[ht][4 * i + 3] * up, qb[ht][i][1]);
+                    if constexpr (PARTS == 2) {
+                        split2<PARTS>(x[ht][4 * i] * up, x[ht][4 * i + 1] * up, qb[ht][i][0]);
+                        split2<PARTS>(x[ht][4 * i + 2] * up, x[ht][4 * i + 3] * up, qb[ht][i][1]);
+                    }
                     sum += (x[ht][4 * i] + x[ht][4 * i + 1]) + (x[ht][4 * i + 2] + x[ht][4 * i + 3]);
+                }
+                if constexpr (PARTS == 1) {
+#pragma unroll
+                    for (int w = 0; w < KW; ++w)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {   // the low nibbles of a word's bytes are its values 0, 4, 1 and 5, the high ones 2, 6, 3 and 7
+                            int v[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) v[j] = __float2int_rn(x[ht][8 * w + 2 * y + (j & 1) * 4 + (j >> 1)] * up);
+                            qb[ht][2 * w + y][0][0] = __byte_perm(__byte_perm(v[0], v[1], 0x0051), __byte_perm(v[2], v[3], 0x0051), 0x5410);
+                            qb[ht][2 * w + y][1][0] = __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
+                        }
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -606,61 +636,87 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // N chunks of sixteen keys, from c0 (those from `stop` on are dead), whose rows lie at `at` (K; V's are PLANE further on) and factors at `fac`
             // (SPECIAL: dead keys among them, or a distance bias; a copy of its own, for the plain steps' sake)
             const bool biased_call = a.slopes != nullptr;
-            auto step = [&](auto special, int c0, int stop, const unsigned char* at, const unsigned char* fac) {
+            auto step = [&](auto special, int c0, int stop, unsigned char* at, const unsigned char* fac) {
                 constexpr bool SPECIAL = decltype(special)::value;
                 const bool edge = SPECIAL && (c0 < t_lo || c0 + 16 * N > stop), biased = SPECIAL && biased_call;
                 // chunk n: keys c0 + 16 n + kr0 and + 8 + kr0
                 float s[N][HT][4];
-                uint32_t kf[N][2], vf[N][2];
+                uint32_t k_lo[N][KW], k_hi[N][KW];
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    uint32_t k_lo[KW], k_hi[KW];
-                    lds_words<KW>(k_lo, at + (16 * n + kr0) * RB + t4 * (RB / 4));
-                    lds_words<KW>(k_hi, at + (16 * n + kr0 + 8) * RB + t4 * (RB / 4));
+                    lds_words<KW>(k_lo[n], at + (16 * n + kr0) * RB + t4 * (RB / 4));
+                    lds_words<KW>(k_hi[n], at + (16 * n + kr0 + 8) * RB + t4 * (RB / 4));
+                }
+                // a key's factors, a lane each: (scales of K and, times 2^-exponent, of V | z of K | z of V times 2^-exponent | exponent)
+                auto dead = [&](int key) { return edge && !((key >= t_lo || key < keep) && key < stop); };
+                {
+                    const int at_key = lane & (16 * N - 1);
+                    uint32_t kf, vf;
+                    lds_words<1>(&kf, fac + 4 * at_key);
+                    lds_words<1>(&vf, fac + PLANE + 4 * at_key);
+                    if (dead(c0 + at_key)) kf = vf = 0u;
+                    const float kz = fmaf(PARTS == 1 ? -7.5f : -0.5f, q4_scale(kf), q4_mid(kf));
+                    const int of_scale = static_cast<int>(vf << 16 & 0x7f800000u), of_mid = static_cast<int>(vf & 0x7f800000u);
+                    const int top = min(__vimax3_s32(of_scale, of_mid - (MID << 23), (LEAST + 127) << 23), 253 << 23);   // (NaN: any)
+                    const float ve = __int_as_float(0x4b000000 | top >> 23) - 8388735.f;   // (2^23 + 127)
+                    const float down = __int_as_float((254 << 23) - top), vs = q4_scale(vf) * down, vz = fmaf(-0.5f, vs, q4_mid(vf) * down);
+                    __syncwarp();
+                    *reinterpret_cast<uint4*>(at + 16 * at_key) = make_uint4((__float_as_uint(vs) & 0xffff0000u) | (kf & 0xffffu), __float_as_uint(kz), __float_as_uint(vz), __float_as_uint(ve));
+                }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        lds_words<1>(&kf[n][i], fac + 4 * (16 * n + kr0 + 8 * i));
-                        lds_words<1>(&vf[n][i], fac + PLANE + 4 * (16 * n + kr0 + 8 * i));
-                    }
+                for (int n = 0; n < N; ++n) {
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) s[n][ht][0] = s[n][ht][1] = s[n][ht][2] = s[n][ht][3] = 0.f;
+                    if constexpr (PARTS == 1) {
+                        int hi[HT][4], lo[HT][4];
 #pragma unroll
-                    for (int w = 0; w < KW; ++w)
+                        for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t a0 = k_lo[w] >> (8 * x), a1 = k_hi[w] >> (8 * x);
-                            const uint32_t af[4] = {codes_low(a0, k1024), codes_low(a1, k1024), codes_high(a0, k1024), codes_high(a1, k1024)};
+                            for (int i = 0; i < 4; ++i) hi[ht][i] = lo[ht][i] = 0;
 #pragma unroll
-                            for (int ht = 0; ht < HT; ++ht)
+                        for (int w = 0; w < KW; ++w) {
+                            const uint32_t af[4] = {k_lo[n][w] & 0x0f0f0f0fu, k_hi[n][w] & 0x0f0f0f0fu, k_lo[n][w] >> 4 & 0x0f0f0f0fu, k_hi[n][w] >> 4 & 0x0f0f0f0fu};
 #pragma unroll
-                                for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
+                            for (int ht = 0; ht < HT; ++ht) {
+                                mma_u8s8(hi[ht], af, qb[ht][2 * w][0][0], qb[ht][2 * w + 1][0][0]);
+                                mma_u8u8(lo[ht], af, qb[ht][2 * w][1][0], qb[ht][2 * w + 1][1][0]);
+                            }
                         }
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[n][ht][i] = static_cast<float>(hi[ht][i] * 256 + lo[ht][i]);
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < KW; ++w)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t a0 = k_lo[n][w] >> (8 * x), a1 = k_hi[n][w] >> (8 * x);
+                                const uint32_t af[4] = {codes_low(a0, k1024), codes_low(a1, k1024), codes_high(a0, k1024), codes_high(a1, k1024)};
+#pragma unroll
+                                for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
+                            }
+                    }
                 }
                 // score + exponent of the two keys of a chunk; of V 2^-exponent, and scale and z times that
                 float sc[N][HT][4], down[N][2], vs[N][2], vz[N][2];
                 bool raise = false;
+                __syncwarp();
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
                     const int key[2] = {c0 + 16 * n + kr0, c0 + 16 * n + 8 + kr0};
-                    bool live[2] = {true, true};
-                    if (edge) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            live[i] = (key[i] >= t_lo || key[i] < keep) && key[i] < stop;
-                            if (!live[i]) kf[n][i] = vf[n][i] = 0u;
-                        }
-                    }
                     float ks[2], kz[2], ve[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        ks[i] = q4_scale(kf[n][i]);
-                        kz[i] = fmaf(-0.5f, ks[i], q4_mid(kf[n][i]));
-                        const int of_scale = static_cast<int>(vf[n][i] << 16 & 0x7f800000u), of_mid = static_cast<int>(vf[n][i] & 0x7f800000u);
-                        const int top = min(__vimax3_s32(of_scale, of_mid - (MID << 23), (LEAST + 127) << 23), 253 << 23);   // (NaN: any)
-                        ve[i] = __int_as_float(0x4b000000 | top >> 23) - 8388735.f;   // (2^23 + 127)
-                        down[n][i] = __int_as_float((254 << 23) - top);
-                        vs[n][i] = q4_scale(vf[n][i]) * down[n][i];
-                        vz[n][i] = fmaf(-0.5f, vs[n][i], q4_mid(vf[n][i]) * down[n][i]);
+                        const uint4 f = *reinterpret_cast<const uint4*>(at + 16 * (16 * n + kr0 + 8 * i));
+                        ks[i] = q4_scale(f.x);
+                        vs[n][i] = q4_mid(f.x);
+                        kz[i] = __uint_as_float(f.y);
+                        vz[n][i] = __uint_as_float(f.z);
+                        ve[i] = __uint_as_float(f.w);
+                        down[n][i] = ex2(-ve[i]);
                     }
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) {
@@ -671,9 +727,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             if (biased) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
                             if (WEIGH) {
                                 const int g = 8 * ht + 2 * t4 + c;
-                                if (g < nG && live[y]) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w - ve[y];
+                                if (g < nG && !dead(key[y])) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w - ve[y];
                             }
-                            if (edge && !live[y]) w = -INFINITY;
+                            if (dead(key[y])) w = -INFINITY;
                             sc[n][ht][i] = w;
                             raise |= w > limit[ht][c];
                         }
@@ -757,13 +813,14 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             };
 
             while (ok && k0 < k_stop) {
-                __syncwarp();  // every lane has read the stage before this one: its place may be overwritten
+                fence_async();
+                __syncwarp();  // every lane is done with the stage before this one, its writes there ordered in front of the copy that overwrites them
                 if (k_next < k_stop) issue(st + S - 1 < S ? st + S - 1 : st - 1);
                 const int end = stage_end(k0);
                 ok = mbar_wait(bars + 8 * st, (parity >> st) & 1u);
                 if (!ok) break;
                 parity ^= 1u << st;
-                const unsigned char* src = q4_smem + warp * (S * STAGE) + st * STAGE;
+                unsigned char* src = q4_smem + warp * (S * STAGE) + st * STAGE;
                 if (++st == S) st = 0;
                 const int n = end - k0;
                 // (a second chunk behind the stage's last key reads what an earlier stage left, as dead keys)
@@ -876,6 +933,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             }
             turn = g - r.n_heads;
         }
+        fence_async();
         if (!__syncthreads_or(active && !whole)) continue;   // (the rings are free again behind this)
         // (request, head)s that several blocks have ranges of: the last block to bring its partial result joins them all
         if (lane == 0) {

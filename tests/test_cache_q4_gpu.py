@@ -314,6 +314,53 @@ def test_scores_far_apart_and_rows_that_are_not_numbers():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_a_query_that_is_not_finite(dtype, value):
+    """... spoils its own head's output and no other's."""
+    H, kv, D, P = 6, 2, 128, 64
+    lens = [70, 130]
+    table, n_pages = tables(lens, P, 71)
+    pool = filled(table, lens, kv, D, P, 72, n_pages).to(DEV)
+    q = rnd(2, H * D, dtype=dtype, seed=73)
+    ref = plain.decode(q, pool, table, torch.tensor(lens) - 1, H, kv, D, P, D ** -0.5)
+    q[1, 4 * D + 9] = value
+    out, _ = run_decode(q, pool, table, lens, H, kv, D, P)
+    got = out.view(2, H, D)
+    assert torch.isnan(got[1, 4]).all()
+    got[1, 4] = ref[0][1, 4].to(DEV, dtype)
+    check(out, ref, dtype, H, D)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_queries_of_very_different_sizes(dtype):
+    """Heads of 2^-100 to 2^100, heads of zeros, and heads with one element 2^10 times the others.  Whole numbers of 16 bits hold such a head's small elements to
+    2^-15 of the largest: half a unit each, so a score is off by at most that times the row's sum of |scale (code - 7.5)|, and a weight by as much of itself."""
+    H, kv, D, P = 8, 1, 128, 64
+    lens = [150]
+    table, n_pages = tables(lens, P, 81)
+    pool = filled(table, lens, kv, D, P, 82, n_pages)
+    q = rnd(1, H * D, seed=83).view(H, D)
+    q[0] *= 2.0 ** -100
+    q[1] *= 2.0 ** -110
+    q[2] = 0
+    q[3, 5], q[4, 127] = 2.0 ** 10, -2.0 ** 10
+    q = q.reshape(1, -1).to(dtype)
+    out, ctx = run_decode(q, pool.to(DEV), table, lens, H, kv, D, P)
+    ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
+    if dtype == BF16:
+        got, want = out.cpu().double().view(H, D), ref[0][0]
+        codes, scale, mid = plain.fields(pool[table[0, :3].long()], P, D)
+        live = torch.arange(3 * P) < lens[0]
+        rows = (scale.unsqueeze(-1) * (codes.double() - 7.5)).abs()[:, 0, 0].reshape(-1, D).sum(1)[live]
+        values = plain.values(pool[table[0, :3].long()], P, D)[:, 1, 0].reshape(-1, D)[live].abs().max()
+        for h in (3, 4):
+            off = float(2.0 ** -15 * 2.0 ** 10 * rows.max() * D ** -0.5)    # of a score; the weights' change is at most twice that of their sum
+            assert ((got[h] - want[h]).abs() <= 2 * off * values + 2.0 ** -8 * want[h].abs() + ref[1][0, h] + SUMS * ref[2][0, h]).all()
+            out.view(H, D)[h] = want[h].to(DEV, dtype)
+    check(out, ref, dtype, H, D)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("kind", ["spread", "hidden", "large", "level"])
 def test_values_of_very_different_sizes(dtype, kind):
     """Rows of v from 2^-30 to 2^30 side by side; rows 2^60 times the others' size whose keys weigh nothing; rows near the type's largest number; and
