@@ -1000,26 +1000,41 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 }
 
 // weights[page][kvh][offset] += sum over the heads of the group of 2^(score - M) / denominator, for every key of the listed requests: scores,
-// maxima and denominators as the kernel above left them.  One thread per key; a slot is added to once per request that lists it, so the sum
-// does not depend on the order (an atomic: a request may be listed twice).
+// maxima and denominators as the kernel above left them.  WG_KEYS keys per thread, whose pages are looked up in front of the wait for that kernel and
+// whose scores are on their way together (bound by such latencies: with one key per thread a call for 8 requests of 4,096 keys on 16 heads took 29.9 us,
+// with four 29.0, with eight 29.6).
+// A slot is added to once per request that lists it, so the sum does not depend on the order (an atomic: a request may be listed twice).
 #define WG_THREADS 256
+#define WG_KEYS 4
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_kernel(Q4Args a, float* __restrict__ weights) {
-    pdl_entry();
-    pdl_trigger();
     const int item = blockIdx.z, kvh = blockIdx.y, G = a.nh / a.nkv, P = a.page_tokens;
     const int seg = a.items[item];
     const int n = min(a.seg_ctx[seg] + 1, a.table_stride * P);
-    const int t = blockIdx.x * WG_THREADS + threadIdx.x;
-    if (t >= n) return;
-    const float* at = a.scores + ((static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P + t) * G;
-    const float2* ml = reinterpret_cast<const float2*>(a.lse) + static_cast<size_t>(item) * a.nh + static_cast<size_t>(kvh) * G;
-    float sum = 0.f;
-    for (int g = 0; g < G; ++g) {
-        const float2 v = __ldg(ml + g);
-        sum = fmaf(ex2(at[g] - v.x), v.y, sum);
+    const int t0 = blockIdx.x * (WG_THREADS * WG_KEYS) + threadIdx.x;
+    const int* table = a.block_table + static_cast<size_t>(seg) * a.table_stride;
+    float* at[WG_KEYS];
+#pragma unroll
+    for (int u = 0; u < WG_KEYS; ++u) {
+        const int t = t0 + u * WG_THREADS, i = t / P;
+        at[u] = t < n ? weights + (static_cast<size_t>(table[i]) * a.nkv + kvh) * P + (t - i * P) : nullptr;
     }
-    const int page = a.block_table[static_cast<size_t>(seg) * a.table_stride + t / P];
-    atomicAdd(weights + (static_cast<size_t>(page) * a.nkv + kvh) * P + t % P, sum);
+    pdl_entry();
+    pdl_trigger();
+    if (t0 >= n) return;
+    const float* score = a.scores + ((static_cast<size_t>(item) * a.nkv + kvh) * a.table_stride * P + t0) * G;
+    const float2* ml = reinterpret_cast<const float2*>(a.lse) + static_cast<size_t>(item) * a.nh + static_cast<size_t>(kvh) * G;
+    float sum[WG_KEYS];
+#pragma unroll
+    for (int u = 0; u < WG_KEYS; ++u) sum[u] = 0.f;
+    for (int g = 0; g < G; ++g) {
+        const float2 v = ml[g];
+#pragma unroll
+        for (int u = 0; u < WG_KEYS; ++u)
+            if (at[u]) sum[u] = fmaf(ex2(score[static_cast<size_t>(u) * WG_THREADS * G + g] - v.x), v.y, sum[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < WG_KEYS; ++u)
+        if (at[u]) atomicAdd(at[u], sum[u]);
 }
 
 template <typename T, int HD, int HT, int N, int W, int S, int SK, bool WEIGH>
@@ -1091,7 +1106,7 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
     }
 #undef Q4_GO
     if (code || !v.weights) return code;
-    const dim3 grid(ceil_div(a.table_stride * a.page_tokens, WG_THREADS), a.nkv, n);
+    const dim3 grid(ceil_div(a.table_stride * a.page_tokens, WG_THREADS * WG_KEYS), a.nkv, n);
     locus_launch(q4_weigh_kernel, grid, WG_THREADS, 0, stream, a, v.weights);
     return locus_launch_status();
 }
