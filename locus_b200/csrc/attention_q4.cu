@@ -34,15 +34,22 @@
 //
 // The cut: every (request, key/value head) is cut into ranges of one length, a warp each (plan_ranges).  The warps of a block that have ranges of
 // one (request, head) join them in shared memory; what covers it whole is the output, else the block leaves one partial result, and the block that
-// is the last to do so joins those, in ascending order.  (With one partial result per warp, joined by the last warp, a request of 131,000 tokens took 270 us, most of it in that.)
+// is the last to do so joins those, in ascending order; in both joins the heads go round the block's warps.  (With one partial result per warp, joined
+// by the last warp, a request of 131,000 tokens took 270 us, most of it in that.)
 //
 // Memory: a warp's ring in shared memory is filled by bulk copies, up to 64 keys at a time: codes and factors of K, then of V.  (A whole page of
-// 64 tokens is one run of bytes per plane; of other pages a lane each asks for the codes and the factors.)  Every wait is bounded: when the limit runs out the warp records it in the module's error
-// word, waits for its other copies with the same limit and goes on to the end without a further copy.
+// 64 tokens is one run of bytes per plane; of other pages a lane each asks for the codes and the factors.)  Every wait is bounded: when the limit
+// runs out the warp records it in the module's error word, waits for its other copies with the same limit and goes on to the end without a further copy.
 // What a key's four factors come to is worked out by one lane and left in the place of its chunks' codes of K, which are in registers by then: all
 // four lanes of a row of fragments need it (64 requests of up to 8,192 keys: 50.1 -> 47.7 us; scores by bytes before that: 52.6 -> 50.1).
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
+//
+// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 162 registers, 104 KB of copies on their way per SM): the instructions that take codes
+// apart and the latencies between them, at three warps a scheduler; the copies alone (no arithmetic) take 12.7 us of the 23.6 of 8 requests of
+// 4,096 keys (71 MB, 3.0 TB/s), 41 of the 47.5 of 64 requests of 777 to 8,192 keys (28 heads on 4; 171 MB, 3.6 TB/s).  For few keys it is latency:
+// descriptors and cut 2.6 to 4 us, first page ids and rows 2.5, joins 1 to 4.  Sixteen warps of 128 registers, eight of 255, one or four chunks at a
+// time, smaller stages: all slower (25 to 28 us for 8 requests of 4,096 keys).
 //
 // With weights: the scores are written out as they are formed, and a second kernel (q4_weigh_kernel) adds every key's p_t, summed over the heads
 // of its group, to a number per (slot, key/value head).  The softmax's denominator is known only behind the last range.
@@ -175,7 +182,7 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 // the codes in bits 0 .. 3 of a register's halves, less 7: 0x6400 | n is 1024 + n.  (Mask and exponent in one LOP3 need one of the two constants in
-// a register; from two immediates the compiler makes two instructions, which cost a quarter of the loop's time.)
+// a register; from two immediates the compiler makes two instructions.)
 __device__ __forceinline__ uint32_t codes_low(uint32_t x, uint32_t k1024) {
     return bits(__hsub2(halves((x & 0x000f000fu) | k1024), halves(0x64076407u)));
 }
@@ -263,7 +270,7 @@ __device__ __forceinline__ int q4_blocks(const int* table, int ranges, int n_vh)
 // some warps may have nothing to do but fewer (request, head)s are joined across blocks.  The cost of a cut, in keys: rounds over the grid x
 // (length + cost_range), and cost_join once where blocks join, and cost_merge per partial result of the longest item.  Lengths
 // from what fills every warp once, 2 % apart, some shorter and longer ones, and the longest item's.
-// (8 requests of 4,096 keys on 16 heads: twelve ranges, a block each, 24.5 us; thirteen, unit after unit, 29.5.)
+// (8 requests of 4,096 keys on 16 heads: by whole blocks 23.6 us, unit after unit 24.4; 64 requests of 777 to 8,192 keys on 4: 56.5 and 47.5.)
 template <int W>
 __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int cost_range, int cost_join,
                                            int cost_merge) {
