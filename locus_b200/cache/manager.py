@@ -224,6 +224,13 @@ class CacheManager:
         el = torch.empty((), dtype=self.dtype).element_size()
         return sum(len(g.calls) * g.spec.elements_per_token() * el for g in self.groups)
 
+    def staging_bytes_per_token(self) -> int:
+        """What steps with portions of prompts take beside pools of 4 bits, per token of the pools: a layer's rows in the model's type."""
+        if self.kv_bits != 4:
+            return 0
+        el = torch.empty((), dtype=self.dtype).element_size()
+        return sum(g.spec.planes * g.spec.n_kv_heads * g.spec.head_dim * el for g in self.groups)
+
     def pages_for(self, n_tokens: int) -> int:
         return -(-n_tokens // self.page_tokens)
 

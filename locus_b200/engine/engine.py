@@ -11,6 +11,7 @@ from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
 
+from .. import kernels as K
 from ..cache.manager import CacheManager
 from ..sampling.sampler import GREEDY, Sampler, SamplingParams
 from .scheduler import Request, Scheduler, SchedulerConfig, Status
@@ -66,6 +67,8 @@ class Engine:
         plan = model.plan
         weigh = keep_tokens > 0
         if kv_bits:
+            if max_running > K.Q4_MAX_ITEMS:
+                raise ValueError(f"kv_bits: at most {K.Q4_MAX_ITEMS} requests at once (max_running {max_running})")
             mixers = [model.blocks[call.layer].mixer for call in plan.order]
             paged = [m for m in mixers if m.cache_needs()[0] is not None]
             if not all(m.reads_q4 for m in paged):
@@ -83,14 +86,13 @@ class Engine:
         if kv_fraction > 0:
             if not (kv_fraction <= 1.0) or model.device.type != "cuda":
                 raise ValueError("kv_fraction is a share (0, 1] of the free memory of a CUDA device")
-            per_token = CacheManager(model.cache_needs(), page_tokens=page_tokens, n_pages=0, n_state_slots=1,
-                                     max_seq_tokens=1, dtype=model.dtype, allocate_device=False, kv_bits=kv_bits, weigh=weigh).bytes_per_token()
+            empty = CacheManager(model.cache_needs(), page_tokens=page_tokens, n_pages=0, n_state_slots=1,
+                                 max_seq_tokens=1, dtype=model.dtype, allocate_device=False, kv_bits=kv_bits, weigh=weigh)
+            per_token = empty.bytes_per_token() + empty.staging_bytes_per_token()
             free, _ = torch.cuda.mem_get_info(model.device)
             ctx = int(free * kv_fraction) // max(1, per_token * page_tokens) * page_tokens
             if ctx < page_tokens:
                 raise ValueError(f"kv_fraction {kv_fraction} of {free} free bytes holds no page of {page_tokens} tokens")
-            if max_seq_tokens <= 0:
-                max_seq_tokens = min(plan.max_positions, ctx)
         if ctx <= 0:
             ctx = min(plan.max_positions, 4096)
         if max_seq_tokens <= 0:   # (an evicted request's positions may go beyond the pool)

@@ -1347,7 +1347,7 @@ def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     held as one of sixteen codes per element and two bfloat16: scale = (max - min) / 15 and mid = (min + max) / 2, and stands for
     mid + scale * (code - 7.5); a row with a value that is not finite reads as NaN.  The angles' product and reduction are 64 bits.
     ``weights`` float32 [n_pages, n_kv_heads, page_tokens]: set to 0 for the slots written (see :func:`attn_decode_q4`).  ``n_heads`` 0 with
-    ``q_out`` None: rows of k and v alone."""
+    ``q_out`` None: rows of k and v alone.  The slots of a call are different ones."""
     what = "rope_kv_write_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
     T, width = qkv.shape
@@ -1421,7 +1421,7 @@ def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Te
     needed any more may go back) or of ``dst_table``'s, which must be other pages than any that ``block_table`` lists.  ``kept`` int32 [layers,
     n_items, n_kv_heads, keep]: which keys stayed, -1 behind the keys of a request that has fewer than ``keep``, and stays whole.  Each head keeps keys
     of its own; every head of a request has the same number.  Keys keep the rotation of the position that they were written at.
-    ``max_tokens``: at least the tokens of the longest request."""
+    No page may be listed for two of the requests, and no request twice: rows move while others are read.  ``max_tokens``: at least the tokens of the longest request."""
     what = "evict_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens, 1)
     layers, pages = pool.shape[:2]
@@ -1488,7 +1488,8 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
     ``part_o``, ``part_ml``: scratch for :func:`decode_units_q4` partial results; ``counters`` (int32, n_items * n_heads) must be zero before
     the call and is zero after it.  ``weights`` float32 [n_pages, n_kv_heads, page_tokens] (without a window or chunks): the softmax weight that
     each key gets, summed over the query heads of its group, is added to the key's slot; ``scores`` is scratch for that, float32 with
-    n_items * n_heads * block_table.shape[1] * page_tokens elements."""
+    n_items * n_heads * block_table.shape[1] * page_tokens elements.  Calls that may run at the same time (on two streams, from two graphs) need
+    scratch and counters of their own."""
     what = "attn_decode_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
     if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:

@@ -35,6 +35,15 @@ def test_pages_and_bytes():
     assert mk(kv_bits=0, weigh=False).groups[0].pool.dtype == torch.float32
 
 
+def test_what_portions_take_beside_the_pools():
+    """A layer's rows in the model's type for every group: the staging buffer has the shape of a layer's pool."""
+    other = PagedKvSpec(1, 128)
+    needs = [(SPEC, None, None), (SPEC, None, None), (other, None, None)]
+    assert mk(needs).staging_bytes_per_token() == (2 * 2 * 64 + 2 * 128) * 4
+    assert mk(needs, dtype=torch.bfloat16).staging_bytes_per_token() == (2 * 2 * 64 + 2 * 128) * 2
+    assert mk(needs, kv_bits=0, weigh=False).staging_bytes_per_token() == 0
+
+
 @pytest.mark.parametrize("needs,over,says", [
     (None, dict(kv_bits=8), "kv_bits 8"),
     (None, dict(kv_bits=0), "beside a cache of 4 bits"),

@@ -203,9 +203,26 @@ def test_engines_that_are_refused(tmp_path):
     window = make_model_dir(tmp_path / "w", "C", raw=dict(CASES["window64"]))
     small = make_model_dir(tmp_path / "s", "A")
     for d, args, says in ((folder, dict(keep_tokens=10), "kv_bits"), (folder, dict(kv_bits=4, keep_tokens=10, keep_first=8, keep_recent=8), "keep_tokens 10"),
-                          (folder, dict(kv_bits=3), "kv_bits 3"), (window, dict(kv_bits=4, keep_tokens=64), "window"), (small, dict(kv_bits=4), "heads of 64")):
+                          (folder, dict(kv_bits=3), "kv_bits 3"), (folder, dict(kv_bits=4, max_running=1025), "at most 1024"), (window, dict(kv_bits=4, keep_tokens=64), "window"), (small, dict(kv_bits=4), "heads of 64")):
         with pytest.raises(ValueError, match=says):
             Engine.from_model_dir(d, page_tokens=16, ctx=256, **args)
+
+
+@pytest.mark.parametrize("keep", [0, 64])
+def test_a_share_of_the_memory_covers_the_staging_buffer(tmp_path, keep):
+    """kv_fraction bounds the pools and the buffer that a prompt's portion is laid out in, and leaves an evicted request's positions alone."""
+    from locus_b200.engine.engine import Engine
+
+    raw = CASES["heads64"]
+    folder = make_model_dir(tmp_path, "A", raw=dict(raw))
+    free, share = torch.cuda.mem_get_info(DEV)[0], 2e-4
+    eng = Engine.from_model_dir(folder, page_tokens=16, kv_bits=4, keep_tokens=keep, kv_fraction=share)
+    c = eng.cache
+    assert 0 < c.n_pages * 16 * (c.bytes_per_token() + c.staging_bytes_per_token()) <= free * share
+    assert c.max_seq_tokens == (raw["max_position_embeddings"] if keep else min(raw["max_position_embeddings"], c.n_pages * 16))
+    assert len(eng.generate([random_tokens(30, raw["vocab_size"], 3)], 4)[0]) == 4
+    staged = [t for k, t in eng.runner.rt._bufs.items() if k[0] == "attention.q4_wide"]
+    assert len(staged) == 1 and staged[0].numel() * staged[0].element_size() == c.n_pages * 16 * c.staging_bytes_per_token()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
