@@ -1291,6 +1291,7 @@ _Q4_EXPAND = struct.Struct("@6P8q")
 _Q4_EVICT = struct.Struct("@6P12q")
 _Q4_DECODE = struct.Struct("@15P15qd")
 _q4_entries = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (asked only behind a check that there are CUDA tensors)
 
 
 def _q4_entry(module: str, name: str):
@@ -1334,11 +1335,6 @@ def _q4_weights(what: str, weights: torch.Tensor, lead, n_kv_heads: int, page_to
         raise KernelError(f"{what}: weights must be float32 {list(lead) + [n_kv_heads, page_tokens]}")
 
 
-def _q4_aligned(what: str, addresses: int, step: int, names: str) -> None:
-    if addresses % step:
-        raise KernelError(f"{what}: {names} must start at multiples of {step} bytes")
-
-
 def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], q_out: Optional[torch.Tensor],
                      pool: torch.Tensor, slots: torch.Tensor, *, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int,
                      interleaved: bool, page_tokens: int, write_kv: bool = True, weights: Optional[torch.Tensor] = None) -> None:
@@ -1354,28 +1350,36 @@ def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     if width != (n_heads + 2 * n_kv_heads) * head_dim or n_heads < 0:
         raise KernelError(f"{what}: qkv width {width} for {n_heads} heads on {n_kv_heads} of {head_dim}")
     if q_out is None:
-        _need(n_heads == 0, "rope_kv_write_q4: q_out may only be left out without query heads")
+        if n_heads != 0:
+            raise KernelError("rope_kv_write_q4: q_out may only be left out without query heads")
         q_out = qkv
-    _need(qkv.dtype is q_out.dtype, "rope_kv_write_q4: qkv and q_out share one element type")
-    _need(q_out.numel() >= T * n_heads * head_dim, "rope_kv_write_q4: q_out is too small")
-    _need(positions.dtype is torch.int32 and positions.numel() >= T, "rope_kv_write_q4: positions must be int32, one per row")
-    _need(slots.dtype is torch.int32 and slots.numel() >= T, "rope_kv_write_q4: slots must be int32, one per row")
+    if not (qkv.dtype is q_out.dtype):
+        raise KernelError("rope_kv_write_q4: qkv and q_out share one element type")
+    if not (q_out.numel() >= T * n_heads * head_dim):
+        raise KernelError("rope_kv_write_q4: q_out is too small")
+    if not (positions.dtype is torch.int32 and positions.numel() >= T):
+        raise KernelError("rope_kv_write_q4: positions must be int32, one per row")
+    if not (slots.dtype is torch.int32 and slots.numel() >= T):
+        raise KernelError("rope_kv_write_q4: slots must be int32, one per row")
     if weights is not None:
         _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
     freq = 0
     if inv_freq is not None:
-        _need(0 <= rot_dim <= head_dim and rot_dim % 2 == 0, "rope_kv_write_q4: rot_dim must be even and at most the heads' size")
-        _need(inv_freq.dtype is torch.float32 and inv_freq.numel() == rot_dim // 2, "rope_kv_write_q4: inv_freq must be float32 [rot_dim / 2]")
+        if not (0 <= rot_dim <= head_dim and rot_dim % 2 == 0):
+            raise KernelError("rope_kv_write_q4: rot_dim must be even and at most the heads' size")
+        if not (inv_freq.dtype is torch.float32 and inv_freq.numel() == rot_dim // 2):
+            raise KernelError("rope_kv_write_q4: inv_freq must be float32 [rot_dim / 2]")
         freq = inv_freq.data_ptr()
     dev = qkv.get_device()
     if not (dev >= 0 and dev == q_out.get_device() == pool.get_device() == positions.get_device() == slots.get_device()
             and (inv_freq is None or (dev == inv_freq.get_device() and inv_freq.is_contiguous()))
             and (weights is None or (dev == weights.get_device() and weights.is_contiguous()))
             and qkv.is_contiguous() and q_out.is_contiguous() and pool.is_contiguous() and positions.is_contiguous() and slots.is_contiguous()
-            and dev == torch.cuda.current_device()):
+            and dev == _current_device()):
         _q4_here(what, qkv=qkv, positions=positions, inv_freq=inv_freq, q_out=q_out, pool=pool, slots=slots, weights=weights)
     x, q, base = qkv.data_ptr(), q_out.data_ptr(), pool.data_ptr()
-    _q4_aligned(what, x | q | base, 16, "qkv, q_out and the pool")
+    if (x | q | base) & 15:
+        raise KernelError("rope_kv_write_q4: qkv, q_out and the pool must start at multiples of 16 bytes")
     code = _q4_entry("cache_q4", "locus_rope_kv_write_q4")(
         _Q4_WRITE.pack(x, positions.data_ptr(), freq, q, base, slots.data_ptr(), 0 if weights is None else weights.data_ptr(), dtype_code(qkv.dtype), T,
                        n_heads, n_kv_heads, head_dim, rot_dim, 1 if interleaved else 0, page_tokens, 1 if write_kv else 0), _q4_stream(dev))
@@ -1391,19 +1395,25 @@ def expand_q4(pool: torch.Tensor, out: torch.Tensor, *, segs: Optional[torch.Ten
     ``max_keys``: at least the rows of the longest of these segments."""
     what = "expand_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)
-    _need(out.shape == (pool.shape[0], 2, n_kv_heads, page_tokens, head_dim), "expand_q4: out must have the pool's pages in the model's type")
-    _need(block_table.dtype is torch.int32 and block_table.dim() == 2, "expand_q4: block_table must be int32 [segments, width]")
-    _need(segs is None or (segs.dtype is torch.int32 and segs.numel() >= n_segs), "expand_q4: segs must be int32, one per segment to expand")
-    _need(segs is not None or min(seg_ctx.numel(), seg_qn.numel(), block_table.shape[0]) >= n_segs, "expand_q4: fewer segments than n_segs")
-    _need(seg_ctx.dtype is torch.int32 and seg_qn.dtype is torch.int32, "expand_q4: seg_ctx and seg_qn must be int32")
+    if not (out.shape == (pool.shape[0], 2, n_kv_heads, page_tokens, head_dim)):
+        raise KernelError("expand_q4: out must have the pool's pages in the model's type")
+    if not (block_table.dtype is torch.int32 and block_table.dim() == 2):
+        raise KernelError("expand_q4: block_table must be int32 [segments, width]")
+    if not (segs is None or (segs.dtype is torch.int32 and segs.numel() >= n_segs)):
+        raise KernelError("expand_q4: segs must be int32, one per segment to expand")
+    if not (segs is not None or min(seg_ctx.numel(), seg_qn.numel(), block_table.shape[0]) >= n_segs):
+        raise KernelError("expand_q4: fewer segments than n_segs")
+    if not (seg_ctx.dtype is torch.int32 and seg_qn.dtype is torch.int32):
+        raise KernelError("expand_q4: seg_ctx and seg_qn must be int32")
     dev = pool.get_device()
     if not (dev >= 0 and dev == out.get_device() == seg_ctx.get_device() == seg_qn.get_device() == block_table.get_device()
             and (segs is None or (dev == segs.get_device() and segs.is_contiguous()))
             and pool.is_contiguous() and out.is_contiguous() and seg_ctx.is_contiguous() and seg_qn.is_contiguous()
-            and block_table.is_contiguous() and dev == torch.cuda.current_device()):
+            and block_table.is_contiguous() and dev == _current_device()):
         _q4_here(what, pool=pool, out=out, segs=segs, seg_ctx=seg_ctx, seg_qn=seg_qn, block_table=block_table)
     base, to = pool.data_ptr(), out.data_ptr()
-    _q4_aligned(what, base | to, 16, "the pool and out")
+    if (base | to) & 15:
+        raise KernelError("expand_q4: the pool and out must start at multiples of 16 bytes")
     code = _q4_entry("cache_q4", "locus_expand_q4")(
         _Q4_EXPAND.pack(base, to, 0 if segs is None else segs.data_ptr(), seg_ctx.data_ptr(), seg_qn.data_ptr(), block_table.data_ptr(), dtype_code(out.dtype), n_segs,
                         block_table.shape[1], n_kv_heads, head_dim, page_tokens, max_keys, min_new), _q4_stream(dev))
@@ -1428,8 +1438,10 @@ def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Te
     _q4_weights(what, weights, (layers, pages), n_kv_heads, page_tokens)
     if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
         raise KernelError(f"{what}: keep {keep} with the first {first} and the last {recent}")
-    _need(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= n_items, "evict_q4: block_table must be int32 [requests, width]")
-    _need(n_tokens.dtype is torch.int32 and n_tokens.numel() >= n_items, "evict_q4: n_tokens must be int32, one per request")
+    if not (block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= n_items):
+        raise KernelError("evict_q4: block_table must be int32 [requests, width]")
+    if not (n_tokens.dtype is torch.int32 and n_tokens.numel() >= n_items):
+        raise KernelError("evict_q4: n_tokens must be int32, one per request")
     if kept.dtype is not torch.int32 or kept.shape != (layers, n_items, n_kv_heads, keep):
         raise KernelError(f"{what}: kept must be int32 {[layers, n_items, n_kv_heads, keep]}")
     width = block_table.shape[1]
@@ -1437,15 +1449,16 @@ def evict_q4(pool: torch.Tensor, weights: torch.Tensor, *, block_table: torch.Te
         raise KernelError(f"{what}: max_tokens {max_tokens} beyond what block_table describes")
     to = block_table if dst_table is None else dst_table
     if dst_table is not None:
-        _need(to.dtype is torch.int32 and to.dim() == 2 and to.shape[0] >= n_items and to.shape[1] * page_tokens >= min(keep, max_tokens),
-              "evict_q4: dst_table must be int32 [requests, pages for the keys that stay]")
+        if not (to.dtype is torch.int32 and to.dim() == 2 and to.shape[0] >= n_items and to.shape[1] * page_tokens >= min(keep, max_tokens)):
+            raise KernelError("evict_q4: dst_table must be int32 [requests, pages for the keys that stay]")
     dev = pool.get_device()
     if not (dev >= 0 and dev == weights.get_device() == block_table.get_device() == to.get_device() == n_tokens.get_device() == kept.get_device()
             and pool.is_contiguous() and weights.is_contiguous() and block_table.is_contiguous() and to.is_contiguous() and n_tokens.is_contiguous()
-            and kept.is_contiguous() and dev == torch.cuda.current_device()):
+            and kept.is_contiguous() and dev == _current_device()):
         _q4_here(what, pool=pool, weights=weights, block_table=block_table, n_tokens=n_tokens, kept=kept, dst_table=dst_table)
     base = pool.data_ptr()
-    _q4_aligned(what, base, 16, "the pool")
+    if base & 15:
+        raise KernelError("evict_q4: the pool must start at multiples of 16 bytes")
     code = _q4_entry("cache_q4", "locus_evict_q4")(
         _Q4_EVICT.pack(base, weights.data_ptr(), block_table.data_ptr(), to.data_ptr(), n_tokens.data_ptr(), kept.data_ptr(), width, to.shape[1],
                        n_items, layers, pages, n_kv_heads, head_dim, page_tokens, keep, first, recent, max_tokens), _q4_stream(dev))
@@ -1495,24 +1508,33 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
     if n_heads <= 0 or n_kv_heads <= 0 or n_heads % n_kv_heads:
         raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv_heads} kv heads")
     width = n_heads * head_dim
-    _need(q.dtype is out.dtype and q.numel() % width == 0 and out.numel() % width == 0, "attn_decode_q4: q and out must be rows of whole heads, of one element type")
-    _need(block_table.dtype is torch.int32 and block_table.dim() == 2, "attn_decode_q4: block_table must be int32 [segments, width]")
+    if not (q.dtype is out.dtype and q.numel() % width == 0 and out.numel() >= q.numel()):
+        raise KernelError("attn_decode_q4: q and out must be rows of whole heads, of one element type")
+    if not (block_table.dtype is torch.int32 and block_table.dim() == 2):
+        raise KernelError("attn_decode_q4: block_table must be int32 [segments, width]")
     pages = block_table.shape[1]
-    _need(n_items <= Q4_MAX_ITEMS, "attn_decode_q4: at most 1024 requests")
-    _need(items.dtype is torch.int32 and items.numel() >= n_items, "attn_decode_q4: items must be int32, one per request")
-    _need(counters.dtype is torch.int32 and counters.numel() >= n_items * n_heads, "attn_decode_q4: counters must be int32 [n_items * n_heads]")
-    _need(seg_q0.dtype is torch.int32 and seg_ctx.dtype is torch.int32, "attn_decode_q4: seg_q0 and seg_ctx must be int32")
-    _need(part_o.dtype is torch.float32 and part_ml.dtype is torch.float32, "attn_decode_q4: float32 scratch")
+    if n_items > Q4_MAX_ITEMS:
+        raise KernelError("attn_decode_q4: at most 1024 requests")
+    if not (items.dtype is torch.int32 and items.numel() >= n_items):
+        raise KernelError("attn_decode_q4: items must be int32, one per request")
+    if not (counters.dtype is torch.int32 and counters.numel() >= n_items * n_heads):
+        raise KernelError("attn_decode_q4: counters must be int32 [n_items * n_heads]")
+    if not (seg_q0.dtype is torch.int32 and seg_ctx.dtype is torch.int32):
+        raise KernelError("attn_decode_q4: seg_q0 and seg_ctx must be int32")
+    if not (part_o.dtype is torch.float32 and part_ml.dtype is torch.float32):
+        raise KernelError("attn_decode_q4: float32 scratch")
     floats, part, to, at, lse = part_o.numel(), part_o.data_ptr(), 0, 0, 0
     if weights is not None:
         _q4_weights(what, weights, pool.shape[:1], n_kv_heads, page_tokens)
-        _need(window == 0 and chunk == 0, "attn_decode_q4: weights go with neither a window nor chunks")
-        _need(scores is not None and scores.dtype is torch.float32 and scores.numel() >= n_items * n_heads * pages * page_tokens,
-              "attn_decode_q4: scores too small for weights")
+        if not (window == 0 and chunk == 0):
+            raise KernelError("attn_decode_q4: weights go with neither a window nor chunks")
+        if not (scores is not None and scores.dtype is torch.float32 and scores.numel() >= n_items * n_heads * pages * page_tokens):
+            raise KernelError("attn_decode_q4: scores too small for weights")
         floats = max(0, (floats - 2 * n_items * n_heads) // 4 * 4)   # a head's maximum and denominator lie behind the partial results
         to, at, lse = weights.data_ptr(), scores.data_ptr(), part + 4 * floats
     max_units = min(floats // head_dim, part_ml.numel() // 2)
-    _need(max_units >= n_items * n_heads * (2 if keep_first > 0 and window > 0 else 1), "attn_decode_q4: scratch too small")
+    if not (max_units >= n_items * n_heads * (2 if keep_first > 0 and window > 0 else 1)):
+        raise KernelError("attn_decode_q4: scratch too small")
     sink_flag, sink_at, slopes_at = 0, 0, 0
     if sink is not False:
         if isinstance(sink, torch.Tensor):
@@ -1532,12 +1554,14 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
             and counters.is_contiguous() and (weights is None or (dev == weights.get_device() == scores.get_device()
                                                                   and weights.is_contiguous() and scores.is_contiguous()))
             and (sink_at == 0 or dev == sink.get_device()) and (slopes is None or dev == slopes.get_device())
-            and dev == torch.cuda.current_device()):
+            and dev == _current_device()):
         _q4_here(what, q=q, pool=pool, out=out, seg_q0=seg_q0, seg_ctx=seg_ctx, block_table=block_table, items=items, part_o=part_o, part_ml=part_ml,
                  counters=counters, slopes=slopes, weights=weights, scores=scores, sink=sink if sink_at else None)
     qp, base, ml = q.data_ptr(), pool.data_ptr(), part_ml.data_ptr()
-    _q4_aligned(what, qp | base | part, 16, "q, the pool and part_o")
-    _q4_aligned(what, ml, 8, "part_ml")
+    if (qp | base | part) & 15:
+        raise KernelError("attn_decode_q4: q, the pool and part_o must start at multiples of 16 bytes")
+    if ml & 7:
+        raise KernelError("attn_decode_q4: part_ml must start at multiples of 8 bytes")
     code = _q4_entry("attention_q4", "locus_attn_decode_q4")(
         _Q4_DECODE.pack(qp, base, out.data_ptr(), seg_q0.data_ptr(), seg_ctx.data_ptr(), block_table.data_ptr(), items.data_ptr(), part, ml,
                         counters.data_ptr(), sink_at, slopes_at, to, at, lse, dtype_code(q.dtype), pages, n_items, n_heads, n_kv_heads, head_dim,

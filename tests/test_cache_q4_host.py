@@ -108,6 +108,8 @@ REFUSED = [
     (K.attn_decode_q4, decode_args, dict(W, scores=torch.zeros(2 * NH * 2 * P - 1)), "scores"),
     (K.attn_decode_q4, decode_args, dict(W, weights=torch.zeros(3, KV, P, dtype=torch.bfloat16)), "weights"),
     (K.attn_decode_q4, decode_args, {}, "CUDA tensor"),
+    (K.attn_decode_q4, decode_args, dict(out=torch.zeros(1, NH * D)), "rows of whole heads"),
+    (K.attn_decode_q4, decode_args, dict(n_kv_heads=0, pool=torch.zeros(3, 2, 0, P * (D // 2 + 4), dtype=torch.uint8)), "multiple"),
 ]
 
 
