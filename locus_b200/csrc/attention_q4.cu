@@ -225,6 +225,7 @@ struct Bool {
 // The cut of a step's keys into ranges.
 #define Q4_MAX_ITEMS 1024
 #define Q4_CAND 64        // candidate range lengths looked at
+#define Q4_ODD 16         // what ranges that do not end where stages of 64 keys do cost more, in keys: a further stage, asked for in pieces
 
 // What a warp of a block does in a round.
 struct Q4Unit {
@@ -268,9 +269,10 @@ __device__ __forceinline__ int q4_blocks(const int* table, int ranges, int n_vh)
 // Fills the plan (all threads of the block; ends with a barrier) and returns the length, 0 when not even one range per item fits max_ranges.
 // Two ways to deal the units to blocks, for each of Q4_CAND lengths: `packed`, unit after unit, W to a block, and by whole blocks (q4_blocks), where
 // some warps may have nothing to do but fewer (request, head)s are joined across blocks.  The cost of a cut, in keys: rounds over the grid x
-// (length + cost_range), and cost_join once where blocks join, and cost_merge per partial result of the longest item.  Lengths
+// (length + cost_range, and Q4_ODD), and cost_join once where blocks join, and cost_merge per partial result of the longest item.  Lengths
 // from what fills every warp once, 2 % apart, some shorter and longer ones, and the longest item's.
-// (8 requests of 4,096 keys on 16 heads: by whole blocks 23.6 us, unit after unit 24.4; 64 requests of 777 to 8,192 keys on 4: 56.5 and 47.5.)
+// (8 requests of 4,096 keys on 16 heads: by whole blocks 23.6 us, unit after unit 24.4; 64 requests of 777 to 8,192 keys on 4: 56.5 and 47.5.
+// One request of 4,096 keys on 16: ranges of 48 keys 14.5, of 64 13.2.)
 template <int W>
 __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int cost_range, int cost_join,
                                            int cost_merge) {
@@ -336,7 +338,7 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int c = lane + 32 * k, ranges = pl.ranges[c];
-            const int most = min(my_len[k], longest) + cost_range, merge = cost_merge * (static_cast<int>(static_cast<float>(longest) * my_inv[k]) / W);
+            const int most = min(my_len[k], longest) + (my_len[k] & 63 ? Q4_ODD : 0) + cost_range, merge = cost_merge * (static_cast<int>(static_cast<float>(longest) * my_inv[k]) / W);
             auto consider = [&](int loads, bool joins, int packed) {
                 const float rounds = floorf((static_cast<float>(loads) + static_cast<float>(gridDim.x - 1)) * grid_inv);
                 const float cost = fminf(rounds * static_cast<float>(most) + static_cast<float>(merge + (joins ? cost_join : 0)), 16777215.f);
