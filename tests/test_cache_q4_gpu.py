@@ -421,6 +421,49 @@ def test_decode_adds_the_weights_up(dtype, H, kv, D, P, lens):
     assert torch.equal(weights.cpu().permute(0, 2, 1)[~held], start.permute(0, 2, 1)[~held])
 
 
+def test_weights_of_long_requests():
+    """Lengths around what a block of the adding kernel takes."""
+    H, kv, D, P = 4, 2, 64, 64
+    lens = [256, 257, 1023, 1024, 1025, 2100]
+    table, n_pages = tables(lens, P, 65)
+    pool = filled(table, lens, kv, D, P, 66, n_pages).to(DEV)
+    q = rnd(len(lens), H * D, dtype=F32, seed=67)
+    weights = torch.zeros(n_pages, kv, P, device=DEV)
+    out, ctx = run_decode(q, pool, table, lens, H, kv, D, P, weights=weights)
+    ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
+    check(out, ref, F32, H, D)
+    want = torch.zeros(n_pages, kv, P, dtype=torch.float64)
+    for (page, h, off), w in ref[3].items():
+        want[page, h, off] += w
+    # (scores of up to some ten, off by some units of 2^-24 each: a weight by as much of itself)
+    assert ((weights.cpu().double() - want).abs() <= 2.0 ** -17 * want).all()
+
+
+def test_calls_at_the_same_time_with_scratch_of_their_own():
+    H, kv, D, P = 8, 2, 128, 64
+    cases = []
+    for i, lens in enumerate(([700, 30, 1500], [64] * 20)):
+        table, n_pages = tables(lens, P, 101 + i)
+        pool = filled(table, lens, kv, D, P, 103 + i, n_pages).to(DEV)
+        q = rnd(len(lens), H * D, dtype=BF16, seed=105 + i).to(DEV)
+        n, units = len(lens), K.decode_units_q4(len(lens), H, DEV)
+        i32 = lambda x: torch.tensor(x, dtype=I32, device=DEV)  # noqa: E731
+        kw = dict(seg_q0=i32(list(range(n))), seg_ctx=i32([x - 1 for x in lens]), block_table=table.to(DEV), items=i32(list(range(n))), n_items=n, n_heads=H,
+                  scale=D ** -0.5, window=0, part_o=torch.empty(units * D, device=DEV), part_ml=torch.empty(2 * units, device=DEV),
+                  counters=torch.zeros(n * H, dtype=I32, device=DEV), **sizes(kv, D, P))
+        want, _ = run_decode(q, pool, table, lens, H, kv, D, P)
+        cases.append((torch.cuda.Stream(), q, pool, torch.empty_like(q), kw, want))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for stream, q, pool, out, kw, _ in cases:
+            with torch.cuda.stream(stream):
+                out.fill_(9.0)
+                K.attn_decode_q4(q, pool, out, **kw)
+        torch.cuda.synchronize()
+        for _, _, _, out, kw, want in cases:
+            assert torch.equal(out, want) and not kw["counters"].any()
+
+
 def test_weights_of_a_request_that_is_listed_twice():
     H, kv, D, P, lens = 4, 2, 64, 16, [40, 40]
     table, n_pages = tables([40], P, 71)
