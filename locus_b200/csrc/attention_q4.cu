@@ -1011,10 +1011,32 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 // weights[page][kvh][offset] += sum over the heads of the group of 2^(score - M) / denominator, for every key of the listed requests: scores,
 // maxima and denominators as the kernel above left them.  WG_KEYS keys per thread, whose pages are looked up in front of the wait for that kernel and
 // whose scores are on their way together (bound by such latencies: with one key per thread a call for 8 requests of 4,096 keys on 16 heads took 29.9 us,
-// with four 29.0, with eight 29.6).
+// with four 29.0, with eight 29.6; of 64 requests 157).
 // A slot is added to once per request that lists it, so the sum does not depend on the order (an atomic: a request may be listed twice).
 #define WG_THREADS 256
 #define WG_KEYS 4
+// Groups of one head: four keys in a row, whose scores are one load and whose weights one atomic of 16 bytes.  (8 requests of 4,096 keys 27.4 us, 64 149, of which 129 without
+// weights.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
+__global__ void __launch_bounds__(WG_THREADS) q4_weigh_one_kernel(Q4Args a, float* __restrict__ weights) {
+    const int item = blockIdx.z, h = blockIdx.y, P = a.page_tokens;
+    const int seg = a.items[item];
+    const int n = min(a.seg_ctx[seg] + 1, a.table_stride * P);
+    const int t = 4 * (blockIdx.x * WG_THREADS + threadIdx.x), i = t / P;
+    float* at = t < n ? weights + (static_cast<size_t>(a.block_table[static_cast<size_t>(seg) * a.table_stride + i]) * a.nkv + h) * P + (t - i * P) : nullptr;
+    pdl_entry();
+    pdl_trigger();
+    if (t >= n) return;
+    const float4 s = *reinterpret_cast<const float4*>(a.scores + (static_cast<size_t>(item) * a.nkv + h) * a.table_stride * P + t);
+    const float2 ml = reinterpret_cast<const float2*>(a.lse)[static_cast<size_t>(item) * a.nh + h];
+    const float w[4] = {ex2(s.x - ml.x) * ml.y, ex2(s.y - ml.x) * ml.y, ex2(s.z - ml.x) * ml.y, ex2(s.w - ml.x) * ml.y};
+    if (t + 4 <= n) {
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3]) : "memory");
+    } else {
+#pragma unroll
+        for (int u = 0; u < 3; ++u)
+            if (t + u < n) atomicAdd(at + u, w[u]);
+    }
+}
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_kernel(Q4Args a, float* __restrict__ weights) {
     const int item = blockIdx.z, kvh = blockIdx.y, G = a.nh / a.nkv, P = a.page_tokens;
     const int seg = a.items[item];
@@ -1087,7 +1109,7 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
         return LOCUS_ERR_UNSUPPORTED;
     const int keep_first = v.window == 0 ? 0 : static_cast<int>(v.keep_first);
     if (v.max_units < v.n_items * v.nh * (keep_first > 0 ? 2 : 1)) return LOCUS_ERR_UNSUPPORTED;
-    if (v.weights && (v.scores == nullptr || v.lse == nullptr || v.window > 0 || v.chunk > 0)) return LOCUS_ERR_UNSUPPORTED;
+    if (v.weights && (((reinterpret_cast<uintptr_t>(v.weights) | reinterpret_cast<uintptr_t>(v.scores)) & 15) != 0 || v.scores == nullptr || v.lse == nullptr || v.window > 0 || v.chunk > 0)) return LOCUS_ERR_UNSUPPORTED;
     int dev = 0, n_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n_sm <= 0)
         return static_cast<int>(cudaGetLastError());
@@ -1116,6 +1138,7 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
 #undef Q4_GO
     if (code || !v.weights) return code;
     const dim3 grid(ceil_div(a.table_stride * a.page_tokens, WG_THREADS * WG_KEYS), a.nkv, n);
-    locus_launch(q4_weigh_kernel, grid, WG_THREADS, 0, stream, a, v.weights);
+    if (a.nh == a.nkv) locus_launch(q4_weigh_one_kernel, grid, WG_THREADS, 0, stream, a, v.weights);
+    else locus_launch(q4_weigh_kernel, grid, WG_THREADS, 0, stream, a, v.weights);
     return locus_launch_status();
 }

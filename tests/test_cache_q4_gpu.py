@@ -421,6 +421,24 @@ def test_decode_adds_the_weights_up(dtype, H, kv, D, P, lens):
     assert torch.equal(weights.cpu().permute(0, 2, 1)[~held], start.permute(0, 2, 1)[~held])
 
 
+def test_addresses_that_break_the_alignment_are_refused():
+    H, kv, D, P, lens = 2, 2, 64, 16, [20]
+    table, n_pages = tables(lens, P, 68)
+    pool = filled(table, lens, kv, D, P, 69, n_pages).to(DEV)
+    off = lambda n: torch.zeros(n + 1, device=DEV)[1:]  # noqa: E731
+    with pytest.raises(K.KernelError, match="weights and scores"):
+        run_decode(rnd(1, H * D), pool, table, lens, H, kv, D, P, weights=off(n_pages * kv * P).view(n_pages, kv, P))
+    i32 = lambda x: torch.tensor(x, dtype=I32, device=DEV)  # noqa: E731
+    kw = dict(seg_q0=i32([0]), seg_ctx=i32([19]), block_table=table.to(DEV), items=i32([0]), n_items=1, n_heads=H, scale=1.0, window=0,
+              counters=torch.zeros(H, dtype=I32, device=DEV), **sizes(kv, D, P))
+    q, out = torch.zeros(1, H * D, device=DEV), torch.zeros(1, H * D, device=DEV)
+    for over, says in ((dict(part_o=off(64 * D)), "part_o"), (dict(part_ml=off(64)), "part_ml")):
+        with pytest.raises(K.KernelError, match=says):
+            K.attn_decode_q4(q, pool, out, **{**kw, "part_o": torch.zeros(64 * D, device=DEV), "part_ml": torch.zeros(64, device=DEV), **over})
+    with pytest.raises(K.KernelError, match="q, the pool"):
+        K.attn_decode_q4(off(H * D).view(1, -1), pool, out, part_o=torch.zeros(64 * D, device=DEV), part_ml=torch.zeros(64, device=DEV), **kw)
+
+
 def test_weights_of_long_requests():
     """Lengths around what a block of the adding kernel takes."""
     H, kv, D, P = 4, 2, 64, 64
