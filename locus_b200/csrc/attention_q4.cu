@@ -45,11 +45,11 @@
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
 //
-// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 162 registers, 104 KB of copies on their way per SM): the instructions that take codes
+// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 164 registers, 104 KB of copies on their way per SM): the instructions that take codes
 // apart and the latencies between them, at three warps a scheduler; the copies alone (no arithmetic) take 12.7 us of the 23.6 of 8 requests of
 // 4,096 keys (71 MB, 3.0 TB/s), 41 of the 47.5 of 64 requests of 777 to 8,192 keys (28 heads on 4; 171 MB, 3.6 TB/s).  For few keys it is latency:
 // descriptors and cut 2.6 to 4 us, first page ids and rows 2.5, joins 1 to 4.  Sixteen warps of 128 registers, eight of 255, one or four chunks at a
-// time, smaller stages: all slower (25 to 28 us for 8 requests of 4,096 keys).
+// time, smaller stages: all slower (24.3 to 28 us for 8 requests of 4,096 keys).
 //
 // With weights: the scores are written out as they are formed, and a second kernel (q4_weigh_kernel) adds every key's p_t, summed over the heads
 // of its group, to a number per (slot, key/value head).  The softmax's denominator is known only behind the last range.
