@@ -2,20 +2,21 @@
 //
 //   o_h = sum_t p_t v_t   p = softmax over the keys in sight of scale * q_h . k_t (a sink, a distance bias: as in attention.cu)
 //
-// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5), so
+// with k_t and v_t read straight from their codes.  A row is mid + scale (code - 7.5) = z + scale (code - 7), z = mid - scale / 2, and codes less 7 are
+// small whole numbers that float16 holds exactly, so
 //
-//   q . k_t = scale_t (q . code_t) + (mid_t - 7.5 scale_t) sum(q)              the product on the tensor cores, the rest per score in float32
-//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t (mid_t - scale_t / 2)   the same for the values
+//   q . k_t = scale_t (q . (code_t - 7)) + z_t sum(q)                      the product on the tensor cores, the rest per score in float32
+//   o       = sum_t (p_t scale_t) (code_t - 7) + sum_t p_t z_t             the same for the values
 //
-// The tensor cores' operands:
-//   * scores of a bfloat16 model: codes as unsigned bytes (a mask, and a shift for every other one) times q as whole numbers of 16 bits, in a signed
-//     and an unsigned byte: a power of two per head brings its largest element to 2^14 .. 2^15 (taken out of the scores again).  Elements down to 2^-7 of
-//     the largest are exact, smaller ones off by at most 2^-15 of the largest, which itself stands for anything within 2^-9; sums are exact.
-//   * scores of a float32 model: codes less 7 and q in float16, q scaled likewise and in two parts, 22 bits and more;
-//   * values: codes less 7 in float16 (exact): a nibble n under the exponent of 1024 is 1024 + n, in the next four bits 1024 + 16 n, and one addition
-//     or multiply-add (two codes an instruction) leaves n - 7.  (A nibble alone is the subnormal number n 2^-24 and would need neither, but the tensor
-//     cores align what they add by the operands' exponent fields: sums of such products were off by 1e-4.  The 7 is taken off the codes rather than
-//     out of the sums, where it would grow over the keys and lose what cancels.)
+// The tensor cores' operands are float16:
+//   * codes less 7: a nibble n under the exponent of 1024 is 1024 + n, in the next four bits 1024 + 16 n, and one addition or multiply-add (two
+//     codes an instruction) leaves n - 7.  (A nibble alone is the subnormal number n 2^-24 and would need neither, but the tensor cores align what
+//     they add by the operands' exponent fields: sums of such products were off by 1e-4.  The 7 is taken off the codes rather than out of the
+//     sums, where it would grow over the keys and lose what cancels.)
+//   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
+//     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more.  (Codes of K as
+//     unsigned bytes against q as whole numbers in two bytes take three instructions a word instead of nine, 64 requests of up to 8,192 keys 47.3 us
+//     instead of 51.1, but the keys' weights were then off by 4e-6 instead of 2e-7; with three bytes it is 51.5.)
 //   * the weights p_t scale_t in float16, formed relative to the running maximum M of score_t + e_t, e_t the exponent of the key's own scale (of its mid
 //     less 20 where that is more), so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the
 //     largest where that is more; two parts for a float32 model).  The unrounded p_t enter the denominator and the sum of the middles.
@@ -24,8 +25,8 @@
 //
 // A warp takes a range of keys of one (request, key/value head) for up to 16 query heads that share it, in the transposed form (16 keys in the M
 // dimension of mma.sync m16n8k16, eight heads in N):
-//   S^T [16 keys x 8 heads] = C_k [16 x hd] . Q^T           (m16n8k32 with bytes) a lane's words of a key row hold eight codes each, in a word's low and
-//                             high nibbles four dimensions as the A fragment wants them;
+//   S^T [16 keys x 8 heads] = (C_k - 7) [16 x hd] . Q^T     a lane's words of a key row hold eight codes each, two neighbouring dimensions in a
+//                             register's halves as the A fragment wants them;
 //   O^T [hd x 8 heads] += (C_v - 7)^T [hd x 16 keys] . P^T  the A fragment wants one dimension of two keys in a register: a byte permute joins
 //                             the same byte of two keys' words, and its two nibbles are two dimensions (two row tiles' halves).
 // A group of more heads is served by several warps (that each read its rows, from the L2 after the first).
@@ -41,15 +42,15 @@
 // 64 tokens is one run of bytes per plane; of other pages a lane each asks for the codes and the factors.)  Every wait is bounded: when the limit
 // runs out the warp records it in the module's error word, waits for its other copies with the same limit and goes on to the end without a further copy.
 // What a key's four factors come to is worked out by one lane and left in the place of its chunks' codes of K, which are in registers by then: all
-// four lanes of a row of fragments need it (64 requests of up to 8,192 keys: 50.1 -> 47.7 us; scores by bytes before that: 52.6 -> 50.1).
+// four lanes of a row of fragments need it (64 requests of up to 8,192 keys: 52.6 -> 51.1 us).
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
 //
-// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 164 registers, 104 KB of copies on their way per SM): the instructions that take codes
-// apart and the latencies between them, at three warps a scheduler; the copies alone (no arithmetic) take 12.7 us of the 23.6 of 8 requests of
-// 4,096 keys (71 MB, 3.0 TB/s), 41 of the 47.5 of 64 requests of 777 to 8,192 keys (28 heads on 4; 171 MB, 3.6 TB/s).  For few keys it is latency:
+// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 162 registers, 104 KB of copies on their way per SM): the instructions that take codes
+// apart and the latencies between them, at three warps a scheduler; the copies alone (no arithmetic) take 12.7 us of the 25.5 of 8 requests of
+// 4,096 keys (71 MB, 2.8 TB/s), 41 of the 51.1 of 64 requests of 777 to 8,192 keys (28 heads on 4; 171 MB, 3.3 TB/s).  For few keys it is latency:
 // descriptors and cut 2.6 to 4 us, first page ids and rows 2.5, joins 1 to 4.  Sixteen warps of 128 registers, eight of 255, one or four chunks at a
-// time, smaller stages: all slower (24.3 to 28 us for 8 requests of 4,096 keys).
+// time, smaller stages: slower by 3 to 18 % (for 8 requests of 4,096 keys).
 //
 // With weights: the scores are written out as they are formed, and a second kernel (q4_weigh_kernel) adds every key's p_t, summed over the heads
 // of its group, to a number per (slot, key/value head).  The softmax's denominator is known only behind the last range.
@@ -155,19 +156,6 @@ __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// codes as unsigned bytes times signed (unsigned) bytes, summed in 32-bit whole numbers
-__device__ __forceinline__ void mma_u8s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_u8u8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // transpose of an 8 x 8 matrix of 16-bit elements held as mma fragments (two elements of a row per lane)
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
     uint32_t r;
@@ -271,7 +259,7 @@ __device__ __forceinline__ int q4_blocks(const int* table, int ranges, int n_vh)
 // some warps may have nothing to do but fewer (request, head)s are joined across blocks.  The cost of a cut, in keys: rounds over the grid x
 // (length + cost_range, and Q4_ODD), and cost_join once where blocks join, and cost_merge per partial result of the longest item.  Lengths
 // from what fills every warp once, 2 % apart, some shorter and longer ones, and the longest item's.
-// (8 requests of 4,096 keys on 16 heads: by whole blocks 23.6 us, unit after unit 24.4; 64 requests of 777 to 8,192 keys on 4: 56.5 and 47.5.
+// (8 requests of 4,096 keys on 16 heads: by whole blocks 25.5 us, unit after unit 3 % more; 64 requests of 777 to 8,192 keys on 4: unit after unit 51.1, 19 % more.
 // One request of 4,096 keys on 16: ranges of 48 keys 14.5, of 64 13.2.)
 template <int W>
 __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int cost_range, int cost_join,
@@ -596,23 +584,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * KW; ++i) {
-                    if constexpr (PARTS == 2) {
-                        split2<PARTS>(x[ht][4 * i] * up, x[ht][4 * i + 1] * up, qb[ht][i][0]);
-                        split2<PARTS>(x[ht][4 * i + 2] * up, x[ht][4 * i + 3] * up, qb[ht][i][1]);
-                    }
+                    split2<PARTS>(x[ht][4 * i] * up, x[ht][4 * i + 1] * up, qb[ht][i][0]);
+                    split2<PARTS>(x[ht][4 * i + 2] * up, x[ht][4 * i + 3] * up, qb[ht][i][1]);
                     sum += (x[ht][4 * i] + x[ht][4 * i + 1]) + (x[ht][4 * i + 2] + x[ht][4 * i + 3]);
-                }
-                if constexpr (PARTS == 1) {
-#pragma unroll
-                    for (int w = 0; w < KW; ++w)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {   // the low nibbles of a word's bytes are its values 0, 4, 1 and 5, the high ones 2, 6, 3 and 7
-                            int v[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) v[j] = __float2int_rn(x[ht][8 * w + 2 * y + (j & 1) * 4 + (j >> 1)] * up);
-                            qb[ht][2 * w + y][0][0] = __byte_perm(__byte_perm(v[0], v[1], 0x0051), __byte_perm(v[2], v[3], 0x0051), 0x5410);
-                            qb[ht][2 * w + y][1][0] = __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
-                        }
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -664,7 +638,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     lds_words<1>(&kf, fac + 4 * at_key);
                     lds_words<1>(&vf, fac + PLANE + 4 * at_key);
                     if (dead(c0 + at_key)) kf = vf = 0u;
-                    const float kz = fmaf(PARTS == 1 ? -7.5f : -0.5f, q4_scale(kf), q4_mid(kf));
+                    const float kz = fmaf(-0.5f, q4_scale(kf), q4_mid(kf));
                     const int of_scale = static_cast<int>(vf << 16 & 0x7f800000u), of_mid = static_cast<int>(vf & 0x7f800000u);
                     const int top = min(__vimax3_s32(of_scale, of_mid - (MID << 23), (LEAST + 127) << 23), 253 << 23);   // (NaN: any)
                     const float ve = __int_as_float(0x4b000000 | top >> 23) - 8388735.f;   // (2^23 + 127)
@@ -676,38 +650,17 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 for (int n = 0; n < N; ++n) {
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) s[n][ht][0] = s[n][ht][1] = s[n][ht][2] = s[n][ht][3] = 0.f;
-                    if constexpr (PARTS == 1) {
-                        int hi[HT][4], lo[HT][4];
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht)
+                    for (int w = 0; w < KW; ++w)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) hi[ht][i] = lo[ht][i] = 0;
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t a0 = k_lo[n][w] >> (8 * x), a1 = k_hi[n][w] >> (8 * x);
+                            const uint32_t af[4] = {codes_low(a0, k1024), codes_low(a1, k1024), codes_high(a0, k1024), codes_high(a1, k1024)};
 #pragma unroll
-                        for (int w = 0; w < KW; ++w) {
-                            const uint32_t af[4] = {k_lo[n][w] & 0x0f0f0f0fu, k_hi[n][w] & 0x0f0f0f0fu, k_lo[n][w] >> 4 & 0x0f0f0f0fu, k_hi[n][w] >> 4 & 0x0f0f0f0fu};
+                            for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                            for (int ht = 0; ht < HT; ++ht) {
-                                mma_u8s8(hi[ht], af, qb[ht][2 * w][0][0], qb[ht][2 * w + 1][0][0]);
-                                mma_u8u8(lo[ht], af, qb[ht][2 * w][1][0], qb[ht][2 * w + 1][1][0]);
-                            }
+                                for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
                         }
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[n][ht][i] = static_cast<float>(hi[ht][i] * 256 + lo[ht][i]);
-                    } else {
-#pragma unroll
-                        for (int w = 0; w < KW; ++w)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const uint32_t a0 = k_lo[n][w] >> (8 * x), a1 = k_hi[n][w] >> (8 * x);
-                                const uint32_t af[4] = {codes_low(a0, k1024), codes_low(a1, k1024), codes_high(a0, k1024), codes_high(a1, k1024)};
-#pragma unroll
-                                for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                                    for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
-                            }
-                    }
                 }
                 // score + exponent of the two keys of a chunk; of V 2^-exponent, and scale and z times that
                 float sc[N][HT][4], down[N][2], vs[N][2], vz[N][2];
@@ -1010,13 +963,13 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 
 // weights[page][kvh][offset] += sum over the heads of the group of 2^(score - M) / denominator, for every key of the listed requests: scores,
 // maxima and denominators as the kernel above left them.  WG_KEYS keys per thread, whose pages are looked up in front of the wait for that kernel and
-// whose scores are on their way together (bound by such latencies: with one key per thread a call for 8 requests of 4,096 keys on 16 heads took 29.9 us,
-// with four 29.0, with eight 29.6; of 64 requests 157).
+// whose scores are on their way together (bound by such latencies: with one key per thread a call for 8 requests of 4,096 keys on 16 heads took 3 %
+// more, with eight 2 %).
 // A slot is added to once per request that lists it, so the sum does not depend on the order (an atomic: a request may be listed twice).
 #define WG_THREADS 256
 #define WG_KEYS 4
-// Groups of one head: four keys in a row, whose scores are one load and whose weights one atomic of 16 bytes.  (8 requests of 4,096 keys 27.4 us, 64 149, of which 129 without
-// weights.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
+// Groups of one head: four keys in a row, whose scores are one load and whose weights one atomic of 16 bytes.  (8 requests of 4,096 keys 29.4 us, 64 164, of which 143 without
+// weights; by the other kernel 1 and 8 more.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_one_kernel(Q4Args a, float* __restrict__ weights) {
     const int item = blockIdx.z, h = blockIdx.y, P = a.page_tokens;
     const int seg = a.items[item];

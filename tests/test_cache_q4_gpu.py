@@ -439,6 +439,25 @@ def test_addresses_that_break_the_alignment_are_refused():
         K.attn_decode_q4(off(H * D).view(1, -1), pool, out, part_o=torch.zeros(64 * D, device=DEV), part_ml=torch.zeros(64, device=DEV), **kw)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,kv,D,lens", [(8, 2, 256, [9]), (8, 2, 128, [9, 300]), (4, 4, 128, [1500]), (7, 1, 64, [40]), (24, 2, 128, [70])])
+def test_weights_are_float32(dtype, H, kv, D, lens):
+    """Whatever the model's type: scores of up to ten, formed in three roundings of half a unit of 2^-23, move a weight by 1.3e-6 of itself at most, q's
+    24 or 22 bits by less; in the norm over the keys that is below 2^-19."""
+    P = 64
+    for seed in (12, 13, 14):
+        table, n_pages = tables(lens, P, 3)
+        pool = filled(table, lens, kv, D, P, 11, n_pages).to(DEV)
+        q = rnd(len(lens), H * D, dtype=dtype, seed=seed)
+        weights = torch.zeros(n_pages, kv, P, device=DEV)
+        out, ctx = run_decode(q, pool, table, lens, H, kv, D, P, weights=weights)
+        ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
+        want = torch.zeros(n_pages, kv, P, dtype=torch.float64)
+        for (page, h, off), w in ref[3].items():
+            want[page, h, off] += w
+        assert float((weights.cpu().double() - want).norm() / want.norm()) <= 2.0 ** -19
+
+
 def test_weights_of_long_requests():
     """Lengths around what a block of the adding kernel takes."""
     H, kv, D, P = 4, 2, 64, 64
