@@ -968,8 +968,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 // A slot is added to once per request that lists it, so the sum does not depend on the order (an atomic: a request may be listed twice).
 #define WG_THREADS 256
 #define WG_KEYS 4
-// Groups of one head: four keys in a row, whose scores are one load and whose weights one atomic of 16 bytes.  (8 requests of 4,096 keys 29.4 us, 64 164, of which 143 without
-// weights; by the other kernel 1 and 8 more.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
+// Groups of one head: four keys in a row, whose scores are one load and whose weights one atomic of 16 bytes.  (8 requests of 4,096 keys
+// 29.4 us, 64 164, of which 143 without weights; by the other kernel 1 and 8 more.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_one_kernel(Q4Args a, float* __restrict__ weights) {
     const int item = blockIdx.z, h = blockIdx.y, P = a.page_tokens;
     const int seg = a.items[item];
