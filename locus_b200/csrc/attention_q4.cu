@@ -188,6 +188,11 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* out) {
         out[1] = bits(__floats2half2_rn(a - f.x, b - f.y));
     }
 }
+// x 2^k in two factors: 2^k alone falls below float32's range where x 2^k does not
+__device__ __forceinline__ float scale2(float x, float k) {
+    const float a = fmaxf(k, -100.f);
+    return x * exp2f(a) * exp2f(k - a);
+}
 __device__ __forceinline__ float pow2i(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }   // -126 .. 127
 
 __device__ __forceinline__ void load8(const float* p, float* v) {
@@ -441,6 +446,12 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
     constexpr uint32_t STAGE = 2 * PLANE;
     constexpr float RAISE = 4.f, TOP = 10.f;   // weights are 2^TOP at M, at most 2^(TOP + RAISE + 1/2), times scale / 2^exponent < 2: below 65,504
     constexpr int LEAST = -64;                 // smallest exponent that is taken out (smaller scales leave smaller weights)
+    // Denominators are kept apart from the weights that enter the sums: a row of zeros beside rows of 2^100 has a weight that adds nothing to
+    // these (relative to their size it is below 2^-126) and a probability like theirs.  A warp's is relative to the largest score at the last
+    // raise (relative to `from`, terms of large rows would be rounded beside exponents of 100, denominators 1e-6 off); a key that raises nothing
+    // scores at most NEAR - LEAST above that, so its term stays in range.  (Values of more than 2^(NEAR - RAISE) raise at every key near M.)  A part's
+    // is relative to its sums' `from` less LIFT, where the largest key's term lies between 2^(TOP - 126 + LIFT) and 2^(TOP - LEAST + RAISE + LIFT).
+    constexpr float NEAR = 40.f, LIFT = 20.f;
     constexpr int MID = 20;                    // a mid's exponent counts less this: products with z / 2^exponent < 2^(MID + 2) stay in range
     extern __shared__ __align__(16) unsigned char q4_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -601,7 +612,8 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
             // gq + 8; columns are heads 2 t4 + {0, 1}.  l, z: this lane's share of the keys.
             float o[HT][MT][4], l[HT][2], z[HT][2], slope[HT][2];
             // A weight times 2^exponent is formed relative to `from`, up to `limit`: M - TOP and M + RAISE; no live key yet: limit -infinity.
-            float limit[HT][2], from[HT][2];
+            // l is relative to `s_from`.
+            float limit[HT][2], from[HT][2], s_from[HT][2];
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
@@ -610,7 +622,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 for (int c = 0; c < 2; ++c) {
                     const int g = 8 * ht + 2 * t4 + c;
                     limit[ht][c] = -INFINITY;
-                    l[ht][c] = z[ht][c] = from[ht][c] = 0.f;
+                    l[ht][c] = z[ht][c] = from[ht][c] = s_from[ht][c] = 0.f;
                     slope[ht][c] = a.slopes && g < nG ? slope_log2(a.slopes, h0 + g) : 0.f;
                 }
             }
@@ -662,14 +674,14 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                                 for (int y = PARTS - 1; y >= 0; --y) mma_f16(s[n][ht], af, qb[ht][2 * w + x][0][y], qb[ht][2 * w + x][1][y]);
                         }
                 }
-                // score + exponent of the two keys of a chunk; of V 2^-exponent, and scale and z times that
-                float sc[N][HT][4], down[N][2], vs[N][2], vz[N][2];
+                // scores; of the two keys of a chunk V's exponent, and scale and z of V times 2^-exponent
+                float sc[N][HT][4], ve[N][2], vs[N][2], vz[N][2];
                 bool raise = false;
                 __syncwarp();
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
                     const int key[2] = {c0 + 16 * n + kr0, c0 + 16 * n + 8 + kr0};
-                    float ks[2], kz[2], ve[2];
+                    float ks[2], kz[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint4 f = *reinterpret_cast<const uint4*>(at + 16 * (16 * n + kr0 + 8 * i));
@@ -677,23 +689,22 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                         vs[n][i] = q4_mid(f.x);
                         kz[i] = __uint_as_float(f.y);
                         vz[n][i] = __uint_as_float(f.z);
-                        ve[i] = __uint_as_float(f.w);
-                        down[n][i] = ex2(-ve[i]);
+                        ve[n][i] = __uint_as_float(f.w);
                     }
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int c = i & 1, y = i >> 1;
-                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], fmaf(kz[y], sq[ht][c], ve[y]));
+                            float w = fmaf(s[n][ht][i], ks[y] * hq[ht][c], kz[y] * sq[ht][c]);
                             if (biased) w = fmaf(slope[ht][c], static_cast<float>(key[y] - p), w);
                             if (WEIGH) {
                                 const int g = 8 * ht + 2 * t4 + c;
-                                if (g < nG && !dead(key[y])) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w - ve[y];
+                                if (g < nG && !dead(key[y])) scores[static_cast<size_t>(key[y]) * G + 8 * ht + c] = w;
                             }
                             if (dead(key[y])) w = -INFINITY;
                             sc[n][ht][i] = w;
-                            raise |= w > limit[ht][c];
+                            raise |= w + ve[n][y] > limit[ht][c];
                         }
                     }
                 }
@@ -702,18 +713,25 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaxf(sc[0][ht][c], sc[0][ht][2 + c]);
+                            float top = fmaxf(sc[0][ht][c] + ve[0][0], sc[0][ht][2 + c] + ve[0][1]), top_s = fmaxf(sc[0][ht][c], sc[0][ht][2 + c]);
 #pragma unroll
-                            for (int n = 1; n < N; ++n) top = fmaxf(top, fmaxf(sc[n][ht][c], sc[n][ht][2 + c]));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            for (int n = 1; n < N; ++n) {
+                                top = fmaxf(top, fmaxf(sc[n][ht][c] + ve[n][0], sc[n][ht][2 + c] + ve[n][1]));
+                                top_s = fmaxf(top_s, fmaxf(sc[n][ht][c], sc[n][ht][2 + c]));
+                            }
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) {
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                                top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, x));
+                            }
                             const bool none = limit[ht][c] == -INFINITY;   // (no live key so far)
                             const float now = none ? rintf(top) - TOP : fmaxf(from[ht][c], rintf(top) - TOP);
+                            const float s_now = none ? rintf(top_s) : fmaxf(s_from[ht][c], rintf(top_s));
                             const float corr = none ? 0.f : ex2(from[ht][c] - now);
-                            limit[ht][c] = now + (TOP + RAISE);
+                            l[ht][c] = none ? 0.f : l[ht][c] * ex2(s_from[ht][c] - s_now);
+                            s_from[ht][c] = s_now == -INFINITY ? 0.f : s_now;
+                            limit[ht][c] = fminf(now + (TOP + RAISE), s_now + NEAR);
                             from[ht][c] = now == -INFINITY ? 0.f : now;
-                            l[ht][c] *= corr;
                             z[ht][c] *= corr;
 #pragma unroll
                             for (int j = 0; j < MT; ++j) {
@@ -729,10 +747,10 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                     for (int ht = 0; ht < HT; ++ht) {
                         float e[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) e[i] = ex2(sc[n][ht][i] - from[ht][i & 1]);
+                        for (int i = 0; i < 4; ++i) e[i] = ex2(sc[n][ht][i] + ve[n][i >> 1] - from[ht][i & 1]);
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            l[ht][c] = fmaf(e[c], down[n][0], fmaf(e[2 + c], down[n][1], l[ht][c]));
+                            l[ht][c] += ex2(sc[n][ht][c] - s_from[ht][c]) + ex2(sc[n][ht][2 + c] - s_from[ht][c]);
                             z[ht][c] = fmaf(e[c], vz[n][0], fmaf(e[2 + c], vz[n][1], z[ht][c]));
                         }
                         // P^T as the B fragment: the transpose of the accumulator layout, 8 keys at a time
@@ -828,7 +846,9 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                             *reinterpret_cast<float4*>(po + 8 * w) = make_float4(low(t[0]), low(t[2]), high(t[0]), high(t[2]));
                             *reinterpret_cast<float4*>(po + 8 * w + 4) = make_float4(low(t[1]), low(t[3]), high(t[1]), high(t[3]));
                         }
-                        if (gq == 0) *reinterpret_cast<float2*>(res + 8 * HT * HD + 2 * g) = make_float2(limit[ht][c] == -INFINITY ? -INFINITY : from[ht][c], lc);
+                        if (gq == 0)
+                            *reinterpret_cast<float2*>(res + 8 * HT * HD + 2 * g) =
+                                limit[ht][c] == -INFINITY ? make_float2(-INFINITY, lc) : make_float2(from[ht][c], scale2(lc, s_from[ht][c] - from[ht][c] + LIFT));
                     }
                 }
             }
@@ -836,18 +856,34 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
         __syncthreads();
         // joins: the weight of a part whose sums are relative to ml.x, relative to M (a part without a live key: 0; NaN stays)
         auto part_weight = [](float2 ml, float M) { return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M); };
+        auto part_sum = [](float2 ml, float M) { return ml.x == -INFINITY && ml.y == 0.f ? 0.f : scale2(ml.y, ml.x - M); };
         auto finish = [&](int g, const float* acc, float L, float M, int h_first, int at_row, int at_item) {
             const int h = h_first + g;
-            // (the sink: one more term of score 0; scores are in base 2)
-            const float full = a.sink ? L + sink_term2(a.sink_val, h, M) : L;
-            const float inv = 1.0f / full;
+            // (the sink: one more term, of score 0 or its own; scores are in base 2.  One far above all scores: everything less 2^60)
+            float ref = M - LIFT, full = L, lift = exp2f(LIFT);
+            if (a.sink) {
+                const float high = sink_term2(a.sink_val, h, ref + 60.f);
+                if (high > 1.f) {
+                    ref += 60.f;
+                    lift *= 0x1p-60f;
+                    full = fmaf(L, 0x1p-60f, high);
+                } else {
+                    full += sink_term2(a.sink_val, h, ref);
+                }
+            }
+            const float inv = lift / full;
             T* dst = static_cast<T*>(a.out) + (static_cast<size_t>(at_row) * a.nh + h) * HD + lane * DL;
 #pragma unroll
             for (int d = 0; d < DL; d += 2) {
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(dst + d) = make_float2(acc[d] * inv, acc[d + 1] * inv);
                 else *reinterpret_cast<__nv_bfloat162*>(dst + d) = __floats2bfloat162_rn(acc[d] * inv, acc[d + 1] * inv);
             }
-            if (WEIGH && lane == 0) *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(at_item) * a.nh + h)) = make_float2(M, inv);
+            if (WEIGH && lane == 0) {
+                // (the denominator's own exponent goes to what scores are relative to, so that no weight above 2^-126 is flushed)
+                const int k = min(max(static_cast<int>(__float_as_uint(full) >> 23 & 255u) - 127, -126), 126);
+                *reinterpret_cast<float2*>(a.lse + 2 * (static_cast<size_t>(at_item) * a.nh + h)) =
+                    make_float2(ref + static_cast<float>(k), 1.f / (full * pow2i(-k)));
+            }
         };
         // what a (request, head) that a warp leads is, and the first of its heads that this warp takes: the block's heads go round the warps
         struct Led {
@@ -868,7 +904,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                 const float2 mine = lane < r.n ? *reinterpret_cast<const float2*>(ml + (at + lane) * RES_STEP) : make_float2(-INFINITY, 0.f);
                 const float M = warp_max(mine.x);
                 const float w = part_weight(mine, M);
-                const float L = warp_sum(w == 0.f ? 0.f : mine.y * w);
+                const float L = warp_sum(part_sum(mine, M));
                 float acc[DL];
 #pragma unroll
                 for (int d = 0; d < DL; ++d) acc[d] = 0.f;
@@ -938,7 +974,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
                                                 : make_float2(0.f, 0.f);
                     const float top = fmaxf(M, warp_max(mine.x)), corr = M == -INFINITY ? 0.f : exp2f(M - top);
                     const float w = part_weight(mine, top);
-                    L = (M == -INFINITY && L == 0.f ? 0.f : L * corr) + warp_sum(w == 0.f ? 0.f : mine.y * w);
+                    L = part_sum(make_float2(M, L), top) + warp_sum(part_sum(mine, top));
 #pragma unroll
                     for (int d = 0; d < DL; ++d) acc[d] = k0 == 0 ? 0.f : acc[d] * corr;
                     M = top;

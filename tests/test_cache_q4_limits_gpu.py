@@ -1,0 +1,91 @@
+"""The cache held in 4 bits at the ends of its range, on the GPU, against tests/plain_q4.py in 64 bits: rows of very different sizes beside one
+another, and how exact the weights and outputs are whatever the rows hold.  Bounds are derived at each test."""
+import math
+
+import pytest
+import torch
+
+import locus_b200.kernels as K
+import plain_q4 as plain
+from test_cache_q4_gpu import BF16, DEV, F32, check, gen, poison, rnd, run_decode, tables
+
+pytestmark = pytest.mark.gpu
+
+
+def pool_of(table, n_pages, rows, P):
+    """A pool of one key/value head that holds rows[b] [2, n, D] (keys, values) of request b."""
+    D = rows[0].shape[-1]
+    pool = poison(n_pages, 1, D, P)
+    for b, x in enumerate(rows):
+        codes, scale, mid = plain.codes_of(x)
+        for pg in range(-(-x.shape[1] // P)):
+            m = min(P, x.shape[1] - pg * P)
+            full = [torch.zeros(2, 1, P, D, dtype=torch.int64), torch.full((2, 1, P), math.nan, dtype=torch.float64), torch.zeros(2, 1, P, dtype=torch.float64)]
+            for f, y in zip(full, (codes, scale, mid)):
+                f[:, 0, :m] = y[:, pg * P:pg * P + m]
+            pool[int(table[b, pg])] = plain.pack(*full, P, D)
+    return pool.to(DEV)
+
+
+def check_or_zero(out, ref, dtype, H, D):
+    """Rows of zeros give zeros (a bound relative to what they hold would be zero over zero)."""
+    if not ref[0].any():
+        assert not out.any()
+    else:
+        check(out, ref, dtype, H, D)
+
+
+def received(ref, n_pages, P):
+    want = torch.zeros(n_pages, 1, P, dtype=torch.float64)
+    for at, w in ref[3].items():
+        want[at] += w
+    return want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("where", ["first", "last", "mixed"])
+@pytest.mark.parametrize("large,small", [(2.0 ** 74, 0.0), (2.0 ** 120, 0.0), (2.0 ** 120, 2.0 ** -60), (1.0, 0.0)])
+def test_rows_of_zeros_beside_large_rows(dtype, where, large, small):
+    """Scores alike, half of the values large, the others next to nothing: these add nothing to the output but count in the denominator, inside a
+    warp's range, among the ranges of a block (65 keys, 700) and among blocks (5,000)."""
+    H, D, P = 3, 128, 64
+    lens = [5000, 700, 65]
+    table, n_pages = tables(lens, P, 3)
+    rows = []
+    for b, n in enumerate(lens):
+        k, v = 0.02 * rnd(n, D, seed=4 + b), rnd(n, D, seed=14 + b)
+        at = torch.arange(n)
+        tiny = at < n // 2 if where == "first" else at >= n - n // 2 if where == "last" else rnd(n, seed=24 + b) > 0
+        v *= torch.where(tiny, small, large).unsqueeze(1)
+        rows.append(torch.stack([k, v]))
+    pool = pool_of(table, n_pages, rows, P)
+    q = rnd(len(lens), H * D, dtype=dtype, seed=5)
+    weights = torch.zeros(n_pages, 1, P, device=DEV)
+    out, ctx = run_decode(q, pool, table, lens, H, 1, D, P, weights=weights)
+    alone, _ = run_decode(q, pool, table, lens, H, 1, D, P)
+    assert torch.equal(out, alone) and torch.isfinite(out).all()
+    ref = plain.decode(q, pool, table, ctx, H, 1, D, P, D ** -0.5)
+    check(out, ref, dtype, H, D)
+    want = received(ref, n_pages, P)
+    # (scores below one, a few roundings of 2^-24; the exponentials, 2^-22 each; the denominator's sum over the keys)
+    assert ((weights.cpu().double() - want).abs() <= 2.0 ** -18 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [0.0, 2.0 ** 100])
+def test_a_sink_far_above_the_scores(dtype, value):
+    """Sinks from far below to far above the keys' scores, over rows of zeros and over large ones: the weights are the keys' share."""
+    H, D, P = 5, 128, 64
+    lens = [200]
+    table, n_pages = tables(lens, P, 33)
+    pool = pool_of(table, n_pages, [torch.stack([0.02 * rnd(200, D, seed=34), value * rnd(200, D, seed=35)])], P)
+    q = rnd(1, H * D, dtype=dtype, seed=36)
+    for sinks in ([-60.0, 0.0, 5.0, 9.0, 3.0], [50.0, 55.0, 52.0, 51.0, 60.0]):
+        sink = torch.tensor(sinks)
+        weights = torch.zeros(n_pages, 1, P, device=DEV)
+        out, ctx = run_decode(q, pool, table, lens, H, 1, D, P, weights=weights, sink=sink)
+        ref = plain.decode(q, pool, table, ctx, H, 1, D, P, D ** -0.5, sink=sink)
+        check_or_zero(out, ref, dtype, H, D)
+        want = received(ref, n_pages, P)
+        # as above, and the sink's exponent: 60 / ln 2 = 87 in base 2, a product rounded once (2^-18) and taken off (2^-18)
+        assert ((weights.cpu().double() - want).abs() <= 2.0 ** -16 * want).all()
