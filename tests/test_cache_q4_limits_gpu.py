@@ -89,3 +89,25 @@ def test_a_sink_far_above_the_scores(dtype, value):
         want = received(ref, n_pages, P)
         # as above, and the sink's exponent: 60 / ln 2 = 87 in base 2, a product rounded once (2^-18) and taken off (2^-18)
         assert ((weights.cpu().double() - want).abs() <= 2.0 ** -16 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,lens", [(1, [300, 64]), (7, [130])])
+def test_weights_do_not_depend_on_the_sizes_of_values(dtype, H, lens):
+    """A key's weight is formed of its score, whatever its value holds: rows of zeros, of 2^-60, 2^60 and 2^100 leave it as exact as rows of ordinary size.
+    Scores of up to two: rounded a few times by 2^-24 of two, less the largest one (2^-24 of four), the exponential 2^-22; taken together 2^-20.5 of a
+    weight, in the norm over the keys 2^-21.  (A score rounded beside an exponent of 64 or more would be off by up to 2^-18 each time.)"""
+    D, P = 128, 64
+    table, n_pages = tables(lens, P, 43)
+    keys = [0.5 * rnd(n, D, seed=44 + b) for b, n in enumerate(lens)]
+    q = rnd(len(lens), H * D, dtype=dtype, seed=45)
+    for size in (1.0, 0.0, 2.0 ** -60, 2.0 ** 60, 2.0 ** 100):
+        rows = [torch.stack([k, size * rnd(k.shape[0], D, seed=46 + b)]) for b, k in enumerate(keys)]
+        pool = pool_of(table, n_pages, rows, P)
+        weights = torch.zeros(n_pages, 1, P, device=DEV)
+        out, ctx = run_decode(q, pool, table, lens, H, 1, D, P, weights=weights)
+        ref = plain.decode(q, pool, table, ctx, H, 1, D, P, D ** -0.5)
+        check_or_zero(out, ref, dtype, H, D)
+        want = received(ref, n_pages, P)
+        off = (weights.cpu().double() - want).norm() / want.norm()
+        assert float(off) <= 2.0 ** -21, f"values of {size:g}: off by {float(off):.3g}"
