@@ -1094,11 +1094,14 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
         v.page_tokens <= 0 || v.page_tokens % 16 != 0 || v.n_items > Q4_MAX_ITEMS || v.table_stride <= 0 || v.nkv > 65535 || v.counters == nullptr ||
         !mask_ok(static_cast<int>(v.window), static_cast<int>(v.chunk), static_cast<int>(v.keep_first)) ||
         ((reinterpret_cast<uintptr_t>(v.q) | reinterpret_cast<uintptr_t>(v.pool) | reinterpret_cast<uintptr_t>(v.part_o)) & 15) != 0 ||
-        (reinterpret_cast<uintptr_t>(v.part_ml) & 7) != 0)
+        (reinterpret_cast<uintptr_t>(v.part_ml) & 7) != 0 ||
+        (reinterpret_cast<uintptr_t>(v.out) & (v.dt == LOCUS_DT_F32 ? 7 : 3)) != 0)   // (two elements a store)
         return LOCUS_ERR_UNSUPPORTED;
     const int keep_first = v.window == 0 ? 0 : static_cast<int>(v.keep_first);
     if (v.max_units < v.n_items * v.nh * (keep_first > 0 ? 2 : 1)) return LOCUS_ERR_UNSUPPORTED;
-    if (v.weights && (((reinterpret_cast<uintptr_t>(v.weights) | reinterpret_cast<uintptr_t>(v.scores)) & 15) != 0 || v.scores == nullptr || v.lse == nullptr || v.window > 0 || v.chunk > 0)) return LOCUS_ERR_UNSUPPORTED;
+    if (v.weights && (((reinterpret_cast<uintptr_t>(v.weights) | reinterpret_cast<uintptr_t>(v.scores)) & 15) != 0 || v.scores == nullptr || v.lse == nullptr ||
+                      (reinterpret_cast<uintptr_t>(v.lse) & 7) != 0 || v.window > 0 || v.chunk > 0))
+        return LOCUS_ERR_UNSUPPORTED;
     int dev = 0, n_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n_sm <= 0)
         return static_cast<int>(cudaGetLastError());

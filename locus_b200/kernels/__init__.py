@@ -1562,10 +1562,13 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
         raise KernelError("attn_decode_q4: q, the pool and part_o must start at multiples of 16 bytes")
     if ml & 7:
         raise KernelError("attn_decode_q4: part_ml must start at multiples of 8 bytes")
+    op = out.data_ptr()
+    if op & (7 if out.dtype is torch.float32 else 3):
+        raise KernelError("attn_decode_q4: out must start at multiples of two elements")
     if (to | at) & 15:
         raise KernelError("attn_decode_q4: weights and scores must start at multiples of 16 bytes")
     code = _q4_entry("attention_q4", "locus_attn_decode_q4")(
-        _Q4_DECODE.pack(qp, base, out.data_ptr(), seg_q0.data_ptr(), seg_ctx.data_ptr(), block_table.data_ptr(), items.data_ptr(), part, ml,
+        _Q4_DECODE.pack(qp, base, op, seg_q0.data_ptr(), seg_ctx.data_ptr(), block_table.data_ptr(), items.data_ptr(), part, ml,
                         counters.data_ptr(), sink_at, slopes_at, to, at, lse, dtype_code(q.dtype), pages, n_items, n_heads, n_kv_heads, head_dim,
                         page_tokens, window, chunk, max_units, Q4_COST_RANGE, Q4_COST_JOIN, Q4_COST_MERGE, keep_first if window > 0 else 0, sink_flag, scale),
         _q4_stream(dev))

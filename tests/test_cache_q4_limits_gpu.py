@@ -111,3 +111,21 @@ def test_weights_do_not_depend_on_the_sizes_of_values(dtype, H, lens):
         want = received(ref, n_pages, P)
         off = (weights.cpu().double() - want).norm() / want.norm()
         assert float(off) <= 2.0 ** -21, f"values of {size:g}: off by {float(off):.3g}"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_an_output_that_starts_between_two_elements_is_refused(dtype):
+    H, D, P = 2, 64, 16
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    pool = pool_of(torch.tensor([[0]], dtype=torch.int32), 1, [rnd(2, 9, D, seed=51)], P)
+    q = rnd(1, H * D, dtype=dtype, seed=52).to(DEV)
+    kw = dict(seg_q0=i32([0]), seg_ctx=i32([8]), block_table=i32([[0]]), items=i32([0]), n_items=1, n_heads=H, n_kv_heads=1, head_dim=D, page_tokens=P, window=0,
+              scale=1.0, part_o=torch.zeros(64 * D, device=DEV), part_ml=torch.zeros(128, device=DEV), counters=torch.zeros(H, dtype=torch.int32, device=DEV))
+    room = torch.full((H * D + 4,), 7.0, dtype=dtype, device=DEV)
+    with pytest.raises(K.KernelError, match="out must start"):
+        K.attn_decode_q4(q, pool, room[1:1 + H * D].view(1, -1), **kw)
+    assert (room == 7).all()
+    K.attn_decode_q4(q, pool, room[2:2 + H * D].view(1, -1), **kw)   # (two elements further on is a place for two)
+    want = torch.empty_like(q)
+    K.attn_decode_q4(q, pool, want, **kw)
+    assert torch.equal(room[2:2 + H * D], want[0]) and (room[:2] == 7).all() and (room[2 + H * D:] == 7).all()
