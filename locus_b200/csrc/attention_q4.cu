@@ -240,6 +240,8 @@ struct Q4Plan {
     int len, packed, n_blocks;
 };
 
+// position of a segment's query, held to what its row of the table describes (and to -1, no key: no page is read then)
+__device__ __forceinline__ int q4_position(const Q4Args& a, int seg) { return max(-1, min(a.seg_ctx[seg], a.table_stride * a.page_tokens - 1)); }
 // first key that a query at position p sees (besides kept first tokens), rounded down to 16
 __device__ __forceinline__ int q4_first(const Q4Args& a, int p) { return first_key(a.window, a.chunk, p) & ~15; }
 // kept first tokens of an item that lie in front of its window's first chunk: a range of their own, the item's first
@@ -272,7 +274,7 @@ __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_it
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int longest = 1, total = 0;
     for (int i = tid; i < n_items; i += 32 * W) {
-        const int seg = a.items[i], p = a.seg_ctx[seg], row = a.seg_q0[seg];
+        const int seg = a.items[i], p = q4_position(a, seg), row = a.seg_q0[seg];
         const int first = q4_first(a, p);
         pl.row[i] = row;
         pl.pos[i] = p;
@@ -1009,7 +1011,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_one_kernel(Q4Args a, float* __restrict__ weights) {
     const int item = blockIdx.z, h = blockIdx.y, P = a.page_tokens;
     const int seg = a.items[item];
-    const int n = min(a.seg_ctx[seg] + 1, a.table_stride * P);
+    const int n = q4_position(a, seg) + 1;
     const int t = 4 * (blockIdx.x * WG_THREADS + threadIdx.x), i = t / P;
     float* at = t < n ? weights + (static_cast<size_t>(a.block_table[static_cast<size_t>(seg) * a.table_stride + i]) * a.nkv + h) * P + (t - i * P) : nullptr;
     pdl_entry();
@@ -1029,7 +1031,7 @@ __global__ void __launch_bounds__(WG_THREADS) q4_weigh_one_kernel(Q4Args a, floa
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_kernel(Q4Args a, float* __restrict__ weights) {
     const int item = blockIdx.z, kvh = blockIdx.y, G = a.nh / a.nkv, P = a.page_tokens;
     const int seg = a.items[item];
-    const int n = min(a.seg_ctx[seg] + 1, a.table_stride * P);
+    const int n = q4_position(a, seg) + 1;
     const int t0 = blockIdx.x * (WG_THREADS * WG_KEYS) + threadIdx.x;
     const int* table = a.block_table + static_cast<size_t>(seg) * a.table_stride;
     float* at[WG_KEYS];
@@ -1091,7 +1093,7 @@ extern "C" int locus_attn_decode_q4(const Q4DecodeCall* call, cudaStream_t strea
     const Q4DecodeCall& v = *call;
     if (v.n_items <= 0) return 0;
     if ((v.dt != LOCUS_DT_F32 && v.dt != LOCUS_DT_BF16) || v.nkv <= 0 || v.nh <= 0 || v.nh % v.nkv != 0 || !q4_head_ok(static_cast<int>(v.hd)) ||
-        v.page_tokens <= 0 || v.page_tokens % 16 != 0 || v.n_items > Q4_MAX_ITEMS || v.table_stride <= 0 || v.nkv > 65535 || v.counters == nullptr ||
+        v.page_tokens <= 0 || v.page_tokens % 16 != 0 || v.n_items > Q4_MAX_ITEMS || v.table_stride <= 0 || v.table_stride > 0x7fffffff / v.page_tokens || v.nkv > 65535 || v.counters == nullptr ||
         !mask_ok(static_cast<int>(v.window), static_cast<int>(v.chunk), static_cast<int>(v.keep_first)) ||
         ((reinterpret_cast<uintptr_t>(v.q) | reinterpret_cast<uintptr_t>(v.pool) | reinterpret_cast<uintptr_t>(v.part_o)) & 15) != 0 ||
         (reinterpret_cast<uintptr_t>(v.part_ml) & 7) != 0 ||

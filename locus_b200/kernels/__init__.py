@@ -1496,7 +1496,8 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
                    weights: Optional[torch.Tensor] = None, scores: Optional[torch.Tensor] = None) -> None:
     """:func:`attn_decode` over a cache held in 4 bits (``pool`` uint8 [n_pages, 2, n_kv_heads, :func:`q4_page_bytes`], written by
     :func:`rope_kv_write_q4`): the codes are multiplied as they are, nothing is laid out in between.  q and out float32 or bfloat16, any number of
-    query heads per key/value head; masks, sinks and distance biases as there.
+    query heads per key/value head; masks, sinks and distance biases as there.  A position behind what its row of ``block_table`` describes counts as
+    the last that it describes.
 
     ``part_o``, ``part_ml``: scratch for :func:`decode_units_q4` partial results; ``counters`` (int32, n_items * n_heads) must be zero before
     the call and is zero after it.  ``weights`` float32 [n_pages, n_kv_heads, page_tokens] (without a window or chunks): the softmax weight that

@@ -129,3 +129,39 @@ def test_an_output_that_starts_between_two_elements_is_refused(dtype):
     want = torch.empty_like(q)
     K.attn_decode_q4(q, pool, want, **kw)
     assert torch.equal(room[2:2 + H * D], want[0]) and (room[:2] == 7).all() and (room[2 + H * D:] == 7).all()
+
+
+@pytest.mark.parametrize("H", [1, 6])
+def test_positions_behind_the_table_and_in_front_of_it(H):
+    """A position behind what a request's row describes counts as the last that it describes, one below zero sees no key: neither reads pages of the next
+    row or adds to another request's weights."""
+    D, P = 64, 16
+    lens = [48, 30, 48, 17]
+    table, n_pages = tables(lens, P, 61)
+    pool = pool_of(table, n_pages, [rnd(2, n, D, seed=62 + b) for b, n in enumerate(lens)], P)
+    q = rnd(4, H * D, seed=67)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    units = K.decode_units_q4(4, H, DEV)
+
+    def run(ctx):
+        out, weights = torch.full((4, H * D), 9.0, device=DEV), torch.zeros(n_pages, 1, P, device=DEV)
+        scores = torch.full((4 * H * 3 * P + 64,), 5.0, device=DEV)
+        kw = dict(seg_q0=i32(range(4)), seg_ctx=i32(ctx), block_table=table.to(DEV), items=i32(range(4)), n_items=4, n_heads=H, n_kv_heads=1, head_dim=D,
+                  page_tokens=P, window=0, scale=D ** -0.5, part_o=torch.empty(units * D + 64, device=DEV), part_ml=torch.empty(2 * units, device=DEV),
+                  counters=torch.zeros(4 * H, dtype=torch.int32, device=DEV))
+        K.attn_decode_q4(q.to(DEV), pool, out, weights=weights, scores=scores, **kw)
+        assert (scores[-64:] == 5).all() and K.attn_q4_error() == 0
+        alone = torch.empty_like(out)
+        K.attn_decode_q4(q.to(DEV), pool, alone, **kw)
+        assert torch.equal(out.view(torch.int32), alone.view(torch.int32))
+        return out, weights
+
+    want, weights = run([47, 29, 47, 16])
+    for far in (48, 1000, 2 ** 31 - 1):
+        got, now = run([far, 29, far, 16])
+        assert torch.equal(got, want) and torch.equal(now, weights)
+    got, now = run([47, -1, 47, -100])
+    assert torch.equal(got[::2], want[::2]) and torch.isnan(got[1::2]).all()
+    used = torch.zeros(n_pages, dtype=torch.bool)
+    used[table[::2].reshape(-1).long()] = True
+    assert torch.equal(now[used.to(DEV)], weights[used.to(DEV)]) and not now[~used.to(DEV)].any()

@@ -23,3 +23,9 @@ def decode_call(**over):
 ], ids=lambda o: "-".join(f"{k}{v - AT if v >= AT else v}" for k, v in o.items()))
 def test_addresses_that_a_store_cannot_take_are_refused_before_a_launch(over):
     assert decode_call(**over) == K.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("over", [dict(table_stride=0), dict(table_stride=1 << 27), dict(table_stride=1 << 40), dict(page_tokens=8), dict(n_items=1025)],
+                         ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()))
+def test_tables_that_describe_no_position_or_too_many_are_refused(over):
+    assert decode_call(**over) == K.ERR_UNSUPPORTED
