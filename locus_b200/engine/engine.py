@@ -50,7 +50,9 @@ class Engine:
         plain attention with heads of 64, 128 or 256.  ``keep_tokens`` > 0 (with 4 bits): a request that holds a page's tokens more than that
         lets go of the keys that received the least attention so far, in each layer and for each key/value head, down to ``keep_tokens``: the
         first ``keep_first``, the last ``keep_recent`` (0: a quarter) and the heaviest others stay.  Weights are counted from single tokens
-        and from the last token of every portion of a prompt.  A preempted request is evicted from anew as its tokens are fed again."""
+        and from the last token of every portion of a prompt.  A preempted request is evicted from anew as its tokens are fed again.  The pool
+        holds at least ``keep_tokens``, a page and a portion: it is made so large where no size is given; a smaller one shortens the portions (``chunk``) to what it
+        leaves, and one that leaves less than a page is refused."""
         from ..models.model import load_model
 
         model = load_model(model_dir, parse_dtype(dtype), device)
@@ -66,6 +68,8 @@ class Engine:
                    keep_tokens: int = 0, keep_first: int = 4, keep_recent: int = 0) -> "Engine":
         plan = model.plan
         weigh = keep_tokens > 0
+        if keep_tokens < 0:
+            raise ValueError(f"keep_tokens {keep_tokens}")
         if kv_bits:
             if max_running > K.Q4_MAX_ITEMS:
                 raise ValueError(f"kv_bits: at most {K.Q4_MAX_ITEMS} requests at once (max_running {max_running})")
@@ -77,12 +81,10 @@ class Engine:
                 raise ValueError("keep_tokens: a mixer of this model has a window, chunks or a distance bias, or reads pages in another way")
         elif weigh:
             raise ValueError("keep_tokens goes with a cache of 4 bits (kv_bits=4)")
-        bound = 0
         if weigh:
             keep_recent = keep_recent if keep_recent > 0 else keep_tokens // 4
             if keep_first < 0 or keep_first + keep_recent > keep_tokens:
                 raise ValueError(f"keep_tokens {keep_tokens} with the first {keep_first} and the last {keep_recent}")
-            bound = keep_tokens + page_tokens + min(chunk, max_batch_tokens)
         if kv_fraction > 0:
             if not (kv_fraction <= 1.0) or model.device.type != "cuda":
                 raise ValueError("kv_fraction is a share (0, 1] of the free memory of a CUDA device")
@@ -93,10 +95,24 @@ class Engine:
             ctx = int(free * kv_fraction) // max(1, per_token * page_tokens) * page_tokens
             if ctx < page_tokens:
                 raise ValueError(f"kv_fraction {kv_fraction} of {free} free bytes holds no page of {page_tokens} tokens")
-        if ctx <= 0:
+        given = ctx > 0
+        if not given:
             ctx = min(plan.max_positions, 4096)
         if max_seq_tokens <= 0:   # (an evicted request's positions may go beyond the pool)
             max_seq_tokens = plan.max_positions if weigh else min(plan.max_positions, ctx)
+        bound = 0
+        if weigh:
+            # A request lets go of keys behind the step in which it comes to hold keep_tokens and a page: the pool has to hold that and a portion.
+            portion, least = min(chunk, max_batch_tokens), keep_tokens + page_tokens
+            if not given:
+                ctx = max(ctx, min(least + portion, max_seq_tokens))
+            room = -(-ctx // page_tokens) * page_tokens - least
+            if room < portion and least + room < max_seq_tokens:
+                if room < min(portion, page_tokens):
+                    raise ValueError(f"keep_tokens {keep_tokens}: a cache of {ctx} tokens is full before a request holds {least} and lets go of keys "
+                                     f"(it has to hold at least {least + min(portion, page_tokens)})")
+                chunk = portion = room
+            bound = least + portion
         n_pages = -(-ctx // page_tokens)
         cache = CacheManager(model.cache_needs(), page_tokens=page_tokens, n_pages=n_pages,
                              n_state_slots=max_running, max_seq_tokens=max_seq_tokens, dtype=model.dtype,

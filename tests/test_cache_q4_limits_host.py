@@ -1,8 +1,13 @@
 """The cache held in 4 bits on the host: what the native entry points refuse before they touch a device, and the sizes that an engine gives such a
 cache."""
-import pytest
+from types import SimpleNamespace
 
+import pytest
+import torch
+
+import locus_b200.engine.engine as engine_module
 import locus_b200.kernels as K
+from locus_b200.parts.base import Mixer, PagedKvSpec
 
 BF16, F32 = 1, 0
 AT = 1 << 20   # an address that nothing on the host or the device reads: every call here ends before its launch
@@ -29,3 +34,103 @@ def test_addresses_that_a_store_cannot_take_are_refused_before_a_launch(over):
                          ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()))
 def test_tables_that_describe_no_position_or_too_many_are_refused(over):
     assert decode_call(**over) == K.ERR_UNSUPPORTED
+
+
+# ---------------------------------------------------------------------------
+# an engine whose requests let go of keys: the pool, the portions and the scheduler, with a model of one layer that computes nothing
+
+
+class StandInRunner:
+    """Logits of token 1 for every wanted place; checks that every entry has room and counts what requests hold."""
+
+    def __init__(self, model, cache, **kw):
+        self.cache, self.most, self.longest = cache, 0, 0
+
+    def step(self, entries):
+        rows = 0
+        for e in entries:
+            assert e.seq.n_tokens + len(e.tokens) <= self.cache.capacity(e.seq)
+            self.cache.commit(e.seq, len(e.tokens))
+            self.most, self.longest = max(self.most, e.seq.n_tokens), max(self.longest, len(e.tokens))
+            rows += len(e.want)
+        return torch.zeros(rows, 4)
+
+
+class StandInSampler:
+    def __init__(self, device, n):
+        pass
+
+    def sample(self, logits, params, seeds, counters, histories=None):
+        return [1] * len(logits)
+
+
+class StandInMixer(Mixer):
+    reads_q4 = weighs = True
+
+    def cache_needs(self):
+        return PagedKvSpec(1, 64), None
+
+
+def stand_in_model(max_positions):
+    mixer = StandInMixer("")
+    plan = SimpleNamespace(max_positions=max_positions, order=[SimpleNamespace(layer=0)], eos_token_id=-1)
+    return SimpleNamespace(plan=plan, blocks=[SimpleNamespace(mixer=mixer)], dtype=torch.bfloat16, device=torch.device("cpu"),
+                           cache_needs=lambda: [mixer.cache_needs() + (None,)])
+
+
+@pytest.fixture
+def engine_of(monkeypatch):
+    monkeypatch.setattr(engine_module, "ModelRunner", StandInRunner)
+    monkeypatch.setattr(engine_module, "Sampler", StandInSampler)
+    monkeypatch.setattr(K, "evict_q4", lambda *a, **kw: None)
+
+    def make(max_positions=32768, **kw):
+        return engine_module.Engine.from_model(stand_in_model(max_positions), kv_bits=4, **kw)
+
+    return make
+
+
+def finish(eng, *requests):
+    ids = [eng.submit([2] * n, new) for n, new in requests]
+    eng.run_to_completion()
+    got = [eng.get(i) for i in ids]
+    assert [(r.status.value, r.error) for r in got] == [("done", "")] * len(ids)
+    assert [len(r.generated) for r in got] == [new for _, new in requests]
+    assert eng.cache.free_pages() == eng.cache.total_pages()
+    eng.cache.check_invariants()
+
+
+def test_a_pool_of_no_given_size_holds_what_a_request_holds_before_it_lets_go(engine_of):
+    eng = engine_of(keep_tokens=4096, keep_first=4, keep_recent=1024)
+    assert eng.cache.total_pages() * 64 >= 4096 + 64 + 2048 == eng.cache.bound
+    finish(eng, (100, 4300), (7000, 30))
+    assert eng.stats()["evictions"] >= 4 and eng.runner.longest <= 2048 and eng.runner.most <= eng.cache.bound
+    # as before where nothing is let go of, and where a request cannot become as long
+    assert engine_of().cache.total_pages() == 64 and engine_of(keep_tokens=100, chunk=512).cache.total_pages() == 64
+    small = engine_of(max_positions=1000, keep_tokens=4096)
+    assert small.cache.total_pages() == 16
+    finish(small, (500, 400))
+
+
+@pytest.mark.parametrize("ctx", [1024 + 128, 1500, 2000, 3000, 3136, 4096])
+def test_portions_of_a_pool_of_a_given_size_leave_room_for_what_stays(engine_of, ctx):
+    """Requests longer than the pool finish in it, alone and beside one another, preempted behind an eviction as well."""
+    eng = engine_of(keep_tokens=1024, ctx=ctx, max_running=4)
+    pool = eng.cache.total_pages() * 64
+    assert eng.cache.bound <= pool and eng.cfg.chunk == (2048 if ctx >= 3136 else pool - 1024 - 64)
+    finish(eng, (100, 2 * pool))
+    assert eng.stats()["evictions"] > 0 and eng.runner.most <= eng.cache.bound and eng.runner.longest <= eng.cfg.chunk
+    finish(eng, (3000, 300), (50, 1900), (700, 1500))
+    assert eng.stats()["preemptions"] > 0 or ctx >= 3000
+
+
+@pytest.mark.parametrize("ctx,chunk,least", [(1024, 2048, 1152), (1151 - 64, 2048, 1152), (1088, 16, 1104), (512, 64, 1152)])
+def test_a_pool_too_small_to_let_go_of_keys_is_refused(engine_of, ctx, chunk, least):
+    with pytest.raises(ValueError, match=f"at least {least}"):
+        engine_of(keep_tokens=1024, ctx=ctx, chunk=chunk)
+    finish(engine_of(keep_tokens=1024, ctx=least, chunk=chunk), (1500, 30))
+
+
+def test_a_negative_count_of_tokens_is_refused(engine_of):
+    with pytest.raises(ValueError, match="keep_tokens -1"):
+        engine_of(keep_tokens=-1)
