@@ -91,10 +91,16 @@ class Engine:
             empty = CacheManager(model.cache_needs(), page_tokens=page_tokens, n_pages=0, n_state_slots=1,
                                  max_seq_tokens=1, dtype=model.dtype, allocate_device=False, kv_bits=kv_bits, weigh=weigh)
             per_token = empty.bytes_per_token() + empty.staging_bytes_per_token()
+            scratch = 0
+            if kv_bits:   # (shared by layers of one size)
+                table = keep_tokens + page_tokens + min(chunk, max_batch_tokens)
+                table = -(-min(table, max_seq_tokens or plan.max_positions) // page_tokens) * page_tokens
+                scratch = 4 * sum(n for _, n in {kn for m in paged for kn in m.q4_scratch(max_running, table, weigh, model.device).items()})
             free, _ = torch.cuda.mem_get_info(model.device)
-            ctx = int(free * kv_fraction) // max(1, per_token * page_tokens) * page_tokens
+            ctx = (int(free * kv_fraction) - scratch) // max(1, per_token * page_tokens) * page_tokens
             if ctx < page_tokens:
-                raise ValueError(f"kv_fraction {kv_fraction} of {free} free bytes holds no page of {page_tokens} tokens")
+                raise ValueError(f"kv_fraction {kv_fraction} of {free} free bytes holds no page of {page_tokens} tokens"
+                                 + (f" beside {scratch} bytes of scratch" if scratch else ""))
         given = ctx > 0
         if not given:
             ctx = min(plan.max_positions, 4096)

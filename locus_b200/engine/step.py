@@ -70,6 +70,11 @@ class ModelRunner:
         self.rt = Runtime(self.device, model.dtype, max_tokens, max_segments, self.max_wanted)
         model.bind(self.rt)
         self.layer_caches = cache.layer_caches()
+        if cache.kv_bits == 4:
+            # the staging and scratch of such a cache are large: here, with the pools, and not at the first step that wants them
+            for call, lc in zip(model.plan.order, self.layer_caches):
+                if lc.pool is not None:
+                    model.blocks[call.layer].mixer.reserve_q4(self.rt, lc, cache.table_width * cache.page_tokens)
         G = len(cache.groups)
         W = cache.table_width
         # the parts' own step plans (work lists of their kernels), one of each kind, behind the descriptors

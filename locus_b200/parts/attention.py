@@ -38,7 +38,7 @@ float32 arithmetic, so that padded heads take a rotation there too.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Dict, Optional
 
 import torch
 
@@ -314,6 +314,25 @@ class Attention(Mixer):
     def weighs(self) -> bool:
         return not (self.window or self.chunk or self.cache_window or self.slopes is not None)
 
+    def q4_scratch(self, max_segments, table_tokens, weigh, device):
+        units = K.decode_units_q4(max_segments, self.n_heads, device, fixed_ranges=self.keep_first > 0)
+        # (behind the partial results a pair of numbers per request and head, for the weights)
+        sizes = {"attention.q4_part_o": units * self.head_dim + 2 * max_segments * self.n_heads + 4, "attention.q4_part_ml": 2 * units}
+        if weigh:
+            sizes["attention.q4_scores"] = max_segments * self.n_heads * table_tokens
+        return sizes
+
+    def _q4_bufs(self, rt, cache, table_tokens) -> Dict[str, torch.Tensor]:
+        sizes = self.q4_scratch(rt.max_segments, table_tokens, cache.weights is not None, rt.device)
+        return {k: rt.buf(k, (n,), torch.float32) for k, n in sizes.items()}
+
+    def _q4_wide(self, rt, cache, page_tokens) -> torch.Tensor:
+        return rt.buf("attention.q4_wide", (cache.pool.shape[0], 2, self.n_kv_heads, page_tokens, self.head_dim), rt.dtype)
+
+    def reserve_q4(self, rt, cache, table_tokens) -> None:
+        self._q4_bufs(rt, cache, table_tokens)
+        self._q4_wide(rt, cache, cache.page_tokens)
+
     def kernel_modules(self, dtype):
         special = bool(self.keep_first or self.sink)   # such an attention runs on the kernels that know of both
         return (["elementwise", "gemm_simt", "gemv", "attention"] + (["short_conv"] if self.shaped else [])
@@ -424,7 +443,7 @@ class Attention(Mixer):
         if q4:
             if tiles["n_chunk_items"]:
                 # the kernels of portions read ordinary pages: those of the portions' requests, laid out for this layer
-                pool = rt.buf("attention.q4_wide", (pool.shape[0], 2, self.n_kv_heads, gb.page_tokens, self.head_dim), rt.dtype)
+                pool = self._q4_wide(rt, cache, gb.page_tokens)
                 K.expand_q4(cache.pool, pool, segs=None, n_segs=batch.n_seg, seg_ctx=batch.seg_ctx, seg_qn=batch.seg_qn, min_new=2,
                             block_table=gb.block_table, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, page_tokens=gb.page_tokens,
                             max_keys=batch.longest)
@@ -484,21 +503,17 @@ class Attention(Mixer):
             n, (items, seg_q0, seg_ctx) = tiles["n_last"], tiles["last"]
         if not n:
             return
-        units = K.decode_units_q4(rt.max_segments, self.n_heads, rt.device, fixed_ranges=self.keep_first > 0)
-        # (behind the partial results a pair of numbers per request and head, for the weights)
-        part_o = rt.buf("attention.q4_part_o", (units * self.head_dim + 2 * rt.max_segments * self.n_heads + 4,), torch.float32)
-        part_ml = rt.buf("attention.q4_part_ml", (2 * units,), torch.float32)
+        bufs = self._q4_bufs(rt, cache, gb.block_table.shape[1] * gb.page_tokens)
         counters = rt.shared_object(
             ("attention.counters", rt.max_segments * self.n_heads),
             lambda: torch.zeros(rt.max_segments * self.n_heads, dtype=torch.int32, device=rt.device),
         )
         weigh = {}
         if cache.weights is not None:
-            weigh = dict(weights=cache.weights, scores=rt.buf(
-                "attention.q4_scores", (rt.max_segments * self.n_heads * gb.block_table.shape[1] * gb.page_tokens,), torch.float32))
+            weigh = dict(weights=cache.weights, scores=bufs["attention.q4_scores"])
         args = {k: v for k, v in common.items() if k not in ("seg_qn", "seg_q0", "seg_ctx")}
-        K.attn_decode_q4(q, cache.pool, o, seg_q0=seg_q0, seg_ctx=seg_ctx, items=items, n_items=n, part_o=part_o, part_ml=part_ml,
-                         counters=counters, **weigh, **extra, **args)
+        K.attn_decode_q4(q, cache.pool, o, seg_q0=seg_q0, seg_ctx=seg_ctx, items=items, n_items=n, part_o=bufs["attention.q4_part_o"],
+                         part_ml=bufs["attention.q4_part_ml"], counters=counters, **weigh, **extra, **args)
 
 
 register_mixer("attention", Attention)

@@ -280,6 +280,14 @@ class Mixer(Part):
     reads_q4 = False
     weighs = False
 
+    def q4_scratch(self, max_segments: int, table_tokens: int, weigh: bool, device) -> Dict[str, int]:
+        """Buffers of a runtime that the mixer takes in steps on a cache of 4 bits, and their sizes in float32 elements: for up to
+        ``max_segments`` requests whose block table describes ``table_tokens`` each."""
+        return {}
+
+    def reserve_q4(self, rt: "Runtime", cache: "LayerCache", table_tokens: int) -> None:
+        """Have ``rt`` allocate what steps on ``cache`` (4 bits) take, the staging buffer of portions included."""
+
     # A part with ``can_overwrite`` takes ``accumulate=False`` in ``forward``: it then WRITES its output into
     # ``residual`` (float32 rows whose old contents do not matter) instead of adding to it.
     can_overwrite = False

@@ -103,6 +103,13 @@ class ParallelMixers(Mixer):
     def weighs(self) -> bool:
         return all(b.weighs for b in self.branches if b.cache_needs()[0] is not None)
 
+    def q4_scratch(self, max_segments, table_tokens, weigh, device):
+        return {k: n for b in self.branches for k, n in b.q4_scratch(max_segments, table_tokens, weigh, device).items()}
+
+    def reserve_q4(self, rt, cache, table_tokens) -> None:
+        for b in self.branches:
+            b.reserve_q4(rt, cache, table_tokens)
+
     def _cache_of(self, i, cache):
         """The layer's cache as branch ``i`` sees it: with its own stretch of the state slot."""
         if i not in self._state_at or cache.state is None:

@@ -7,6 +7,7 @@ import torch
 
 import locus_b200.engine.engine as engine_module
 import locus_b200.kernels as K
+from locus_b200.cache import CacheManager
 from locus_b200.parts.base import Mixer, PagedKvSpec
 
 BF16, F32 = 1, 0
@@ -71,11 +72,11 @@ class StandInMixer(Mixer):
         return PagedKvSpec(1, 64), None
 
 
-def stand_in_model(max_positions):
-    mixer = StandInMixer("")
-    plan = SimpleNamespace(max_positions=max_positions, order=[SimpleNamespace(layer=0)], eos_token_id=-1)
-    return SimpleNamespace(plan=plan, blocks=[SimpleNamespace(mixer=mixer)], dtype=torch.bfloat16, device=torch.device("cpu"),
-                           cache_needs=lambda: [mixer.cache_needs() + (None,)])
+def stand_in_model(max_positions, *mixers):
+    mixers = mixers or (StandInMixer(""),)
+    plan = SimpleNamespace(max_positions=max_positions, order=[SimpleNamespace(layer=i) for i in range(len(mixers))], eos_token_id=-1)
+    return SimpleNamespace(plan=plan, blocks=[SimpleNamespace(mixer=m) for m in mixers], dtype=torch.bfloat16, device=torch.device("cpu"),
+                           cache_needs=lambda: [m.cache_needs() + (None,) for m in mixers])
 
 
 @pytest.fixture
@@ -134,3 +135,56 @@ def test_a_pool_too_small_to_let_go_of_keys_is_refused(engine_of, ctx, chunk, le
 def test_a_negative_count_of_tokens_is_refused(engine_of):
     with pytest.raises(ValueError, match="keep_tokens -1"):
         engine_of(keep_tokens=-1)
+
+
+# ---------------------------------------------------------------------------
+# what a cache of 4 bits takes beside its pools
+
+
+@pytest.mark.parametrize("weigh", [False, True])
+def test_the_scratch_of_a_cache_of_4_bits_is_known_beforehand(weigh, tmp_path, monkeypatch):
+    """What the mixers say they take is what a runner holds once it is built, before its first step: nothing is left to be found out with the pool in place."""
+    from locus_b200.engine.step import ModelRunner
+    from locus_b200.models import load_model
+    from tiny_configs import config, make_model_dir
+    import emulated_kernels
+
+    emulated_kernels.install(monkeypatch)
+    model = load_model(make_model_dir(tmp_path, "A", raw=dict(config("A"), head_dim=64, num_key_value_heads=2)), torch.float32, "cpu")
+    cache = CacheManager(model.cache_needs(), page_tokens=16, n_pages=8, n_state_slots=3, max_seq_tokens=300, dtype=torch.float32, device="cpu", kv_bits=4, weigh=weigh)
+    runner = ModelRunner(model, cache, max_tokens=32, max_segments=3)
+    mixer = model.blocks[0].mixer
+    said = mixer.q4_scratch(3, cache.table_width * 16, weigh, "cpu")
+    held = {k[0]: t for k, t in runner.rt._bufs.items() if k[0].startswith("attention.q4")}
+    assert {k: t.numel() for k, t in held.items() if k != "attention.q4_wide"} == said
+    assert ("attention.q4_scores" in said) == weigh and (not weigh or said["attention.q4_scores"] == 3 * mixer.n_heads * 19 * 16)
+    wide = held["attention.q4_wide"]
+    assert wide.numel() * wide.element_size() == cache.n_pages * 16 * cache.staging_bytes_per_token()
+    plain_cache = CacheManager(model.cache_needs(), page_tokens=16, n_pages=8, n_state_slots=3, max_seq_tokens=300, dtype=torch.float32, device="cpu")
+    assert not any(k[0].startswith("attention.q4") for k in ModelRunner(model, plain_cache, max_tokens=32, max_segments=3).rt._bufs)
+
+
+def test_a_share_of_the_memory_covers_the_scratch(engine_of, monkeypatch):
+    """1,024 requests that keep 8,192 tokens: their scores alone are more than a gigabyte."""
+    free = 8 << 30
+    scratch = {"part": 10 << 20, "scores": 28 * 1024 * 10304}
+
+    class Device:   # of a model that computes nothing: only its kind is looked at
+        type, index = "cuda", 0
+
+    class WithScratch(StandInMixer):
+        def q4_scratch(self, max_segments, table_tokens, weigh, device):
+            assert (max_segments, table_tokens, weigh) == (1024, 10304, True)
+            return scratch
+
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (free, free))
+    monkeypatch.setattr(engine_module, "CacheManager", lambda *a, **kw: CacheManager(*a, **dict(kw, device="cpu", allocate_device=False)))
+    model = stand_in_model(32768, WithScratch("0"), WithScratch("1"))
+    model.device = Device()
+    eng = engine_module.Engine.from_model(model, kv_bits=4, keep_tokens=8192, max_running=1024, kv_fraction=0.5)
+    c = eng.cache
+    per = c.bytes_per_token() + c.staging_bytes_per_token()
+    taken = c.n_pages * 64 * per + 4 * sum(scratch.values())   # (the layers share it)
+    assert free // 2 - 64 * per < taken <= free // 2
+    with pytest.raises(ValueError, match="holds no page"):
+        engine_module.Engine.from_model(model, kv_bits=4, keep_tokens=8192, max_running=1024, kv_fraction=0.05)
