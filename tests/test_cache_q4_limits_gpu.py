@@ -7,7 +7,7 @@ import torch
 
 import locus_b200.kernels as K
 import plain_q4 as plain
-from test_cache_q4_gpu import BF16, DEV, F32, check, gen, poison, rnd, run_decode, tables
+from test_cache_q4_gpu import BF16, DECODE, DEV, F32, SUMS, check, filled, poison, rnd, run_decode, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,76 @@ def test_positions_behind_the_table_and_in_front_of_it(H):
     used = torch.zeros(n_pages, dtype=torch.bool)
     used[table[::2].reshape(-1).long()] = True
     assert torch.equal(now[used.to(DEV)], weights[used.to(DEV)]) and not now[~used.to(DEV)].any()
+
+
+# ---------------------------------------------------------------------------
+# what is rounded to fewer bits, no more than that
+
+
+def rounded_once(ref, pool, table, ctx, H, kv, D, P, dtype):
+    """The bound of tests/test_cache_q4_gpu.py with what a bfloat16 model's kernel rounds: every weight times its value's scale once to float16 (2^-11 of
+    it, or 2^-35 of the largest where that is more: subnormal, 2^-25 beside 2^10), the output once.  ``plain_q4.decode`` allows for 2^-8 of a weight."""
+    want, step, mass, _ = ref
+    if dtype == F32:
+        return SUMS * mass
+    floor = torch.zeros_like(want)
+    codes, scale, mid = plain.fields(pool, P, D)
+    for b in range(want.shape[0]):
+        t = torch.arange(int(ctx[b]) + 1)
+        vs = scale[table[b, t // P].long(), 1, :, t % P]                       # [keys, kv]
+        floor[b] = len(t) * 2.0 ** -35 * 8 * vs.max(0).values.repeat_interleave(H // kv).unsqueeze(1)
+    return SUMS * mass + 2.0 ** -8 * want.abs() + 2.0 ** -3 * step + floor
+
+
+def within(out, tol, ref, H, D):
+    got = out.cpu().double().view(-1, H, D)
+    worst = float(((got - ref[0]).abs() / tol).max())
+    assert worst <= 1, f"off by {worst:.2f} times the bound"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,kv,D,P,lens", DECODE)
+def test_attention_to_the_roundings_of_its_operands(dtype, H, kv, D, P, lens):
+    table, n_pages = tables(lens, P, 3, extra_width=2)
+    pool = filled(table, lens, kv, D, P, 71, n_pages).to(DEV)
+    q = rnd(len(lens), H * D, dtype=dtype, seed=72, scale=1.5)
+    out, ctx = run_decode(q, pool, table, lens, H, kv, D, P)
+    ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
+    within(out, rounded_once(ref, pool, table, ctx, H, kv, D, P, dtype), ref, H, D)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_that_cancel(dtype):
+    """Pairs of keys of nearly one weight and opposite values: what is left of the output is small beside the weights, so that their rounding shows.
+    (Weights rounded to bfloat16 would be off by four times the bound.)"""
+    H, D, P = 4, 128, 16
+    lens = [2] * 8 + [4] * 8
+    table, n_pages = tables(lens, P, 73)
+    rows = []
+    for b, n in enumerate(lens):
+        v = rnd(n // 2, D, seed=74 + b)
+        rows.append(torch.stack([0.1 * rnd(n, D, seed=94 + b), torch.stack([v, -v], 1).reshape(n, D)]))
+    pool = pool_of(table, n_pages, rows, P)
+    q = rnd(len(lens), H * D, dtype=dtype, seed=75)
+    out, ctx = run_decode(q, pool, table, lens, H, 1, D, P)
+    ref = plain.decode(q, pool, table, ctx, H, 1, D, P, D ** -0.5)
+    within(out, rounded_once(ref, pool, table, ctx, H, 1, D, P, dtype), ref, H, D)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_queries_of_very_different_sizes_keep_their_small_elements(dtype):
+    """Heads of 2^-100 and 2^-110, of zeros, and heads with one element 2^10 times the others: a bfloat16 query goes in as it is and a float32 one with 22 bits
+    of each element, so every head keeps the bound of ordinary ones."""
+    H, kv, D, P = 8, 1, 128, 64
+    lens = [150]
+    table, n_pages = tables(lens, P, 81)
+    pool = filled(table, lens, kv, D, P, 82, n_pages)
+    q = rnd(1, H * D, seed=83).view(H, D)
+    q[0] *= 2.0 ** -100
+    q[1] *= 2.0 ** -110
+    q[2] = 0
+    q[3, 5], q[4, 127] = 2.0 ** 10, -2.0 ** 10
+    q = q.reshape(1, -1).to(dtype)
+    out, ctx = run_decode(q, pool.to(DEV), table, lens, H, kv, D, P)
+    ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
+    within(out, rounded_once(ref, pool, table, ctx, H, kv, D, P, dtype), ref, H, D)
