@@ -75,6 +75,8 @@ def build_parser() -> argparse.ArgumentParser:
                     help="hold keys and values in 4 bits (default 0: in the model's type)")
     ap.add_argument("--keep-tokens", type=int, default=0, metavar="N",
                     help="with --kv-bits 4: a request lets go of the keys that received the least attention, down to N tokens")
+    ap.add_argument("--keep-first", type=int, default=4, metavar="N", help="with --keep-tokens: the first N tokens stay (default 4)")
+    ap.add_argument("--keep-recent", type=int, default=0, metavar="N", help="with --keep-tokens: the last N tokens stay (default 0: a quarter)")
     ap.add_argument("--concurrent", type=int, default=1, help="submit the prompt N times and report aggregate tok/s")
     ap.add_argument("--batch-decode", action="store_true", help="decode all running requests in one batch (always on here)")
     ap.add_argument("--no-batch-prefill", action="store_true", help="force per-token prompt ingestion")
@@ -149,7 +151,7 @@ def main(argv=None) -> int:
         eng = Engine.from_model_dir(args.model, dtype=args.dtype, ctx=args.ctx, page_tokens=args.page_tokens,
                                     max_batch_tokens=max(args.max_batch_tokens, conc), chunk=chunk,
                                     max_running=max(conc, 1), kv_fraction=args.kv_fraction, kv_bits=args.kv_bits,
-                                    keep_tokens=args.keep_tokens)
+                                    keep_tokens=args.keep_tokens, keep_first=args.keep_first, keep_recent=args.keep_recent)
         plan = eng.model.plan
         cfg = plan.config
         print(f"{torch.cuda.get_device_name(0)} | backend=cuda-sm100a | dtype={args.dtype} | layers={len(plan.layers)} "

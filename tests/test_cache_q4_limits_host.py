@@ -188,3 +188,12 @@ def test_a_share_of_the_memory_covers_the_scratch(engine_of, monkeypatch):
     assert free // 2 - 64 * per < taken <= free // 2
     with pytest.raises(ValueError, match="holds no page"):
         engine_module.Engine.from_model(model, kv_bits=4, keep_tokens=8192, max_running=1024, kv_fraction=0.05)
+
+
+def test_what_stays_can_be_said_on_the_command_line():
+    from locus_b200.cli import build_parser
+
+    a = build_parser().parse_args(["--kv-bits", "4", "--keep-tokens", "4096", "--keep-first", "8", "--keep-recent", "1024", "model", "5,17"])
+    assert (a.kv_bits, a.keep_tokens, a.keep_first, a.keep_recent) == (4, 4096, 8, 1024)
+    a = build_parser().parse_args(["model", "5,17"])
+    assert (a.keep_tokens, a.keep_first, a.keep_recent) == (0, 4, 0)
