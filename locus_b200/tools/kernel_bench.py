@@ -191,7 +191,7 @@ def _bench_attn_decode_q4(args) -> None:
 
 def bench_cache_q4(args) -> None:
     """Rows written for --tokens new tokens; those rows laid out in ordinary pages; --batch requests of --ctx tokens in --layers layers evicted
-    down to --keep (into other pages, so that every call does the same)."""
+    down to --keep, into other pages and in place."""
     P, D, H, kv, T = args.page_tokens, args.head_dim, args.heads, args.kv_heads, args.tokens
     dt = getattr(torch, args.dtype)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda:0")  # noqa: E731
@@ -220,6 +220,10 @@ def bench_cache_q4(args) -> None:
     us = _time(lambda: K.evict_q4(pool, weights, **kw, **size), args.iters, args.graph)
     byts = L * B * kv * (4 * n + min(keep, n) * (2 * 2 * (D // 2 + 4) + 8))
     print(f"evict 4 bits batch={B} ctx={n} -> {keep} layers={L} kv_heads={kv} head_dim={D}: {us:.1f} us/call  {byts / us / 1e3:.1f} GB/s")
+    # in place, as the engine evicts: the lengths stay, so every call does the same again on what the one before left
+    kw["dst_table"] = None
+    us = _time(lambda: K.evict_q4(pool, weights, **kw, **size), args.iters, args.graph)
+    print(f"evict 4 bits in place batch={B} ctx={n} -> {keep} layers={L} kv_heads={kv} head_dim={D}: {us:.1f} us/call  {byts / us / 1e3:.1f} GB/s")
 
 
 def bench_attn_decode(args) -> None:
