@@ -16,10 +16,12 @@
 //   * q times a power of two per head that brings its largest element to 2^14 .. 2^15 (taken out of the scores again): a bfloat16 element loses
 //     bits only if it is 2^-29 of the largest, and then at most 2^-40 of that; a float32 q goes in as two parts, 22 bits and more.  (Codes of K as
 //     unsigned bytes against q as whole numbers in two bytes take three instructions a word instead of nine, 64 requests of up to 8,192 keys 47.3 us
-//     instead of 51.1, but the keys' weights were then off by 4e-6 instead of 2e-7; with three bytes it is 51.5.)
+//     where this took 51.1, but the keys' weights were then off by 4e-6 instead of 2e-7; with three bytes it was 51.5.)
 //   * the weights p_t scale_t in float16, formed relative to the running maximum M of score_t + e_t, e_t the exponent of the key's own scale (of its mid
-//     less 20 where that is more), so that they stay below 2^16, whatever the scales are, and are rounded once (2^-12 of a weight, or 2^-35 of the
-//     largest where that is more; two parts for a float32 model).  The unrounded p_t enter the denominator and the sum of the middles.
+//     less 20 where that is more), so that they stay below 2^16, whatever the scales are, and are rounded once (2^-11 of a weight, or 2^-35 of the
+//     largest where that is more; two parts for a float32 model).  The unrounded p_t enter the sum of the middles.  The denominator is a sum of its own,
+//     of 2^(score - largest score): a weight may vanish beside those of larger values, its probability must not.  (Formed of the weights, the
+//     exponents put back: 2 to 4 % less time, and wrong from rows 2^73 times the others' size on.)
 // For a float32 model the products of each chunk of 16 keys are added to the running sums in float32 registers: in the tensor cores' own accumulation
 // over thousands of keys every step's cut-off adds up (measured behind 8,000 keys: 3.9e-6 of the output's norm against 0.5e-6).
 //
@@ -46,10 +48,11 @@
 // Dead keys of an edge chunk (before a window, behind the range's end) have their factors replaced, as unwritten factors may be any bits; codes of
 // any bits are numbers.
 //
-// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 162 registers, 104 KB of copies on their way per SM): the instructions that take codes
-// apart and the latencies between them, at three warps a scheduler; the copies alone (no arithmetic) take 12.7 us of the 25.5 of 8 requests of
-// 4,096 keys (71 MB, 2.8 TB/s), 41 of the 51.1 of 64 requests of 777 to 8,192 keys (28 heads on 4; 171 MB, 3.3 TB/s).  For few keys it is latency:
-// descriptors and cut 2.6 to 4 us, first page ids and rows 2.5, joins 1 to 4.  Sixteen warps of 128 registers, eight of 255, one or four chunks at a
+// What bounds it (16 + 16 heads of 128, bfloat16; 12 warps of 163 registers, 104 KB of copies on their way per SM): the instructions that take codes
+// apart and the latencies between them, at three warps a scheduler.  A copy of the kernel without the arithmetic (descriptors, cut, copies and joins as
+// they are) takes 37.5 of the 52.1 us of 64 requests of 777 to 8,192 keys (28 heads on 4; 171 MB, 3.3 TB/s): the last keys are there at 31 us instead of
+// 47, of 8 requests of 4,096 keys (71 MB, which the L2 holds from call to call) 11.9 of 25.5.  For few keys it is latency:
+// descriptors and cut 3 to 4 us, first page ids and rows 2 to 2.7, joins 1 to 6.  Sixteen warps of 128 registers, eight of 255, one or four chunks at a
 // time, smaller stages: slower by 3 to 18 % (for 8 requests of 4,096 keys).
 //
 // With weights: the scores are written out as they are formed, and a second kernel (q4_weigh_kernel) adds every key's p_t, summed over the heads
@@ -252,8 +255,8 @@ __device__ __forceinline__ int q4_blocks(const int* table, int ranges, int n_vh)
 // some warps may have nothing to do but fewer (request, head)s are joined across blocks.  The cost of a cut, in keys: rounds over the grid x
 // (length + cost_range, and Q4_ODD), and cost_join once where blocks join, and cost_merge per partial result of the longest item.  Lengths
 // from what fills every warp once, 2 % apart, some shorter and longer ones, and the longest item's.
-// (8 requests of 4,096 keys on 16 heads: by whole blocks 25.5 us, unit after unit 3 % more; 64 requests of 777 to 8,192 keys on 4: unit after unit 51.1, 19 % more.
-// One request of 4,096 keys on 16: ranges of 48 keys 14.5, of 64 13.2.)
+// (8 requests of 4,096 keys on 16 heads: unit after unit 3 % more than by whole blocks; 64 requests of 777 to 8,192 keys on 4: by whole blocks 19 % more than unit after
+// unit.  One request of 4,096 keys on 16: ranges of 48 keys 14.5 us, of 64 13.2.)
 template <int W>
 __device__ __forceinline__ int plan_ranges(Q4Plan& pl, const Q4Args& a, int n_items, int n_vh, long long max_ranges, int cost_range, int cost_join,
                                            int cost_merge) {
@@ -993,7 +996,7 @@ __global__ void __launch_bounds__(32 * W, 1) attn_decode_q4_kernel(Q4Args a, int
 #define WG_THREADS 256
 #define WG_KEYS 4
 // Groups of one head: four keys in a row, whose scores are one load and whose weights one atomic of 16 bytes.  (8 requests of 4,096 keys
-// 29.4 us, 64 164, of which 143 without weights; by the other kernel 1 and 8 more.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
+// 29.1 us, 64 162, of which 151 without weights; by the other kernel 1 and 8 more.  In groups of several heads four keys' scores are 4 G floats in a row, too wide a stride between a warp's lanes.)
 __global__ void __launch_bounds__(WG_THREADS) q4_weigh_one_kernel(Q4Args a, float* __restrict__ weights) {
     const int item = blockIdx.z, h = blockIdx.y, P = a.page_tokens;
     const int seg = a.items[item];

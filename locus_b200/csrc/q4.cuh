@@ -10,7 +10,8 @@
 // A row of equal values has scale 0 and is read as mid; a row that holds a value that is not finite has a scale that is not a number, and so
 // has everything read from it.
 // One pair of factors per token and key/value head: a row is written once, by the step that has it, and never again (factors that several
-// tokens share would have to be revised when the next token comes).  bfloat16 has float32's range, so no row is too large or too small.
+// tokens share would have to be revised when the next token comes).  bfloat16 has float32's range, so no row is too small, nor too large up to 3.38e38
+// (a factor of a row of larger values may round to infinity, or the row be read beyond float32's range).
 // The factors of a page lie together behind its codes: rows of hd / 2 bytes keep the alignment of 16-byte loads and bulk copies (hd / 2 + 4
 // would not), and of a whole page codes and factors are one run.
 // Of the eight values of a little-endian 32-bit word value 2 i lies in nibble i and value 2 i + 1 in nibble i + 4: one shift and one mask

@@ -1341,7 +1341,7 @@ def rope_kv_write_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     """:func:`rope_kv_write` into a cache held in 4 bits: q, rotated, to ``q_out`` in the model's type; k, rotated, and v, neither rounded to
     the model's type first, to the rows of ``slots`` in ``pool`` uint8 [n_pages, 2, n_kv_heads, :func:`q4_page_bytes`].  A row x of a head is
     held as one of sixteen codes per element and two bfloat16: scale = (max - min) / 15 and mid = (min + max) / 2, and stands for
-    mid + scale * (code - 7.5); a row with a value that is not finite reads as NaN.  The angles' product and reduction are 64 bits.
+    mid + scale * (code - 7.5); a row with a value that is not finite reads as NaN (a finite one beyond 3.38e38 may read as infinite).  The angles' product and reduction are 64 bits.
     ``weights`` float32 [n_pages, n_kv_heads, page_tokens]: set to 0 for the slots written (see :func:`attn_decode_q4`).  ``n_heads`` 0 with
     ``q_out`` None: rows of k and v alone.  The slots of a call are different ones."""
     what = "rope_kv_write_q4"
