@@ -1502,7 +1502,7 @@ def attn_decode_q4(q: torch.Tensor, pool: torch.Tensor, out: torch.Tensor, *, se
     ``part_o``, ``part_ml``: scratch for :func:`decode_units_q4` partial results; ``counters`` (int32, n_items * n_heads) must be zero before
     the call and is zero after it.  ``weights`` float32 [n_pages, n_kv_heads, page_tokens] (without a window or chunks): the softmax weight that
     each key gets, summed over the query heads of its group, is added to the key's slot; ``scores`` is scratch for that, float32 with
-    n_items * n_heads * block_table.shape[1] * page_tokens elements.  Calls that may run at the same time (on two streams, from two graphs) need
+    n_items * n_heads * block_table.shape[1] * page_tokens elements, and so are the last 2 * n_items * n_heads + 3 elements of ``part_o``.  Calls that may run at the same time (on two streams, from two graphs) need
     scratch and counters of their own."""
     what = "attn_decode_q4"
     _q4_pool(what, pool, n_kv_heads, head_dim, page_tokens)

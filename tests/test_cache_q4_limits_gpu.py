@@ -238,3 +238,26 @@ def test_queries_of_very_different_sizes_keep_their_small_elements(dtype):
     out, ctx = run_decode(q, pool.to(DEV), table, lens, H, kv, D, P)
     ref = plain.decode(q, pool, table, ctx, H, kv, D, P, D ** -0.5)
     within(out, rounded_once(ref, pool, table, ctx, H, kv, D, P, dtype), ref, H, D)
+
+
+def test_requests_that_are_preempted_behind_an_eviction(tmp_path):
+    """A pool that holds one request's keys, a page and a short portion: requests longer than the pool, beside one another, finish and give everything back, and
+    the same run again gives the same tokens."""
+    from locus_b200.engine.engine import Engine
+    from test_engine_q4_gpu import CASES
+    from tiny_configs import make_model_dir, random_tokens
+
+    raw = CASES["heads64"]
+    folder = make_model_dir(tmp_path, "A", raw=dict(raw))
+    prompts = [random_tokens(n, raw["vocab_size"], n) for n in (40, 150, 90)]
+    seen = []
+    for _ in range(2):
+        eng = Engine.from_model_dir(folder, dtype="bfloat16", kv_bits=4, keep_tokens=48, ctx=96, page_tokens=16, max_running=3)
+        assert eng.cfg.chunk == 32 and eng.cache.bound == 96 and eng.stats()["total_pages"] == 6
+        out = eng.generate(prompts, 80)
+        assert [len(x) for x in out] == [80] * 3
+        stats = eng.stats()
+        assert stats["evictions"] > 6 and stats["preemptions"] > 0 and stats["free_pages"] == 6
+        eng.cache.check_invariants()
+        seen.append(out)
+    assert seen[0] == seen[1]
